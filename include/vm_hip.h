@@ -707,6 +707,93 @@ int vm_hip_add_rmsnorm_stage_f32(float* h, const float* delta, const float* w, v
 int vm_hip_silu_mul_stage_f32(const float* gate_up, void* a_staged, int layout, float* out_f32, int64_t rows,
                               int64_t inter, void* stream);
 
+/* ---- INT8 KV cache (no counterpart in the reference, whose cache is fp32
+ * and grows by Concat) ----------------------------------------------------
+ * Keys (after rotation) and values as 8-bit codes with one fp32 scale for
+ * each token and KV head, quantized as quant.cpp quantizes a column
+ * (src/quant.cpp:74-104): scale = max|x| / 127, code = x times the scale's
+ * reciprocal rounded half away from zero and clamped to +-127, all in fp32.
+ * A row whose largest magnitude is below 2^-119 is stored as zeros with
+ * scale 1; a row that holds an infinity or NaN as zeros with scale NaN, so
+ * that whatever attends to it is NaN.
+ *
+ * k_codes, v_codes  int8 [batch, kv_heads, max_seq, head_dim], 16-byte aligned
+ * k_scales, v_scales f32 [batch, kv_heads, max_seq]
+ *
+ * head_dim is 64 or 128; max_seq * head_dim < 2^31; batch <= 65535.
+ * `pos` is an int32 per sequence in device memory: how many tokens are
+ * cached before the call's.  `counts` (int32 per sequence in device memory,
+ * or NULL: all of them) says how many of the call's `rows` tokens a sequence
+ * really has; what belongs to the others (padding) is left as it was.
+ * dtype is VM_HIP_DTYPE_F32, _F16 or _BF16. */
+typedef struct vm_hip_kv_q8 {
+    int8_t* k_codes;
+    float*  k_scales;
+    int8_t* v_codes;
+    float*  v_scales;
+    int64_t batch, kv_heads, max_seq, head_dim;
+} vm_hip_kv_q8;
+
+/* vm_hip_rope_kv_append_f32 for this cache.  qkv [batch, rows, (heads + 2
+ * kv_heads) * head_dim]; token t of sequence b is rotated at position pos[b]
+ * + t, or pos[b] + depths[b * rows + t] when depths (int32 [batch, rows]) is
+ * given, as a tree's nodes are: siblings share a position, but every node has
+ * its own cache row pos[b] + t.  Each product, difference and sum of the
+ * rotation is rounded to fp32; the rotated key is quantized from there, and
+ * the rotated query rounded once to dtype, q_out [batch, heads, rows,
+ * head_dim].  Tokens whose cache row is outside [0, max_seq) are not written
+ * at all; rotation positions are clamped to the tables' rows [0, max_seq).
+ * qkv and q_out are 16-byte aligned. */
+int vm_hip_kv_q8_append(const vm_hip_kv_q8* cache, const void* qkv, int dtype, int64_t rows, int64_t heads,
+                        const float* cos_table, const float* sin_table, const int32_t* pos, const int32_t* counts,
+                        const int32_t* depths, void* q_out, void* stream);
+
+/* The cache's rows first .. first + rows - 1 as numbers (code times scale,
+ * rounded once to dtype): k_out, v_out [batch, kv_heads, rows, head_dim],
+ * 16-byte aligned; either may be NULL.  For kernels that take K and V in
+ * fp32 (vm_hip_attention_f32). */
+int vm_hip_kv_q8_read(const vm_hip_kv_q8* cache, int64_t first, int64_t rows, void* k_out, void* v_out, int dtype,
+                      void* stream);
+
+/* Keeps the accepted path of a tree: for every sequence b and i <
+ * kept_counts[b], the cache row pos[b] + kept[b * width + i] moves to row
+ * pos[b] + i, codes and scales bit for bit.  All rows are read before any is
+ * written, so any indices do (ascending ones are what a path has); an entry
+ * whose source or target row is outside [0, max_seq) is skipped.  width <=
+ * 256 (VM_HIP_KV_Q8_KEEP_MAX); kept_counts are clamped to [0, width]. */
+#define VM_HIP_KV_Q8_KEEP_MAX 256
+int vm_hip_kv_q8_keep(const vm_hip_kv_q8* cache, const int32_t* pos, const int32_t* kept, const int32_t* kept_counts,
+                      int64_t width, void* stream);
+
+/* Attention over the INT8 cache for `rows` tokens of every sequence: one
+ * decoded token, a prompt's chunk, or a tree of drafted tokens, whose keys
+ * and values vm_hip_kv_q8_append has written at cache rows pos[b] + t.
+ *   q    [batch, heads, rows, head_dim] of dtype, as kv_q8_append leaves it;
+ *        query head h reads KV head h / (heads / kv_heads)
+ *   out  [batch, rows, heads * head_dim] of dtype; both 16-byte aligned
+ *   tree uint64 [batch, rows, ceil(rows / 64)] in device memory: token t sees
+ *        every cache row below pos[b] and, of the call's own rows, row pos[b]
+ *        + j where bit j % 64 of word j / 64 is set (a node's ancestors and
+ *        itself).  Bits at or past the sequence's count are ignored.  NULL: a
+ *        chain, token t sees rows up to pos[b] + t.
+ * scale <= 0 means 1/sqrt(head_dim).  A token that sees no row gives zeros.
+ * Cache rows at or past max_seq do not exist.
+ * Scores, maxima, sums and the output are accumulated in fp32; what is
+ * rounded before: with fp32 queries, the query and each weight to 22
+ * significant bits (two fp16 parts); with 16-bit queries, each weight to fp16
+ * (codes and queries are exact).
+ *
+ * workspace: vm_hip_attention_q8_workspace_bytes bytes of device memory (0 is
+ * possible: then workspace may be NULL), 16-byte aligned and zeroed before its
+ * first use; every call leaves it ready for the next one of the same or
+ * smaller size and of any shape.  Calls that share a workspace must not
+ * overlap.  workspace_bytes returns the bytes, or a negative status. */
+int64_t vm_hip_attention_q8_workspace_bytes(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads,
+                                            int64_t head_dim, int64_t max_seq);
+int vm_hip_attention_q8(const vm_hip_kv_q8* cache, const void* q, void* out, int dtype, int64_t rows, int64_t heads,
+                        const int32_t* pos, const int32_t* counts, const uint64_t* tree, float scale, void* workspace,
+                        int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -50,6 +50,12 @@ class QmmMember(ctypes.Structure):
     _fields_ = [("codes", c_void_p), ("scales", c_void_p), ("c", c_void_p), ("n", c_int64)]
 
 
+class KvQ8(ctypes.Structure):
+    """vm_hip_kv_q8 (include/vm_hip.h): device addresses and shape of an INT8 cache."""
+    _fields_ = [("k_codes", c_void_p), ("k_scales", c_void_p), ("v_codes", c_void_p), ("v_scales", c_void_p),
+                ("batch", c_int64), ("kv_heads", c_int64), ("max_seq", c_int64), ("head_dim", c_int64)]
+
+
 def _declare(L: ctypes.CDLL) -> None:
     p = c_void_p
     sig = {
@@ -134,6 +140,11 @@ def _declare(L: ctypes.CDLL) -> None:
         "vm_hip_qmm_staged_f32": ([p, p, p, p, c_int64, c_int64, c_int64, c_int, c_int, p], c_int),
         "vm_hip_add_rmsnorm_stage_f32": ([p, p, p, p, c_int, p, c_int64, c_int64, c_float, p], c_int),
         "vm_hip_silu_mul_stage_f32": ([p, p, c_int, p, c_int64, c_int64, p], c_int),
+        "vm_hip_kv_q8_append": ([POINTER(KvQ8), p, c_int, c_int64, c_int64, p, p, p, p, p, p, p], c_int),
+        "vm_hip_kv_q8_read": ([POINTER(KvQ8), c_int64, c_int64, p, p, c_int, p], c_int),
+        "vm_hip_kv_q8_keep": ([POINTER(KvQ8), p, p, p, c_int64, p], c_int),
+        "vm_hip_attention_q8_workspace_bytes": ([c_int64] * 6, c_int64),
+        "vm_hip_attention_q8": ([POINTER(KvQ8), p, p, c_int, c_int64, c_int64, p, p, p, c_float, p, c_int64, p], c_int),
     }
     for name, (args, res) in sig.items():
         fn = getattr(L, name)
@@ -166,7 +177,9 @@ def exported_symbols() -> list[str]:
             "vm_hip_qmm_add_f32", "vm_hip_attention_decode_chain_f32", "vm_hip_rope_append_f32",
             "vm_hip_qmm_norm_group_f32", "vm_hip_qmm_swiglu_add_f32",
             "vm_hip_qmm_a_layout", "vm_hip_qmm_staged_f32", "vm_hip_add_rmsnorm_stage_f32",
-            "vm_hip_silu_mul_stage_f32", "vm_hip_copy_strided"]
+            "vm_hip_silu_mul_stage_f32", "vm_hip_copy_strided",
+            "vm_hip_kv_q8_append", "vm_hip_kv_q8_read", "vm_hip_kv_q8_keep", "vm_hip_attention_q8_workspace_bytes",
+            "vm_hip_attention_q8"]
 
 
 def open_library() -> ctypes.CDLL:
@@ -360,6 +373,43 @@ def dequant_int8(q: int, scale: int, w: int, rows: int, cols: int, stream=None) 
 
 def dequant_int4(packed: int, scale: int, w: int, rows: int, cols: int, block: int, stream=None) -> None:
     check(open_library().vm_hip_dequant_int4(packed, scale, w, rows, cols, block, _h(stream)))
+
+
+# ---- INT8 cache and attention over it (raw device addresses) ----
+
+def kv_q8_append(cache: KvQ8, qkv: int, dtype: int, rows: int, heads: int, cos: int, sin: int, pos: int, counts,
+                 depths, q_out: int, stream=None) -> None:
+    """vm_hip_kv_q8_append: rotate q and k, quantize k and v into the cache rows pos[b] + t."""
+    check(open_library().vm_hip_kv_q8_append(byref(cache), qkv, dtype, rows, heads, cos, sin, pos, counts, depths,
+                                             q_out, _h(stream)))
+
+
+def kv_q8_read(cache: KvQ8, first: int, rows: int, k_out, v_out, dtype: int, stream=None) -> None:
+    """vm_hip_kv_q8_read: cache rows first .. first + rows - 1 as numbers."""
+    check(open_library().vm_hip_kv_q8_read(byref(cache), first, rows, k_out, v_out, dtype, _h(stream)))
+
+
+def kv_q8_keep(cache: KvQ8, pos: int, kept: int, kept_counts: int, width: int, stream=None) -> None:
+    """vm_hip_kv_q8_keep: cache rows pos[b] + kept[b, i] to pos[b] + i."""
+    check(open_library().vm_hip_kv_q8_keep(byref(cache), pos, kept, kept_counts, width, _h(stream)))
+
+
+def attention_q8_workspace_bytes(batch: int, rows: int, heads: int, kv_heads: int, head_dim: int, max_seq: int) -> int:
+    return _size(open_library().vm_hip_attention_q8_workspace_bytes(batch, rows, heads, kv_heads, head_dim, max_seq))
+
+
+def attention_q8(cache: KvQ8, q: int, out: int, dtype: int, rows: int, heads: int, pos: int, counts, tree,
+                 scale: float, workspace, workspace_bytes: int, stream=None) -> None:
+    """vm_hip_attention_q8: tokens, prompts or trees of drafted tokens over an INT8 cache."""
+    check(open_library().vm_hip_attention_q8(byref(cache), q, out, dtype, rows, heads, pos, counts, tree, scale,
+                                             workspace, workspace_bytes, _h(stream)))
+
+
+def _size(n: int) -> int:
+    """A size from an entry point that returns bytes or a negative status."""
+    if n < 0:
+        check(n)
+    return n
 
 
 def synchronize() -> None:
