@@ -794,6 +794,95 @@ int vm_hip_attention_q8(const vm_hip_kv_q8* cache, const void* q, void* out, int
                         const int32_t* pos, const int32_t* counts, const uint64_t* tree, float scale, void* workspace,
                         int64_t workspace_bytes, void* stream);
 
+/* ---- INT8 x INT8 matrix product with scales for each token and column (no
+ * counterpart in the reference, whose activations stay in floating point) --
+ * The INT8 weights of vm_hip_qmm_f32 (per-column scales) times activations
+ * quantized to 8 bits with one scale for each token (row):
+ *   C[m, n] = fp32(sum_k a[m, k] w[k, n]) * (a_scale[m] * w_scale[n])
+ * with an exact 32-bit integer sum, one fp32 conversion and two fp32
+ * products, rounded once more to c_dtype when that has 16 bits: the result
+ * does not depend on how the work is split.  Against vm_hip_qmm_f32, whose
+ * activations keep 22 bits, this is the cheaper product of a model whose
+ * activations allow 8 bits.
+ *
+ *   vm_hip_a8_pack   lays the weights' codes [k, n] (vm_hip_pack_int8) out
+ *                    for the matrix cores, once: vm_hip_a8_weights_bytes
+ *                    bytes; the codes are not needed afterwards
+ *   vm_hip_a8_stage  quantizes rows of activations a [rows, k] (dtype F32,
+ *                    F16 or BF16) as the INT8 cache quantizes a head's row
+ *                    (above: max / 127, zeros below 2^-119, NaN for a row
+ *                    that is not finite) into vm_hip_a8_stage_bytes bytes;
+ *                    one staged buffer serves every product of those rows
+ *                    (q | k | v, gate | up)
+ *   vm_hip_qmm_a8    the product: scale [n] fp32, c [rows, n] of c_dtype
+ *
+ * Buffers of packed weights and staged rows are 16-byte aligned; a, codes,
+ * scale and c as their elements are.  1 <= k <= 131072 (the largest sum then
+ * fits 32 bits); rows == 0 or n == 0 is a no-op.
+ * workspace: vm_hip_qmm_a8_workspace_bytes bytes (0 is possible: then it may
+ * be NULL), 16-byte aligned and zeroed before its first use; every call
+ * leaves it ready for the next one of any shape it is large enough for.
+ * Calls that share a workspace must not overlap.  The functions that return
+ * bytes return a negative status for a shape that the product refuses. */
+#define VM_HIP_A8_MAX_K 131072
+int64_t vm_hip_a8_weights_bytes(int64_t k, int64_t n);
+int64_t vm_hip_a8_stage_bytes(int64_t rows, int64_t k);
+int64_t vm_hip_qmm_a8_workspace_bytes(int64_t rows, int64_t k, int64_t n);
+int vm_hip_a8_pack(const int8_t* codes, int64_t k, int64_t n, void* packed, void* stream);
+int vm_hip_a8_stage(const void* a, int dtype, int64_t rows, int64_t k, void* staged, void* stream);
+int vm_hip_qmm_a8(const void* staged, const void* packed, const float* scale, void* c, int c_dtype, int64_t rows,
+                  int64_t k, int64_t n, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- Logits under rules, and the greedy token (no counterpart in the
+ * reference, which takes the argmax of bare logits) -------------------------
+ * logits [seqs, rows, vocab] of dtype (F32, F16 or BF16): `rows` positions of
+ * every sequence, 1 when tokens are decoded one by one, the nodes of a tree of
+ * drafted tokens when they are verified.  In fp32, for every value x of a row
+ *   n  how often its token stands in the sequence's history and, with
+ *      `drafted`, on the row's path
+ *   if n > 0:  x = x > 0 ? x / repetition : x * repetition;
+ *              x = (x - n * frequency) - presence
+ *   x = x + bias of its token; where the token is listed several times the
+ *      last entry counts
+ *   x = -infinity where the token is not allowed (whatever x is)
+ * with every step rounded to fp32; out (may be logits itself, or NULL) gets x
+ * rounded once to dtype, and tokens [seqs, rows] (int32, or NULL) the lowest
+ * index of the largest fp32 x, NaN skipped, or -1 where no token has more
+ * than -infinity.  Rows t >= counts[s] (int32 per sequence, or NULL: all
+ * rows count) are padding: nothing of theirs is written.
+ *
+ * A pointer of the rules that is NULL leaves its rule out (repetition 1,
+ * frequency and presence 0, no bias, everything allowed).  Tokens outside
+ * [0, vocab) match nothing; lengths are clamped to [0, stride].
+ * logits and out are aligned as their elements are. */
+typedef struct vm_hip_logits_rules {
+    const int32_t*  history;          /* [seqs, history_stride]                    */
+    const int32_t*  history_lengths;  /* [seqs], with history                      */
+    int64_t         history_stride;
+    const float*    repetition;       /* [seqs]                                    */
+    const float*    frequency;        /* [seqs]                                    */
+    const float*    presence;         /* [seqs]                                    */
+    const int32_t*  bias_tokens;      /* [seqs, bias_stride]                       */
+    const float*    bias_values;      /* [seqs, bias_stride], with bias_tokens     */
+    const int32_t*  bias_lengths;     /* [seqs], with bias_tokens                  */
+    int64_t         bias_stride;
+    const uint32_t* allowed;          /* [seqs, rows, ceil(vocab / 32)], bit 1: may */
+    const int32_t*  drafted;          /* [seqs, rows]: the token of each row's node */
+    const uint64_t* tree;             /* [seqs, rows, ceil(rows / 64)]: the nodes on
+                                       * a row's path, itself among them; NULL with
+                                       * drafted: rows 0 .. t                       */
+} vm_hip_logits_rules;
+
+/* workspace: vm_hip_logits_rules_workspace_bytes bytes, 16-byte aligned and
+ * zeroed before its first use; needed for tokens (NULL otherwise); every call
+ * leaves it ready for the next one of any shape it is large enough for.  Calls
+ * that share a workspace must not overlap.  seqs * rows <= 65536, vocab <
+ * 2^31; workspace_bytes returns a negative status otherwise. */
+int64_t vm_hip_logits_rules_workspace_bytes(int64_t seqs, int64_t rows, int64_t vocab);
+int vm_hip_logits_rules_apply(const vm_hip_logits_rules* rules, const void* logits, void* out, int dtype,
+                              int32_t* tokens, int64_t seqs, int64_t rows, int64_t vocab, const int32_t* counts,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

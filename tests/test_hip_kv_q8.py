@@ -66,6 +66,13 @@ def same(a, b):
         assert np.array_equal(a[k].view(np.uint8), b[k].view(np.uint8)), k
 
 
+def assert_equal(got, want):
+    """Bit for bit (any NaN for a NaN), with a short message."""
+    assert got.shape == want.shape
+    differ = ~((got == want) | (np.isnan(got) & np.isnan(want)))
+    assert not differ.any(), f"{differ.sum()} of {differ.size} differ, first at {np.argwhere(differ)[0]}: {got[differ][0]!r}, not {want[differ][0]!r}"
+
+
 def dev(hip, a):
     return hip.DeviceBuffer.from_array(a)
 

@@ -7,6 +7,7 @@
 #include <cmath>
 #include <cstdint>
 
+#include "vm_device.h"
 #include "vm_hip.h"
 
 namespace vmhip {
@@ -18,6 +19,31 @@ struct F16 {
 struct BF16 {
     uint16_t bits;
 };
+
+template <typename T>
+__device__ __forceinline__ float widen(T v);
+template <>
+__device__ __forceinline__ float widen<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float widen<F16>(F16 v) { return static_cast<float>(__builtin_bit_cast(_Float16, v.bits)); }
+template <>
+__device__ __forceinline__ float widen<BF16>(BF16 v) { return __uint_as_float(static_cast<uint32_t>(v.bits) << 16); }
+
+// An fp32 value rounded to nearest even.  (The empty statement keeps the
+// compiler from folding the product that made v into its conversion to fp16,
+// v_fma_mixlo_f16: that skips the product's own rounding to fp32, which
+// results are defined with.)
+template <typename T>
+__device__ __forceinline__ T narrow(float v);
+template <>
+__device__ __forceinline__ float narrow<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ F16 narrow<F16>(float v) {
+    asm("" : "+v"(v));
+    return F16{__builtin_bit_cast(uint16_t, static_cast<_Float16>(v))};
+}
+template <>
+__device__ __forceinline__ BF16 narrow<BF16>(float v) { return BF16{f32_to_bf16_ref(v)}; }
 
 // Checks of the cache that every entry point shares (VM_HIP_EINVAL with a
 // message that names `who`).

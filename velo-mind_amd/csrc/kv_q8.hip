@@ -46,26 +46,6 @@ struct alignas(sizeof(T) * N) Vec {
     T e[N];
 };
 
-template <typename T>
-__device__ __forceinline__ float widen(T v);
-template <>
-__device__ __forceinline__ float widen<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ float widen<F16>(F16 v) { return static_cast<float>(__builtin_bit_cast(_Float16, v.bits)); }
-template <>
-__device__ __forceinline__ float widen<BF16>(BF16 v) { return __uint_as_float(static_cast<uint32_t>(v.bits) << 16); }
-
-template <typename T>
-__device__ __forceinline__ T narrow(float v);
-template <>
-__device__ __forceinline__ float narrow<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ F16 narrow<F16>(float v) {
-    return F16{__builtin_bit_cast(uint16_t, static_cast<_Float16>(v))};
-}
-template <>
-__device__ __forceinline__ BF16 narrow<BF16>(float v) { return BF16{f32_to_bf16_ref(v)}; }
-
 // ---- Append.  Sixteen lanes own one head row of one token: lane i holds
 // elements i D / 32 .. of the lower half and the same of the upper half, the
 // pairs that a rotation combines, so the row's maximum is four DPP steps away

@@ -1,0 +1,431 @@
+// INT8 x INT8 matrix product: activations quantized per row, weights per
+// column, exact 32-bit integer sums on v_mfma_i32_32x32x32_i8.
+//
+//   C[m, n] = fp32(sum_k a[m, k] w[k, n]) * (a_scale[m] * w_scale[n])
+//
+// Both operands lie in blocks of 32 rows (columns) x 64 k, 2 KB each: 16-byte
+// chunk kc * 32 + r holds row r's k = 16 kc .. + 15 (kc 0..3), so a wave reads
+// the operand of one MFMA (32 rows x 32 k: lane l row l % 32, k 16 (l / 32) ..
+// + 15) as 1 KB of adjacent bytes.  A panel of 32 columns is contiguous along
+// k.  Rows and columns are padded to 32 (padding is read, never used), k to 64
+// with zeros.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <cstring>
+
+#include "kv_q8.h"
+#include "vm_device.h"
+#include "vm_internal.h"
+
+namespace vmhip {
+namespace {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kT = 256;
+constexpr int kBlockBytes = 2048;
+constexpr int kMaxTiles = 4096;          // tiles that several workgroups may share
+constexpr int64_t kTicketBytes = kMaxTiles * 4;
+constexpr int kMaxSplits = 16;
+
+int64_t blocks32(int64_t x) { return (x + 31) / 32; }
+int64_t steps64(int64_t k) { return (k + 63) / 64; }
+int64_t staged_codes(int64_t rows, int64_t k) { return blocks32(rows) * steps64(k) * kBlockBytes; }
+
+// ---- Weights: thread (column, 16-k chunk) gathers 16 bytes of its column;
+// 32 lanes read 32 adjacent bytes of a row and write 512 adjacent ones.
+__global__ __launch_bounds__(kT) void a8_pack_kernel(const int8_t* __restrict__ w, int8_t* __restrict__ out, int64_t k,
+                                                     int64_t n, int64_t steps, int64_t chunks) {
+    for (int64_t u = static_cast<int64_t>(blockIdx.x) * kT + threadIdx.x; u < chunks;
+         u += static_cast<int64_t>(gridDim.x) * kT) {
+        const int64_t block = u >> 7;          // (panel, step)
+        const int c = static_cast<int>(u & 127);
+        const int64_t col = block / steps * 32 + (c & 31);
+        const int64_t k0 = block % steps * 64 + (c >> 5) * 16;
+        alignas(16) int8_t e[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) e[i] = col < n && k0 + i < k ? w[(k0 + i) * n + col] : int8_t(0);
+        *reinterpret_cast<u32x4*>(out + u * 16) = *reinterpret_cast<const u32x4*>(e);
+    }
+}
+
+// ---- Activations: WPR waves hold a row, 16 adjacent values a lane and chunk.
+template <typename T>
+__device__ __forceinline__ void load16(const T* p, int valid, float (&x)[16]);
+template <>
+__device__ __forceinline__ void load16<float>(const float* p, int valid, float (&x)[16]) {
+    if (valid >= 16) {
+        __builtin_memcpy(x, p, 64);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = i < valid ? p[i] : 0.0f;
+    }
+}
+template <bool kBf16>
+__device__ __forceinline__ void load16_half(const uint16_t* p, int valid, float (&x)[16]) {
+    uint16_t h[16];
+    if (valid >= 16) {
+        __builtin_memcpy(h, p, 32);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) h[i] = i < valid ? p[i] : uint16_t(0);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        x[i] = kBf16 ? __uint_as_float(static_cast<uint32_t>(h[i]) << 16)
+                     : static_cast<float>(__builtin_bit_cast(_Float16, h[i]));
+}
+template <>
+__device__ __forceinline__ void load16<F16>(const F16* p, int valid, float (&x)[16]) {
+    load16_half<false>(&p->bits, valid, x);
+}
+template <>
+__device__ __forceinline__ void load16<BF16>(const BF16* p, int valid, float (&x)[16]) {
+    load16_half<true>(&p->bits, valid, x);
+}
+
+constexpr int kHeld = 4;   // chunks of a lane kept in registers between the two passes
+
+template <typename T, int WPR>
+__global__ __launch_bounds__(kT) void a8_stage_kernel(const T* __restrict__ a, int8_t* __restrict__ out,
+                                                      float* __restrict__ scales, int64_t rows, int k, int steps) {
+    __shared__ uint32_t wave_max[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * (4 / WPR) + wave / WPR;
+    const bool ok = row < rows;
+    const int first = (wave % WPR) * 64 + lane;   // this lane's chunks: first, first + 64 WPR, ..
+    const int chunks = steps * 4;
+    const T* src = a + (ok ? row : 0) * k;
+    float x[kHeld][16];
+    uint32_t m = 0;
+    for (int c = first, u = 0; c < chunks; c += 64 * WPR, ++u) {
+        float y[16];
+        load16(src + c * 16, ok ? k - c * 16 : 0, y);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(y[i]) & 0x7fffffffu);
+#pragma unroll
+        for (int h = 0; h < kHeld; ++h)
+            if (h == u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[h][i] = y[i];
+    }
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), s, 64)));
+    if (WPR > 1) {
+        if (lane == 0) wave_max[wave] = m;
+        __syncthreads();
+#pragma unroll
+        for (int v = 0; v < 4; ++v) m = max(m, wave_max[v]);
+    }
+    if (!ok) return;
+    const Q8Scale q8 = q8_scale(m);
+    int8_t* dst = out + (row >> 5) * steps * kBlockBytes + (row & 31) * 16;
+    for (int c = first, u = 0; c < chunks; c += 64 * WPR, ++u) {
+        float y[16];
+        if (u < kHeld) {
+#pragma unroll
+            for (int h = 0; h < kHeld; ++h)
+                if (h == u)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) y[i] = x[h][i];
+        } else {
+            load16(src + c * 16, k - c * 16, y);
+        }
+        alignas(16) int8_t e[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) e[i] = q8_code(y[i], q8.inv);
+        *reinterpret_cast<u32x4*>(dst + (c >> 2) * static_cast<int64_t>(kBlockBytes) + (c & 3) * 512) =
+            *reinterpret_cast<const u32x4*>(e);
+    }
+    if (first == 0) scales[row] = q8.scale;
+}
+
+// ---- The product.
+struct Args {
+    const int8_t* a;
+    const float* a_scale;
+    const int8_t* w;
+    const float* w_scale;
+    void* c;
+    unsigned* tickets;
+    int* parts;
+    int64_t rows, n;
+    int row_blocks, steps, panels, tiles_m, splits;
+    int vec;   // c takes four columns at once
+};
+
+template <typename T>
+struct alignas(sizeof(T) * 4) Four {
+    T e[4];
+};
+
+// Four adjacent columns of a row.
+template <typename T>
+__device__ __forceinline__ void epilogue4(const Args& g, int64_t row, int64_t col, i32x4 s) {
+    if (row >= g.rows || col >= g.n) return;
+    const float as = g.a_scale[row];
+    T* c = static_cast<T*>(g.c) + row * g.n + col;
+    Four<T> y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        y.e[i] = narrow<T>(static_cast<float>(s[i]) * (as * (col + i < g.n ? g.w_scale[col + i] : 0.0f)));
+    if (g.vec) {
+        *reinterpret_cast<Four<T>*>(c) = y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (col + i < g.n) c[i] = y.e[i];
+    }
+}
+
+// Tiles of 32 MB rows x 32 columns.  The four waves of a workgroup share the
+// k range of its tile step by step, operands straight from global memory into
+// registers (a wave's loads of a step are 1 KB each), and their sums meet in
+// LDS.  Where the tiles are few, several workgroups share a tile's k range,
+// store their sums in the workspace and the last one adds them (integers: the
+// order does not matter).
+template <typename T, int MB>
+__global__ __launch_bounds__(kT) void qmm_a8_kernel(const Args g) {
+    __shared__ __align__(16) int sums[3][MB * 32 * 32];
+    __shared__ unsigned ticket;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int id = static_cast<int>(blockIdx.x);
+    const int split = id % g.splits;
+    id /= g.splits;
+    const int tile = id;
+    const int tm = id % g.tiles_m, panel = id / g.tiles_m;
+    // this wave's k steps
+    const int ways = 4 * g.splits, way = 4 * split + wave;
+    const int s0 = static_cast<int>(static_cast<int64_t>(g.steps) * way / ways);
+    const int s1 = static_cast<int>(static_cast<int64_t>(g.steps) * (way + 1) / ways);
+    const int8_t* wp = g.w + static_cast<int64_t>(panel) * g.steps * kBlockBytes + lane * 16;
+    const int8_t* ap[MB];
+#pragma unroll
+    for (int b = 0; b < MB; ++b)
+        ap[b] = g.a + static_cast<int64_t>(min(tm * MB + b, g.row_blocks - 1)) * g.steps * kBlockBytes + lane * 16;
+    i32x16 acc[MB];
+#pragma unroll
+    for (int b = 0; b < MB; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[b][e] = 0;
+    for (int s = s0; s < s1; ++s) {
+        const int64_t o = static_cast<int64_t>(s) * kBlockBytes;
+        i32x4 wv[2], av[MB][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            wv[h] = *reinterpret_cast<const i32x4*>(wp + o + 1024 * h);
+#pragma unroll
+            for (int b = 0; b < MB; ++b) av[b][h] = *reinterpret_cast<const i32x4*>(ap[b] + o + 1024 * h);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int b = 0; b < MB; ++b) acc[b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(av[b][h], wv[h], acc[b], 0, 0, 0);
+    }
+    // Element e of lane l: row 8 (e / 4) + 4 (l / 32) + e % 4, column l % 32.
+    if (wave > 0) {
+#pragma unroll
+        for (int b = 0; b < MB; ++b)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                sums[wave - 1][(b * 32 + 8 * (e / 4) + 4 * (lane / 32) + e % 4) * 32 + lane % 32] = acc[b][e];
+    }
+    __syncthreads();
+    if (wave == 0) {
+#pragma unroll
+        for (int b = 0; b < MB; ++b)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int at = (b * 32 + 8 * (e / 4) + 4 * (lane / 32) + e % 4) * 32 + lane % 32;
+                sums[0][at] += acc[b][e];
+            }
+    }
+    __syncthreads();
+    i32x4 mine[MB];
+#pragma unroll
+    for (int b = 0; b < MB; ++b) {
+        const int at = (b * kT + threadIdx.x) * 4;
+        mine[b] = *reinterpret_cast<const i32x4*>(&sums[0][at]) + *reinterpret_cast<const i32x4*>(&sums[1][at]) +
+                  *reinterpret_cast<const i32x4*>(&sums[2][at]);
+    }
+    constexpr uint32_t kPart = MB * 32 * 32 * 4;
+    if (g.splits > 1) {
+        char* tile_parts = reinterpret_cast<char*>(g.parts) + static_cast<int64_t>(tile) * g.splits * kPart;
+        const __amdgpu_buffer_rsrc_t prs = buffer_rsrc(tile_parts, kPart * static_cast<uint32_t>(g.splits));
+#pragma unroll
+        for (int b = 0; b < MB; ++b)
+            coherent_store16(prs, split * kPart + (b * kT + threadIdx.x) * 16, __builtin_bit_cast(u32x4, mine[b]));
+        publish_partials();
+        __syncthreads();
+        if (threadIdx.x == 0) ticket = ticket_take(g.tickets + tile, g.splits);
+        __syncthreads();
+        if (ticket != static_cast<unsigned>(g.splits - 1)) return;
+        if (threadIdx.x == 0) __hip_atomic_store(g.tickets + tile, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        for (int s = 0; s < g.splits; ++s) {
+            if (s == split) continue;
+#pragma unroll
+            for (int b = 0; b < MB; ++b)
+                mine[b] += __builtin_bit_cast(i32x4, coherent_load16(prs, s * kPart + (b * kT + threadIdx.x) * 16));
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < MB; ++b) {
+        const int at = b * kT + threadIdx.x;   // row at / 8, columns 4 (at % 8) ..
+        epilogue4<T>(g, static_cast<int64_t>(tm) * MB * 32 + at / 8, static_cast<int64_t>(panel) * 32 + 4 * (at % 8), mine[b]);
+    }
+}
+
+struct Plan {
+    int mb, splits;
+    int64_t tiles_m, panels, bytes;
+};
+
+Plan plan(int64_t rows, int64_t k, int64_t n) {
+    Plan p;
+    const int64_t rb = blocks32(rows);
+    p.mb = rb <= 1 ? 1 : rb <= 2 ? 2 : 4;
+    p.tiles_m = (rb + p.mb - 1) / p.mb;
+    p.panels = blocks32(n);
+    const int64_t tiles = p.tiles_m * p.panels;
+    // Few tiles: enough workgroups to fill the GPU twice, a step a wave at least.
+    int64_t s = tiles < 512 ? (512 + tiles - 1) / tiles : 1;
+    s = std::min<int64_t>({s, kMaxSplits, std::max<int64_t>(steps64(k) / 4, 1)});
+    p.splits = static_cast<int>(s);
+    p.bytes = s > 1 ? kTicketBytes + tiles * s * p.mb * 4096 : 0;
+    return p;
+}
+
+int check_a8(int64_t rows, int64_t k, int64_t n, const char* who) {
+    const std::string w(who);
+    if (k < 1 || k > VM_HIP_A8_MAX_K) return fail_inval(w + ": k must be in [1, 131072]");
+    if (rows < 0 || rows > (1 << 24) || n < 0 || n > (1 << 24)) return fail_inval(w + ": rows or n out of range");
+    if (blocks32(rows) * blocks32(n) > (1 << 30)) return fail_inval(w + ": too many outputs for one call");
+    return 0;
+}
+
+bool known_dtype(int d) { return d == VM_HIP_DTYPE_F32 || d == VM_HIP_DTYPE_F16 || d == VM_HIP_DTYPE_BF16; }
+bool off(const void* p, unsigned m) { return (reinterpret_cast<uintptr_t>(p) & m) != 0; }
+unsigned element_mask(int d) { return d == VM_HIP_DTYPE_F32 ? 3 : 1; }
+
+template <typename T>
+int stage(const void* a, int64_t rows, int64_t k, void* staged, hipStream_t stream) {
+    float* scales = reinterpret_cast<float*>(static_cast<char*>(staged) + staged_codes(rows, k));
+    const int steps = static_cast<int>(steps64(k));
+    // A wave a row where that fills the GPU, else four: the row's loads are a chain.
+    if (rows >= 2048 && k <= 4096)
+        hipLaunchKernelGGL((a8_stage_kernel<T, 1>), dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(kT), 0, stream,
+                           static_cast<const T*>(a), static_cast<int8_t*>(staged), scales, rows, static_cast<int>(k), steps);
+    else
+        hipLaunchKernelGGL((a8_stage_kernel<T, 4>), dim3(static_cast<unsigned>(rows)), dim3(kT), 0, stream,
+                           static_cast<const T*>(a), static_cast<int8_t*>(staged), scales, rows, static_cast<int>(k), steps);
+    return check_launch("a8_stage", stream);
+}
+
+template <typename T>
+void launch(const Args& g, int mb, int64_t grid, hipStream_t stream) {
+    const dim3 d(static_cast<unsigned>(grid));
+    if (mb == 1)
+        hipLaunchKernelGGL((qmm_a8_kernel<T, 1>), d, dim3(kT), 0, stream, g);
+    else if (mb == 2)
+        hipLaunchKernelGGL((qmm_a8_kernel<T, 2>), d, dim3(kT), 0, stream, g);
+    else
+        hipLaunchKernelGGL((qmm_a8_kernel<T, 4>), d, dim3(kT), 0, stream, g);
+}
+
+}  // namespace
+}  // namespace vmhip
+
+using namespace vmhip;
+
+extern "C" {
+
+int64_t vm_hip_a8_weights_bytes(int64_t k, int64_t n) {
+    clear_error();
+    VM_TRY(check_a8(1, k, n, "a8_weights_bytes"));
+    return blocks32(n) * steps64(k) * kBlockBytes;
+}
+
+int64_t vm_hip_a8_stage_bytes(int64_t rows, int64_t k) {
+    clear_error();
+    VM_TRY(check_a8(rows, k, 1, "a8_stage_bytes"));
+    return staged_codes(rows, k) + blocks32(rows) * 32 * 4;
+}
+
+int64_t vm_hip_qmm_a8_workspace_bytes(int64_t rows, int64_t k, int64_t n) {
+    clear_error();
+    VM_TRY(check_a8(rows, k, n, "qmm_a8_workspace_bytes"));
+    return rows && n ? plan(rows, k, n).bytes : 0;
+}
+
+int vm_hip_a8_pack(const int8_t* codes, int64_t k, int64_t n, void* packed, void* stream) {
+    clear_error();
+    VM_TRY(check_a8(1, k, n, "a8_pack"));
+    if (n == 0) return 0;
+    if (!codes || !packed) return fail_inval("a8_pack: null pointer");
+    if (off(packed, 15)) return fail_inval("a8_pack: packed must be 16-byte aligned");
+    const int64_t chunks = blocks32(n) * steps64(k) * (kBlockBytes / 16);
+    const int64_t blocks = std::min<int64_t>((chunks + kT - 1) / kT, 65536);
+    auto s = static_cast<hipStream_t>(stream);
+    hipLaunchKernelGGL(a8_pack_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kT), 0, s, codes,
+                       static_cast<int8_t*>(packed), k, n, steps64(k), chunks);
+    return check_launch("a8_pack", s);
+}
+
+int vm_hip_a8_stage(const void* a, int dtype, int64_t rows, int64_t k, void* staged, void* stream) {
+    clear_error();
+    VM_TRY(check_a8(rows, k, 1, "a8_stage"));
+    if (!known_dtype(dtype)) return fail_inval("a8_stage: dtype must be F32, F16 or BF16");
+    if (rows == 0) return 0;
+    if (!a || !staged) return fail_inval("a8_stage: null pointer");
+    if (off(staged, 15) || off(a, element_mask(dtype))) return fail_inval("a8_stage: unaligned pointer");
+    auto s = static_cast<hipStream_t>(stream);
+    if (dtype == VM_HIP_DTYPE_F16) return stage<F16>(a, rows, k, staged, s);
+    if (dtype == VM_HIP_DTYPE_BF16) return stage<BF16>(a, rows, k, staged, s);
+    return stage<float>(a, rows, k, staged, s);
+}
+
+int vm_hip_qmm_a8(const void* staged, const void* packed, const float* scale, void* c, int c_dtype, int64_t rows,
+                  int64_t k, int64_t n, void* workspace, int64_t workspace_bytes, void* stream) {
+    clear_error();
+    VM_TRY(check_a8(rows, k, n, "qmm_a8"));
+    if (!known_dtype(c_dtype)) return fail_inval("qmm_a8: c_dtype must be F32, F16 or BF16");
+    if (rows == 0 || n == 0) return 0;
+    if (!staged || !packed || !scale || !c) return fail_inval("qmm_a8: null pointer");
+    if (off(staged, 15) || off(packed, 15) || off(scale, 3) || off(c, element_mask(c_dtype)))
+        return fail_inval("qmm_a8: unaligned pointer");
+    const Plan p = plan(rows, k, n);
+    if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes || off(workspace, 15)))
+        return fail_inval("qmm_a8: workspace smaller than vm_hip_qmm_a8_workspace_bytes or unaligned");
+    Args g;
+    g.a = static_cast<const int8_t*>(staged);
+    g.a_scale = reinterpret_cast<const float*>(g.a + staged_codes(rows, k));
+    g.w = static_cast<const int8_t*>(packed);
+    g.w_scale = scale;
+    g.c = c;
+    g.tickets = static_cast<unsigned*>(workspace);
+    g.parts = p.bytes > 0 ? reinterpret_cast<int*>(static_cast<char*>(workspace) + kTicketBytes) : nullptr;
+    g.rows = rows;
+    g.n = n;
+    g.row_blocks = static_cast<int>(blocks32(rows));
+    g.steps = static_cast<int>(steps64(k));
+    g.panels = static_cast<int>(p.panels);
+    g.tiles_m = static_cast<int>(p.tiles_m);
+    g.splits = p.splits;
+    const unsigned e = c_dtype == VM_HIP_DTYPE_F32 ? 4 : 2;
+    g.vec = n % 4 == 0 && !off(c, 4 * e - 1);
+    const int64_t grid = p.tiles_m * p.panels * p.splits;
+    auto s = static_cast<hipStream_t>(stream);
+    if (c_dtype == VM_HIP_DTYPE_F16)
+        launch<F16>(g, p.mb, grid, s);
+    else if (c_dtype == VM_HIP_DTYPE_BF16)
+        launch<BF16>(g, p.mb, grid, s);
+    else
+        launch<float>(g, p.mb, grid, s);
+    return check_launch("qmm_a8", s);
+}
+
+}  // extern "C"

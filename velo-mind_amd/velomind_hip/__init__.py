@@ -56,6 +56,14 @@ class KvQ8(ctypes.Structure):
                 ("batch", c_int64), ("kv_heads", c_int64), ("max_seq", c_int64), ("head_dim", c_int64)]
 
 
+class LogitsRules(ctypes.Structure):
+    """vm_hip_logits_rules (include/vm_hip.h): device addresses of the rules; what is left out stays NULL."""
+    _fields_ = [("history", c_void_p), ("history_lengths", c_void_p), ("history_stride", c_int64),
+                ("repetition", c_void_p), ("frequency", c_void_p), ("presence", c_void_p), ("bias_tokens", c_void_p),
+                ("bias_values", c_void_p), ("bias_lengths", c_void_p), ("bias_stride", c_int64), ("allowed", c_void_p),
+                ("drafted", c_void_p), ("tree", c_void_p)]
+
+
 def _declare(L: ctypes.CDLL) -> None:
     p = c_void_p
     sig = {
@@ -145,6 +153,15 @@ def _declare(L: ctypes.CDLL) -> None:
         "vm_hip_kv_q8_keep": ([POINTER(KvQ8), p, p, p, c_int64, p], c_int),
         "vm_hip_attention_q8_workspace_bytes": ([c_int64] * 6, c_int64),
         "vm_hip_attention_q8": ([POINTER(KvQ8), p, p, c_int, c_int64, c_int64, p, p, p, c_float, p, c_int64, p], c_int),
+        "vm_hip_a8_weights_bytes": ([c_int64, c_int64], c_int64),
+        "vm_hip_a8_stage_bytes": ([c_int64, c_int64], c_int64),
+        "vm_hip_qmm_a8_workspace_bytes": ([c_int64] * 3, c_int64),
+        "vm_hip_a8_pack": ([p, c_int64, c_int64, p, p], c_int),
+        "vm_hip_a8_stage": ([p, c_int, c_int64, c_int64, p, p], c_int),
+        "vm_hip_qmm_a8": ([p, p, p, p, c_int, c_int64, c_int64, c_int64, p, c_int64, p], c_int),
+        "vm_hip_logits_rules_workspace_bytes": ([c_int64] * 3, c_int64),
+        "vm_hip_logits_rules_apply": ([POINTER(LogitsRules), p, p, c_int, p, c_int64, c_int64, c_int64, p, p, c_int64, p],
+                                      c_int),
     }
     for name, (args, res) in sig.items():
         fn = getattr(L, name)
@@ -179,7 +196,9 @@ def exported_symbols() -> list[str]:
             "vm_hip_qmm_a_layout", "vm_hip_qmm_staged_f32", "vm_hip_add_rmsnorm_stage_f32",
             "vm_hip_silu_mul_stage_f32", "vm_hip_copy_strided",
             "vm_hip_kv_q8_append", "vm_hip_kv_q8_read", "vm_hip_kv_q8_keep", "vm_hip_attention_q8_workspace_bytes",
-            "vm_hip_attention_q8"]
+            "vm_hip_attention_q8", "vm_hip_a8_weights_bytes", "vm_hip_a8_stage_bytes", "vm_hip_qmm_a8_workspace_bytes",
+            "vm_hip_a8_pack", "vm_hip_a8_stage", "vm_hip_qmm_a8", "vm_hip_logits_rules_workspace_bytes",
+            "vm_hip_logits_rules_apply"]
 
 
 def open_library() -> ctypes.CDLL:
@@ -403,6 +422,48 @@ def attention_q8(cache: KvQ8, q: int, out: int, dtype: int, rows: int, heads: in
     """vm_hip_attention_q8: tokens, prompts or trees of drafted tokens over an INT8 cache."""
     check(open_library().vm_hip_attention_q8(byref(cache), q, out, dtype, rows, heads, pos, counts, tree, scale,
                                              workspace, workspace_bytes, _h(stream)))
+
+
+# ---- INT8 x INT8 products and logits under rules (raw device addresses) ----
+
+def a8_weights_bytes(k: int, n: int) -> int:
+    return _size(open_library().vm_hip_a8_weights_bytes(k, n))
+
+
+def a8_stage_bytes(rows: int, k: int) -> int:
+    return _size(open_library().vm_hip_a8_stage_bytes(rows, k))
+
+
+def qmm_a8_workspace_bytes(rows: int, k: int, n: int) -> int:
+    return _size(open_library().vm_hip_qmm_a8_workspace_bytes(rows, k, n))
+
+
+def a8_pack(codes: int, k: int, n: int, packed: int, stream=None) -> None:
+    """vm_hip_a8_pack: INT8 codes [k, n] laid out for qmm_a8."""
+    check(open_library().vm_hip_a8_pack(codes, k, n, packed, _h(stream)))
+
+
+def a8_stage(a: int, dtype: int, rows: int, k: int, staged: int, stream=None) -> None:
+    """vm_hip_a8_stage: activations to INT8 with a scale for each row."""
+    check(open_library().vm_hip_a8_stage(a, dtype, rows, k, staged, _h(stream)))
+
+
+def qmm_a8(staged: int, packed: int, scale: int, c: int, c_dtype: int, rows: int, k: int, n: int, workspace,
+           workspace_bytes: int, stream=None) -> None:
+    """vm_hip_qmm_a8: staged rows times packed weights."""
+    check(open_library().vm_hip_qmm_a8(staged, packed, scale, c, c_dtype, rows, k, n, workspace, workspace_bytes,
+                                       _h(stream)))
+
+
+def logits_rules_workspace_bytes(seqs: int, rows: int, vocab: int) -> int:
+    return _size(open_library().vm_hip_logits_rules_workspace_bytes(seqs, rows, vocab))
+
+
+def logits_rules(rules: LogitsRules, logits: int, out, dtype: int, tokens, seqs: int, rows: int, vocab: int, counts,
+                 workspace, workspace_bytes: int, stream=None) -> None:
+    """vm_hip_logits_rules_apply: penalties, biases and masks on logits, and the greedy token of each row."""
+    check(open_library().vm_hip_logits_rules_apply(byref(rules), logits, out, dtype, tokens, seqs, rows, vocab, counts,
+                                                   workspace, workspace_bytes, _h(stream)))
 
 
 def _size(n: int) -> int:
