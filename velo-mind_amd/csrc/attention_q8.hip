@@ -54,7 +54,9 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
 constexpr int kBlock = 32;             // keys of a block
+constexpr int kLeast = 2 * kWaves;     // blocks that are worth a workgroup
 constexpr int kMaxSplits = 64;
 constexpr int kMaxUnits = 1024;        // workgroup groups that split their keys
 constexpr int64_t kTicketBytes = kMaxUnits * 4;
@@ -92,14 +94,19 @@ __device__ __forceinline__ half8 join(half2v a, half2v b, half2v c, half2v d) {
     return half8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
-// Maximum over the lanes of a row's four groups (lanes lr + 16 g).
+// Maximum and sum over the lanes of a row's four groups (lanes lr + 16 g).
 __device__ __forceinline__ float max_groups(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16, 64));
-    return fmaxf(v, __shfl_xor(v, 32, 64));
+    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    unsigned q[2];
+    __builtin_memcpy(q, &p, sizeof q);
+    v = fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
+    const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    __builtin_memcpy(q, &h, sizeof q);
+    return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
 }
 __device__ __forceinline__ float sum_groups(float v) {
-    v += __shfl_xor(v, 16, 64);
-    return v + __shfl_xor(v, 32, 64);
+    v = swap_rows_add(v, v);
+    return swap_halves_add(v, v);
 }
 
 template <typename T>
@@ -146,81 +153,89 @@ __device__ __forceinline__ void store4(BF16* p, const float* y) {
 }
 
 // One workgroup's place: which rows, and which 32-key blocks of its keys.
-// Both the kernel's waves and the last arrival's merge go by it.
-template <int RW>
 struct Place {
     int b, kh, tile, split, unit;
     int g, p0, n_tok, n_keys;   // group size, cached tokens, real tokens, cache rows that exist
     int active, first, last;    // workgroups that share the keys; this one's blocks
 };
 
-template <int RW>
-__device__ __forceinline__ Place<RW> place(const Args& a) {
-    Place<RW> w;
+// Workgroups go to the XCDs in turn.  The tiles of a (sequence, head, share of
+// the keys) read the same codes, so where the count of those allows they are
+// placed on one XCD, next to each other, the tiles that see the most keys
+// first; else they are as far apart as the others are many.
+template <int RT>
+__device__ __forceinline__ Place place(const Args& a) {
+    Place w;
     int id = static_cast<int>(blockIdx.x);
-    w.split = id % a.splits;
-    id /= a.splits;
-    w.unit = id;
-    w.tile = id % a.tiles;
-    id /= a.tiles;
-    w.kh = id % a.kv_heads;
-    w.b = id / a.kv_heads;
+    const int shares = a.batch * a.kv_heads * a.splits;
+    int share;
+    if (shares % 8 == 0) {
+        const int j = id / 8;
+        w.tile = a.tiles - 1 - j % a.tiles;
+        share = j / a.tiles * 8 + id % 8;
+    } else {
+        w.tile = a.tiles - 1 - id / shares;
+        share = id % shares;
+    }
+    w.split = share % a.splits;
+    share /= a.splits;
+    w.unit = share * a.tiles + w.tile;
+    w.kh = share % a.kv_heads;
+    w.b = share / a.kv_heads;
     w.g = a.heads / a.kv_heads;
     // (clamped where nothing changes: rows past max_seq, or all before row 0)
     w.p0 = max(min(a.pos[w.b], a.max_seq), -(1 << 21));
     w.n_tok = a.counts ? min(max(a.counts[w.b], 0), a.rows) : a.rows;
-    const int64_t end = static_cast<int64_t>(w.p0) + w.n_tok;
-    w.n_keys = static_cast<int>(min(max(end, int64_t(0)), static_cast<int64_t>(a.max_seq)));
+    w.n_keys = min(max(w.p0 + w.n_tok, 0), a.max_seq);
     // A chain's tile sees the rows up to its last token's.
     int seen = w.n_keys;
-    if (!a.tree) {
-        const int t_last = min((w.tile * 16 * RW + 16 * RW - 1) / w.g, w.n_tok - 1);
-        seen = static_cast<int>(min(static_cast<int64_t>(seen), max(static_cast<int64_t>(w.p0) + t_last + 1, int64_t(0))));
-    }
+    if (!a.tree) seen = min(seen, max(w.p0 + min((w.tile * 16 * RT + 16 * RT - 1) / w.g, w.n_tok - 1) + 1, 0));
     const int blocks = (seen + kBlock - 1) / kBlock;
-    constexpr int kLeast = 2 * (4 / RW);   // blocks that are worth a workgroup
-    const int share = max((blocks + a.splits - 1) / a.splits, kLeast);
-    w.active = max((blocks + share - 1) / share, 1);
-    w.first = w.split * share;
-    w.last = min(blocks, w.first + share);
+    const int each = max((blocks + a.splits - 1) / a.splits, kLeast);
+    w.active = max((blocks + each - 1) / each, 1);
+    w.first = w.split * each;
+    w.last = min(blocks, w.first + each);
     return w;
 }
 
-template <typename T, int D, int RW>
+template <typename T, int D, int RT>
 __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a) {
     constexpr int H = D / 64;              // 64-dim slabs
     constexpr int NC = D / 32;             // k-steps of a score
     constexpr int ND = D / 16;             // dim tiles; codes of a key that a lane reads
-    constexpr int KS = 4 / RW;
     constexpr bool kTwo = sizeof(T) == 4;  // fp32 operands: two fp16 parts
     constexpr int NP = kTwo ? 2 : 1;
-    __shared__ __align__(16) float scales_lds[4][2 * kBlock];
-    __shared__ __align__(16) float merge_o[KS > 1 ? (KS - 1) * RW * 16 * D : 4];
-    __shared__ float merge_ml[KS > 1 ? (KS - 1) * RW * 16 * 2 : 1];
+    constexpr int kRows = 16 * RT;
+    constexpr float kHeadroom = 1.0f;      // log2 units that a weight may exceed 1 by
+    __shared__ __align__(16) float scales_lds[kWaves][2 * kBlock];
+    __shared__ __align__(16) float merge_o[kWaves][kRows * D];
+    __shared__ float merge_m[kWaves][kRows], merge_l[kWaves][kRows];
     __shared__ unsigned ticket;
 
-    const Place<RW> w = place<RW>(a);
+    const Place w = place<RT>(a);
     if (w.split >= w.active) return;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wr = wave % RW, kg = wave / RW;
     const int lr = lane & 15, lg = lane >> 4;
-    const int r = (w.tile * RW + wr) * 16 + lr;     // query row of this lane
-    const int t = r / w.g, head = w.kh * w.g + r % w.g;
-    const bool row_ok = t < w.n_tok;                // (rows past the last token's have t >= rows >= n_tok)
-    const int t_first = (w.tile * RW + wr) * 16 / w.g;   // the wave's first token
-    const bool wave_ok = t_first < w.n_tok;
-    // Rows below `whole` are seen by every token of the wave.
+    const int r0 = w.tile * kRows;                  // the tile's first row, (token, head of the group)
+    const int t_first = r0 / w.g;
+    if (t_first >= w.n_tok) return;                 // padding only
+    // Rows below `whole` are seen by every token of the tile.
     const int whole = min(a.tree ? w.p0 : w.p0 + t_first + 1, w.n_keys);
 
-    // Q^T operand: Q[r][64 h + 16 lg + 8 s + j] in qf[.][2 h + s], scaled by the
-    // power of two that puts the row's largest magnitude in [2^13, 2^14).
-    half8 qf[NP][NC];
-    float row_factor;
-    {
+    // Q^T operands: Q[row][64 h + 16 lg + 8 s + j] in qf[.][.][2 h + s], scaled by
+    // the power of two that puts the row's largest magnitude in [2^13, 2^14).
+    half8 qf[RT][NP][NC];
+    float row_factor[RT];   // of a score's log2
+    int token[RT];          // -1: no row
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int r = r0 + 16 * rt + lr, t = r / w.g;
+        const bool row_ok = t < w.n_tok;
+        token[rt] = row_ok ? t : -1;
         float x[H][16];
         const T* qp = static_cast<const T*>(a.q) +
-                      ((static_cast<int64_t>(w.b) * a.heads + head) * a.rows + t) * D + 16 * lg;
+                      ((static_cast<int64_t>(w.b) * a.heads + w.kh * w.g + r % w.g) * a.rows + t) * D + 16 * lg;
         uint32_t m = 0;
 #pragma unroll
         for (int h = 0; h < H; ++h) {
@@ -237,16 +252,15 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
         m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 32, 64)));
         const bool finite = m < 0x7f800000u;
         const int up = 14 - exponent_above(__uint_as_float(m));
-        // exp2's argument: log2(e) times the score
-        row_factor = finite ? ldexpf(a.scale * 1.44269504f, -up) : NAN;
+        row_factor[rt] = finite ? ldexpf(a.scale * 1.44269504f, -up) : NAN;
 #pragma unroll
         for (int h = 0; h < H; ++h)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const float v = finite ? ldexpf(x[h][e], up) : 0.0f;
                 const _Float16 hi = static_cast<_Float16>(v);
-                qf[0][2 * h + e / 8][e % 8] = hi;
-                if (kTwo) qf[NP - 1][2 * h + e / 8][e % 8] = static_cast<_Float16>(v - static_cast<float>(hi));
+                qf[rt][0][2 * h + e / 8][e % 8] = hi;
+                if (kTwo) qf[rt][NP - 1][2 * h + e / 8][e % 8] = static_cast<_Float16>(v - static_cast<float>(hi));
             }
     }
 
@@ -284,17 +298,26 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
         }
     };
 
-    f32x4 acc[ND];   // O^T[dim ND (4 lg + e) + db][row lr] 2^(14 - v_exp)
+    f32x4 acc[RT][ND];   // O^T[dim ND (4 lg + e) + db][row lr] 2^(14 - v_exp)
+    float m_run[RT];     // the score (less the row's factor) that weighs 1
+    float limit[RT];     // how far a score may pass it (log2); -inf before the first key
+    float l_run[RT];     // sum of this lane's keys' weights
 #pragma unroll
-    for (int db = 0; db < ND; ++db) acc[db] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m_run = -INFINITY, l_run = 0.0f;   // l: this lane's keys only
-    int v_exp = -200;                        // E of the weights' unit
+    for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+        for (int db = 0; db < ND; ++db) acc[rt][db] = f32x4{0.f, 0.f, 0.f, 0.f};
+        m_run[rt] = l_run[rt] = 0.0f;
+        limit[rt] = -INFINITY;
+    }
+    int v_exp = -200;   // E of the weights' unit 2^(E - 14)
 
     auto compute = [&](int block, const Codes& c) {
         const int k0 = block * kBlock;
         float* sl = scales_lds[wave];
         sl[lane] = c.s;                       // keys' scales, then values'
-        f32x4 st[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        f32x4 st[RT][2];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) st[rt][0] = st[rt][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int h = 0; h < H; ++h)
 #pragma unroll
@@ -304,8 +327,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
                     const uint32_t u0 = c.k[bt][h][2 * s] ^ 0x80808080u, u1 = c.k[bt][h][2 * s + 1] ^ 0x80808080u;
                     const half8 kf = join(widen_low(u0), widen_high(u0), widen_low(u1), widen_high(u1));
 #pragma unroll
-                    for (int p = 0; p < NP; ++p)
-                        st[bt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[p][2 * h + s], st[bt], 0, 0, 0);
+                    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                        for (int p = 0; p < NP; ++p)
+                            st[rt][bt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[rt][p][2 * h + s], st[rt][bt], 0, 0, 0);
                 }
         __builtin_amdgcn_wave_barrier();
         float sk[8], sv[8];
@@ -315,60 +340,83 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
             sv[j] = sl[kBlock + 8 * lg + j];
         }
         __builtin_amdgcn_wave_barrier();
-        uint32_t sees = 0xffu;   // bit j: row lr sees key k0 + 8 lg + j
         const bool masked = k0 + kBlock > whole;
-        if (masked) {
-            const int key0 = k0 + 8 * lg;
-            const int node0 = key0 - w.p0;   // of the call's own rows; negative: cached before
-            if (a.tree) {
-                const uint64_t* tw = a.tree + (static_cast<int64_t>(w.b) * a.rows + (row_ok ? t : 0)) * a.words;
-                const int lo = max(node0, 0), wi = lo >> 6, sh = lo & 63;
-                const uint64_t w0 = wi < a.words ? tw[wi] : 0, w1 = wi + 1 < a.words ? tw[wi + 1] : 0;
-                const uint64_t win = sh ? w0 >> sh | w1 << (64 - sh) : w0;
-                const int before = min(max(-node0, 0), 8);   // keys of the eight that were cached before
-                sees = static_cast<uint32_t>(win) << before | ((1u << before) - 1);
-            } else {
-                const int n = t - node0 + 1;   // keys of the eight up to the token's own
-                sees = n >= 8 ? 0xffu : n > 0 ? (1u << n) - 1 : 0u;
+        // Scores less the row's reference (and its factor), and whether that or
+        // the weights' unit has to move: rarely, after the first blocks.
+        uint32_t sees[RT];   // bit j: the row sees key k0 + 8 lg + j
+        float mt[RT];
+        float top = sv[0];   // (NaN is skipped)
+#pragma unroll
+        for (int j = 1; j < 8; ++j) top = fmaxf(top, sv[j]);
+        bool moves = top == top && exponent_above(top) > v_exp;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            sees[rt] = 0xffu;
+            if (masked) {
+                const int key0 = k0 + 8 * lg;
+                const int node0 = key0 - w.p0;   // of the call's own rows; negative: cached before
+                if (a.tree) {
+                    const uint64_t* tw = a.tree + (static_cast<int64_t>(w.b) * a.rows + max(token[rt], 0)) * a.words;
+                    const int lo = max(node0, 0), wi = lo >> 6, sh = lo & 63;
+                    const uint64_t w0 = wi < a.words ? tw[wi] : 0, w1 = wi + 1 < a.words ? tw[wi + 1] : 0;
+                    const uint64_t win = sh ? w0 >> sh | w1 << (64 - sh) : w0;
+                    const int before = min(max(-node0, 0), 8);   // keys of the eight that were cached before
+                    sees[rt] = static_cast<uint32_t>(win) << before | ((1u << before) - 1);
+                } else {
+                    const int n = token[rt] - node0 + 1;   // keys of the eight up to the token's own
+                    sees[rt] = n >= 8 ? 0xffu : n > 0 ? (1u << n) - 1 : 0u;
+                }
+                const int n = w.n_keys - key0;
+                sees[rt] &= n >= 8 ? 0xffu : n > 0 ? (1u << n) - 1 : 0u;
+                if (token[rt] < 0) sees[rt] = 0;
             }
-            const int n = w.n_keys - key0;
-            sees &= n >= 8 ? 0xffu : n > 0 ? (1u << n) - 1 : 0u;
-            if (!row_ok) sees = 0;
-        }
-        float v[8];
-        float mt = -INFINITY, top = 0.0f;
+            mt[rt] = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            v[j] = st[j / 4][j % 4] * (sk[j] * row_factor);
-            if (masked && !(sees >> j & 1)) v[j] = -INFINITY;
-            mt = fmaxf(mt, v[j]);
-            top = fmaxf(top, sv[j]);   // (NaN is skipped)
+            for (int j = 0; j < 8; ++j) {
+                float v = fmaf(st[rt][j / 4][j % 4], sk[j], -m_run[rt]);
+                if (masked && !(sees[rt] >> j & 1)) v = -INFINITY;
+                st[rt][j / 4][j % 4] = v;
+                mt[rt] = fmaxf(mt[rt], v);
+            }
+            moves = moves || mt[rt] * row_factor[rt] > limit[rt];
         }
-        mt = max_groups(mt);
-        top = max_groups(top);
-        const float m_new = fmaxf(m_run, mt);
-        const float m_ref = m_new == -INFINITY ? 0.0f : m_new;
-        const int e_new = max(v_exp, exponent_above(top));
-        const float alpha = __builtin_amdgcn_exp2f(m_run - m_ref);
-        const float fall = ldexpf(alpha, v_exp - e_new);
-        float ls = 0.0f;
-        half8 ph, pl;
+        if (__any(moves)) {
+            top = max_groups(top);
+            const int e_new = top == top ? max(v_exp, exponent_above(top)) : v_exp;
+            const float grown = ldexpf(1.0f, v_exp - e_new);
+            v_exp = e_new;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float p = __builtin_amdgcn_exp2f(v[j] - m_ref);
-            ls += p;
-            float x = p * ldexpf(sv[j], 14 - e_new);
-            if (masked && !(sees >> j & 1)) x = 0.0f;   // (0 times a NaN scale)
-            const _Float16 hi = static_cast<_Float16>(x);
-            ph[j] = hi;
-            if (kTwo) pl[j] = static_cast<_Float16>(x - static_cast<float>(hi));
+            for (int rt = 0; rt < RT; ++rt) {
+                const float most = max_groups(mt[rt]);
+                const bool first = limit[rt] == -INFINITY;
+                const bool seen = most > -INFINITY && row_factor[rt] == row_factor[rt];
+                const float up = !seen ? 0.0f : first ? most : fmaxf(most, 0.0f);
+                m_run[rt] += up;
+                const float fall = first ? 1.0f : __builtin_amdgcn_exp2f(-up * row_factor[rt]);
+                if (seen) limit[rt] = kHeadroom;
+                l_run[rt] *= fall;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) st[rt][j / 4][j % 4] -= up;
+#pragma unroll
+                for (int db = 0; db < ND; ++db) acc[rt][db] *= fall * grown;
+            }
         }
-        l_run = fmaf(l_run, alpha, ls);
-        m_run = m_new;
-        v_exp = e_new;
-        if (__any(fall != 1.0f)) {
+        float su[8];
 #pragma unroll
-            for (int db = 0; db < ND; ++db) acc[db] *= fall;
+        for (int j = 0; j < 8; ++j) su[j] = ldexpf(sv[j], 14 - v_exp);
+        half8 pf[RT][NP];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float p = __builtin_amdgcn_exp2f(st[rt][j / 4][j % 4] * row_factor[rt]);
+                float x = p * su[j];
+                if (masked && !(sees[rt] >> j & 1)) p = x = 0.0f;   // (whatever the factor and the scale are)
+                l_run[rt] += p;
+                const _Float16 hi = static_cast<_Float16>(x);
+                pf[rt][0][j] = hi;
+                if (kTwo) pf[rt][NP - 1][j] = static_cast<_Float16>(x - static_cast<float>(hi));
+            }
         }
         // V^T: four dim tiles from four adjacent codes of eight keys.
 #pragma unroll
@@ -387,164 +435,180 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
 #pragma unroll
             for (int db = 0; db < 4; ++db) {
                 const half8 vf = join(f[db][0], f[db][1], f[db][2], f[db][3]);
-                acc[4 * d4 + db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph, acc[4 * d4 + db], 0, 0, 0);
-                if (kTwo) acc[4 * d4 + db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl, acc[4 * d4 + db], 0, 0, 0);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                    for (int p = 0; p < NP; ++p)
+                        acc[rt][4 * d4 + db] =
+                            __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rt][p], acc[rt][4 * d4 + db], 0, 0, 0);
             }
         }
     };
 
-    if (wave_ok) {
+    {
         Codes c0, c1;
-        int block = w.first + kg;
+        int block = w.first + wave;
         if (block < w.last) {
             load(block, c0);
             while (true) {
-                if (block + KS < w.last) load(block + KS, c1);
+                if (block + kWaves < w.last) load(block + kWaves, c1);
                 compute(block, c0);
-                block += KS;
+                block += kWaves;
                 if (block >= w.last) break;
-                if (block + KS < w.last) load(block + KS, c0);
+                if (block + kWaves < w.last) load(block + kWaves, c0);
                 compute(block, c1);
-                block += KS;
+                block += kWaves;
                 if (block >= w.last) break;
             }
         }
     }
-    l_run = sum_groups(l_run);
-    float o[4][ND];   // dims ND (4 lg + e) + db of row lr
+    // Every wave's triple to LDS (outputs without their unit); then thread
+    // (row, four dims) merges the four.
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int rt = 0; rt < RT; ++rt) {
+        const float l = sum_groups(l_run[rt]);
+        float* d = merge_o[wave] + (16 * rt + lr) * D + 4 * ND * lg;
 #pragma unroll
-        for (int db = 0; db < ND; ++db) o[e][db] = ldexpf(acc[db][e], v_exp - 14);
-
-    // Merge the key groups into group 0.
-    if constexpr (KS > 1) {
-        if (kg > 0) {
-            float* d = merge_o + (((kg - 1) * RW + wr) * 16 + lr) * D + 4 * ND * lg;
+        for (int e = 0; e < 4; ++e)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+            for (int u = 0; u < ND / 4; ++u) {
+                float y[4];
 #pragma unroll
-                for (int u = 0; u < ND / 4; ++u) store4(d + ND * e + 4 * u, &o[e][4 * u]);
-            if (lg == 0) {
-                merge_ml[(((kg - 1) * RW + wr) * 16 + lr) * 2] = m_run;
-                merge_ml[(((kg - 1) * RW + wr) * 16 + lr) * 2 + 1] = l_run;
+                for (int i = 0; i < 4; ++i) y[i] = ldexpf(acc[rt][4 * u + i][e], v_exp - 14);
+                store4(d + ND * e + 4 * u, y);
             }
-        }
-        __syncthreads();
-        if (kg == 0) {
-            float m = m_run;
-#pragma unroll
-            for (int k = 0; k < KS - 1; ++k) m = fmaxf(m, merge_ml[((k * RW + wr) * 16 + lr) * 2]);
-            const float m_ref = m == -INFINITY ? 0.0f : m;
-            const float f0 = __builtin_amdgcn_exp2f(m_run - m_ref);
-            l_run *= f0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int db = 0; db < ND; ++db) o[e][db] *= f0;
-#pragma unroll
-            for (int k = 0; k < KS - 1; ++k) {
-                const float* ml = merge_ml + ((k * RW + wr) * 16 + lr) * 2;
-                const float f = __builtin_amdgcn_exp2f(ml[0] - m_ref);
-                l_run = fmaf(ml[1], f, l_run);
-                const float* s = merge_o + ((k * RW + wr) * 16 + lr) * D + 4 * ND * lg;
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-#pragma unroll
-                    for (int db = 0; db < ND; ++db) o[e][db] = fmaf(s[ND * e + db], f, o[e][db]);
-            }
-            m_run = m;
-        }
-    }
-    if (w.active == 1) {
-        if (kg == 0 && row_ok) {
-            const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;   // (no row seen: zeros)
-            T* d = static_cast<T*>(a.out) + ((static_cast<int64_t>(w.b) * a.rows + t) * a.heads + head) * D + 4 * ND * lg;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int u = 0; u < ND / 4; ++u) {
-                    const float y[4] = {o[e][4 * u] * inv, o[e][4 * u + 1] * inv, o[e][4 * u + 2] * inv,
-                                        o[e][4 * u + 3] * inv};
-                    store4(d + ND * e + 4 * u, y);
-                }
-        }
-        return;
-    }
-    // Several workgroups share the keys: [16 RW][D] outputs, then maxima and sums.
-    constexpr uint32_t kPart = 16 * RW * (D + 2) * 4;
-    char* unit_parts = a.parts + static_cast<int64_t>(w.unit) * a.splits * kPart;
-    if (kg == 0) {
-        const __amdgpu_buffer_rsrc_t prs = buffer_rsrc(unit_parts + static_cast<int64_t>(w.split) * kPart, kPart);
-        const uint32_t at = static_cast<uint32_t>(wr * 16 + lr) * D * 4 + 16 * ND * lg;
-        if (row_ok) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int u = 0; u < ND / 4; ++u)
-                    coherent_store16(prs, at + 4 * ND * e + 16 * u,
-                                     u32x4{__float_as_uint(o[e][4 * u]), __float_as_uint(o[e][4 * u + 1]),
-                                           __float_as_uint(o[e][4 * u + 2]), __float_as_uint(o[e][4 * u + 3])});
-        }
         if (lg == 0) {
-            float* ml = reinterpret_cast<float*>(unit_parts + static_cast<int64_t>(w.split) * kPart) + 16 * RW * D;
-            coherent_store(ml + wr * 16 + lr, m_run);
-            coherent_store(ml + 16 * RW + wr * 16 + lr, l_run);
+            merge_m[wave][16 * rt + lr] = limit[rt] == -INFINITY ? -INFINITY : m_run[rt] * row_factor[rt];
+            merge_l[wave][16 * rt + lr] = l;
         }
-        publish_partials();
     }
+    __syncthreads();
+    constexpr int kItems = kRows * D / 4 / kThreads;   // of a thread
+    constexpr uint32_t kPart = kRows * (D + 2) * 4;
+    char* unit_parts = a.parts + static_cast<int64_t>(w.unit) * a.splits * kPart;
+    const __amdgpu_buffer_rsrc_t prs = buffer_rsrc(unit_parts, kPart * static_cast<uint32_t>(a.splits));
+    const auto put = [&](int row, int d4, const float* y, float l) {
+        const int r = r0 + row, t = r / w.g;
+        if (t >= w.n_tok) return;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;   // (no row seen: zeros)
+        const float z[4] = {y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv};
+        store4(static_cast<T*>(a.out) +
+                   ((static_cast<int64_t>(w.b) * a.rows + t) * a.heads + w.kh * w.g + r % w.g) * D + 4 * d4,
+               z);
+    };
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+        const int item = i * kThreads + threadIdx.x, row = item / (D / 4), d4 = item % (D / 4);
+        float m = merge_m[0][row];
+#pragma unroll
+        for (int k = 1; k < kWaves; ++k) m = fmaxf(m, merge_m[k][row]);
+        const float m_ref = m == -INFINITY ? 0.0f : m;
+        float l = 0.0f, y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) {
+            const float f = __builtin_amdgcn_exp2f(merge_m[k][row] - m_ref);
+            l = fmaf(merge_l[k][row], f, l);
+            const float4 o = *reinterpret_cast<const float4*>(&merge_o[k][row * D + 4 * d4]);
+            y[0] = fmaf(o.x, f, y[0]);
+            y[1] = fmaf(o.y, f, y[1]);
+            y[2] = fmaf(o.z, f, y[2]);
+            y[3] = fmaf(o.w, f, y[3]);
+        }
+        if (w.active == 1) {
+            put(row, d4, y, l);
+            continue;
+        }
+        // Several workgroups share the keys: [rows][D] outputs, then maxima and sums.
+        const uint32_t part = static_cast<uint32_t>(w.split) * kPart;
+        coherent_store16(prs, part + static_cast<uint32_t>(item) * 16,
+                         u32x4{__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3])});
+        if (d4 == 0) {
+            float* ml = reinterpret_cast<float*>(unit_parts + part) + kRows * D;
+            coherent_store(ml + row, m);
+            coherent_store(ml + kRows + row, l);
+        }
+    }
+    if (w.active == 1) return;
+    publish_partials();
     __syncthreads();
     if (threadIdx.x == 0) ticket = ticket_take(a.tickets + w.unit, w.active);
     __syncthreads();
     if (ticket != static_cast<unsigned>(w.active - 1)) return;
     if (threadIdx.x == 0) __hip_atomic_store(a.tickets + w.unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    // The last arrival: thread (row, 4 dims), workgroups in order.
-    for (int item = threadIdx.x; item < 16 * RW * (D / 4); item += kThreads) {
-        const int row = item / (D / 4), d4 = item % (D / 4);
-        const int rr = w.tile * RW * 16 + row, tt = rr / w.g;
-        if (tt >= w.n_tok) continue;
-        float m = -INFINITY;
-        for (int s = 0; s < w.active; ++s)
-            m = fmaxf(m, coherent_load(reinterpret_cast<const float*>(unit_parts + static_cast<int64_t>(s) * kPart) +
-                                       16 * RW * D + row));
-        const float m_ref = m == -INFINITY ? 0.0f : m;
-        float l = 0.0f, y[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int s = 0; s < w.active; ++s) {
-            const char* part = unit_parts + static_cast<int64_t>(s) * kPart;
-            const float* ml = reinterpret_cast<const float*>(part) + 16 * RW * D;
-            const float f = __builtin_amdgcn_exp2f(coherent_load(ml + row) - m_ref);
-            l = fmaf(coherent_load(ml + 16 * RW + row), f, l);
-            const u32x4 x = coherent_load16(buffer_rsrc(part, kPart), static_cast<uint32_t>(item) * 16);
+    // The last arrival merges: the factor of every (workgroup, row) first, in
+    // LDS, then thread (row, four dims) adds the workgroups in order, eight
+    // loads in flight.
+    float* factor = merge_o[0];   // [active][rows]: at most 64 x 16 RT floats
+    float* total = merge_m[0];
+    static_assert(kMaxSplits * kRows <= kWaves * kRows * D, "factors fit");
+    for (int row = threadIdx.x / 16; row < kRows; row += kThreads / 16) {
+        const int s0 = threadIdx.x % 16;
+        float mv[kMaxSplits / 16], lv[kMaxSplits / 16], m = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = fmaf(__uint_as_float(x[e]), f, y[e]);
+        for (int u = 0; u < kMaxSplits / 16; ++u) {
+            const int s = s0 + 16 * u;
+            const float* ml = reinterpret_cast<const float*>(unit_parts + static_cast<int64_t>(s) * kPart) + kRows * D + row;
+            mv[u] = s < w.active ? coherent_load(ml) : -INFINITY;
+            lv[u] = s < w.active ? coherent_load(ml + kRows) : 0.0f;
         }
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] *= inv;
-        store4(static_cast<T*>(a.out) +
-                   ((static_cast<int64_t>(w.b) * a.rows + tt) * a.heads + w.kh * w.g + rr % w.g) * D + 4 * d4,
-               y);
+        for (int u = 0; u < kMaxSplits / 16; ++u) m = fmaxf(m, mv[u]);
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        const float m_ref = m == -INFINITY ? 0.0f : m;
+        float l = 0.0f;
+#pragma unroll
+        for (int u = 0; u < kMaxSplits / 16; ++u) {
+            const int s = s0 + 16 * u;
+            const float f = __builtin_amdgcn_exp2f(mv[u] - m_ref);
+            l = fmaf(lv[u], f, l);
+            if (s < w.active) factor[s * kRows + row] = f;
+        }
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) l += __shfl_xor(l, o, 64);
+        if (s0 == 0) total[row] = l;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+        const int item = i * kThreads + threadIdx.x, row = item / (D / 4), d4 = item % (D / 4);
+        float y[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int s0 = 0; s0 < w.active; s0 += 8) {
+            u32x4 x[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                x[u] = s0 + u < w.active ? coherent_load16(prs, static_cast<uint32_t>(s0 + u) * kPart + item * 16)
+                                         : u32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const float f = s0 + u < w.active ? factor[(s0 + u) * kRows + row] : 0.0f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = fmaf(__uint_as_float(x[u][e]), f, y[e]);
+            }
+        }
+        put(row, d4, y, total[row]);
     }
 }
 
-// Row blocks of a workgroup, tiles, and workgroups that share a tile's keys.
+// 16-row tiles of a wave, row tiles, and workgroups that share a tile's keys.
 struct Plan {
-    int rw, splits;
+    int rt, splits;
     int64_t tiles, units;
     int64_t bytes;
 };
 
-Plan plan(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, int64_t d, int64_t max_seq) {
+Plan plan(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, int64_t d, int64_t max_seq, bool two) {
     Plan p;
     const int64_t r = rows * (heads / kv_heads);
-    p.rw = r <= 16 ? 1 : r <= 32 ? 2 : 4;
-    p.tiles = (r + 16 * p.rw - 1) / (16 * p.rw);
+    const int most_tiles = d == 64 ? (two ? 2 : 4) : (two ? 1 : 2);
+    p.rt = r <= 16 ? 1 : r <= 32 ? std::min(2, most_tiles) : most_tiles;
+    p.tiles = (r + 16 * p.rt - 1) / (16 * p.rt);
     p.units = batch * kv_heads * p.tiles;
-    const int64_t most = (max_seq + kBlock * 2 * (4 / p.rw) - 1) / (kBlock * 2 * (4 / p.rw));
+    const int64_t most = (max_seq + kBlock * kLeast - 1) / (kBlock * kLeast);
     int64_t s = p.units > 0 && p.units < kTargetGroups ? (kTargetGroups + p.units - 1) / p.units : 1;
     s = std::min<int64_t>(std::min<int64_t>(s, kMaxSplits), most);
     p.splits = static_cast<int>(std::max<int64_t>(s, 1));
-    p.bytes = p.splits > 1 ? kTicketBytes + p.units * p.splits * (16 * p.rw * (d + 2) * 4) : 0;
+    p.bytes = p.splits > 1 ? kTicketBytes + p.units * p.splits * (16 * p.rt * (d + 2) * 4) : 0;
     return p;
 }
 
@@ -555,24 +619,24 @@ int check_shape(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, in
     if (rows < 0 || rows > (1 << 20) || heads < 1 || heads > 65536 || heads % kv_heads ||
         rows * (heads / kv_heads) > (1 << 30))
         return fail_inval("attention_q8: bad rows or heads");
-    if (batch && rows && plan(batch, rows, heads, kv_heads, d, max_seq).units > (1 << 30))
+    if (batch && rows && plan(batch, rows, heads, kv_heads, d, max_seq, true).units > (1 << 30))
         return fail_inval("attention_q8: too many rows for one call");
     return 0;
 }
 
-template <typename T, int D, int RW>
+template <typename T, int D, int RT>
 void launch(const Args& a, int64_t grid, hipStream_t stream) {
-    hipLaunchKernelGGL((attention_q8_kernel<T, D, RW>), dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((attention_q8_kernel<T, D, RT>), dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, stream, a);
 }
 
-template <typename T, int D>
-void launch_rows(const Args& a, int rw, int64_t grid, hipStream_t stream) {
-    if (rw == 1)
-        launch<T, D, 1>(a, grid, stream);
-    else if (rw == 2)
-        launch<T, D, 2>(a, grid, stream);
+template <typename T>
+void launch_rows(const Args& a, int64_t d, int rt, int64_t grid, hipStream_t stream) {
+    if (d == 128)
+        rt == 1 ? launch<T, 128, 1>(a, grid, stream) : launch<T, 128, 2>(a, grid, stream);
+    else if (rt == 1)
+        launch<T, 64, 1>(a, grid, stream);
     else
-        launch<T, D, 4>(a, grid, stream);
+        rt == 2 ? launch<T, 64, 2>(a, grid, stream) : launch<T, 64, 4>(a, grid, stream);
 }
 
 }  // namespace
@@ -587,7 +651,8 @@ int64_t vm_hip_attention_q8_workspace_bytes(int64_t batch, int64_t rows, int64_t
     clear_error();
     VM_TRY(check_shape(batch, rows, heads, kv_heads, head_dim, max_seq));
     if (batch == 0 || rows == 0) return 0;
-    return plan(batch, rows, heads, kv_heads, head_dim, max_seq).bytes;
+    return std::max(plan(batch, rows, heads, kv_heads, head_dim, max_seq, false).bytes,
+                    plan(batch, rows, heads, kv_heads, head_dim, max_seq, true).bytes);
 }
 
 int vm_hip_attention_q8(const vm_hip_kv_q8* cache, const void* q, void* out, int dtype, int64_t rows, int64_t heads,
@@ -603,9 +668,12 @@ int vm_hip_attention_q8(const vm_hip_kv_q8* cache, const void* q, void* out, int
     if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15)
         return fail_inval("attention_q8: q and out must be 16-byte aligned");
     if (!(scale < INFINITY)) return fail_inval("attention_q8: scale must be finite");
-    const Plan p = plan(cache->batch, rows, heads, cache->kv_heads, cache->head_dim, cache->max_seq);
-    if (p.bytes > 0 &&
-        (!workspace || workspace_bytes < p.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0))
+    const Plan p = plan(cache->batch, rows, heads, cache->kv_heads, cache->head_dim, cache->max_seq,
+                        dtype == VM_HIP_DTYPE_F32);
+    const int64_t need = vm_hip_attention_q8_workspace_bytes(cache->batch, rows, heads, cache->kv_heads, cache->head_dim,
+                                                             cache->max_seq);
+    if (need > 0 &&
+        (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0))
         return fail_inval("attention_q8: workspace smaller than vm_hip_attention_q8_workspace_bytes or unaligned");
     Args a;
     a.kc = cache->k_codes;
@@ -630,13 +698,12 @@ int vm_hip_attention_q8(const vm_hip_kv_q8* cache, const void* q, void* out, int
     a.scale = scale > 0.0f ? scale : 1.0f / std::sqrt(static_cast<float>(cache->head_dim));
     const int64_t grid = p.units * p.splits;
     auto s = static_cast<hipStream_t>(stream);
-    const bool wide = cache->head_dim == 128;
     if (dtype == VM_HIP_DTYPE_F32)
-        wide ? launch_rows<float, 128>(a, p.rw, grid, s) : launch_rows<float, 64>(a, p.rw, grid, s);
+        launch_rows<float>(a, cache->head_dim, p.rt, grid, s);
     else if (dtype == VM_HIP_DTYPE_F16)
-        wide ? launch_rows<F16, 128>(a, p.rw, grid, s) : launch_rows<F16, 64>(a, p.rw, grid, s);
+        launch_rows<F16>(a, cache->head_dim, p.rt, grid, s);
     else
-        wide ? launch_rows<BF16, 128>(a, p.rw, grid, s) : launch_rows<BF16, 64>(a, p.rw, grid, s);
+        launch_rows<BF16>(a, cache->head_dim, p.rt, grid, s);
     return check_launch("attention_q8", s);
 }
 
