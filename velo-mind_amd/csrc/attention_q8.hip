@@ -605,7 +605,7 @@ Plan plan(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, int64_t 
     p.tiles = (r + 16 * p.rt - 1) / (16 * p.rt);
     p.units = batch * kv_heads * p.tiles;
     const int64_t most = (max_seq + kBlock * kLeast - 1) / (kBlock * kLeast);
-    int64_t s = p.units > 0 && p.units < kTargetGroups ? (kTargetGroups + p.units - 1) / p.units : 1;
+    int64_t s = p.units > 0 && p.units < kTargetGroups ? kTargetGroups / p.units : 1;
     s = std::min<int64_t>(std::min<int64_t>(s, kMaxSplits), most);
     p.splits = static_cast<int>(std::max<int64_t>(s, 1));
     p.bytes = p.splits > 1 ? kTicketBytes + p.units * p.splits * (16 * p.rt * (d + 2) * 4) : 0;
