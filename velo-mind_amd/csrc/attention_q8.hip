@@ -40,6 +40,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "kv_q8.h"
 #include "vm_device.h"
@@ -311,7 +312,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
     }
     int v_exp = -200;   // E of the weights' unit 2^(E - 14)
 
-    auto compute = [&](int block, const Codes& c) {
+    // kMasked: some row does not see the whole block (or the block ends past the
+    // cache).  Two copies of the code: the masks cost a quarter of a block's time.
+    auto compute = [&](auto masked_tag, int block, const Codes& c) {
+        constexpr bool kMasked = decltype(masked_tag)::value;
         const int k0 = block * kBlock;
         float* sl = scales_lds[wave];
         sl[lane] = c.s;                       // keys' scales, then values'
@@ -340,7 +344,6 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
             sv[j] = sl[kBlock + 8 * lg + j];
         }
         __builtin_amdgcn_wave_barrier();
-        const bool masked = k0 + kBlock > whole;
         // Scores less the row's reference (and its factor), and whether that or
         // the weights' unit has to move: rarely, after the first blocks.
         uint32_t sees[RT];   // bit j: the row sees key k0 + 8 lg + j
@@ -352,7 +355,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             sees[rt] = 0xffu;
-            if (masked) {
+            if (kMasked) {
                 const int key0 = k0 + 8 * lg;
                 const int node0 = key0 - w.p0;   // of the call's own rows; negative: cached before
                 if (a.tree) {
@@ -374,7 +377,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 float v = fmaf(st[rt][j / 4][j % 4], sk[j], -m_run[rt]);
-                if (masked && !(sees[rt] >> j & 1)) v = -INFINITY;
+                if (kMasked && !(sees[rt] >> j & 1)) v = -INFINITY;
                 st[rt][j / 4][j % 4] = v;
                 mt[rt] = fmaxf(mt[rt], v);
             }
@@ -411,8 +414,11 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
             for (int j = 0; j < 8; ++j) {
                 float p = __builtin_amdgcn_exp2f(st[rt][j / 4][j % 4] * row_factor[rt]);
                 float x = p * su[j];
-                if (masked && !(sees[rt] >> j & 1)) p = x = 0.0f;   // (whatever the factor and the scale are)
+                if (kMasked && !(sees[rt] >> j & 1)) p = x = 0.0f;   // (whatever the factor and the scale are)
                 l_run[rt] += p;
+                // (Both parts have to come from one rounding of x: folded into its
+                // product, the first part's conversion would round another value.)
+                if (kTwo) asm("" : "+v"(x));
                 const _Float16 hi = static_cast<_Float16>(x);
                 pf[rt][0][j] = hi;
                 if (kTwo) pf[rt][NP - 1][j] = static_cast<_Float16>(x - static_cast<float>(hi));
@@ -445,21 +451,28 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
         }
     };
 
+    // A wave's blocks, the next one's codes on their way while one is computed;
+    // the blocks that need masks come last.
     {
         Codes c0, c1;
         int block = w.first + wave;
-        if (block < w.last) {
-            load(block, c0);
-            while (true) {
-                if (block + kWaves < w.last) load(block + kWaves, c1);
-                compute(block, c0);
-                block += kWaves;
-                if (block >= w.last) break;
-                if (block + kWaves < w.last) load(block + kWaves, c0);
-                compute(block, c1);
-                block += kWaves;
-                if (block >= w.last) break;
+        if (block < w.last) load(block, c0);
+        while (block < w.last && (block + 1) * kBlock <= whole) {
+            if (block + kWaves < w.last) load(block + kWaves, c1);
+            compute(std::false_type{}, block, c0);
+            block += kWaves;
+            if (block >= w.last || (block + 1) * kBlock > whole) {
+                c0 = c1;
+                break;
             }
+            if (block + kWaves < w.last) load(block + kWaves, c0);
+            compute(std::false_type{}, block, c1);
+            block += kWaves;
+        }
+        for (; block < w.last; block += kWaves) {
+            if (block + kWaves < w.last) load(block + kWaves, c1);
+            compute(std::true_type{}, block, c0);
+            c0 = c1;
         }
     }
     // Every wave's triple to LDS (outputs without their unit); then thread
