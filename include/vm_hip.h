@@ -853,7 +853,8 @@ int vm_hip_qmm_a8(const void* staged, const void* packed, const float* scale, vo
  *
  * A pointer of the rules that is NULL leaves its rule out (repetition 1,
  * frequency and presence 0, no bias, everything allowed).  Tokens outside
- * [0, vocab) match nothing; lengths are clamped to [0, stride].
+ * [0, vocab) match nothing; lengths are clamped to [0, stride], strides are
+ * at most 2^30.
  * logits and out are aligned as their elements are. */
 typedef struct vm_hip_logits_rules {
     const int32_t*  history;          /* [seqs, history_stride]                    */
@@ -875,8 +876,7 @@ typedef struct vm_hip_logits_rules {
 
 /* workspace: vm_hip_logits_rules_workspace_bytes bytes, 16-byte aligned and
  * zeroed before its first use; needed for tokens (NULL otherwise); every call
- * leaves it ready for the next one of any shape it is large enough for.  Calls
- * that share a workspace must not overlap.  seqs * rows <= 65536, vocab <
+ * leaves it zeroed again.  Calls that share a workspace must not overlap.  seqs * rows <= 65536, vocab <
  * 2^31; workspace_bytes returns a negative status otherwise. */
 int64_t vm_hip_logits_rules_workspace_bytes(int64_t seqs, int64_t rows, int64_t vocab);
 int vm_hip_logits_rules_apply(const vm_hip_logits_rules* rules, const void* logits, void* out, int dtype,

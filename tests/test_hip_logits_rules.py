@@ -112,7 +112,7 @@ def run(hip, a, use, dtype, counts=None, in_place=False, ws=None, stream=None):
     hip.logits_rules(r.rules, x.addr, out.addr, dtype, tokens.addr, seqs, rows, vocab, dc.addr if dc else None, ws.addr, ws.nbytes, stream)
     if stream is not None:
         stream.synchronize()
-    assert (ws.download(np.uint32, (65536,)) == 0).all(), "tickets left behind"
+    assert (ws.download(np.uint8, (ws.nbytes,)) == 0).all(), "the workspace is not zero again"
     return host_typed(out, a["logits"].shape, dtype), tokens.download(np.int32, (seqs, rows))
 
 

@@ -67,6 +67,6 @@ def test_logits_arguments():
                 dict(bias_tokens=P, bias_values=P, bias_stride=4), dict(bias_tokens=P, bias_values=P, bias_lengths=P, bias_stride=-1)]:
         _refused(H.logits_rules, H.LogitsRules(**bad), *ok[1:])
     assert H.open_library().vm_hip_logits_rules_apply(None, P, P, 0, P, 2, 3, 1000, None, P, need, None) == H.EINVAL
-    for bad in [(-1, 1, 10), (65537, 1, 10), (1, 1, 0), (1, 1, 1 << 31), (1, 65536, 0x7fffffff)]:
+    for bad in [(-1, 1, 10), (65537, 1, 10), (1, 1, 0), (1, 1, 1 << 31)]:
         _refused(H.logits_rules_workspace_bytes, *bad)
     H.logits_rules(r, None, None, H.DTYPE_F32, None, 0, 3, 1000, None, None, 0)

@@ -59,9 +59,11 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kBlock = 32;             // keys of a block
 constexpr int kLeast = 2 * kWaves;     // blocks that are worth a workgroup
 constexpr int kMaxSplits = 64;
-constexpr int kMaxUnits = 1024;        // workgroup groups that split their keys
-constexpr int64_t kTicketBytes = kMaxUnits * 4;
+constexpr int kMaxUnits = 512;         // workgroup groups that split their keys
+constexpr int kTicketStride = 16;      // a ticket has a 64-byte line of its own
+constexpr int64_t kTicketBytes = kMaxUnits * kTicketStride * 4;
 constexpr int kTargetGroups = 512;     // workgroups that fill 256 compute units twice
+static_assert(kTargetGroups <= kMaxUnits, "calls of more units do not split");
 
 struct Args {
     const int8_t* kc;
@@ -544,10 +546,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
     if (w.active == 1) return;
     publish_partials();
     __syncthreads();
-    if (threadIdx.x == 0) ticket = ticket_take(a.tickets + w.unit, w.active);
+    if (threadIdx.x == 0) ticket = ticket_take(a.tickets + w.unit * kTicketStride, w.active);
     __syncthreads();
     if (ticket != static_cast<unsigned>(w.active - 1)) return;
-    if (threadIdx.x == 0) __hip_atomic_store(a.tickets + w.unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (threadIdx.x == 0) __hip_atomic_store(a.tickets + w.unit * kTicketStride, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     // The last arrival merges: the factor of every (workgroup, row) first, in
     // LDS, then thread (row, four dims) adds the workgroups in order, eight
     // loads in flight.
@@ -613,11 +615,18 @@ struct Plan {
 Plan plan(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, int64_t d, int64_t max_seq, bool two) {
     Plan p;
     const int64_t r = rows * (heads / kv_heads);
-    const int most_tiles = d == 64 ? (two ? 2 : 4) : (two ? 1 : 2);
-    p.rt = r <= 16 ? 1 : r <= 32 ? std::min(2, most_tiles) : most_tiles;
+    const int64_t most = (max_seq + kBlock * kLeast - 1) / (kBlock * kLeast);
+    // More tiles a wave share the codes' widening, as far as registers go (fp32,
+    // 64 dims: four spill; 16-bit, 128 dims, one wave per SIMD instead of two: 340
+    // us against 201 for 24 tokens of 64 heads over 131000 keys; one tile: 303);
+    // fewer where the keys cannot be shared out to enough workgroups (16 tokens
+    // of 32 heads over 2000 keys: 9.0 us with one, 12.0 with two or four).
+    p.rt = d == 64 && !two ? 4 : 2;
+    while (p.rt > 1 && (r <= 8 * p.rt ||
+                        batch * kv_heads * ((r + 16 * p.rt - 1) / (16 * p.rt)) * std::min<int64_t>(most, kMaxSplits) < kTargetGroups))
+        p.rt /= 2;
     p.tiles = (r + 16 * p.rt - 1) / (16 * p.rt);
     p.units = batch * kv_heads * p.tiles;
-    const int64_t most = (max_seq + kBlock * kLeast - 1) / (kBlock * kLeast);
     int64_t s = p.units > 0 && p.units < kTargetGroups ? kTargetGroups / p.units : 1;
     s = std::min<int64_t>(std::min<int64_t>(s, kMaxSplits), most);
     p.splits = static_cast<int>(std::max<int64_t>(s, 1));

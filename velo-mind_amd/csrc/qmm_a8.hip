@@ -27,8 +27,9 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kT = 256;
 constexpr int kBlockBytes = 2048;
-constexpr int kMaxTiles = 4096;          // tiles that several workgroups may share
-constexpr int64_t kTicketBytes = kMaxTiles * 4;
+constexpr int kMaxTiles = 512;           // tiles that several workgroups may share
+constexpr int kTicketStride = 16;        // a ticket has a 64-byte line of its own
+constexpr int64_t kTicketBytes = kMaxTiles * kTicketStride * 4;
 constexpr int kMaxSplits = 16;
 
 int64_t blocks32(int64_t x) { return (x + 31) / 32; }
@@ -261,10 +262,10 @@ __global__ __launch_bounds__(kT) void qmm_a8_kernel(const Args g) {
             coherent_store16(prs, split * kPart + (b * kT + threadIdx.x) * 16, __builtin_bit_cast(u32x4, mine[b]));
         publish_partials();
         __syncthreads();
-        if (threadIdx.x == 0) ticket = ticket_take(g.tickets + tile, g.splits);
+        if (threadIdx.x == 0) ticket = ticket_take(g.tickets + tile * kTicketStride, g.splits);
         __syncthreads();
         if (ticket != static_cast<unsigned>(g.splits - 1)) return;
-        if (threadIdx.x == 0) __hip_atomic_store(g.tickets + tile, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (threadIdx.x == 0) __hip_atomic_store(g.tickets + tile * kTicketStride, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         for (int s = 0; s < g.splits; ++s) {
             if (s == split) continue;
 #pragma unroll
@@ -292,7 +293,7 @@ Plan plan(int64_t rows, int64_t k, int64_t n) {
     p.panels = blocks32(n);
     const int64_t tiles = p.tiles_m * p.panels;
     // Few tiles: enough workgroups to fill the GPU twice, a step a wave at least.
-    int64_t s = tiles < 512 ? (512 + tiles - 1) / tiles : 1;
+    int64_t s = tiles < kMaxTiles ? (kMaxTiles + tiles - 1) / tiles : 1;
     s = std::min<int64_t>({s, kMaxSplits, std::max<int64_t>(steps64(k) / 4, 1)});
     p.splits = static_cast<int>(s);
     p.bytes = s > 1 ? kTicketBytes + tiles * s * p.mb * 4096 : 0;
