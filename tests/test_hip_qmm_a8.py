@@ -58,7 +58,8 @@ def test_products(hip, m, k, n, dtype):
 
 
 @pytest.mark.parametrize("m,k,n", [(7, 28672, 40), (3, 131072, 33), (40, 20000, 64), (2100, 512, 96), (2049, 100, 33),
-                                   (530, 1100, 1030), (1024, 64, 2048), (700, 8192, 600)])
+                                   (530, 1100, 1030), (1024, 64, 2048), (700, 8192, 600),
+                                   (2049, 130, 8200), (4100, 64, 4160), (300, 2500, 16500)])
 @pytest.mark.parametrize("dtype", [0, 5])
 def test_long_rows_and_large_outputs(hip, m, k, n, dtype):
     print(f"case qmm_a8 large m={m} k={k} n={n} dtype={dtype}", flush=True)

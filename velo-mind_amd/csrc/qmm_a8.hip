@@ -163,16 +163,14 @@ struct alignas(sizeof(T) * 4) Four {
     T e[4];
 };
 
-// Four adjacent columns of a row.
+// Four adjacent columns of a row, ws their scales.
 template <typename T>
-__device__ __forceinline__ void epilogue4(const Args& g, int64_t row, int64_t col, i32x4 s) {
+__device__ __forceinline__ void epilogue4(const Args& g, int64_t row, int64_t col, i32x4 s, float as, const float (&ws)[4]) {
     if (row >= g.rows || col >= g.n) return;
-    const float as = g.a_scale[row];
     T* c = static_cast<T*>(g.c) + row * g.n + col;
     Four<T> y;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        y.e[i] = narrow<T>(static_cast<float>(s[i]) * (as * (col + i < g.n ? g.w_scale[col + i] : 0.0f)));
+    for (int i = 0; i < 4; ++i) y.e[i] = narrow<T>(static_cast<float>(s[i]) * (as * ws[i]));
     if (g.vec) {
         *reinterpret_cast<Four<T>*>(c) = y;
     } else {
@@ -208,6 +206,14 @@ __global__ __launch_bounds__(kT) void qmm_a8_kernel(const Args g) {
 #pragma unroll
     for (int b = 0; b < MB; ++b)
         ap[b] = g.a + static_cast<int64_t>(min(tm * MB + b, g.row_blocks - 1)) * g.steps * kBlockBytes + lane * 16;
+    // This thread's outputs: columns 4 (thread % 8) .., rows thread / 8 + 32 b.
+    const int64_t row0 = static_cast<int64_t>(tm) * MB * 32 + threadIdx.x / 8;
+    const int64_t col0 = static_cast<int64_t>(panel) * 32 + 4 * (threadIdx.x % 8);
+    float as[MB], ws[4];
+#pragma unroll
+    for (int b = 0; b < MB; ++b) as[b] = g.a_scale[min(row0 + 32 * b, g.rows - 1)];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ws[i] = g.w_scale[min(col0 + i, g.n - 1)];
     i32x16 acc[MB];
 #pragma unroll
     for (int b = 0; b < MB; ++b)
@@ -274,20 +280,153 @@ __global__ __launch_bounds__(kT) void qmm_a8_kernel(const Args g) {
         }
     }
 #pragma unroll
-    for (int b = 0; b < MB; ++b) {
-        const int at = b * kT + threadIdx.x;   // row at / 8, columns 4 (at % 8) ..
-        epilogue4<T>(g, static_cast<int64_t>(tm) * MB * 32 + at / 8, static_cast<int64_t>(panel) * 32 + 4 * (at % 8), mine[b]);
+    for (int b = 0; b < MB; ++b) epilogue4<T>(g, row0 + 32 * b, col0, mine[b], as[b], ws);
+}
+
+// ---- Large products: tiles of BM x BN by four waves (2 x 2), 64 k a stage.
+// A stage's blocks come in by 16-byte loads (two blocks a load of the
+// workgroup), wait in registers, kAhead stages early, and go to one of three
+// LDS buffers as they are, so every LDS access is 1 KB of adjacent bytes.  A
+// wave reads the operands of the next 32 k while it multiplies these, across
+// stages too (the stage after next is being written meanwhile: the barrier at
+// a stage's end orders both), so the matrix cores wait for neither LDS nor
+// memory.
+template <typename T, int BM, int BN>
+__global__ __launch_bounds__(kT, 1) void qmm_a8_tile_kernel(const Args g) {
+    constexpr int PA = BM / 32, PB = BN / 32;   // blocks of a stage
+    constexpr int MT = BM / 64, NT = BN / 64;   // a wave's 32 x 32 tiles
+    constexpr int LA = PA / 2, LB = PB / 2;     // loads of a stage
+    constexpr int kAhead = BM + BN >= 512 ? 2 : 6;
+    constexpr int kStage = (PA + PB) * kBlockBytes;
+    __shared__ __align__(16) int8_t lds[3 * kStage];
+    const int tiles_n = (g.panels + PB - 1) / PB, tiles_m = (g.row_blocks + PA - 1) / PA;
+    // Workgroups go to the XCDs in turn: an XCD's are the row tiles of every
+    // eighth column tile, which share that column's weights in its L2.
+    const int xcd = static_cast<int>(blockIdx.x) % 8, j = static_cast<int>(blockIdx.x) / 8;
+    // (scalars, which the buffer descriptors have to be made of)
+    const int tm = __builtin_amdgcn_readfirstlane(j % tiles_m);
+    const int tn = __builtin_amdgcn_readfirstlane(j / tiles_m * 8 + xcd);
+    if (tn >= tiles_n) return;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wr = wave / 2, wc = wave % 2;
+
+    // Blocks past the operands' ends, and stages past the last, read as zeros.
+    const uint32_t pitch = static_cast<uint32_t>(g.steps) * kBlockBytes;
+    const __amdgpu_buffer_rsrc_t ars = buffer_rsrc(g.a + static_cast<int64_t>(tm) * PA * pitch,
+                                                   static_cast<uint32_t>(min(PA, g.row_blocks - tm * PA)) * pitch);
+    const __amdgpu_buffer_rsrc_t brs = buffer_rsrc(g.w + static_cast<int64_t>(tn) * PB * pitch,
+                                                   static_cast<uint32_t>(min(PB, g.panels - tn * PB)) * pitch);
+    const uint32_t from = static_cast<uint32_t>(tid >> 7) * pitch + static_cast<uint32_t>(tid & 127) * 16;
+    struct Stage {
+        u32x4 a[LA], b[LB];
+    };
+    const auto load = [&](int stage, Stage& t) {
+        const uint32_t o = stage < g.steps ? from + static_cast<uint32_t>(stage) * kBlockBytes : 0x80000000u;
+#pragma unroll
+        for (int u = 0; u < LA; ++u) t.a[u] = buffer_load16(ars, o + 2 * u * pitch);
+#pragma unroll
+        for (int u = 0; u < LB; ++u) t.b[u] = buffer_load16(brs, o + 2 * u * pitch);
+    };
+    const auto store = [&](const Stage& t, int8_t* to) {
+#pragma unroll
+        for (int u = 0; u < LA; ++u) *reinterpret_cast<u32x4*>(to + u * 2 * kBlockBytes + tid * 16) = t.a[u];
+#pragma unroll
+        for (int u = 0; u < LB; ++u) *reinterpret_cast<u32x4*>(to + (PA + 2 * u) * kBlockBytes + tid * 16) = t.b[u];
+    };
+    i32x4 fa[2][MT], fb[2][NT];   // operands of this and the next 32 k
+    const auto fetch = [&](const int8_t* stage, int h) {
+        const int8_t* la = stage + wr * MT * kBlockBytes + h * 1024 + lane * 16;
+        const int8_t* lb = stage + (PA + wc * NT) * kBlockBytes + h * 1024 + lane * 16;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) fa[h][i] = *reinterpret_cast<const i32x4*>(la + i * kBlockBytes);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) fb[h][n] = *reinterpret_cast<const i32x4*>(lb + n * kBlockBytes);
+    };
+    i32x16 acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][n][e] = 0;
+    const auto multiply = [&](int h) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+                acc[i][n] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[h][i], fb[h][n], acc[i][n], 0, 0, 0);
+    };
+
+    Stage ring[kAhead];
+    {
+        Stage t0, t1;
+        load(0, t0);
+        load(1, t1);
+#pragma unroll
+        for (int d = 0; d < kAhead; ++d) load(2 + d, ring[d]);
+        store(t0, lds);
+        store(t1, lds + kStage);
     }
+    __syncthreads();
+    int8_t *now = lds, *next = lds + kStage, *after = lds + 2 * kStage;
+    fetch(now, 0);
+    const auto advance = [&](int stage, Stage& t, bool more) {
+        fetch(now, 1);
+        multiply(0);
+        store(t, after);   // stage + 2
+        if (more) load(stage + 2 + kAhead, t);
+        fetch(next, 0);
+        multiply(1);
+        __syncthreads();
+        int8_t* first = now;
+        now = next;
+        next = after;
+        after = first;
+    };
+    int stage = 0;
+    for (; stage + kAhead <= g.steps; stage += kAhead) {
+#pragma unroll
+        for (int d = 0; d < kAhead; ++d) advance(stage + d, ring[d], true);
+    }
+#pragma unroll
+    for (int d = 0; d < kAhead - 1; ++d)
+        if (stage + d < g.steps) advance(stage + d, ring[d], false);
+    // Element e of lane l: row 8 (e / 4) + 4 (l / 32) + e % 4, column l % 32.
+    // All the scales first: a load between two stores would wait for them.
+    float as[MT][16], ws[NT];
+    const int64_t row0 = (static_cast<int64_t>(tm) * PA + wr * MT) * 32 + 4 * (lane / 32);
+    const int64_t col0 = (static_cast<int64_t>(tn) * PB + wc * NT) * 32 + lane % 32;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) as[i][e] = g.a_scale[min(row0 + 32 * i + 8 * (e / 4) + e % 4, g.rows - 1)];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) ws[n] = g.w_scale[min(col0 + 32 * n, g.n - 1)];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int64_t row = row0 + 32 * i + 8 * (e / 4) + e % 4;
+            T* c = static_cast<T*>(g.c) + row * g.n + col0;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+                if (row < g.rows && col0 + 32 * n < g.n)
+                    c[32 * n] = narrow<T>(static_cast<float>(acc[i][n][e]) * (as[i][e] * ws[n]));
+        }
 }
 
 struct Plan {
     int mb, splits;
+    int tile;   // edge of the LDS kernel's tiles; 0: the other kernel
     int64_t tiles_m, panels, bytes;
 };
 
 Plan plan(int64_t rows, int64_t k, int64_t n) {
     Plan p;
     const int64_t rb = blocks32(rows);
+    const auto tiles_of = [&](int64_t edge) { return (rb * 32 + edge - 1) / edge * ((n + edge - 1) / edge); };
+    p.tile = rows <= 128 ? 0 : tiles_of(256) >= 256 ? 256 : tiles_of(128) >= 128 ? 128 : 0;
     p.mb = rb <= 1 ? 1 : rb <= 2 ? 2 : 4;
     p.tiles_m = (rb + p.mb - 1) / p.mb;
     p.panels = blocks32(n);
@@ -296,6 +435,12 @@ Plan plan(int64_t rows, int64_t k, int64_t n) {
     int64_t s = tiles < kMaxTiles ? (kMaxTiles + tiles - 1) / tiles : 1;
     s = std::min<int64_t>({s, kMaxSplits, std::max<int64_t>(steps64(k) / 4, 1)});
     p.splits = static_cast<int>(s);
+    if (p.tile) {
+        p.tiles_m = (rb * 32 + p.tile - 1) / p.tile;
+        p.splits = 1;
+        p.bytes = 0;
+        return p;
+    }
     p.bytes = s > 1 ? kTicketBytes + tiles * s * p.mb * 4096 : 0;
     return p;
 }
@@ -327,8 +472,18 @@ int stage(const void* a, int64_t rows, int64_t k, void* staged, hipStream_t stre
 }
 
 template <typename T>
-void launch(const Args& g, int mb, int64_t grid, hipStream_t stream) {
-    const dim3 d(static_cast<unsigned>(grid));
+void launch(const Args& g, const Plan& p, hipStream_t stream) {
+    const int mb = p.mb;
+    if (p.tile) {
+        const int64_t tiles_n = (p.panels * 32 + p.tile - 1) / p.tile;
+        const dim3 d(static_cast<unsigned>(p.tiles_m * ((tiles_n + 7) / 8) * 8));
+        if (p.tile == 256)
+            hipLaunchKernelGGL((qmm_a8_tile_kernel<T, 256, 256>), d, dim3(kT), 0, stream, g);
+        else
+            hipLaunchKernelGGL((qmm_a8_tile_kernel<T, 128, 128>), d, dim3(kT), 0, stream, g);
+        return;
+    }
+    const dim3 d(static_cast<unsigned>(p.tiles_m * p.panels * p.splits));
     if (mb == 1)
         hipLaunchKernelGGL((qmm_a8_kernel<T, 1>), d, dim3(kT), 0, stream, g);
     else if (mb == 2)
@@ -418,14 +573,13 @@ int vm_hip_qmm_a8(const void* staged, const void* packed, const float* scale, vo
     g.splits = p.splits;
     const unsigned e = c_dtype == VM_HIP_DTYPE_F32 ? 4 : 2;
     g.vec = n % 4 == 0 && !off(c, 4 * e - 1);
-    const int64_t grid = p.tiles_m * p.panels * p.splits;
     auto s = static_cast<hipStream_t>(stream);
     if (c_dtype == VM_HIP_DTYPE_F16)
-        launch<F16>(g, p.mb, grid, s);
+        launch<F16>(g, p, s);
     else if (c_dtype == VM_HIP_DTYPE_BF16)
-        launch<BF16>(g, p.mb, grid, s);
+        launch<BF16>(g, p, s);
     else
-        launch<float>(g, p.mb, grid, s);
+        launch<float>(g, p, s);
     return check_launch("qmm_a8", s);
 }
 
