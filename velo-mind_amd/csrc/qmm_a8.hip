@@ -53,7 +53,11 @@ __global__ __launch_bounds__(kT) void a8_pack_kernel(const int8_t* __restrict__ 
     }
 }
 
-// ---- Activations: WPR waves hold a row, 16 adjacent values a lane and chunk.
+// ---- Activations: a workgroup a row, 16 adjacent values a lane and chunk, read
+// once (the first kHeld chunks of a lane wait in registers for the maximum).
+// 16 x 2048 fp32 2.6 us, 512 x 2048 4.6, 2048 x 8192 bf16 23 (50 MB: HBM at half
+// its rate; with codes gathered in LDS, so that 64 adjacent bytes are written
+// instead of 16, it took as long there and half as long again at 512 rows).
 template <typename T>
 __device__ __forceinline__ void load16(const T* p, int valid, float (&x)[16]);
 template <>
@@ -90,21 +94,19 @@ __device__ __forceinline__ void load16<BF16>(const BF16* p, int valid, float (&x
 
 constexpr int kHeld = 4;   // chunks of a lane kept in registers between the two passes
 
-template <typename T, int WPR>
-__global__ __launch_bounds__(kT) void a8_stage_kernel(const T* __restrict__ a, int8_t* __restrict__ out,
-                                                      float* __restrict__ scales, int64_t rows, int k, int steps) {
+template <typename T>
+__global__ __launch_bounds__(kT) void a8_stage_row_kernel(const T* __restrict__ a, int8_t* __restrict__ out,
+                                                          float* __restrict__ scales, int k, int steps) {
     __shared__ uint32_t wave_max[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * (4 / WPR) + wave / WPR;
-    const bool ok = row < rows;
-    const int first = (wave % WPR) * 64 + lane;   // this lane's chunks: first, first + 64 WPR, ..
+    const int64_t row = blockIdx.x;
     const int chunks = steps * 4;
-    const T* src = a + (ok ? row : 0) * k;
+    const T* src = a + row * k;
     float x[kHeld][16];
     uint32_t m = 0;
-    for (int c = first, u = 0; c < chunks; c += 64 * WPR, ++u) {
+    for (int c = threadIdx.x, u = 0; c < chunks; c += kT, ++u) {
         float y[16];
-        load16(src + c * 16, ok ? k - c * 16 : 0, y);
+        load16(src + c * 16, k - c * 16, y);
 #pragma unroll
         for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(y[i]) & 0x7fffffffu);
 #pragma unroll
@@ -115,16 +117,13 @@ __global__ __launch_bounds__(kT) void a8_stage_kernel(const T* __restrict__ a, i
     }
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), s, 64)));
-    if (WPR > 1) {
-        if (lane == 0) wave_max[wave] = m;
-        __syncthreads();
+    if (lane == 0) wave_max[wave] = m;
+    __syncthreads();
 #pragma unroll
-        for (int v = 0; v < 4; ++v) m = max(m, wave_max[v]);
-    }
-    if (!ok) return;
+    for (int v = 0; v < 4; ++v) m = max(m, wave_max[v]);
     const Q8Scale q8 = q8_scale(m);
     int8_t* dst = out + (row >> 5) * steps * kBlockBytes + (row & 31) * 16;
-    for (int c = first, u = 0; c < chunks; c += 64 * WPR, ++u) {
+    for (int c = threadIdx.x, u = 0; c < chunks; c += kT, ++u) {
         float y[16];
         if (u < kHeld) {
 #pragma unroll
@@ -141,7 +140,7 @@ __global__ __launch_bounds__(kT) void a8_stage_kernel(const T* __restrict__ a, i
         *reinterpret_cast<u32x4*>(dst + (c >> 2) * static_cast<int64_t>(kBlockBytes) + (c & 3) * 512) =
             *reinterpret_cast<const u32x4*>(e);
     }
-    if (first == 0) scales[row] = q8.scale;
+    if (threadIdx.x == 0) scales[row] = q8.scale;
 }
 
 // ---- The product.
@@ -283,20 +282,19 @@ __global__ __launch_bounds__(kT) void qmm_a8_kernel(const Args g) {
     for (int b = 0; b < MB; ++b) epilogue4<T>(g, row0 + 32 * b, col0, mine[b], as[b], ws);
 }
 
-// ---- Large products: tiles of BM x BN by four waves (2 x 2), 64 k a stage.
-// A stage's blocks come in by 16-byte loads (two blocks a load of the
-// workgroup), wait in registers, kAhead stages early, and go to one of three
+// ---- Large products: tiles of BM x BN by 2 x WN waves, 64 k a stage.  A
+// stage's blocks come in by 16-byte loads (WN blocks a load of the workgroup), wait in registers, kAhead stages early, and go to one of three
 // LDS buffers as they are, so every LDS access is 1 KB of adjacent bytes.  A
 // wave reads the operands of the next 32 k while it multiplies these, across
 // stages too (the stage after next is being written meanwhile: the barrier at
 // a stage's end orders both), so the matrix cores wait for neither LDS nor
 // memory.
-template <typename T, int BM, int BN>
-__global__ __launch_bounds__(kT, 1) void qmm_a8_tile_kernel(const Args g) {
-    constexpr int PA = BM / 32, PB = BN / 32;   // blocks of a stage
-    constexpr int MT = BM / 64, NT = BN / 64;   // a wave's 32 x 32 tiles
-    constexpr int LA = PA / 2, LB = PB / 2;     // loads of a stage
-    constexpr int kAhead = BM + BN >= 512 ? 2 : 6;
+template <typename T, int BM, int BN, int WN>
+__global__ __launch_bounds__(128 * WN, WN / 2) void qmm_a8_tile_kernel(const Args g) {
+    constexpr int PA = BM / 32, PB = BN / 32;       // blocks of a stage
+    constexpr int MT = BM / 64, NT = BN / WN / 32;  // a wave's 32 x 32 tiles
+    constexpr int LA = PA / WN, LB = PB / WN;       // loads of a stage, WN blocks each
+    constexpr int kAhead = 6;
     constexpr int kStage = (PA + PB) * kBlockBytes;
     __shared__ __align__(16) int8_t lds[3 * kStage];
     const int tiles_n = (g.panels + PB - 1) / PB, tiles_m = (g.row_blocks + PA - 1) / PA;
@@ -309,7 +307,7 @@ __global__ __launch_bounds__(kT, 1) void qmm_a8_tile_kernel(const Args g) {
     if (tn >= tiles_n) return;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wr = wave / 2, wc = wave % 2;
+    const int wr = wave / WN, wc = wave % WN;
 
     // Blocks past the operands' ends, and stages past the last, read as zeros.
     const uint32_t pitch = static_cast<uint32_t>(g.steps) * kBlockBytes;
@@ -324,15 +322,15 @@ __global__ __launch_bounds__(kT, 1) void qmm_a8_tile_kernel(const Args g) {
     const auto load = [&](int stage, Stage& t) {
         const uint32_t o = stage < g.steps ? from + static_cast<uint32_t>(stage) * kBlockBytes : 0x80000000u;
 #pragma unroll
-        for (int u = 0; u < LA; ++u) t.a[u] = buffer_load16(ars, o + 2 * u * pitch);
+        for (int u = 0; u < LA; ++u) t.a[u] = buffer_load16(ars, o + WN * u * pitch);
 #pragma unroll
-        for (int u = 0; u < LB; ++u) t.b[u] = buffer_load16(brs, o + 2 * u * pitch);
+        for (int u = 0; u < LB; ++u) t.b[u] = buffer_load16(brs, o + WN * u * pitch);
     };
     const auto store = [&](const Stage& t, int8_t* to) {
 #pragma unroll
-        for (int u = 0; u < LA; ++u) *reinterpret_cast<u32x4*>(to + u * 2 * kBlockBytes + tid * 16) = t.a[u];
+        for (int u = 0; u < LA; ++u) *reinterpret_cast<u32x4*>(to + u * WN * kBlockBytes + tid * 16) = t.a[u];
 #pragma unroll
-        for (int u = 0; u < LB; ++u) *reinterpret_cast<u32x4*>(to + (PA + 2 * u) * kBlockBytes + tid * 16) = t.b[u];
+        for (int u = 0; u < LB; ++u) *reinterpret_cast<u32x4*>(to + (PA + WN * u) * kBlockBytes + tid * 16) = t.b[u];
     };
     i32x4 fa[2][MT], fb[2][NT];   // operands of this and the next 32 k
     const auto fetch = [&](const int8_t* stage, int h) {
@@ -418,30 +416,34 @@ __global__ __launch_bounds__(kT, 1) void qmm_a8_tile_kernel(const Args g) {
 
 struct Plan {
     int mb, splits;
-    int tile;   // edge of the LDS kernel's tiles; 0: the other kernel
+    int wn;   // waves along n of the LDS kernel's 128 x 128 tiles; 0: the other kernel
     int64_t tiles_m, panels, bytes;
 };
 
 Plan plan(int64_t rows, int64_t k, int64_t n) {
     Plan p;
     const int64_t rb = blocks32(rows);
-    const auto tiles_of = [&](int64_t edge) { return (rb * 32 + edge - 1) / edge * ((n + edge - 1) / edge); };
-    p.tile = rows <= 128 ? 0 : tiles_of(256) >= 256 ? 256 : tiles_of(128) >= 128 ? 128 : 0;
+    // Large outputs: 128 x 128 tiles through LDS, with eight waves a tile where
+    // there is not one for each compute unit (512 x 5632 outputs: 20.2 us
+    // against 22.2 with four and 21.4 without LDS; 1000 x 5632: 31.6 with four,
+    // 34.4 with eight, 35.5 without; 1000 x 2048: 18.6 without, 20.9 with eight).
+    const int64_t tiles = (rows + 127) / 128 * ((n + 127) / 128);
+    p.wn = rows <= 128 || tiles < 160 ? 0 : tiles < 256 ? 4 : 2;
     p.mb = rb <= 1 ? 1 : rb <= 2 ? 2 : 4;
     p.tiles_m = (rb + p.mb - 1) / p.mb;
     p.panels = blocks32(n);
-    const int64_t tiles = p.tiles_m * p.panels;
+    const int64_t parts = p.tiles_m * p.panels;
     // Few tiles: enough workgroups to fill the GPU twice, a step a wave at least.
-    int64_t s = tiles < kMaxTiles ? (kMaxTiles + tiles - 1) / tiles : 1;
+    int64_t s = parts < kMaxTiles ? (kMaxTiles + parts - 1) / parts : 1;
     s = std::min<int64_t>({s, kMaxSplits, std::max<int64_t>(steps64(k) / 4, 1)});
     p.splits = static_cast<int>(s);
-    if (p.tile) {
-        p.tiles_m = (rb * 32 + p.tile - 1) / p.tile;
+    if (p.wn) {
+        p.tiles_m = (rows + 127) / 128;
         p.splits = 1;
         p.bytes = 0;
         return p;
     }
-    p.bytes = s > 1 ? kTicketBytes + tiles * s * p.mb * 4096 : 0;
+    p.bytes = s > 1 ? kTicketBytes + parts * s * p.mb * 4096 : 0;
     return p;
 }
 
@@ -460,27 +462,22 @@ unsigned element_mask(int d) { return d == VM_HIP_DTYPE_F32 ? 3 : 1; }
 template <typename T>
 int stage(const void* a, int64_t rows, int64_t k, void* staged, hipStream_t stream) {
     float* scales = reinterpret_cast<float*>(static_cast<char*>(staged) + staged_codes(rows, k));
-    const int steps = static_cast<int>(steps64(k));
-    // A wave a row where that fills the GPU, else four: the row's loads are a chain.
-    if (rows >= 2048 && k <= 4096)
-        hipLaunchKernelGGL((a8_stage_kernel<T, 1>), dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(kT), 0, stream,
-                           static_cast<const T*>(a), static_cast<int8_t*>(staged), scales, rows, static_cast<int>(k), steps);
-    else
-        hipLaunchKernelGGL((a8_stage_kernel<T, 4>), dim3(static_cast<unsigned>(rows)), dim3(kT), 0, stream,
-                           static_cast<const T*>(a), static_cast<int8_t*>(staged), scales, rows, static_cast<int>(k), steps);
+    hipLaunchKernelGGL(a8_stage_row_kernel<T>, dim3(static_cast<unsigned>(rows)), dim3(kT), 0, stream,
+                       static_cast<const T*>(a), static_cast<int8_t*>(staged), scales, static_cast<int>(k),
+                       static_cast<int>(steps64(k)));
     return check_launch("a8_stage", stream);
 }
 
 template <typename T>
 void launch(const Args& g, const Plan& p, hipStream_t stream) {
     const int mb = p.mb;
-    if (p.tile) {
-        const int64_t tiles_n = (p.panels * 32 + p.tile - 1) / p.tile;
+    if (p.wn) {
+        const int64_t tiles_n = (g.n + 127) / 128;
         const dim3 d(static_cast<unsigned>(p.tiles_m * ((tiles_n + 7) / 8) * 8));
-        if (p.tile == 256)
-            hipLaunchKernelGGL((qmm_a8_tile_kernel<T, 256, 256>), d, dim3(kT), 0, stream, g);
+        if (p.wn == 4)
+            hipLaunchKernelGGL((qmm_a8_tile_kernel<T, 128, 128, 4>), d, dim3(512), 0, stream, g);
         else
-            hipLaunchKernelGGL((qmm_a8_tile_kernel<T, 128, 128>), d, dim3(kT), 0, stream, g);
+            hipLaunchKernelGGL((qmm_a8_tile_kernel<T, 128, 128, 2>), d, dim3(256), 0, stream, g);
         return;
     }
     const dim3 d(static_cast<unsigned>(p.tiles_m * p.panels * p.splits));
