@@ -84,14 +84,19 @@ struct Args {
 // log2 of the power of two just above v (v >= 0 finite; 0 and subnormals: -126).
 __device__ __forceinline__ int exponent_above(float v) { return static_cast<int>(__float_as_uint(v) >> 23) - 126; }
 
-// Bytes 0, 1 (2, 3) of u = code ^ 0x80 as two fp16 codes.
-__device__ __forceinline__ half2v widen_low(uint32_t u) {
-    return __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) -
-           half2v{static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
+// Bytes 0, 1 (2, 3) of u = code ^ 0x80 as two fp16 codes, or 1152 more.
+template <bool kExact = true>
+__device__ __forceinline__ half2v widen_bits(uint32_t bits) {
+    const half2v v = __builtin_bit_cast(half2v, bits);
+    return kExact ? v - half2v{static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)} : v;
 }
+template <bool kExact = true>
+__device__ __forceinline__ half2v widen_low(uint32_t u) {
+    return widen_bits<kExact>(__builtin_amdgcn_perm(0x64646464u, u, 0x04010400u));
+}
+template <bool kExact = true>
 __device__ __forceinline__ half2v widen_high(uint32_t u) {
-    return __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) -
-           half2v{static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
+    return widen_bits<kExact>(__builtin_amdgcn_perm(0x64646464u, u, 0x04030402u));
 }
 __device__ __forceinline__ half8 join(half2v a, half2v b, half2v c, half2v d) {
     return half8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
@@ -226,47 +231,6 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
     // Rows below `whole` are seen by every token of the tile.
     const int whole = min(a.tree ? w.p0 : w.p0 + t_first + 1, w.n_keys);
 
-    // Q^T operands: Q[row][64 h + 16 lg + 8 s + j] in qf[.][.][2 h + s], scaled by
-    // the power of two that puts the row's largest magnitude in [2^13, 2^14).
-    half8 qf[RT][NP][NC];
-    float row_factor[RT];   // of a score's log2
-    int token[RT];          // -1: no row
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int r = r0 + 16 * rt + lr, t = r / w.g;
-        const bool row_ok = t < w.n_tok;
-        token[rt] = row_ok ? t : -1;
-        float x[H][16];
-        const T* qp = static_cast<const T*>(a.q) +
-                      ((static_cast<int64_t>(w.b) * a.heads + w.kh * w.g + r % w.g) * a.rows + t) * D + 16 * lg;
-        uint32_t m = 0;
-#pragma unroll
-        for (int h = 0; h < H; ++h) {
-            if (row_ok) {
-                load_query(qp + 64 * h, x[h]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) x[h][e] = 0.0f;
-            }
-#pragma unroll
-            for (int e = 0; e < 16; ++e) m = max(m, __float_as_uint(x[h][e]) & 0x7fffffffu);
-        }
-        m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 16, 64)));
-        m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 32, 64)));
-        const bool finite = m < 0x7f800000u;
-        const int up = 14 - exponent_above(__uint_as_float(m));
-        row_factor[rt] = finite ? ldexpf(a.scale * 1.44269504f, -up) : NAN;
-#pragma unroll
-        for (int h = 0; h < H; ++h)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float v = finite ? ldexpf(x[h][e], up) : 0.0f;
-                const _Float16 hi = static_cast<_Float16>(v);
-                qf[rt][0][2 * h + e / 8][e % 8] = hi;
-                if (kTwo) qf[rt][NP - 1][2 * h + e / 8][e % 8] = static_cast<_Float16>(v - static_cast<float>(hi));
-            }
-    }
-
     const int64_t head_row = (static_cast<int64_t>(w.b) * a.kv_heads + w.kh) * a.max_seq;
     const uint32_t code_bytes = static_cast<uint32_t>(w.n_keys) * D;   // loads past it give zeros
     const __amdgpu_buffer_rsrc_t krs = buffer_rsrc(a.kc + head_row * D, code_bytes);
@@ -301,6 +265,59 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
         }
     };
 
+    // The first block's codes are on their way while the queries are prepared.
+    Codes c0, c1;
+    int block = w.first + wave;
+    if (block < w.last) load(block, c0);
+
+    // Q^T operands: Q[row][64 h + 16 lg + 8 s + j] in qf[.][.][2 h + s], scaled by
+    // the power of two that puts the row's largest magnitude in [2^13, 2^14).
+    // One-part queries meet codes that are still 1152 too large (a subtraction
+    // less for each pair), and their scores start 1152 sum(Q) too low: that costs
+    // the fp32 sums 1152 / |code| of their precision, which 16 bits do not see.
+    half8 qf[RT][NP][NC];
+    float start[RT];
+    float row_factor[RT];   // of a score's log2
+    int token[RT];          // -1: no row
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int r = r0 + 16 * rt + lr, t = r / w.g;
+        const bool row_ok = t < w.n_tok;
+        token[rt] = row_ok ? t : -1;
+        float x[H][16];
+        const T* qp = static_cast<const T*>(a.q) +
+                      ((static_cast<int64_t>(w.b) * a.heads + w.kh * w.g + r % w.g) * a.rows + t) * D + 16 * lg;
+        uint32_t m = 0;
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            if (row_ok) {
+                load_query(qp + 64 * h, x[h]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[h][e] = 0.0f;
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) m = max(m, __float_as_uint(x[h][e]) & 0x7fffffffu);
+        }
+        m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 16, 64)));
+        m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 32, 64)));
+        const bool finite = m < 0x7f800000u;
+        const int up = 14 - exponent_above(__uint_as_float(m));
+        row_factor[rt] = finite ? ldexpf(a.scale * 1.44269504f, -up) : NAN;
+        float sum = 0.0f;
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float v = finite ? ldexpf(x[h][e], up) : 0.0f;
+                const _Float16 hi = static_cast<_Float16>(v);
+                qf[rt][0][2 * h + e / 8][e % 8] = hi;
+                if (kTwo) qf[rt][NP - 1][2 * h + e / 8][e % 8] = static_cast<_Float16>(v - static_cast<float>(hi));
+                sum += static_cast<float>(hi);
+            }
+        start[rt] = kTwo ? 0.0f : -1152.0f * sum_groups(sum);
+    }
+
     f32x4 acc[RT][ND];   // O^T[dim ND (4 lg + e) + db][row lr] 2^(14 - v_exp)
     float m_run[RT];     // the score (less the row's factor) that weighs 1
     float limit[RT];     // how far a score may pass it (log2); -inf before the first key
@@ -323,7 +340,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
         sl[lane] = c.s;                       // keys' scales, then values'
         f32x4 st[RT][2];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) st[rt][0] = st[rt][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int rt = 0; rt < RT; ++rt) st[rt][0] = st[rt][1] = f32x4{start[rt], start[rt], start[rt], start[rt]};
 #pragma unroll
         for (int h = 0; h < H; ++h)
 #pragma unroll
@@ -331,7 +348,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
 #pragma unroll
                 for (int bt = 0; bt < 2; ++bt) {
                     const uint32_t u0 = c.k[bt][h][2 * s] ^ 0x80808080u, u1 = c.k[bt][h][2 * s + 1] ^ 0x80808080u;
-                    const half8 kf = join(widen_low(u0), widen_high(u0), widen_low(u1), widen_high(u1));
+                    const half8 kf = join(widen_low<kTwo>(u0), widen_high<kTwo>(u0), widen_low<kTwo>(u1), widen_high<kTwo>(u1));
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -456,9 +473,6 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
     // A wave's blocks, the next one's codes on their way while one is computed;
     // the blocks that need masks come last.
     {
-        Codes c0, c1;
-        int block = w.first + wave;
-        if (block < w.last) load(block, c0);
         while (block < w.last && (block + 1) * kBlock <= whole) {
             if (block + kWaves < w.last) load(block + kWaves, c1);
             compute(std::false_type{}, block, c0);
@@ -553,6 +567,15 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
     // The last arrival merges: the factor of every (workgroup, row) first, in
     // LDS, then thread (row, four dims) adds the workgroups in order, eight
     // loads in flight.
+    constexpr int kFirst = kItems <= 2 ? 8 : 0;   // workgroups whose outputs are requested before the factors
+    u32x4 early[kItems][kFirst + 1];
+#pragma unroll
+    for (int i = 0; i < kItems; ++i)
+#pragma unroll
+        for (int u = 0; u < kFirst; ++u)
+            early[i][u] = u < w.active ? coherent_load16(prs, static_cast<uint32_t>(u) * kPart +
+                                                                  (i * kThreads + threadIdx.x) * 16)
+                                       : u32x4{0, 0, 0, 0};
     float* factor = merge_o[0];   // [active][rows]: at most 64 x 16 RT floats
     float* total = merge_m[0];
     static_assert(kMaxSplits * kRows <= kWaves * kRows * D, "factors fit");
@@ -592,7 +615,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
             u32x4 x[8];
 #pragma unroll
             for (int u = 0; u < 8; ++u)
-                x[u] = s0 + u < w.active ? coherent_load16(prs, static_cast<uint32_t>(s0 + u) * kPart + item * 16)
+                x[u] = s0 < kFirst ? early[i][kFirst ? u : 0] : s0 + u < w.active ? coherent_load16(prs, static_cast<uint32_t>(s0 + u) * kPart + item * 16)
                                          : u32x4{0, 0, 0, 0};
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
@@ -657,8 +680,10 @@ void launch_rows(const Args& a, int64_t d, int rt, int64_t grid, hipStream_t str
         rt == 1 ? launch<T, 128, 1>(a, grid, stream) : launch<T, 128, 2>(a, grid, stream);
     else if (rt == 1)
         launch<T, 64, 1>(a, grid, stream);
-    else
-        rt == 2 ? launch<T, 64, 2>(a, grid, stream) : launch<T, 64, 4>(a, grid, stream);
+    else if (rt == 2)
+        launch<T, 64, 2>(a, grid, stream);
+    else if constexpr (sizeof(T) == 2)   // (plan() gives fp32 two tiles at most)
+        launch<T, 64, 4>(a, grid, stream);
 }
 
 }  // namespace
