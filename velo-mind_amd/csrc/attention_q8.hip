@@ -27,8 +27,8 @@
 // Widening: code ^ 0x80 behind the byte 0x64 is fp16 1152 + code, one packed
 // subtraction away.
 //
-// Weights meet fp16 as p sv 2^(14 - E), 2^E above the largest sv seen: what
-// the second part cannot hold is below 2^-39 of the largest.
+// Weights meet fp16 as p sv 2^(8 - E), 2^E above the largest sv seen and p
+// below 2^7: what the second part cannot hold is below 2^-32 of the largest.
 //
 // A workgroup of four waves takes 16 RW query rows and a share of the keys;
 // its KS = 4 / RW key groups take turns at 32-key blocks, and their (max,
@@ -214,7 +214,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
     constexpr bool kTwo = sizeof(T) == 4;  // fp32 operands: two fp16 parts
     constexpr int NP = kTwo ? 2 : 1;
     constexpr int kRows = 16 * RT;
-    constexpr float kHeadroom = 1.0f;      // log2 units that a weight may exceed 1 by
+    // A weight may exceed 1 by this much (log2) before its row's reference moves:
+    // with one unit some row of a wave moved in most blocks.
+    constexpr float kHeadroom = 7.0f;
+    constexpr int kUnit = 8;               // weights in units of 2^(E - kUnit): below 2^15
     __shared__ __align__(16) float scales_lds[kWaves][2 * kBlock];
     __shared__ __align__(16) float merge_o[kWaves][kRows * D];
     __shared__ float merge_m[kWaves][kRows], merge_l[kWaves][kRows];
@@ -318,7 +321,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
         start[rt] = kTwo ? 0.0f : -1152.0f * sum_groups(sum);
     }
 
-    f32x4 acc[RT][ND];   // O^T[dim ND (4 lg + e) + db][row lr] 2^(14 - v_exp)
+    f32x4 acc[RT][ND];   // O^T[dim ND (4 lg + e) + db][row lr] 2^(kUnit - v_exp)
     float m_run[RT];     // the score (less the row's factor) that weighs 1
     float limit[RT];     // how far a score may pass it (log2); -inf before the first key
     float l_run[RT];     // sum of this lane's keys' weights
@@ -329,7 +332,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
         m_run[rt] = l_run[rt] = 0.0f;
         limit[rt] = -INFINITY;
     }
-    int v_exp = -200;   // E of the weights' unit 2^(E - 14)
+    int v_exp = -200;   // E
 
     // kMasked: some row does not see the whole block (or the block ends past the
     // cache).  Two copies of the code: the masks cost a quarter of a block's time.
@@ -425,7 +428,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
         }
         float su[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) su[j] = ldexpf(sv[j], 14 - v_exp);
+        for (int j = 0; j < 8; ++j) su[j] = ldexpf(sv[j], kUnit - v_exp);
         half8 pf[RT][NP];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
@@ -503,7 +506,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
             for (int u = 0; u < ND / 4; ++u) {
                 float y[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) y[i] = ldexpf(acc[rt][4 * u + i][e], v_exp - 14);
+                for (int i = 0; i < 4; ++i) y[i] = ldexpf(acc[rt][4 * u + i][e], v_exp - kUnit);
                 store4(d + ND * e + 4 * u, y);
             }
         if (lg == 0) {
