@@ -30,11 +30,20 @@
 // Weights meet fp16 as p sv 2^(8 - E), 2^E above the largest sv seen and p
 // below 2^7: what the second part cannot hold is below 2^-32 of the largest.
 //
-// A workgroup of four waves takes 16 RW query rows and a share of the keys;
-// its KS = 4 / RW key groups take turns at 32-key blocks, and their (max,
-// sum, output) triples are merged through LDS.  Where few workgroups would
-// leave the GPU idle the keys are split over several of them; each stores its
-// triple in the workspace, and the one that draws the last ticket merges.
+// A workgroup of four waves takes 16 RT query rows and a share of the keys;
+// its waves take turns at 32-key blocks, the next block's codes in registers
+// while one is computed, and their (reference, sum, output) triples are merged
+// through LDS.  Where few workgroups would leave the GPU idle the keys are
+// split over several of them; each stores its triple in the workspace, and the
+// one that draws the last ticket merges.
+//
+// MI355X, passes back to back: 32 tokens over ragged caches of up to 8000, 64
+// heads of 128, bf16: 86 us, 4.7 TB/s of codes and scales (HBM: a large copy
+// reaches 4.8); 1000 rows of 32 heads of 64 behind 3001 cached, f16: 55 us, 520
+// TFLOP/s; 24 nodes of 64 heads of 128 over 131000, bf16: 183 us, 560 TFLOP/s
+// (VALU: widening and softmax, about 340 instructions beside 32 MFMAs a block of
+// 32 keys x 32 rows); one token of 32 heads over 2000: 7.3 us, 16 nodes: 7.9
+// (the chain position - codes - LDS merge - ticket - join).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
