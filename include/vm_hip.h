@@ -777,7 +777,9 @@ int vm_hip_kv_q8_keep(const vm_hip_kv_q8* cache, const int32_t* pos, const int32
  *        itself).  Bits at or past the sequence's count are ignored.  NULL: a
  *        chain, token t sees rows up to pos[b] + t.
  * scale <= 0 means 1/sqrt(head_dim).  A token that sees no row gives zeros.
- * Cache rows at or past max_seq do not exist.
+ * Cache rows at or past max_seq do not exist; a token whose own row does not
+ * (kv_q8_append left its q alone) gets unspecified values.  Scores have to stay
+ * below 2^112 in magnitude.
  * Scores, maxima, sums and the output are accumulated in fp32; what is
  * rounded before: with fp32 queries, the query and each weight to 22
  * significant bits (two fp16 parts); with 16-bit queries, each weight to fp16

@@ -209,3 +209,32 @@ def test_one_workspace_for_several_shapes_and_replays(hip):
         want, wt = expect(a, ALL, 0)
         assert np.array_equal(out.download(np.float32, want.shape), want)
         assert np.array_equal(tokens.download(np.int32, (2, 2)), wt)
+
+
+def test_two_streams(hip):
+    sets = []
+    for i in range(2):
+        a = inputs(2, 3, 30000, 50, 6, 0, 20 + i)
+        sets.append((a, Rules(hip, a, ALL), dev(hip, a["logits"]), dev(hip, np.zeros_like(a["logits"])), dev(hip, np.zeros((2, 3), np.int32)),
+                     dev(hip, np.zeros(hip.logits_rules_workspace_bytes(2, 3, 30000), np.uint8)), hip.Stream()))
+    hip.synchronize()
+    print("case logits two streams", flush=True)
+    for _ in range(20):
+        for a, r, x, out, tokens, ws, s in sets:
+            hip.logits_rules(r.rules, x.addr, out.addr, 0, tokens.addr, 2, 3, 30000, None, ws.addr, ws.nbytes, s)
+    for a, r, x, out, tokens, ws, s in sets:
+        s.synchronize()
+        want, wt = expect(a, ALL, 0)
+        assert_equal(out.download(np.float32, want.shape), want)
+        assert_equal(tokens.download(np.int32, (2, 3)), wt)
+
+
+def test_long_histories(hip):
+    # histories longer than a workgroup holds in registers (4096 tokens), for
+    # several chunks of the vocabulary and rows
+    print("case logits long histories", flush=True)
+    a = inputs(2, 5, 5000, 13001, 1500, 0, 30)
+    a["history_lengths"][:] = [13001, 9000]
+    check(hip, a, ALL, 0)
+    a = inputs(1, 1, 2000000, 9000, 3, 5, 31)
+    check(hip, a, ALL, 5)

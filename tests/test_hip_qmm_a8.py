@@ -162,3 +162,26 @@ def test_packed_int8_weights_of_the_framework(hip):
     dense = codes.astype(np.float64) * scale.astype(np.float64)
     bound = (np.abs(a).max(1) / 254 * (1 + 1e-5))[:, None] * np.abs(dense).sum(0)[None, :]
     assert np.all(np.abs(got - a.astype(np.float64) @ dense) <= bound)
+
+
+def test_two_streams(hip):
+    # products that share a staged buffer and its weights, each with its own
+    # workspace and output, on two streams at once
+    m, k, n = 12, 4096, 96
+    a = np.random.default_rng(9).standard_normal((m, k)).astype(np.float32)
+    codes, scale = weights(k, n, 9)
+    da, dc, ds = dev(hip, a), dev(hip, codes), dev(hip, scale)
+    staged, packed = hip.DeviceBuffer(hip.a8_stage_bytes(m, k)), hip.DeviceBuffer(hip.a8_weights_bytes(k, n))
+    hip.a8_pack(dc.addr, k, n, packed.addr)
+    hip.a8_stage(da.addr, 0, m, k, staged.addr)
+    need = hip.qmm_a8_workspace_bytes(m, k, n)
+    assert need > 0   # several workgroups share a tile here
+    sets = [(hip.Stream(), dev(hip, np.zeros((m, n), np.float32)), dev(hip, np.zeros(need, np.uint8))) for _ in range(2)]
+    hip.synchronize()
+    print("case qmm_a8 two streams", flush=True)
+    for _ in range(30):
+        for s, out, ws in sets:
+            hip.qmm_a8(staged.addr, packed.addr, ds.addr, out.addr, 0, m, k, n, ws.addr, need, s)
+    for s, out, _ in sets:
+        s.synchronize()
+        assert_equal(out.download(np.float32, (m, n)), expect(a, codes, scale, 0))
