@@ -49,6 +49,17 @@ __device__ __forceinline__ BF16 narrow<BF16>(float v) { return BF16{f32_to_bf16_
 // message that names `who`).
 int check_kv_q8(const vm_hip_kv_q8* c, const char* who);
 
+// The same pointer, by an offset of zero that the compiler does not know: keeps
+// the element-wise branch of a guarded vector access apart from the vector
+// branch (with the first element in common, it was taken out of both, and what
+// was left of 16 bytes became a 4- and a 12-byte access).
+template <typename T>
+__device__ __forceinline__ T* apart(T* p) {
+    int zero = 0;
+    asm("" : "+v"(zero));
+    return p + zero;
+}
+
 struct Q8Scale {
     float scale;   // what a code stands for
     float inv;     // what a value is multiplied by before it is rounded

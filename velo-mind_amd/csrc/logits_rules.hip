@@ -59,6 +59,7 @@ __device__ __forceinline__ void load4<float>(const float* p, int valid, float (&
     if (valid >= 4) {
         __builtin_memcpy(x, p, 16);
     } else {
+        p = apart(p);
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[i] = i < valid ? p[i] : 0.0f;
     }
@@ -67,6 +68,7 @@ __device__ __forceinline__ void load4_bits(const uint16_t* p, int valid, uint16_
     if (valid >= 4) {
         __builtin_memcpy(h, p, 8);
     } else {
+        p = apart(p);
 #pragma unroll
         for (int i = 0; i < 4; ++i) h[i] = i < valid ? p[i] : uint16_t(0);
     }
@@ -90,6 +92,7 @@ __device__ __forceinline__ void store4(float* p, int valid, const float (&x)[4])
     if (valid >= 4) {
         __builtin_memcpy(p, x, 16);
     } else {
+        p = apart(p);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (i < valid) p[i] = x[i];
@@ -99,6 +102,7 @@ __device__ __forceinline__ void store4_bits(uint16_t* p, int valid, const uint16
     if (valid >= 4) {
         __builtin_memcpy(p, h, 8);
     } else {
+        p = apart(p);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (i < valid) p[i] = h[i];
@@ -174,8 +178,9 @@ __global__ __launch_bounds__(kT, 3) void logits_rules_kernel(const Args a) {
             if (i + 4 <= stride) {
                 __builtin_memcpy(h[u], history + i, 16);
             } else {
+                const int32_t* p = apart(history);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) h[u][e] = i + e < stride ? history[i + e] : -1;
+                for (int e = 0; e < 4; ++e) h[u][e] = i + e < stride ? p[i + e] : -1;
             }
         }
     };

@@ -65,6 +65,7 @@ __device__ __forceinline__ void load16<float>(const float* p, int valid, float (
     if (valid >= 16) {
         __builtin_memcpy(x, p, 64);
     } else {
+        p = apart(p);
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] = i < valid ? p[i] : 0.0f;
     }
@@ -75,6 +76,7 @@ __device__ __forceinline__ void load16_half(const uint16_t* p, int valid, float 
     if (valid >= 16) {
         __builtin_memcpy(h, p, 32);
     } else {
+        p = apart(p);
 #pragma unroll
         for (int i = 0; i < 16; ++i) h[i] = i < valid ? p[i] : uint16_t(0);
     }
@@ -438,9 +440,12 @@ Plan plan(int64_t rows, int64_t k, int64_t n) {
     p.tiles_m = (rb + p.mb - 1) / p.mb;
     p.panels = blocks32(n);
     const int64_t parts = p.tiles_m * p.panels;
-    // Few tiles: enough workgroups to fill the GPU twice, a step a wave at least.
-    int64_t s = parts < kMaxTiles ? (kMaxTiles + parts - 1) / parts : 1;
-    s = std::min<int64_t>({s, kMaxSplits, std::max<int64_t>(steps64(k) / 4, 1)});
+    // Few tiles: workgroups that fill the GPU twice share the k, as long as a
+    // wave keeps five steps (16 x 5632 x 2048: 10.5 us with four, 11.4 with eight,
+    // 13.8 with one; 16 x 2048 x 5632: 8.6 with one, 9.3 with three; 32 x 8192 x
+    // 8192: 17.7 with two, 19.6 with one).
+    int64_t s = parts < kMaxTiles ? kMaxTiles / parts : 1;
+    s = std::max<int64_t>(std::min<int64_t>({s, kMaxSplits, steps64(k) / 20}), 1);
     p.splits = static_cast<int>(s);
     if (p.wn) {
         p.tiles_m = (rows + 127) / 128;
