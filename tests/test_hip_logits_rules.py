@@ -230,7 +230,7 @@ def test_two_streams(hip):
 
 
 def test_long_histories(hip):
-    # histories longer than a workgroup holds in registers (4096 tokens), for
+    # histories longer than a workgroup holds in registers, for
     # several chunks of the vocabulary and rows
     print("case logits long histories", flush=True)
     a = inputs(2, 5, 5000, 13001, 1500, 0, 30)

@@ -4,7 +4,7 @@
 // A workgroup takes up to four rows of one sequence and a range of the
 // vocabulary, 1024 tokens (four a thread) at a time.  For each such chunk it
 // counts in LDS how often its tokens stand in the history, which its threads
-// keep in registers (up to 4096 tokens; every workgroup of a sequence reads
+// keep in registers (up to 2048 tokens; every workgroup of a sequence reads
 // the whole history: a few KB from L2, against a counting pass and a
 // vocabulary of counts in memory), notes the last bias entry of each (integer
 // maximum: the order of arrival does not matter) and counts the nodes on each
@@ -12,9 +12,9 @@
 // thread keeps its best value of each row; at the end the workgroup's best go
 // to the workspace, and the last workgroup of a row (atomic ticket) reduces
 // the candidates, lowest index on ties.  64 x 128256 fp32 behind 6000 tokens of
-// history: 31 us, 2.1 TB/s (instructions and waiting in turn: without the
-// history 28, without the reduction 25); 1 x 32000: 7.2 us (the chain lists -
-// LDS - biases - ticket).
+// history: 25.2 us, 2.7 TB/s (instructions and waiting in turn; with twice the
+// history in registers three workgroups fit a compute unit instead of four:
+// 29.2); 1 x 32000: 6.6 us (the chain lists - LDS - biases - ticket).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -37,7 +37,7 @@ constexpr int kTicketStride = 16;
 
 constexpr int kChunk = 4 * kT;        // tokens that a workgroup holds at a time
 constexpr int kRowBatch = 4;          // rows of a workgroup
-constexpr int kTargetGroups = 768;    // workgroups that are resident together
+constexpr int kTargetGroups = 1024;    // workgroups that are resident together
 
 struct Args {
     vm_hip_logits_rules r;
@@ -147,7 +147,7 @@ __device__ __forceinline__ void wave_best(uint64_t (&k)[N]) {
 }
 
 template <typename T, int RB>
-__global__ __launch_bounds__(kT, 3) void logits_rules_kernel(const Args a) {
+__global__ __launch_bounds__(kT, 4) void logits_rules_kernel(const Args a) {
 #pragma clang fp contract(off)
     __shared__ __align__(16) int seen_lds[kChunk];        // occurrences in the history
     __shared__ __align__(16) int entry_lds[kChunk];       // last bias entry + 1, 0: none
@@ -167,7 +167,7 @@ __global__ __launch_bounds__(kT, 3) void logits_rules_kernel(const Args a) {
     const bool penalties = a.r.repetition || a.r.frequency || a.r.presence;
     const bool histories = a.r.history && penalties, paths = a.r.drafted && penalties;
     // The lists, by their strides: the lengths are still on their way.
-    constexpr int kVec = 4;
+    constexpr int kVec = 2;
     const int stride = histories ? static_cast<int>(a.r.history_stride) : 0;
     const int32_t* history = a.r.history + seq * a.r.history_stride;
     int32_t h[kVec][4];

@@ -301,7 +301,7 @@ __global__ __launch_bounds__(128 * WN, WN / 2) void qmm_a8_tile_kernel(const Arg
     constexpr int PA = BM / 32, PB = BN / 32;       // blocks of a stage
     constexpr int MT = BM / 64, NT = BN / WN / 32;  // a wave's 32 x 32 tiles
     constexpr int LA = PA / WN, LB = PB / WN;       // loads of a stage, WN blocks each
-    constexpr int kAhead = 6;
+    constexpr int kAhead = WN == 2 ? 3 : 6;
     constexpr int kStage = (PA + PB) * kBlockBytes;
     __shared__ __align__(16) int8_t lds[3 * kStage];
     const int tiles_n = (g.panels + PB - 1) / PB, tiles_m = (g.row_blocks + PA - 1) / PA;
