@@ -98,10 +98,15 @@ constexpr int kHeld = 4;   // chunks of a lane kept in registers between the two
 
 template <typename T>
 __global__ __launch_bounds__(kT) void a8_stage_row_kernel(const T* __restrict__ a, int8_t* __restrict__ out,
-                                                          float* __restrict__ scales, int k, int steps) {
+                                                          float* __restrict__ scales, int64_t rows, int k, int steps,
+                                                          int spread) {
     __shared__ uint32_t wave_max[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t row = blockIdx.x;
+    // Workgroups go to the XCDs in turn; the 32 rows of a block, whose codes
+    // share lines, to one of them (rows of 256 at a time).
+    int64_t row = blockIdx.x;
+    if (spread) row = (row & ~int64_t(255)) | (row & 7) << 5 | (row & 255) >> 3;
+    if (row >= rows) return;
     const int chunks = steps * 4;
     const T* src = a + row * k;
     float x[kHeld][16];
@@ -472,9 +477,11 @@ unsigned element_mask(int d) { return d == VM_HIP_DTYPE_F32 ? 3 : 1; }
 template <typename T>
 int stage(const void* a, int64_t rows, int64_t k, void* staged, hipStream_t stream) {
     float* scales = reinterpret_cast<float*>(static_cast<char*>(staged) + staged_codes(rows, k));
-    hipLaunchKernelGGL(a8_stage_row_kernel<T>, dim3(static_cast<unsigned>(rows)), dim3(kT), 0, stream,
-                       static_cast<const T*>(a), static_cast<int8_t*>(staged), scales, static_cast<int>(k),
-                       static_cast<int>(steps64(k)));
+    const bool spread = rows >= 256;
+    const int64_t grid = spread ? (rows + 255) / 256 * 256 : rows;
+    hipLaunchKernelGGL(a8_stage_row_kernel<T>, dim3(static_cast<unsigned>(grid)), dim3(kT), 0, stream,
+                       static_cast<const T*>(a), static_cast<int8_t*>(staged), scales, rows, static_cast<int>(k),
+                       static_cast<int>(steps64(k)), spread ? 1 : 0);
     return check_launch("a8_stage", stream);
 }
 
