@@ -720,7 +720,8 @@ int vm_hip_silu_mul_stage_f32(const float* gate_up, void* a_staged, int layout, 
  * k_codes, v_codes  int8 [batch, kv_heads, max_seq, head_dim], 16-byte aligned
  * k_scales, v_scales f32 [batch, kv_heads, max_seq]
  *
- * head_dim is 64 or 128; max_seq * head_dim < 2^31; batch <= 65535.
+ * head_dim is 64 or 128; max_seq * head_dim < 2^31; batch <= 65535; kv_heads
+ * <= 4096.
  * `pos` is an int32 per sequence in device memory: how many tokens are
  * cached before the call's.  `counts` (int32 per sequence in device memory,
  * or NULL: all of them) says how many of the call's `rows` tokens a sequence
@@ -743,7 +744,8 @@ typedef struct vm_hip_kv_q8 {
  * the rotated query rounded once to dtype, q_out [batch, heads, rows,
  * head_dim].  Tokens whose cache row is outside [0, max_seq) are not written
  * at all; rotation positions are clamped to the tables' rows [0, max_seq).
- * qkv and q_out are 16-byte aligned. */
+ * qkv and q_out are 16-byte aligned; batch * rows * (heads + 2 kv_heads) <
+ * 2^28. */
 int vm_hip_kv_q8_append(const vm_hip_kv_q8* cache, const void* qkv, int dtype, int64_t rows, int64_t heads,
                         const float* cos_table, const float* sin_table, const int32_t* pos, const int32_t* counts,
                         const int32_t* depths, void* q_out, void* stream);
@@ -759,8 +761,8 @@ int vm_hip_kv_q8_read(const vm_hip_kv_q8* cache, int64_t first, int64_t rows, vo
  * kept_counts[b], the cache row pos[b] + kept[b * width + i] moves to row
  * pos[b] + i, codes and scales bit for bit.  All rows are read before any is
  * written, so any indices do (ascending ones are what a path has); an entry
- * whose source or target row is outside [0, max_seq) is skipped.  width <=
- * 256 (VM_HIP_KV_Q8_KEEP_MAX); kept_counts are clamped to [0, width]. */
+ * whose source or target row is outside [0, max_seq) is skipped.  batch *
+ * kv_heads < 2^24, width <= 256 (VM_HIP_KV_Q8_KEEP_MAX); kept_counts are clamped to [0, width]. */
 #define VM_HIP_KV_Q8_KEEP_MAX 256
 int vm_hip_kv_q8_keep(const vm_hip_kv_q8* cache, const int32_t* pos, const int32_t* kept, const int32_t* kept_counts,
                       int64_t width, void* stream);
@@ -779,7 +781,8 @@ int vm_hip_kv_q8_keep(const vm_hip_kv_q8* cache, const int32_t* pos, const int32
  * scale <= 0 means 1/sqrt(head_dim).  A token that sees no row gives zeros.
  * Cache rows at or past max_seq do not exist; a token whose own row does not
  * (kv_q8_append left its q alone) gets unspecified values.  Scores have to stay
- * below 2^112 in magnitude.
+ * below 2^112 in magnitude.  batch * kv_heads times the 16-row tiles of rows *
+ * heads / kv_heads rows is below 2^24 (2^28 rows in all).
  * Scores, maxima, sums and the output are accumulated in fp32; what is
  * rounded before: with fp32 queries, the query and each weight to 22
  * significant bits (two fp16 parts); with 16-bit queries, each weight to fp16
@@ -820,13 +823,16 @@ int vm_hip_attention_q8(const vm_hip_kv_q8* cache, const void* q, void* out, int
  *
  * Buffers of packed weights and staged rows are 16-byte aligned; a, codes,
  * scale and c as their elements are.  1 <= k <= 131072 (the largest sum then
- * fits 32 bits); rows == 0 or n == 0 is a no-op.
+ * fits 32 bits), rows <= 2^23, n <= 2^24 and rows * n <= 2^37; rows == 0 or n
+ * == 0 is a no-op.
  * workspace: vm_hip_qmm_a8_workspace_bytes bytes (0 is possible: then it may
  * be NULL), 16-byte aligned and zeroed before its first use; every call
  * leaves it ready for the next one of any shape it is large enough for.
  * Calls that share a workspace must not overlap.  The functions that return
  * bytes return a negative status for a shape that the product refuses. */
-#define VM_HIP_A8_MAX_K 131072
+#define VM_HIP_A8_MAX_K    131072
+#define VM_HIP_A8_MAX_ROWS (1 << 23)
+#define VM_HIP_A8_MAX_N    (1 << 24)
 int64_t vm_hip_a8_weights_bytes(int64_t k, int64_t n);
 int64_t vm_hip_a8_stage_bytes(int64_t rows, int64_t k);
 int64_t vm_hip_qmm_a8_workspace_bytes(int64_t rows, int64_t k, int64_t n);
@@ -856,7 +862,8 @@ int vm_hip_qmm_a8(const void* staged, const void* packed, const float* scale, vo
  * A pointer of the rules that is NULL leaves its rule out (repetition 1,
  * frequency and presence 0, no bias, everything allowed).  Tokens outside
  * [0, vocab) match nothing; lengths are clamped to [0, stride], strides are
- * at most 2^30.
+ * at most 2^30.  The lists are whole arrays, stride entries for every sequence:
+ * entries past a length may be read, and never count.
  * logits and out are aligned as their elements are. */
 typedef struct vm_hip_logits_rules {
     const int32_t*  history;          /* [seqs, history_stride]                    */

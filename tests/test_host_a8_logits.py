@@ -46,9 +46,9 @@ def test_a8_pack_and_stage_arguments():
 
 
 def test_qmm_a8_arguments():
-    need = H.qmm_a8_workspace_bytes(16, 2048, 512)
+    need = H.qmm_a8_workspace_bytes(16, 8192, 512)
     assert need > 0
-    _each(H.qmm_a8, [P, P, P, P, H.DTYPE_F32, 16, 2048, 512, P, need],
+    _each(H.qmm_a8, [P, P, P, P, H.DTYPE_F32, 16, 8192, 512, P, need],
           [(0, None), (0, P + 8), (1, None), (1, P + 4), (2, None), (2, P + 2), (3, None), (3, P + 2), (4, 2), (5, -1), (6, 0),
            (6, 131073), (7, -1), (8, None), (8, P + 8), (9, need - 1), (9, -1)])
     H.qmm_a8(None, None, None, None, H.DTYPE_F32, 0, 64, 64, None, 0)
@@ -70,3 +70,12 @@ def test_logits_arguments():
     for bad in [(-1, 1, 10), (65537, 1, 10), (1, 1, 0), (1, 1, 1 << 31)]:
         _refused(H.logits_rules_workspace_bytes, *bad)
     H.logits_rules(r, None, None, H.DTYPE_F32, None, 0, 3, 1000, None, None, 0)
+
+
+def test_a8_calls_of_more_threads_than_a_launch_has():
+    assert H.a8_stage_bytes(1 << 23, 1) > 0 and H.a8_weights_bytes(1, 1 << 24) > 0
+    assert H.qmm_a8_workspace_bytes(1 << 18, 64, 1 << 19) == 0
+    _refused(H.a8_stage_bytes, (1 << 23) + 1, 1)
+    _refused(H.a8_stage, P, H.DTYPE_F32, 1 << 24, 1, P)
+    _refused(H.qmm_a8_workspace_bytes, 1 << 19, 64, 1 << 19)
+    _refused(H.qmm_a8, P, P, P, P, H.DTYPE_F32, 1 << 19, 64, 1 << 19, None, 0)

@@ -89,3 +89,13 @@ def test_workspace_bytes():
     assert H.attention_q8_workspace_bytes(64, 512, 32, 8, 64, 4096) == 0   # enough rows to fill the GPU
     one = H.attention_q8_workspace_bytes(1, 1, 32, 4, 64, 4096)
     assert 0 < one <= H.attention_q8_workspace_bytes(1, 1, 32, 4, 64, 100000) < (64 << 20)
+
+
+def test_calls_of_more_threads_than_a_launch_has():
+    many = _cache(batch=4096, kv_heads=4096)
+    _refused(H.kv_q8_keep, many, P, P, P, 4)
+    # 1024 x 65536 tokens of four heads
+    _refused(H.kv_q8_append, _cache(batch=1024, kv_heads=1), P, H.DTYPE_F32, 65536, 2, P, P, P, None, None, P)
+    assert H.attention_q8_workspace_bytes(1024, 65536, 2, 1, 64, 100) == 0
+    _refused(H.attention_q8_workspace_bytes, 4096, 65536, 2, 1, 64, 100)
+    _refused(H.attention_q8, _cache(batch=4096, kv_heads=1), P, P, H.DTYPE_F32, 65536, 2, P, None, None, 1.0, None, 0)

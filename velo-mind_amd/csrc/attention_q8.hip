@@ -676,7 +676,8 @@ int check_shape(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, in
     if (rows < 0 || rows > (1 << 20) || heads < 1 || heads > 65536 || heads % kv_heads ||
         rows * (heads / kv_heads) > (1 << 30))
         return fail_inval("attention_q8: bad rows or heads");
-    if (batch && rows && plan(batch, rows, heads, kv_heads, d, max_seq, true).units > (1 << 30))
+    // (a launch has less than 2^32 threads)
+    if (batch && rows && plan(batch, rows, heads, kv_heads, d, max_seq, true).units >= (1 << 24))
         return fail_inval("attention_q8: too many rows for one call");
     return 0;
 }

@@ -248,7 +248,8 @@ int vm_hip_kv_q8_append(const vm_hip_kv_q8* cache, const void* qkv, int dtype, i
     if (!qkv || !cos_table || !sin_table || !pos || !q_out) return fail_inval("kv_q8_append: null pointer");
     if (!aligned16(qkv) || !aligned16(q_out)) return fail_inval("kv_q8_append: qkv and q_out must be 16-byte aligned");
     const int64_t total = cache->batch * rows * (heads + 2 * cache->kv_heads);
-    if (total > int64_t(0x7fffffff) * (kT / 16)) return fail_inval("kv_q8_append: too many tokens for one call");
+    if (total >= (1 << 28))   // (a launch has less than 2^32 threads)
+        return fail_inval("kv_q8_append: too many tokens for one call");
     auto s = static_cast<hipStream_t>(stream);
     if (dtype == VM_HIP_DTYPE_F16)
         return append<F16>(*cache, qkv, rows, heads, cos_table, sin_table, pos, counts, depths, q_out, total, s);
@@ -278,6 +279,7 @@ int vm_hip_kv_q8_keep(const vm_hip_kv_q8* cache, const int32_t* pos, const int32
     clear_error();
     VM_TRY(check_kv_q8(cache, "kv_q8_keep"));
     if (width < 0 || width > VM_HIP_KV_Q8_KEEP_MAX) return fail_inval("kv_q8_keep: width must be in [0, 256]");
+    if (cache->batch * cache->kv_heads >= (1 << 24)) return fail_inval("kv_q8_keep: too many heads for one call");
     if (width == 0 || cache->batch == 0) return 0;
     if (!pos || !kept || !kept_counts) return fail_inval("kv_q8_keep: null pointer");
     auto s = static_cast<hipStream_t>(stream);

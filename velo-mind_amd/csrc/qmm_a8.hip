@@ -465,8 +465,10 @@ Plan plan(int64_t rows, int64_t k, int64_t n) {
 int check_a8(int64_t rows, int64_t k, int64_t n, const char* who) {
     const std::string w(who);
     if (k < 1 || k > VM_HIP_A8_MAX_K) return fail_inval(w + ": k must be in [1, 131072]");
-    if (rows < 0 || rows > (1 << 24) || n < 0 || n > (1 << 24)) return fail_inval(w + ": rows or n out of range");
-    if (blocks32(rows) * blocks32(n) > (1 << 30)) return fail_inval(w + ": too many outputs for one call");
+    if (rows < 0 || rows > VM_HIP_A8_MAX_ROWS || n < 0 || n > VM_HIP_A8_MAX_N)
+        return fail_inval(w + ": rows or n out of range");
+    if (blocks32(rows) * blocks32(n) > (1 << 27))   // (a launch has less than 2^32 threads)
+        return fail_inval(w + ": too many outputs for one call");
     return 0;
 }
 
