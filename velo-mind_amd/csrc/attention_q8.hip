@@ -40,7 +40,7 @@
 // MI355X, passes back to back: 32 tokens over ragged caches of up to 8000, 64
 // heads of 128, bf16: 86 us, 4.7 TB/s of codes and scales (HBM: a large copy
 // reaches 4.8); 1000 rows of 32 heads of 64 behind 3001 cached, f16: 55 us, 520
-// TFLOP/s; 24 nodes of 64 heads of 128 over 131000, bf16: 183 us, 560 TFLOP/s
+// TFLOP/s; 24 nodes of 64 heads of 128 over 131000, bf16: 180 us, 570 TFLOP/s
 // (VALU: widening and softmax, about 340 instructions beside 32 MFMAs a block of
 // 32 keys x 32 rows); one token of 32 heads over 2000: 7.3 us, 16 nodes: 7.9
 // (the chain position - codes - LDS merge - ticket - join).

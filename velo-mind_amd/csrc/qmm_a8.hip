@@ -55,7 +55,7 @@ __global__ __launch_bounds__(kT) void a8_pack_kernel(const int8_t* __restrict__ 
 
 // ---- Activations: a workgroup a row, 16 adjacent values a lane and chunk, read
 // once (the first kHeld chunks of a lane wait in registers for the maximum).
-// 16 x 2048 fp32 2.6 us, 512 x 2048 4.6, 2048 x 8192 bf16 23 (50 MB: HBM at half
+// 16 x 2048 fp32 2.6 us, 512 x 2048 4.2-4.8, 2048 x 8192 bf16 20 (50 MB: HBM at half
 // its rate; with codes gathered in LDS, so that 64 adjacent bytes are written
 // instead of 16, it took as long there and half as long again at 512 rows).
 template <typename T>
@@ -103,7 +103,8 @@ __global__ __launch_bounds__(kT) void a8_stage_row_kernel(const T* __restrict__ 
     __shared__ uint32_t wave_max[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     // Workgroups go to the XCDs in turn; the 32 rows of a block, whose codes
-    // share lines, to one of them (rows of 256 at a time).
+    // share lines, to one of them (rows of 256 at a time): staging and product
+    // of 512 x 2048 x 5632 20.3 -> 19.7 us, of 1000 rows 30.4 -> 29.2.
     int64_t row = blockIdx.x;
     if (spread) row = (row & ~int64_t(255)) | (row & 7) << 5 | (row & 255) >> 3;
     if (row >= rows) return;
@@ -191,8 +192,8 @@ __device__ __forceinline__ void epilogue4(const Args& g, int64_t row, int64_t co
 // registers (a wave's loads of a step are 1 KB each), and their sums meet in
 // LDS.  Where the tiles are few, several workgroups share a tile's k range,
 // store their sums in the workspace and the last one adds them (integers: the
-// order does not matter).  16 x 2048 x 5632: 6.3 us (1.9 TB/s of weights: the
-// chain of loads, LDS and ticket); 4 x 8192 x 28672: 54 with the staging, 4.4
+// order does not matter).  16 x 2048 x 5632: 5.5 us (2.1 TB/s of weights: the
+// chain of loads and LDS); 4 x 8192 x 28672: 54 with the staging, 4.4
 // TB/s; more steps in flight a wave: slower (512 rows 21.4 -> 28.4 with three: L2
 // delivers 12 TB/s and is what bounds it).
 template <typename T, int MB>
@@ -293,11 +294,12 @@ __global__ __launch_bounds__(kT) void qmm_a8_kernel(const Args g) {
 }
 
 // ---- Large products: tiles of BM x BN by 2 x WN waves, 64 k a stage.  A
-// stage's blocks come in by 16-byte loads (WN blocks a load of the workgroup), wait in registers, kAhead stages early, and go to one of three
-// LDS buffers as they are, so every LDS access is 1 KB of adjacent bytes.  A
+// stage's blocks come in by 16-byte loads (WN blocks a load of the workgroup),
+// wait in registers, kAhead stages early, and go to one of three LDS buffers as
+// they are, so every LDS access is 1 KB of adjacent bytes.  A
 // wave reads the operands of the next 32 k while it multiplies these, across
 // stages too (the stage after next is being written meanwhile: the barrier at
-// a stage's end orders both).  2048 x 8192 x 28672: 548 us, 1.75 POP/s (a large
+// a stage's end orders both).  2048 x 8192 x 28672: 545 us, 1.76 POP/s (a large
 // library product of 8-bit integers reaches 2.1 here): the matrix cores are
 // busy 38 % of the time at the 2 GHz they run at, the rest waits at the stages'
 // barriers and for LDS; 256 x 256 tiles with one wave a SIMD: 620.
@@ -436,7 +438,7 @@ Plan plan(int64_t rows, int64_t k, int64_t n) {
     Plan p;
     const int64_t rb = blocks32(rows);
     // Large outputs: 128 x 128 tiles through LDS, with eight waves a tile where
-    // there is not one for each compute unit (512 x 5632 outputs: 20.2 us
+    // there is not one for each compute unit (512 x 5632 outputs: 20.3 us
     // against 22.2 with four and 21.4 without LDS; 1000 x 5632: 31.6 with four,
     // 34.4 with eight, 35.5 without; 1000 x 2048: 18.6 without, 20.9 with eight).
     const int64_t tiles = (rows + 127) / 128 * ((n + 127) / 128);
