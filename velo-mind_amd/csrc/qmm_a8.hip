@@ -293,23 +293,26 @@ __global__ __launch_bounds__(kT) void qmm_a8_kernel(const Args g) {
     for (int b = 0; b < MB; ++b) epilogue4<T>(g, row0 + 32 * b, col0, mine[b], as[b], ws);
 }
 
-// ---- Large products: tiles of BM x BN by 2 x WN waves, 64 k a stage.  A
-// stage's blocks come in by 16-byte loads (WN blocks a load of the workgroup),
-// wait in registers, kAhead stages early, and go to one of three LDS buffers as
-// they are, so every LDS access is 1 KB of adjacent bytes.  A
-// wave reads the operands of the next 32 k while it multiplies these, across
-// stages too (the stage after next is being written meanwhile: the barrier at
-// a stage's end orders both).  2048 x 8192 x 28672: 545 us, 1.76 POP/s (a large
+// ---- Large products: tiles of BM x BN by 2 x WN waves, 64 k a stage.  The
+// rows' blocks of a stage come in by 16-byte loads (WN blocks a load of the
+// workgroup), wait in registers, kAhead stages early, and go to one of three
+// LDS buffers as they are, so every LDS access is 1 KB of adjacent bytes; the
+// columns' blocks go straight to the operand registers of the two waves that
+// need them (through LDS as well: 570 us, 512 rows 19.6 us against 19.1).  A
+// wave reads the rows of the next 32 k while it multiplies these, across stages
+// too (the stage after next is being written meanwhile: the barrier at a
+// stage's end orders both).  2048 x 8192 x 28672: 546 us, 1.76 POP/s (a large
 // library product of 8-bit integers reaches 2.1 here): the matrix cores are
 // busy 38 % of the time at the 2 GHz they run at, the rest waits at the stages'
-// barriers and for LDS; 256 x 256 tiles with one wave a SIMD: 620.
+// barriers and for operands; with both through LDS, 256 x 256 tiles with one
+// wave a SIMD took 620, and 128 k a stage 725.
 template <typename T, int BM, int BN, int WN>
 __global__ __launch_bounds__(128 * WN, WN / 2) void qmm_a8_tile_kernel(const Args g) {
     constexpr int PA = BM / 32, PB = BN / 32;       // blocks of a stage
     constexpr int MT = BM / 64, NT = BN / WN / 32;  // a wave's 32 x 32 tiles
-    constexpr int LA = PA / WN, LB = PB / WN;       // loads of a stage, WN blocks each
-    constexpr int kAhead = WN == 2 ? 3 : 6;
-    constexpr int kStage = (PA + PB) * kBlockBytes;
+    constexpr int LA = PA / WN;                     // loads of a stage's rows, WN blocks each
+    constexpr int kAhead = WN == 2 ? 3 : 4;
+    constexpr int kStage = PA * kBlockBytes;
     __shared__ __align__(16) int8_t lds[3 * kStage];
     const int tiles_n = (g.panels + PB - 1) / PB, tiles_m = (g.row_blocks + PA - 1) / PA;
     // Workgroups go to the XCDs in turn: an XCD's are the row tiles of every
@@ -330,30 +333,38 @@ __global__ __launch_bounds__(128 * WN, WN / 2) void qmm_a8_tile_kernel(const Arg
     const __amdgpu_buffer_rsrc_t brs = buffer_rsrc(g.w + static_cast<int64_t>(tn) * PB * pitch,
                                                    static_cast<uint32_t>(min(PB, g.panels - tn * PB)) * pitch);
     const uint32_t from = static_cast<uint32_t>(tid >> 7) * pitch + static_cast<uint32_t>(tid & 127) * 16;
-    struct Stage {
-        u32x4 a[LA], b[LB];
+    struct Rows {
+        u32x4 v[LA];
     };
-    const auto load = [&](int stage, Stage& t) {
-        const uint32_t o = stage < g.steps ? from + static_cast<uint32_t>(stage) * kBlockBytes : 0x80000000u;
-#pragma unroll
-        for (int u = 0; u < LA; ++u) t.a[u] = buffer_load16(ars, o + WN * u * pitch);
-#pragma unroll
-        for (int u = 0; u < LB; ++u) t.b[u] = buffer_load16(brs, o + WN * u * pitch);
+    struct Columns {
+        i32x4 v[2][NT];
     };
-    const auto store = [&](const Stage& t, int8_t* to) {
-#pragma unroll
-        for (int u = 0; u < LA; ++u) *reinterpret_cast<u32x4*>(to + u * WN * kBlockBytes + tid * 16) = t.a[u];
-#pragma unroll
-        for (int u = 0; u < LB; ++u) *reinterpret_cast<u32x4*>(to + (PA + WN * u) * kBlockBytes + tid * 16) = t.b[u];
+    const auto at = [&](int stage) {
+        return stage < g.steps ? static_cast<uint32_t>(stage) * kBlockBytes : 0x80000000u;
     };
-    i32x4 fa[2][MT], fb[2][NT];   // operands of this and the next 32 k
+    const auto load_rows = [&](int stage, Rows& t) {
+        const uint32_t o = at(stage) + from;
+#pragma unroll
+        for (int u = 0; u < LA; ++u) t.v[u] = buffer_load16(ars, o + WN * u * pitch);
+    };
+    const uint32_t column = static_cast<uint32_t>(wc * NT) * pitch + lane * 16;
+    const auto load_columns = [&](int stage, Columns& t) {
+        const uint32_t o = at(stage) + column;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+                t.v[h][n] = __builtin_bit_cast(i32x4, buffer_load16(brs, o + n * pitch + 1024 * h));
+    };
+    const auto store = [&](const Rows& t, int8_t* to) {
+#pragma unroll
+        for (int u = 0; u < LA; ++u) *reinterpret_cast<u32x4*>(to + u * WN * kBlockBytes + tid * 16) = t.v[u];
+    };
+    i32x4 fa[2][MT];   // rows of this and the next 32 k
     const auto fetch = [&](const int8_t* stage, int h) {
         const int8_t* la = stage + wr * MT * kBlockBytes + h * 1024 + lane * 16;
-        const int8_t* lb = stage + (PA + wc * NT) * kBlockBytes + h * 1024 + lane * 16;
 #pragma unroll
         for (int i = 0; i < MT; ++i) fa[h][i] = *reinterpret_cast<const i32x4*>(la + i * kBlockBytes);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) fb[h][n] = *reinterpret_cast<const i32x4*>(lb + n * kBlockBytes);
     };
     i32x16 acc[MT][NT];
 #pragma unroll
@@ -362,34 +373,41 @@ __global__ __launch_bounds__(128 * WN, WN / 2) void qmm_a8_tile_kernel(const Arg
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][n][e] = 0;
-    const auto multiply = [&](int h) {
+    const auto multiply = [&](int h, const Columns& t) {
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int n = 0; n < NT; ++n)
-                acc[i][n] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[h][i], fb[h][n], acc[i][n], 0, 0, 0);
+                acc[i][n] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[h][i], t.v[h][n], acc[i][n], 0, 0, 0);
     };
 
-    Stage ring[kAhead];
+    Rows rows[kAhead];
+    Columns columns[kAhead];
     {
-        Stage t0, t1;
-        load(0, t0);
-        load(1, t1);
+        Rows t0, t1;
+        load_rows(0, t0);
+        load_rows(1, t1);
 #pragma unroll
-        for (int d = 0; d < kAhead; ++d) load(2 + d, ring[d]);
+        for (int d = 0; d < kAhead; ++d) {
+            load_columns(d, columns[d]);
+            load_rows(2 + d, rows[d]);
+        }
         store(t0, lds);
         store(t1, lds + kStage);
     }
     __syncthreads();
     int8_t *now = lds, *next = lds + kStage, *after = lds + 2 * kStage;
     fetch(now, 0);
-    const auto advance = [&](int stage, Stage& t, bool more) {
+    const auto advance = [&](int stage, Columns& c, Rows& t, bool more) {
         fetch(now, 1);
-        multiply(0);
+        multiply(0, c);
         store(t, after);   // stage + 2
-        if (more) load(stage + 2 + kAhead, t);
         fetch(next, 0);
-        multiply(1);
+        multiply(1, c);
+        if (more) {
+            load_columns(stage + kAhead, c);
+            load_rows(stage + 2 + kAhead, t);
+        }
         __syncthreads();
         int8_t* first = now;
         now = next;
@@ -399,11 +417,11 @@ __global__ __launch_bounds__(128 * WN, WN / 2) void qmm_a8_tile_kernel(const Arg
     int stage = 0;
     for (; stage + kAhead <= g.steps; stage += kAhead) {
 #pragma unroll
-        for (int d = 0; d < kAhead; ++d) advance(stage + d, ring[d], true);
+        for (int d = 0; d < kAhead; ++d) advance(stage + d, columns[d], rows[d], true);
     }
 #pragma unroll
     for (int d = 0; d < kAhead - 1; ++d)
-        if (stage + d < g.steps) advance(stage + d, ring[d], false);
+        if (stage + d < g.steps) advance(stage + d, columns[d], rows[d], false);
     // Element e of lane l: row 8 (e / 4) + 4 (l / 32) + e % 4, column l % 32.
     // All the scales first: a load between two stores would wait for them.
     float as[MT][16], ws[NT];
@@ -440,7 +458,8 @@ Plan plan(int64_t rows, int64_t k, int64_t n) {
     // Large outputs: 128 x 128 tiles through LDS, with eight waves a tile where
     // there is not one for each compute unit (512 x 5632 outputs: 20.3 us
     // against 22.2 with four and 21.4 without LDS; 1000 x 5632: 31.6 with four,
-    // 34.4 with eight, 35.5 without; 1000 x 2048: 18.6 without, 20.9 with eight).
+    // 34.4 with eight, 35.5 without; 1000 x 2048: 18.6 without, 20.9 with eight;
+    // measured with both operands in LDS, which costs 2-3 % more).
     const int64_t tiles = (rows + 127) / 128 * ((n + 127) / 128);
     p.wn = rows <= 128 || tiles < 160 ? 0 : tiles < 256 ? 4 : 2;
     p.mb = rb <= 1 ? 1 : rb <= 2 ? 2 : 4;
