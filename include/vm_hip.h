@@ -786,7 +786,10 @@ int vm_hip_kv_q8_keep(const vm_hip_kv_q8* cache, const int32_t* pos, const int32
  * Scores, maxima, sums and the output are accumulated in fp32; what is
  * rounded before: with fp32 queries, the query and each weight to 22
  * significant bits (two fp16 parts); with 16-bit queries, each weight to fp16
- * (codes and queries are exact).
+ * (codes and queries are exact).  A weight times its value's scale is held to
+ * no less than 2^-28 of the largest such product of its row (of the rows seen
+ * that kv_q8_append has not stored as zeros): a row's output does not depend
+ * on the size of values that it does not see.
  *
  * workspace: vm_hip_attention_q8_workspace_bytes bytes of device memory (0 is
  * possible: then workspace may be NULL), 16-byte aligned and zeroed before its

@@ -27,8 +27,16 @@
 // Widening: code ^ 0x80 behind the byte 0x64 is fp16 1152 + code, one packed
 // subtraction away.
 //
-// Weights meet fp16 as p sv 2^(8 - E), 2^E above the largest sv seen and p
-// below 2^7: what the second part cannot hold is below 2^-32 of the largest.
+// Weights meet fp16 as p sv 2^(8 - E + u), p below 2^7: 2^E is above the scales of
+// the values that the wave's rows have seen, and u is a row's own.  While all
+// scales that a row may have taken its reference from are 2^(E - 5) at least (and
+// are no zeros' scale, 1), u is 0, and the wave keeps nothing for it.  From then
+// on (`wide`) a row's largest p sv is known, of keys that it sees and that hold
+// more than zeros, and u puts it near 2^8.  What fp16 (its second part, of fp32
+// calls) cannot hold is below 2^-28 of the row's largest p sv either way, whatever
+// the other rows see.  (With one unit for all a wave's rows, from all its keys,
+// values were lost beside rows of zeros and beside large values that a row does
+// not see; the units cost 2 us of 58 for 1000 rows behind 3001.)
 //
 // A workgroup of four waves takes 16 RT query rows and a share of the keys;
 // its waves take turns at 32-key blocks, the next block's codes in registers
@@ -109,6 +117,16 @@ __device__ __forceinline__ half2v widen_high(uint32_t u) {
 }
 __device__ __forceinline__ half8 join(half2v a, half2v b, half2v c, half2v d) {
     return half8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
+// Bits of the 16 lanes lr of a lane's group joined.
+__device__ __forceinline__ uint32_t join_rows(uint32_t v) {
+    int x = static_cast<int>(v);
+    x |= __builtin_amdgcn_update_dpp(0, x, 0x121, 0xf, 0xf, false);   // row_ror:1
+    x |= __builtin_amdgcn_update_dpp(0, x, 0x122, 0xf, 0xf, false);
+    x |= __builtin_amdgcn_update_dpp(0, x, 0x124, 0xf, 0xf, false);
+    x |= __builtin_amdgcn_update_dpp(0, x, 0x128, 0xf, 0xf, false);
+    return static_cast<uint32_t>(x);
 }
 
 // Maximum and sum over the lanes of a row's four groups (lanes lr + 16 g).
@@ -226,7 +244,9 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
     // A weight may exceed 1 by this much (log2) before its row's reference moves:
     // with one unit some row of a wave moved in most blocks.
     constexpr float kHeadroom = 7.0f;
-    constexpr int kUnit = 8;               // weights in units of 2^(E - kUnit): below 2^15
+    constexpr int kUnit = 8;               // weights in units of 2^(E - kUnit - u): below 2^15
+    constexpr int kNear = 4;               // scales from 2^(E - 5) up need no u
+    constexpr float kUnset = -3e38f;       // limit of a row that has a reference and no weight yet
     __shared__ __align__(16) float scales_lds[kWaves][2 * kBlock];
     __shared__ __align__(16) float merge_o[kWaves][kRows * D];
     __shared__ float merge_m[kWaves][kRows], merge_l[kWaves][kRows];
@@ -330,10 +350,13 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
         start[rt] = kTwo ? 0.0f : -1152.0f * sum_groups(sum);
     }
 
-    f32x4 acc[RT][ND];   // O^T[dim ND (4 lg + e) + db][row lr] 2^(kUnit - v_exp)
+    f32x4 acc[RT][ND];   // O^T[dim ND (4 lg + e) + db][row lr] 2^(kUnit - v_exp + u)
     float m_run[RT];     // the score (less the row's factor) that weighs 1
     float limit[RT];     // how far a score may pass it (log2); -inf before the first key
     float l_run[RT];     // sum of this lane's keys' weights
+    // Of a row, where scales lie far apart (`wide`); in LDS until the merge needs the place:
+    float* e_run = merge_m[wave] + lr;   // [16 rt] log2 of the row's largest p sv; -inf: none
+    float* unit = merge_l[wave] + lr;    // [16 rt] 2^u
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
@@ -341,7 +364,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
         m_run[rt] = l_run[rt] = 0.0f;
         limit[rt] = -INFINITY;
     }
-    int v_exp = -200;   // E
+    int v_exp = -200;       // E
+    int lowest = 200;       // the smallest scales (log2) of blocks in which a reference moved
+    bool wide = false;      // scales lie far apart, or there may be rows of zeros
+    bool shifted = false;   // some row of the wave has another u than 0
 
     // kMasked: some row does not see the whole block (or the block ends past the
     // cache).  Two copies of the code: the masks cost a quarter of a block's time.
@@ -379,9 +405,9 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
         // the weights' unit has to move: rarely, after the first blocks.
         uint32_t sees[RT];   // bit j: the row sees key k0 + 8 lg + j
         float mt[RT];
-        float top = sv[0];   // (NaN is skipped)
+        float top = fabsf(sv[0]);   // (NaN is skipped)
 #pragma unroll
-        for (int j = 1; j < 8; ++j) top = fmaxf(top, sv[j]);
+        for (int j = 1; j < 8; ++j) top = fmaxf(top, fabsf(sv[j]));
         bool moves = top == top && exponent_above(top) > v_exp;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
@@ -415,10 +441,54 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
             moves = moves || mt[rt] * row_factor[rt] > limit[rt];
         }
         if (__any(moves)) {
-            top = max_groups(top);
-            const int e_new = top == top ? max(v_exp, exponent_above(top)) : v_exp;
-            const float grown = ldexpf(1.0f, v_exp - e_new);
+            uint32_t seen_by = 0xffu;   // keys that some row of the wave sees
+            if (kMasked) {
+                seen_by = sees[0];
+#pragma unroll
+                for (int rt = 1; rt < RT; ++rt) seen_by |= sees[rt];
+                seen_by = join_rows(seen_by);
+            }
+            const auto above_all = [&]() {   // E with this block's keys
+                float most = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (!kMasked || (seen_by >> j & 1)) most = fmaxf(most, fabsf(sv[j]));
+                return __builtin_amdgcn_readfirstlane(max(v_exp, exponent_above(max_groups(most))));
+            };
+            int e_new = above_all();
+            if (!wide) {
+                float least = INFINITY;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (!kMasked || (seen_by >> j & 1)) least = fminf(least, fabsf(sv[j]));
+                lowest = __builtin_amdgcn_readfirstlane(min(lowest, exponent_above(-max_groups(-least))));
+                if (lowest < e_new - kNear || (e_new >= 1 && e_new <= 1 + kNear)) {
+                    wide = true;
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) {
+                        e_run[16 * rt] = limit[rt] == -INFINITY ? -INFINITY : static_cast<float>(v_exp - kNear);
+                        unit[16 * rt] = 1.0f;
+                    }
+                }
+            }
+            if (wide) {   // keys of zeros count for nothing
+                uint32_t holds = 0;   // bit j: key 8 lg + j has another code than 0
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    uint32_t bits = c.v[j][0];
+#pragma unroll
+                    for (int u = 1; u < ND / 4; ++u) bits |= c.v[j][u];
+                    holds |= bits ? 1u << j : 0u;
+                }
+                holds = join_rows(holds);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (!(holds >> j & 1) && sv[j] == sv[j]) sv[j] = 0.0f;
+                e_new = above_all();
+            }
+            const int drop = e_new - v_exp;
             v_exp = e_new;
+            bool any_unit = false;
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 const float most = max_groups(mt[rt]);
@@ -431,30 +501,57 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
                 l_run[rt] *= fall;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) st[rt][j / 4][j % 4] -= up;
+                int more = -drop;   // log2 of what the row's outputs grow by for their units
+                if (wide) {
+                    float w = -INFINITY;   // log2 of the row's largest p sv of this block
 #pragma unroll
-                for (int db = 0; db < ND; ++db) acc[rt][db] *= fall * grown;
+                    for (int j = 0; j < 8; ++j)
+                        if (!kMasked || (sees[rt] >> j & 1))
+                            w = fmaxf(w, fmaf(st[rt][j / 4][j % 4], row_factor[rt], __builtin_amdgcn_logf(fabsf(sv[j]))));
+                    float e = e_run[16 * rt];
+                    if (seen) e = fmaxf(e - up * row_factor[rt], max_groups(w));
+                    e_run[16 * rt] = e;
+                    const bool none = e == -INFINITY;
+                    e += static_cast<float>(kUnit - v_exp);
+                    const int u = none || (e >= kUnit - kNear && e <= kUnit + kNear) ? 0 : kUnit - static_cast<int>(ceilf(fmaxf(e, -100.0f)));
+                    more += u + 1 - exponent_above(unit[16 * rt]);
+                    unit[16 * rt] = ldexpf(1.0f, u);
+                    any_unit |= u != 0;
+                    if (limit[rt] > -INFINITY) limit[rt] = none ? kUnset : kHeadroom - static_cast<float>(max(u, 0));
+                }
+                const float scaled = ldexpf(fall, more);
+#pragma unroll
+                for (int db = 0; db < ND; ++db) acc[rt][db] *= scaled;
             }
+            shifted = __any(any_unit);
         }
         float su[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) su[j] = ldexpf(sv[j], kUnit - v_exp);
         half8 pf[RT][NP];
+        const auto weigh = [&](auto shifted_tag) {
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
+            for (int rt = 0; rt < RT; ++rt) {
+                const float row_unit = decltype(shifted_tag)::value ? unit[16 * rt] : 1.0f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float p = __builtin_amdgcn_exp2f(st[rt][j / 4][j % 4] * row_factor[rt]);
-                float x = p * su[j];
-                if (kMasked && !(sees[rt] >> j & 1)) p = x = 0.0f;   // (whatever the factor and the scale are)
-                l_run[rt] += p;
-                // (Both parts have to come from one rounding of x: folded into its
-                // product, the first part's conversion would round another value.)
-                if (kTwo) asm("" : "+v"(x));
-                const _Float16 hi = static_cast<_Float16>(x);
-                pf[rt][0][j] = hi;
-                if (kTwo) pf[rt][NP - 1][j] = static_cast<_Float16>(x - static_cast<float>(hi));
+                for (int j = 0; j < 8; ++j) {
+                    float p = __builtin_amdgcn_exp2f(st[rt][j / 4][j % 4] * row_factor[rt]);
+                    float x = decltype(shifted_tag)::value ? p * row_unit * su[j] : p * su[j];
+                    if (kMasked && !(sees[rt] >> j & 1)) p = x = 0.0f;   // (whatever the factor and the scale are)
+                    l_run[rt] += p;
+                    // (Both parts have to come from one rounding of x: folded into its
+                    // product, the first part's conversion would round another value.)
+                    if (kTwo) asm("" : "+v"(x));
+                    const _Float16 hi = static_cast<_Float16>(x);
+                    pf[rt][0][j] = hi;
+                    if (kTwo) pf[rt][NP - 1][j] = static_cast<_Float16>(x - static_cast<float>(hi));
+                }
             }
-        }
+        };
+        if (shifted)
+            weigh(std::true_type{});
+        else
+            weigh(std::false_type{});
         // V^T: four dim tiles from four adjacent codes of eight keys.
 #pragma unroll
         for (int d4 = 0; d4 < ND / 4; ++d4) {
@@ -508,6 +605,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         const float l = sum_groups(l_run[rt]);
+        const int back = v_exp - kUnit + (wide ? 1 - exponent_above(unit[16 * rt]) : 0);
         float* d = merge_o[wave] + (16 * rt + lr) * D + 4 * ND * lg;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -515,7 +613,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
             for (int u = 0; u < ND / 4; ++u) {
                 float y[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) y[i] = ldexpf(acc[rt][4 * u + i][e], v_exp - kUnit);
+                for (int i = 0; i < 4; ++i) y[i] = ldexpf(acc[rt][4 * u + i][e], back);
                 store4(d + ND * e + 4 * u, y);
             }
         if (lg == 0) {
