@@ -101,19 +101,15 @@ struct Args {
 // log2 of the power of two just above v (v >= 0 finite; 0 and subnormals: -126).
 __device__ __forceinline__ int exponent_above(float v) { return static_cast<int>(__float_as_uint(v) >> 23) - 126; }
 
-// Bytes 0, 1 (2, 3) of u = code ^ 0x80 as two fp16 codes, or 1152 more.
-template <bool kExact = true>
+// Bytes 0, 1 (2, 3) of u = code ^ 0x80 as two fp16 codes.
 __device__ __forceinline__ half2v widen_bits(uint32_t bits) {
-    const half2v v = __builtin_bit_cast(half2v, bits);
-    return kExact ? v - half2v{static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)} : v;
+    return __builtin_bit_cast(half2v, bits) - half2v{static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
 }
-template <bool kExact = true>
 __device__ __forceinline__ half2v widen_low(uint32_t u) {
-    return widen_bits<kExact>(__builtin_amdgcn_perm(0x64646464u, u, 0x04010400u));
+    return widen_bits(__builtin_amdgcn_perm(0x64646464u, u, 0x04010400u));
 }
-template <bool kExact = true>
 __device__ __forceinline__ half2v widen_high(uint32_t u) {
-    return widen_bits<kExact>(__builtin_amdgcn_perm(0x64646464u, u, 0x04030402u));
+    return widen_bits(__builtin_amdgcn_perm(0x64646464u, u, 0x04030402u));
 }
 __device__ __forceinline__ half8 join(half2v a, half2v b, half2v c, half2v d) {
     return half8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
@@ -304,11 +300,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
 
     // Q^T operands: Q[row][64 h + 16 lg + 8 s + j] in qf[.][.][2 h + s], scaled by
     // the power of two that puts the row's largest magnitude in [2^13, 2^14).
-    // One-part queries meet codes that are still 1152 too large (a subtraction
-    // less for each pair), and their scores start 1152 sum(Q) too low: that costs
-    // the fp32 sums 1152 / |code| of their precision, which 16 bits do not see.
     half8 qf[RT][NP][NC];
-    float start[RT];
     float row_factor[RT];   // of a score's log2
     int token[RT];          // -1: no row
 #pragma unroll
@@ -336,7 +328,6 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
         const bool finite = m < 0x7f800000u;
         const int up = 14 - exponent_above(__uint_as_float(m));
         row_factor[rt] = finite ? ldexpf(a.scale * 1.44269504f, -up) : NAN;
-        float sum = 0.0f;
 #pragma unroll
         for (int h = 0; h < H; ++h)
 #pragma unroll
@@ -345,9 +336,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
                 const _Float16 hi = static_cast<_Float16>(v);
                 qf[rt][0][2 * h + e / 8][e % 8] = hi;
                 if (kTwo) qf[rt][NP - 1][2 * h + e / 8][e % 8] = static_cast<_Float16>(v - static_cast<float>(hi));
-                sum += static_cast<float>(hi);
             }
-        start[rt] = kTwo ? 0.0f : -1152.0f * sum_groups(sum);
     }
 
     f32x4 acc[RT][ND];   // O^T[dim ND (4 lg + e) + db][row lr] 2^(kUnit - v_exp + u)
@@ -378,7 +367,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
         sl[lane] = c.s;                       // keys' scales, then values'
         f32x4 st[RT][2];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) st[rt][0] = st[rt][1] = f32x4{start[rt], start[rt], start[rt], start[rt]};
+        for (int rt = 0; rt < RT; ++rt) st[rt][0] = st[rt][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int h = 0; h < H; ++h)
 #pragma unroll
@@ -386,7 +375,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
 #pragma unroll
                 for (int bt = 0; bt < 2; ++bt) {
                     const uint32_t u0 = c.k[bt][h][2 * s] ^ 0x80808080u, u1 = c.k[bt][h][2 * s + 1] ^ 0x80808080u;
-                    const half8 kf = join(widen_low<kTwo>(u0), widen_high<kTwo>(u0), widen_low<kTwo>(u1), widen_high<kTwo>(u1));
+                    const half8 kf = join(widen_low(u0), widen_high(u0), widen_low(u1), widen_high(u1));
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
