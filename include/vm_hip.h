@@ -860,7 +860,9 @@ int vm_hip_qmm_a8(const void* staged, const void* packed, const float* scale, vo
  * rounded once to dtype, and tokens [seqs, rows] (int32, or NULL) the lowest
  * index of the largest fp32 x, NaN skipped, or -1 where no token has more
  * than -infinity.  Rows t >= counts[s] (int32 per sequence, or NULL: all
- * rows count) are padding: nothing of theirs is written.
+ * rows count) are padding: nothing of theirs is written, and their nodes are
+ * on no row's path (their bits of the tree are ignored, as vm_hip_attention_q8
+ * ignores them).
  *
  * A pointer of the rules that is NULL leaves its rule out (repetition 1,
  * frequency and presence 0, no bias, everything allowed).  Tokens outside

@@ -157,7 +157,8 @@ __global__ __launch_bounds__(kT, 4) void logits_rules_kernel(const Args a) {
     const int range = id % a.ranges;
     id /= a.ranges;
     const int t0 = id % a.groups * RB, seq = id / a.groups;
-    const int n_rows = min((a.counts ? min(a.counts[seq], a.rows) : a.rows) - t0, RB);
+    const int nodes = a.counts ? min(a.counts[seq], a.rows) : a.rows;   // the others are padding
+    const int n_rows = min(nodes - t0, RB);
     if (n_rows <= 0) return;
     const int c0 = static_cast<int>(static_cast<int64_t>(a.chunks) * range / a.ranges);
     const int c1 = static_cast<int>(static_cast<int64_t>(a.chunks) * (range + 1) / a.ranges);
@@ -190,9 +191,9 @@ __global__ __launch_bounds__(kT, 4) void logits_rules_kernel(const Args a) {
     const int first_bias = tid < bias_stride ? bias_tokens[tid] : -1;
     // A thread's (row, node) pairs: the node's token if it lies on the row's
     // path, else one that matches nothing.
-    const int pairs = paths ? n_rows * a.rows : 0;
+    const int pairs = paths ? n_rows * nodes : 0;
     const auto path_token = [&](int pair) {
-        const int r = pair / a.rows, j = pair - r * a.rows;
+        const int r = pair / nodes, j = pair - r * nodes;
         const int token = a.r.drafted[row0 - t0 + j];
         const uint64_t on = a.r.tree ? a.r.tree[(row0 + r) * a.words + j / 64] >> (j & 63) & 1 : j <= t0 + r;
         return on ? token : -1;
@@ -273,7 +274,7 @@ __global__ __launch_bounds__(kT, 4) void logits_rules_kernel(const Args a) {
         for (int pair = tid; pair < pairs; pair += kT) {
             const uint32_t at = place(pair == tid ? first_path : path_token(pair));
             if (at < size) {
-                atomicAdd(&path_lds[pair / a.rows][at], 1);
+                atomicAdd(&path_lds[pair / nodes][at], 1);
                 on_path = 1;
             }
         }
