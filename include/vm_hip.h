@@ -781,12 +781,15 @@ int vm_hip_kv_q8_keep(const vm_hip_kv_q8* cache, const int32_t* pos, const int32
  * scale <= 0 means 1/sqrt(head_dim).  A token that sees no row gives zeros.
  * Cache rows at or past max_seq do not exist; a token whose own row does not
  * (kv_q8_append left its q alone) gets unspecified values.  Scores have to stay
- * below 2^112 in magnitude.  batch * kv_heads times the 16-row tiles of rows *
+ * below 2^112 in magnitude, the keys' scales below 2^98 and the values' below
+ * 2^88 (sums of products before the queries' size and the sum of the weights
+ * are divided out are fp32 too).  batch * kv_heads times the 16-row tiles of rows *
  * heads / kv_heads rows is below 2^24 (2^28 rows in all).
  * Scores, maxima, sums and the output are accumulated in fp32; what is
  * rounded before: with fp32 queries, the query and each weight to 22
  * significant bits (two fp16 parts); with 16-bit queries, each weight to fp16
- * (codes and queries are exact).  A weight times its value's scale is held to
+ * (codes and queries are exact).  A query's values are held to no less than
+ * 2^-38 of the largest of its row.  A weight times its value's scale is held to
  * no less than 2^-28 of the largest such product of its row (of the rows seen
  * that kv_q8_append has not stored as zeros): a row's output does not depend
  * on the size of values that it does not see.

@@ -175,3 +175,16 @@ def test_rows_of_zeros_that_take_nearly_all_the_weight(hip, shape, d, dtype, siz
     cache.host["v_codes"][:, :, 7], cache.host["v_scales"][:, :, 7] = 0, 1.0
     print(f"case attention_q8 zeros' weight {shape} d={d} dtype={dtype} size={size}", flush=True)
     check(hip, cache, q, dtype, pos, None, 0.1)
+
+
+@pytest.mark.parametrize("d,dtype", [(64, 0), (64, 5), (128, 0), (128, 5)])
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_largest_scales(hip, shape, d, dtype):
+    # keys' scales up to 2^98 under queries so small that scores are ordinary
+    # ones, values' scales up to 2^88
+    cache, q = make(hip, shape, d, dtype, 27)
+    cache.host["k_scales"] = np.ldexp(np.minimum(cache.host["k_scales"] * 50, np.float32(0.999)), 98)
+    cache.host["v_scales"] = np.ldexp(np.minimum(cache.host["v_scales"] * 50, np.float32(0.999)), 88)
+    q = np.ldexp(q, -105)
+    print(f"case attention_q8 largest scales {shape} d={d} dtype={dtype}", flush=True)
+    check(hip, cache, q, dtype, shape[4], None, 0.1)
