@@ -46,12 +46,13 @@
 // one that draws the last ticket merges.
 //
 // MI355X, passes back to back: 32 tokens over ragged caches of up to 8000, 64
-// heads of 128, bf16: 86 us, 4.7 TB/s of codes and scales (HBM: a large copy
-// reaches 4.8); 1000 rows of 32 heads of 64 behind 3001 cached, f16: 55 us, 520
-// TFLOP/s; 24 nodes of 64 heads of 128 over 131000, bf16: 180 us, 570 TFLOP/s
-// (VALU: widening and softmax, about 340 instructions beside 32 MFMAs a block of
-// 32 keys x 32 rows); one token of 32 heads over 2000: 7.3 us, 16 nodes: 7.9
-// (the chain position - codes - LDS merge - ticket - join).
+// heads of 128, bf16: 88 us, 4.6 TB/s of codes and scales (HBM: a large copy
+// reaches 4.8 to 5.4); 1000 rows of 32 heads of 64 behind 3001 cached, f16: 58 us,
+// 490 TFLOP/s, f32: 90 us; 24 nodes of 64 heads of 128 over 131000, bf16: 194 us,
+// 530 TFLOP/s (VALU: widening and softmax, ten to twelve instructions beside an
+// MFMA, the matrix cores busy 17 to 20 % of the cycles); one token of 32 heads over
+// 2000: 7.6 us, 16 nodes: 8.2 (the chain position - codes - LDS merge - ticket -
+// join).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -528,6 +529,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
                     float x = decltype(shifted_tag)::value ? p * row_unit * su[j] : p * su[j];
                     if (kMasked && !(sees[rt] >> j & 1)) p = x = 0.0f;   // (whatever the factor and the scale are)
                     l_run[rt] += p;
+                    // 16-bit calls: one part, 2^-12 of the weight, as fp16 outputs are
+                    // rounded (another part would double the second product's MFMAs).
                     // (Both parts have to come from one rounding of x: folded into its
                     // product, the first part's conversion would round another value.)
                     if (kTwo) asm("" : "+v"(x));

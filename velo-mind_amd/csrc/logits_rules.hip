@@ -12,9 +12,10 @@
 // thread keeps its best value of each row; at the end the workgroup's best go
 // to the workspace, and the last workgroup of a row (atomic ticket) reduces
 // the candidates, lowest index on ties.  64 x 128256 fp32 behind 6000 tokens of
-// history: 25.4 us, 2.6 TB/s (instructions and waiting in turn; with twice the
-// history in registers three workgroups fit a compute unit instead of four:
-// 29.2); 1 x 32000: 6.6 us (the chain lists - LDS - biases - ticket).
+// history: 25 us, 2.6 TB/s (waves wait 60 % of their time, VALU instructions are 10
+// us of it; with twice the history in registers three workgroups fit a compute
+// unit instead of four: 29.2); 1 x 32000: 6.6 us (the chain lists - LDS - biases -
+// ticket).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -55,9 +55,11 @@ __global__ __launch_bounds__(kT) void a8_pack_kernel(const int8_t* __restrict__ 
 
 // ---- Activations: a workgroup a row, 16 adjacent values a lane and chunk, read
 // once (the first kHeld chunks of a lane wait in registers for the maximum).
-// 16 x 2048 fp32 2.6 us, 512 x 2048 4.2-4.8, 2048 x 8192 bf16 20 (50 MB: HBM at half
-// its rate; with codes gathered in LDS, so that 64 adjacent bytes are written
-// instead of 16, it took as long there and half as long again at 512 rows).
+// 16 x 2048 fp32 3.1 us, 512 x 2048 3.3-4.8, 2048 x 8192 bf16 19-21 (50 MB: 2.5 TB/s.
+// About 20 VALU instructions a value, the rounding half away from zero among them,
+// are 10 us of it, and a row's loads, maximum and stores follow one another; with
+// codes gathered in LDS, so that 64 adjacent bytes are written instead of 16, it
+// took as long there and half as long again at 512 rows).
 template <typename T>
 __device__ __forceinline__ void load16(const T* p, int valid, float (&x)[16]);
 template <>
@@ -192,10 +194,9 @@ __device__ __forceinline__ void epilogue4(const Args& g, int64_t row, int64_t co
 // registers (a wave's loads of a step are 1 KB each), and their sums meet in
 // LDS.  Where the tiles are few, several workgroups share a tile's k range,
 // store their sums in the workspace and the last one adds them (integers: the
-// order does not matter).  16 x 2048 x 5632: 5.5 us (2.1 TB/s of weights: the
-// chain of loads and LDS); 4 x 8192 x 28672: 54 with the staging, 4.4
-// TB/s; more steps in flight a wave: slower (512 rows 21.4 -> 28.4 with three: L2
-// delivers 12 TB/s and is what bounds it).
+// order does not matter).  16 x 2048 x 5632: 5.5 us (2.1 TB/s of weights; its
+// waves wait for loads 81 % of their time, a step's after the other's); 4 x 8192 x
+// 28672: 40 us (5.9 TB/s, repeated: part of the weights come from the last cache).
 template <typename T, int MB>
 __global__ __launch_bounds__(kT) void qmm_a8_kernel(const Args g) {
     __shared__ __align__(16) int sums[3][MB * 32 * 32];
@@ -303,9 +304,10 @@ __global__ __launch_bounds__(kT) void qmm_a8_kernel(const Args g) {
 // too (the stage after next is being written meanwhile: the barrier at a
 // stage's end orders both).  2048 x 8192 x 28672: 546 us, 1.76 POP/s (a large
 // library product of 8-bit integers reaches 2.1 here): the matrix cores are
-// busy 38 % of the time at the 2 GHz they run at, the rest waits at the stages'
-// barriers and for operands; with both through LDS, 256 x 256 tiles with one
-// wave a SIMD took 620, and 128 k a stage 725.
+// busy 44 % of the cycles, the rest waits at the stages' barriers and for
+// operands (512 x 2048 x 5632, tiles for two of three compute units: 16 us, 10 %);
+// with both through LDS, 256 x 256 tiles with one wave a SIMD took 620, and 128 k a
+// stage 725.
 template <typename T, int BM, int BN, int WN>
 __global__ __launch_bounds__(128 * WN, WN / 2) void qmm_a8_tile_kernel(const Args g) {
     constexpr int PA = BM / 32, PB = BN / 32;       // blocks of a stage
@@ -456,10 +458,11 @@ Plan plan(int64_t rows, int64_t k, int64_t n) {
     Plan p;
     const int64_t rb = blocks32(rows);
     // Large outputs: 128 x 128 tiles through LDS, with eight waves a tile where
-    // there is not one for each compute unit (512 x 5632 outputs: 20.3 us
-    // against 22.2 with four and 21.4 without LDS; 1000 x 5632: 31.6 with four,
-    // 34.4 with eight, 35.5 without; 1000 x 2048: 18.6 without, 20.9 with eight;
-    // measured with both operands in LDS, which costs 2-3 % more).
+    // there is not one for each compute unit.  With the staging, k = 2048, us with
+    // eight waves, with four, without LDS: 300 x 5632 (132 tiles) 18.9, 20.4, 19.9;
+    // 512 x 5632 (176) 20.7, 22.0, 22.3; 1000 x 2048 (128) 20.5, 22.1, 17.8; 2000 x
+    // 2048 (256) 26.7, 27.1, 30.5; 700 x 5632 (264) 32.5, 28.4, 29.8; 1000 x 5632
+    // (352) 34.9, 30.9, 35.1.
     const int64_t tiles = (rows + 127) / 128 * ((n + 127) / 128);
     p.wn = rows <= 128 || tiles < 160 ? 0 : tiles < 256 ? 4 : 2;
     p.mb = rb <= 1 ? 1 : rb <= 2 ? 2 : 4;
@@ -469,7 +472,8 @@ Plan plan(int64_t rows, int64_t k, int64_t n) {
     // Few tiles: workgroups that fill the GPU twice share the k, as long as a
     // wave keeps five steps (16 x 5632 x 2048: 10.5 us with four, 11.4 with eight,
     // 13.8 with one; 16 x 2048 x 5632: 8.6 with one, 9.3 with three; 32 x 8192 x
-    // 8192: 17.7 with two, 19.6 with one).
+    // 8192: 17.7 with two, 19.6 with one; 16 x 2048 x 256, one workgroup for each
+    // of eight panels: 8.3).
     int64_t s = parts < kMaxTiles ? kMaxTiles / parts : 1;
     s = std::max<int64_t>(std::min<int64_t>({s, kMaxSplits, steps64(k) / 20}), 1);
     p.splits = static_cast<int>(s);
