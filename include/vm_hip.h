@@ -792,7 +792,8 @@ int vm_hip_kv_q8_keep(const vm_hip_kv_q8* cache, const int32_t* pos, const int32
  * 2^-38 of the largest of its row.  A weight times its value's scale is held to
  * no less than 2^-28 of the largest such product of its row (of the rows seen
  * that kv_q8_append has not stored as zeros): a row's output does not depend
- * on the size of values that it does not see.
+ * on the size of values that it does not see, as long as those are below 2^100
+ * times its own.
  *
  * workspace: vm_hip_attention_q8_workspace_bytes bytes of device memory (0 is
  * possible: then workspace may be NULL), 16-byte aligned and zeroed before its
