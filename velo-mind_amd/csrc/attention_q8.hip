@@ -30,15 +30,15 @@
 // Weights meet fp16 as p sv 2^(8 - E + u), p below 2^7: 2^E is above the scales of
 // the values that the wave's rows have seen, and u is a row's own.  While all
 // scales that a row may have taken its reference from are 2^(E - 5) at least (and
-// are no zeros' scale, 1), u is 0, and the wave keeps nothing for it.  From then
+// none is that of zeros, 1), u is 0, and the wave keeps nothing for it.  From then
 // on (`wide`) a row's largest p sv is known, of keys that it sees and that hold
 // more than zeros, and u puts it near 2^8.  What fp16 (its second part, of fp32
 // calls) cannot hold is below 2^-28 of the row's largest p sv either way, whatever
 // the other rows see.  (With one unit for all a wave's rows, from all its keys,
 // values were lost beside rows of zeros and beside large values that a row does
-// not see; the units cost 2 us of 58 for 1000 rows behind 3001.  There a block
-// with a row of zeros beside smaller scales moves them again: one such row in a
-// thousand 62 us, one in ten 113; 32 tokens over up to 8000: 88 and 93.)
+// not see; the units cost 2 us of 58 for 1000 rows behind 3001; with rows of zeros in
+// the cache, which every block is then searched for, that call takes 63 to 68 us,
+// a tree of 24 over 131000 215 to 217.)
 //
 // A workgroup of four waves takes 16 RT query rows and a share of the keys;
 // its waves take turns at 32-key blocks, the next block's codes in registers
@@ -393,6 +393,22 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
             sv[j] = sl[kBlock + 8 * lg + j];
         }
         __builtin_amdgcn_wave_barrier();
+        // Keys of zeros count for nothing.
+        const auto drop_zeros = [&]() {
+            uint32_t holds = 0;   // bit j: key 8 lg + j has another code than 0
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                uint32_t bits = c.v[j][0];
+#pragma unroll
+                for (int u = 1; u < ND / 4; ++u) bits |= c.v[j][u];
+                holds |= bits ? 1u << j : 0u;
+            }
+            holds = join_rows(holds);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (!(holds >> j & 1) && sv[j] == sv[j]) sv[j] = 0.0f;
+        };
+        if (wide) drop_zeros();
         // Scores less the row's reference (and its factor), and whether that or
         // the weights' unit has to move: rarely, after the first blocks.
         uint32_t sees[RT];   // bit j: the row sees key k0 + 8 lg + j
@@ -454,7 +470,12 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
                 for (int j = 0; j < 8; ++j)
                     if (!kMasked || (seen_by >> j & 1)) least = fminf(least, fabsf(sv[j]));
                 lowest = __builtin_amdgcn_readfirstlane(min(lowest, exponent_above(-max_groups(-least))));
-                if (lowest < e_new - kNear || (e_new >= 1 && e_new <= 1 + kNear)) {
+                bool one = false;   // (the scale of a row of zeros)
+                if (e_new >= 1 && e_new <= 1 + kNear) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) one |= sv[j] == 1.0f;
+                }
+                if (lowest < e_new - kNear || __any(one)) {
                     wide = true;
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt) {
@@ -463,19 +484,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_q8_kernel(const Args a)
                     }
                 }
             }
-            if (wide) {   // keys of zeros count for nothing
-                uint32_t holds = 0;   // bit j: key 8 lg + j has another code than 0
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    uint32_t bits = c.v[j][0];
-#pragma unroll
-                    for (int u = 1; u < ND / 4; ++u) bits |= c.v[j][u];
-                    holds |= bits ? 1u << j : 0u;
-                }
-                holds = join_rows(holds);
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (!(holds >> j & 1) && sv[j] == sv[j]) sv[j] = 0.0f;
+            if (wide) {
+                drop_zeros();
                 e_new = above_all();
             }
             const int drop = e_new - v_exp;
