@@ -330,7 +330,7 @@ def _prepare_paged(case, seed):
         H = _hip()
         s["H"], s["out"] = H, torch.empty(rows, heads * d, device=DEV, dtype=dt)
         s["cache"] = H.KvPaged(s["k"].data_ptr(), s["v"].data_ptr(), _CODE[case["dtype"]], pages, page, hk, d)
-        nbytes = H.attention_paged_workspace_bytes(b, rows, heads, hk, d, tables.shape[1] * page)
+        nbytes = H.attention_paged_workspace_bytes(b, rows, case["chunk"], heads, hk, d, tables.shape[1] * page)
         s["ws"] = torch.zeros(max(1, nbytes), device=DEV, dtype=torch.uint8)
     return s
 
@@ -369,8 +369,8 @@ def _run_own(s):
                            s["ws"].data_ptr(), s["ws"].numel())
         return s["out"]
     H.attention_paged(s["cache"], s["tables"].data_ptr(), s["tables"].shape[1], s["q"].data_ptr(), s["out"].data_ptr(),
-                      case["batch"], s["q"].shape[0], heads, s["row_start"].data_ptr(), s["lengths"].data_ptr(), 0.0,
-                      s["ws"].data_ptr(), s["ws"].numel())
+                      case["batch"], s["q"].shape[0], case["chunk"], heads, s["row_start"].data_ptr(),
+                      s["lengths"].data_ptr(), 0.0, s["ws"].data_ptr(), s["ws"].numel())
     return s["out"]
 
 
