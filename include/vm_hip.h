@@ -901,6 +901,198 @@ int vm_hip_logits_rules_apply(const vm_hip_logits_rules* rules, const void* logi
                               int32_t* tokens, int64_t seqs, int64_t rows, int64_t vocab, const int32_t* counts,
                               void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---- A step over requests that share a pool of cache pages (no counterpart
+ * in the reference, which serves one sequence) -------------------------------
+ * A request's tokens lie in pages of page_size tokens (16, 32, 64, 128 or
+ * 256); row b of the block tables [batch, max_pages] (int32) says which: token
+ * t is in page tables[b][t / page_size].  Every call works on the rows of all
+ * requests one behind the other, row_start[b] .. row_start[b + 1] - 1 those of
+ * request b, without padding between them; rows past row_start[batch] are
+ * padding of the call's size and are left as they were.
+ *   vm_hip_kv_paged_plan    says which rows a step has and where they go
+ *   vm_hip_kv_paged_append  norms, rotates and stores a projection's rows
+ *   vm_hip_attention_paged  attends to the pages
+ *   vm_hip_kv_paged_release gives the pages of requests that ended back
+ * All of them read lengths, counts, positions, slots and tables on the device,
+ * so that a captured step replays with others; indices that point outside
+ * (a page id, a slot, a position) are never followed: their rows and keys
+ * count as not there.  At most VM_HIP_PAGED_MAX_BATCH requests and
+ * VM_HIP_PAGED_MAX_ROWS rows a call. */
+#define VM_HIP_PAGED_MAX_BATCH 2048
+#define VM_HIP_PAGED_MAX_ROWS  (1 << 24)
+
+/* The cache: k, v [pages, kv_heads, page_size, head_dim] of dtype (F32, F16 or
+ * BF16), 16-byte aligned.  head_dim is 64 or 128, kv_heads <= 4096, pages *
+ * page_size < 2^31. */
+typedef struct vm_hip_kv_paged {
+    void*   k;
+    void*   v;
+    int     dtype;
+    int64_t pages, page_size, kv_heads, head_dim;
+} vm_hip_kv_paged;
+
+/* One step's plan.  Request b has lengths[b] tokens cached and wants counts[b]
+ * more.  It is admitted, in order of b, unless
+ *   - its lengths or counts are negative or it would be longer than
+ *     max_pages * page_size (later ones go on);
+ *   - its rows, behind those of the requests before it (without the too long
+ *     ones), do not fit `rows` (later ones wait too);
+ *   - it wants more new pages than the requests before it left in the pool
+ *     (it and every later one that wants any wait).
+ * Pages are taken from the end of free_pages (int32 [pages], *free_count of
+ * them valid) and written to the tables' entries behind those in use; nothing
+ * else of the tables changes.
+ *   row_start      int32 [batch + 1]: admitted rows in front of each request
+ *   lengths_out    int32 [batch]: lengths with the admitted rows
+ *   free_count_out int32 [1]
+ *   positions      int32 [rows]: a row's token number in its request; -1: padding
+ *   slots          int32 [rows]: page * page_size + place in the page; -1:
+ *                  padding, or a table entry that is no page
+ * lengths_out may be lengths, and free_count_out free_count; nothing else
+ * overlaps.  All pointers are to device memory; batch == 0 is a no-op.
+ * workspace: vm_hip_kv_paged_plan_workspace_bytes bytes, 16-byte aligned and
+ * zeroed before its first use; every call leaves it zeroed.  Calls that share a
+ * workspace must not overlap. */
+typedef struct vm_hip_page_plan {
+    int64_t batch, rows, max_pages, pages, page_size;
+    const int32_t* lengths;
+    const int32_t* counts;
+    const int32_t* free_pages;
+    const int32_t* free_count;
+    int32_t*       tables;
+    int32_t*       row_start;
+    int32_t*       lengths_out;
+    int32_t*       free_count_out;
+    int32_t*       positions;
+    int32_t*       slots;
+} vm_hip_page_plan;
+int64_t vm_hip_kv_paged_plan_workspace_bytes(int64_t batch, int64_t rows);
+int vm_hip_kv_paged_plan(const vm_hip_page_plan* plan, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The pages of every request with finished[b] != 0 (int32 [batch]) go back to
+ * the end of free_pages, in order of requests and tokens; their tables' entries
+ * become -1, their lengths 0, and *free_count grows (never past `pages`). */
+int vm_hip_kv_paged_release(int64_t batch, int64_t max_pages, int64_t pages, int64_t page_size, const int32_t* finished,
+                            int32_t* lengths, int32_t* tables, int32_t* free_pages, int32_t* free_count, void* stream);
+
+/* ---- Rotary positions ------------------------------------------------------
+ * Tables of the cosines and sines of positions first .. first + rows - 1 for
+ * `dim` rotated elements (even, 2 to 128): cos_table, sin_table [rows, dim / 2]
+ * fp32, entry i of position p = cos(p f_i) and sin(p f_i), times the attention
+ * factor, computed in fp64 (off by at most half a step of fp32 and 2^-40).
+ * f_i = theta^(-2 i / dim), theta > 1, scaled for contexts longer than the
+ * trained one (`original` positions):
+ *   PLAIN   not (scaling may be NULL)
+ *   LINEAR  f_i / factor
+ *   BANDS   by the turns t = original f_i / (2 pi) of a pair in the trained
+ *           length: f_i / factor where t <= low, f_i where t >= high, linear in t
+ *           between
+ *   RAMP    the same, linear in the pair's index i between the pairs that turn
+ *           `high` and `low` times, dim ln(original / (2 pi turns)) / (2 ln
+ *           theta) rounded outwards and held to [0, dim - 1]
+ * Positions are below 2^31. */
+#define VM_HIP_ROPE_PLAIN  0
+#define VM_HIP_ROPE_LINEAR 1
+#define VM_HIP_ROPE_BANDS  2
+#define VM_HIP_ROPE_RAMP   3
+typedef struct vm_hip_rope_scaling {
+    int    kind;
+    double factor;      /* not used by PLAIN                */
+    double low, high;   /* turns, BANDS and RAMP            */
+    double original;    /* positions, BANDS and RAMP        */
+    double attention;   /* what cos and sin are multiplied by */
+} vm_hip_rope_scaling;
+int vm_hip_rope_tables(float* cos_table, float* sin_table, int64_t first, int64_t rows, int64_t dim, double theta,
+                       const vm_hip_rope_scaling* scaling, void* stream);
+
+/* The rotation of a head row's first `dim` elements (even, up to head_dim; 0:
+ * none) by tables of `rows` positions: x_a' = x_a cos - x_b sin, x_b' = x_b cos
+ * + x_a sin for the pairs (a, b) = (i, i + dim / 2) (HALVES) or (2 i, 2 i + 1)
+ * (PAIRS).  Positions past the tables take their last row. */
+#define VM_HIP_ROPE_HALVES 0
+#define VM_HIP_ROPE_PAIRS  1
+typedef struct vm_hip_rope {
+    const float* cos_table;   /* [rows, dim / 2] */
+    const float* sin_table;
+    int64_t      rows, dim;
+    int          layout;
+} vm_hip_rope;
+
+/* The norm of a head row in front of the rotation: x / sqrt(mean(x^2) + eps) *
+ * weight, with weights [head_dim] for query and for key heads. */
+typedef struct vm_hip_qk_norm {
+    const float* q_weight;
+    const float* k_weight;
+    float        eps;
+} vm_hip_qk_norm;
+
+/* A projection's rows qkv [rows, (heads + 2 kv_heads) * head_dim] of the
+ * cache's dtype: query and key heads are normed (norm, or NULL) and rotated
+ * (rope, or NULL) at positions[row], in fp32, rounded once; queries go to
+ * q_out [rows, heads * head_dim], keys and values to the cache's slots[row].
+ * A row with a negative position or a slot outside the cache is padding: nothing
+ * of it is written.  Slots that are given twice get one of the rows.  q_out must
+ * not overlap qkv; both are 16-byte aligned. */
+int vm_hip_kv_paged_append(const vm_hip_kv_paged* cache, const void* qkv, int64_t rows, int64_t heads,
+                           const vm_hip_qk_norm* norm, const vm_hip_rope* rope, const int32_t* positions,
+                           const int32_t* slots, void* q_out, void* stream);
+
+/* The same without a cache, for vm_hip_attention_packed: keys to k_out [rows,
+ * kv_heads * head_dim]; values stay in qkv. */
+int vm_hip_qk_norm_rope(const void* qkv, int dtype, int64_t rows, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                        const vm_hip_qk_norm* norm, const vm_hip_rope* rope, const int32_t* positions, void* q_out,
+                        void* k_out, void* stream);
+
+/* Causal attention of whole prompts that lie one behind the other: row i of
+ * request b (rows row_start[b] + i) sees the request's rows 0 .. i.
+ *   q, k, v  rows of dtype, q_stride, k_stride, v_stride elements apart (each a
+ *            multiple of 16 bytes), query head h at h * head_dim of its row,
+ *            with KV head h / (heads / kv_heads); they may be parts of one
+ *            projection's rows
+ *   out      [rows, heads * head_dim] of dtype; all 16-byte aligned
+ * row_start (int32 [batch + 1] in device memory) is held to [0, rows] and to
+ * rising order.  scale <= 0 means 1/sqrt(head_dim).
+ *
+ * Products, maxima, sums and the output are fp32 (with 16-bit rows, each weight
+ * is rounded to 16 bits for its product with the value; fp32 rows are
+ * multiplied in fp32).  Scores below 2^100 in magnitude.  A key or value that a
+ * row does not see takes no part in it, whatever it holds; a value that is not
+ * finite makes the element not finite in every row that sees it.
+ *
+ * workspace: vm_hip_attention_packed_workspace_bytes bytes (0 is possible: then
+ * it may be NULL), 16-byte aligned and zeroed before its first use; every call
+ * leaves it ready for the next one of any shape it is large enough for.  Calls
+ * that share a workspace must not overlap. */
+int64_t vm_hip_attention_packed_workspace_bytes(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads,
+                                                int64_t head_dim);
+int vm_hip_attention_packed(const void* q, const void* k, const void* v, void* out, int dtype, int64_t q_stride,
+                            int64_t k_stride, int64_t v_stride, int64_t batch, int64_t rows, int64_t heads,
+                            int64_t kv_heads, int64_t head_dim, const int32_t* row_start, float scale, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+
+/* Attention over the pages: decoded tokens, chunks of prompts, and both in one
+ * call.  Request b has lengths[b] tokens cached, this call's n = row_start[b +
+ * 1] - row_start[b] rows the last of them (already appended); row i sees tokens
+ * 0 .. lengths[b] - n + i.
+ *   q    [rows, heads * head_dim] of the cache's dtype, out the same; both 16-byte
+ *        aligned
+ *   max_rows  the most rows that one request has (from the counts that were
+ *        planned); a request's rows past it are left as they were.  0: not
+ *        known.  Kernels and the workspace are chosen by it: 1 where all
+ *        requests decode.
+ * max_pages * page_size <= 2^30, and times batch * kv_heads below 2^38.
+ * row_start and lengths are held to [0, rows] and [0, max_pages * page_size];
+ * tokens in table entries that are no page do not exist; a row that sees none
+ * gets zeros.  Roundings, scores, infinities, scale and the workspace are those
+ * of vm_hip_attention_packed; the workspace is that of the largest rows and
+ * max_rows it is used with. */
+int64_t vm_hip_attention_paged_workspace_bytes(int64_t batch, int64_t rows, int64_t max_rows, int64_t heads,
+                                               int64_t kv_heads, int64_t head_dim, int64_t max_tokens);
+int vm_hip_attention_paged(const vm_hip_kv_paged* cache, const int32_t* tables, int64_t max_pages, const void* q,
+                           void* out, int64_t batch, int64_t rows, int64_t max_rows, int64_t heads,
+                           const int32_t* row_start, const int32_t* lengths, float scale, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

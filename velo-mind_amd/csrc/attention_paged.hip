@@ -1,0 +1,1271 @@
+// Causal attention of many requests in one call: over cache pages (decoded
+// tokens and chunks of prompts) and of whole prompts that lie one behind the
+// other.
+//
+//   o_r = sum_j p_rj v_j / sum_j p_rj,   p_rj = exp(scale (q_r . k_j) - m_r),
+//
+// j over the tokens up to the row's own, m_r a reference that is at least the
+// largest score less kHeadroom.  The query heads of a KV head read the same keys,
+// so the (token, head) pairs of a request and KV head are its query rows, r =
+// token G + head.  Both products are computed transposed, S^T = K Q^T and O^T =
+// V^T P^T, so that a query row owns a column of both and its statistics stay in
+// its lanes; keys are numbered inside a tile so that the scores a lane holds
+// are the weights that the second product wants from it.
+//
+// Two kernels.  attention_few_kernel takes requests of at most 16 RT query
+// rows (decoded tokens): K and V straight from memory to operand registers, a
+// wave its own blocks of keys, and the keys of all requests dealt out evenly
+// over the workgroups.  attention_many_kernel takes the others: 32 RT rows a
+// wave, key tiles in LDS for all four waves.  16-bit rows use the 16-bit matrix
+// instructions (weights rounded to 16 bits: half a step of the result's type
+// for each), fp32 rows the fp32 ones.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <type_traits>
+
+#include "kv_paged.h"
+#include "kv_q8.h"
+#include "vm_device.h"
+#include "vm_internal.h"
+
+namespace vmhip {
+namespace {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+constexpr int kMaxBatch = VM_HIP_PAGED_MAX_BATCH;
+constexpr int kMaxSplits = 64;        // workgroups that share a request's keys: few rows,
+constexpr int kManySplits = 16;       // many rows
+constexpr int kTargetGroups = 512;    // workgroups that fill 256 compute units twice
+constexpr int kTicketStride = 16;     // a ticket has a 64-byte line of its own
+constexpr int64_t kTicketBytes = kTargetGroups * kTicketStride * 4;
+constexpr int kRound = 128;           // keys that the waves of attention_few_kernel take at once
+constexpr int kLeast = 2;             // rounds that are worth a workgroup
+// A weight may exceed 1 by this much (log2) before its row's reference moves:
+// references then move in the first blocks and rarely later.
+constexpr float kHeadroom = 7.0f;
+
+struct Args {
+    const void* q;
+    const void* k;
+    const void* v;
+    void* out;
+    const int32_t* row_start;
+    const int32_t* lengths;   // with pages
+    const int32_t* tables;
+    unsigned* tickets;
+    char* parts;
+    int64_t q_stride, k_stride, v_stride;   // elements
+    int64_t max_pages, pages;
+    int batch, rows, max_rows, heads, kv_heads, shift;
+    int few;      // query rows up to which a request is attention_few_kernel's
+    int splits;   // attention_many_kernel: workgroups that share a tile's keys
+    int slots;    // tiles that a KV head's requests may have
+    float c;      // scale / ln 2
+};
+
+// A request's rows and the tokens in front of them.
+struct Request {
+    int start, n, length, p0;   // first row, rows, tokens, tokens in front of the first row (negative: rows without)
+    int todo;                   // rows that are computed
+};
+
+template <bool kPaged>
+__device__ __forceinline__ Request request(const Args& a, int b) {
+    Request r;
+    r.start = min(max(a.row_start[b], 0), a.rows);
+    r.n = min(max(a.row_start[b + 1], r.start), a.rows) - r.start;
+    if (kPaged) {
+        const int64_t most = a.max_pages << a.shift;
+        r.length = static_cast<int>(min(static_cast<int64_t>(max(a.lengths[b], 0)), most));
+    } else {
+        r.length = r.n;
+    }
+    r.p0 = r.length - r.n;
+    r.todo = min(r.n, a.max_rows);
+    return r;
+}
+
+__device__ __forceinline__ float max_halves(float v) {
+    const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    unsigned q[2];
+    __builtin_memcpy(q, &h, sizeof q);
+    return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
+}
+__device__ __forceinline__ float sum_halves(float v) { return swap_halves_add(v, v); }
+// Over the lanes lr + 16 g.
+__device__ __forceinline__ float max_groups(float v) {
+    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    unsigned q[2];
+    __builtin_memcpy(q, &p, sizeof q);
+    return max_halves(fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1])));
+}
+__device__ __forceinline__ float sum_groups(float v) {
+    v = swap_rows_add(v, v);
+    return swap_halves_add(v, v);
+}
+
+// Whether a dword holds an element that is not finite, and the dword without
+// those elements.
+template <typename T>
+__device__ __forceinline__ bool odd_element(uint32_t bits) {
+    if constexpr (sizeof(T) == 4) return (bits & 0x7f800000u) == 0x7f800000u;
+    constexpr uint32_t e = std::is_same<T, F16>::value ? 0x7c00u : 0x7f80u;
+    return (bits & e) == e || (bits >> 16 & e) == e;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t finite_elements(uint32_t bits) {
+    if constexpr (sizeof(T) == 4) return odd_element<T>(bits) ? 0u : bits;
+    constexpr uint32_t e = std::is_same<T, F16>::value ? 0x7c00u : 0x7f80u;
+    if ((bits & e) == e) bits &= 0xffff0000u;
+    if ((bits >> 16 & e) == e) bits &= 0x0000ffffu;
+    return bits;
+}
+template <typename T>
+__device__ __forceinline__ bool odd_vector(u32x4 v) {
+    return odd_element<T>(v.x) || odd_element<T>(v.y) || odd_element<T>(v.z) || odd_element<T>(v.w);
+}
+
+template <typename T>
+__device__ __forceinline__ f32x4 mfma16(u32x4 x, u32x4 y, f32x4 z) {
+    if constexpr (std::is_same<T, F16>::value)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, x), __builtin_bit_cast(half8, y), z, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, x), __builtin_bit_cast(bf8, y), z, 0, 0, 0);
+}
+template <typename T>
+__device__ __forceinline__ f32x16 mfma32(u32x4 x, u32x4 y, f32x16 z) {
+    if constexpr (std::is_same<T, F16>::value)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, x), __builtin_bit_cast(half8, y), z, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8, x), __builtin_bit_cast(bf8, y), z, 0, 0, 0);
+}
+
+// Eight weights as an operand, rounded to nearest.
+template <typename T>
+__device__ __forceinline__ u32x4 pack8(const float* p) {
+    if constexpr (std::is_same<T, F16>::value) {
+        half8 h;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] = static_cast<_Float16>(p[e]);
+        return __builtin_bit_cast(u32x4, h);
+    } else {
+        bf8 h;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] = static_cast<__bf16>(p[e]);
+        return __builtin_bit_cast(u32x4, h);
+    }
+}
+
+__device__ __forceinline__ void store4(float* p, const float* y) { *reinterpret_cast<float4*>(p) = make_float4(y[0], y[1], y[2], y[3]); }
+template <typename T>
+__device__ __forceinline__ void store4(T* p, const float* y) {
+    uint16_t h[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h[e] = narrow<T>(y[e]).bits;
+    *reinterpret_cast<u32x2*>(p) = u32x2{h[0] | static_cast<uint32_t>(h[1]) << 16, h[2] | static_cast<uint32_t>(h[3]) << 16};
+}
+
+// One row's four dims: outputs over the sum of weights; a row that saw nothing: zeros.
+template <typename T>
+__device__ __forceinline__ void put(const Args& a, const Request& q, int kh, int g, int r, int dim, const float* y,
+                                    float l, int d) {
+    const int t = r / g;
+    if (t >= q.todo) return;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float z[4] = {y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv};
+    store4(static_cast<T*>(a.out) + (static_cast<int64_t>(q.start + t) * a.heads + kh * g + r % g) * d + dim, z);
+}
+
+// Parts of a tile's keys in the workspace, [rows][D] outputs, then references
+// (log2) and sums of the rows; the workgroup that draws the last ticket joins
+// them.  part(s): byte offset of workgroup s's; factors: LDS for kMaxSplits x
+// kRows floats, totals for kRows.
+template <typename T, int D, int kRows, typename Part>
+__device__ __forceinline__ void join_parts(const Args& a, const Request& q, int kh, int g, int r0, int active,
+                                           Part part, float* factors, float* totals) {
+    for (int row = threadIdx.x / 16; row < kRows; row += kThreads / 16) {
+        const int s0 = threadIdx.x % 16;
+        float mv[kMaxSplits / 16], lv[kMaxSplits / 16], m = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < kMaxSplits / 16; ++u) {
+            const int s = s0 + 16 * u;
+            const float* ml = reinterpret_cast<const float*>(a.parts + part(min(s, active - 1))) + kRows * D + row;
+            mv[u] = s < active ? coherent_load(ml) : -INFINITY;
+            lv[u] = s < active ? coherent_load(ml + kRows) : 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < kMaxSplits / 16; ++u) m = fmaxf(m, mv[u]);
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        const float m_ref = m == -INFINITY ? 0.0f : m;
+        float l = 0.0f;
+#pragma unroll
+        for (int u = 0; u < kMaxSplits / 16; ++u) {
+            const int s = s0 + 16 * u;
+            const float f = __builtin_amdgcn_exp2f(mv[u] - m_ref);
+            if (s < active) {
+                l = fmaf(lv[u], f, l);
+                factors[s * kRows + row] = f;
+            }
+        }
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) l += __shfl_xor(l, o, 64);
+        if (s0 == 0) totals[row] = l;
+    }
+    __syncthreads();
+    for (int item = threadIdx.x; item < kRows * D / 4; item += kThreads) {
+        const int row = item / (D / 4), d4 = item % (D / 4);
+        float y[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int s0 = 0; s0 < active; s0 += 8) {
+            u32x4 x[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (s0 + u < active)
+                    x[u] = coherent_load16(buffer_rsrc(a.parts + part(s0 + u), kRows * D * 4), item * 16);
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (s0 + u < active) {
+                    const float f = factors[(s0 + u) * kRows + row];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[e] = fmaf(__uint_as_float(x[u][e]), f, y[e]);
+                }
+        }
+        put<T>(a, q, kh, g, r0 + row, 4 * d4, y, totals[row], D);
+    }
+}
+
+constexpr int64_t part_bytes(int64_t rows, int64_t d) { return rows * (d + 2) * 4; }
+
+// Clears the ticket and says whether this workgroup drew the last one.
+__device__ __forceinline__ bool last_arrival(unsigned* counter, int active, unsigned* drawn) {
+    publish_partials();
+    __syncthreads();
+    if (threadIdx.x == 0) *drawn = ticket_take(counter, active);
+    __syncthreads();
+    if (*drawn != static_cast<unsigned>(active - 1)) return false;
+    if (threadIdx.x == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return true;
+}
+
+// ---- Few rows: 16-wide tiles.  A[i][k] and B[k][j] of a 16x16x32 product
+// sit in lane i (j) + 16 (k / 8), element k % 8; of a 16x16x4 fp32 product in lane
+// i (j) + 16 k; D[i][j] in lane j + 16 (i / 4), element i % 4.
+//   S^T  16 bits: tile bt (0, 1) of a 32-key block has key 8 (i / 4) + 4 bt + i %
+//        4 in row i, so that lane group lg = lane / 16 holds keys 8 lg .. + 7;
+//        fp32: one tile of 16 keys, in order, lane group lg holds keys 4 lg .. + 3
+//   K    16 bytes a lane of its key's row, 64 adjacent bytes in four lanes
+//   O^T  16 bits: row i of tile db is dim (D / 16) i + db: a lane reads D / 16
+//        adjacent elements of each of its eight keys and transposes them with
+//        byte permutes; fp32: tile 4 h + u has dim 64 h + 4 i + u: nothing moves
+template <typename T, int D, int RT>
+__global__ __launch_bounds__(kThreads, 2) void attention_few_kernel(const Args a) {
+    constexpr bool kWide = sizeof(T) == 4;
+    constexpr int KB = kWide ? 16 : 32;          // keys of a block
+    constexpr int KPL = KB / 4;                  // of a lane
+    constexpr int NT = KB / 16;                  // score tiles
+    constexpr int KC = D * sizeof(T) / 64;       // 16-byte pieces of a key that a lane reads
+    constexpr int ND = D / 16;                   // dim tiles
+    constexpr int VW = ND * sizeof(T) / 4;       // dwords of a value's row that a lane reads
+    constexpr int kRows = 16 * RT;
+    __shared__ __align__(16) float merge_o[kWaves][kRows * D];
+    __shared__ float merge_m[kWaves][kRows], merge_l[kWaves][kRows];
+    __shared__ int work[kMaxBatch];              // rounds of the requests up to this one, of a KV head
+    __shared__ int waves_sum[kWaves], waves_max[kWaves];
+    __shared__ unsigned ticket;
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lr = lane & 15, lg = lane >> 4;
+    const int g = a.heads / a.kv_heads;
+    const auto rounds_of = [&](const Request& q) {
+        return q.todo > 0 && q.todo * g <= a.few ? max((q.length + kRound - 1) / kRound, 1) : 0;
+    };
+
+    // Rounds of all requests, summed up by every workgroup for itself.
+    int total, longest;
+    {
+        const int each = (a.batch + kThreads - 1) / kThreads, b0 = threadIdx.x * each;
+        int sum = 0, most = 0;
+        for (int b = b0; b < min(b0 + each, a.batch); ++b) {
+            const int w = rounds_of(request<true>(a, b));
+            sum += w;
+            most = max(most, w);
+            work[b] = sum;
+        }
+        int run = sum;
+#pragma unroll
+        for (int s = 1; s < 64; s <<= 1) {
+            const int o = __shfl_up(run, s, 64);
+            if (lane >= s) run += o;
+            most = max(most, __shfl_xor(most, s, 64));
+        }
+        if (lane == 63) waves_sum[wave] = run, waves_max[wave] = most;
+        __syncthreads();
+        int before = run - sum;
+        total = longest = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            if (w < wave) before += waves_sum[w];
+            total += waves_sum[w];
+            longest = max(longest, waves_max[w]);
+        }
+        for (int b = b0; b < min(b0 + each, a.batch); ++b) work[b] += before;
+        __syncthreads();
+    }
+    total *= a.kv_heads;
+    // Shares: even, worth a workgroup, and no more than kMaxSplits of a request's keys.
+    const int per = max(max((total + kTargetGroups - 1) / kTargetGroups, kLeast),
+                        (longest + kMaxSplits - 2) / (kMaxSplits - 1));
+    int pos = static_cast<int>(blockIdx.x) * per;
+    const int end = min(total, pos + per);
+
+    while (pos < end) {
+        // The request, KV head and rounds that this share goes on with.
+        int lo = 0, hi = a.batch - 1;            // the first request with more rounds than pos / kv_heads
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (work[mid] * a.kv_heads > pos)
+                hi = mid;
+            else
+                lo = mid + 1;
+        }
+        const int b = __builtin_amdgcn_readfirstlane(lo);
+        const Request q = request<true>(a, b);
+        const int rounds = rounds_of(q);
+        const int request_start = (work[b] - rounds) * a.kv_heads;
+        const int kh = (pos - request_start) / rounds;
+        const int unit_start = request_start + kh * rounds;
+        const int first = pos - unit_start, last = min(rounds, end - unit_start);
+        const int first_group = unit_start / per;
+        const int active = (unit_start + rounds - 1) / per - first_group + 1;
+        pos = unit_start + last;
+
+        const int64_t row_bytes = D * sizeof(T);
+        const char* kbase = static_cast<const char*>(a.k) + ((static_cast<int64_t>(kh) << a.shift) * row_bytes);
+        const char* vbase = static_cast<const char*>(a.v) + ((static_cast<int64_t>(kh) << a.shift) * row_bytes);
+        const int64_t page_bytes = (static_cast<int64_t>(a.kv_heads) << a.shift) * row_bytes;
+        const int32_t* table = a.tables + static_cast<int64_t>(b) * a.max_pages;
+        const int in_page = (1 << a.shift) - 1;
+        const int last_page = max(q.length - 1, 0) >> a.shift;
+        const int whole = min(q.p0 + 1, q.length);   // keys that every row sees
+
+        struct Ids {
+            int k, v;
+        };
+        // (a block's keys have one page, or, of 16 tokens, two)
+        const auto lookup = [&](int block) {
+            Ids i;
+            i.k = table[min((block * KB + (kWide ? 0 : 8 * (lr / 4))) >> a.shift, last_page)];
+            i.v = table[min((block * KB + KPL * lg) >> a.shift, last_page)];
+            return i;
+        };
+        struct Block {
+            u32x4 k[NT][KC];
+            uint32_t v[KPL][VW];
+            bool there;   // the page of this lane's keys
+        };
+        const auto load = [&](int block, Ids ids, Block& c) {
+            const int k0 = block * KB;
+            const bool k_there = ids.k >= 0 && ids.k < a.pages;
+            c.there = ids.v >= 0 && ids.v < a.pages;
+            const char* kp = kbase + (k_there ? ids.k : 0) * page_bytes + 16 * lg;
+            const char* vp = vbase + (c.there ? ids.v : 0) * page_bytes + 4 * VW * lr;
+#pragma unroll
+            for (int bt = 0; bt < NT; ++bt) {
+                const int key = k0 + (kWide ? lr : 8 * (lr / 4) + 4 * bt + lr % 4);
+                const char* p = kp + (key & in_page) * row_bytes;
+#pragma unroll
+                for (int s = 0; s < KC; ++s) c.k[bt][s] = *reinterpret_cast<const u32x4*>(p + 64 * s);
+            }
+#pragma unroll
+            for (int j = 0; j < KPL; ++j) {
+                const char* p = vp + ((k0 + KPL * lg + j) & in_page) * row_bytes;
+                if constexpr (kWide) {
+                    // (rows of 64 dims apart: tile 4 h + u)
+                    const char* pw = vbase + (c.there ? ids.v : 0) * page_bytes + 16 * lr + ((k0 + KPL * lg + j) & in_page) * row_bytes;
+#pragma unroll
+                    for (int h = 0; h < D / 64; ++h) {
+                        const u32x4 x = *reinterpret_cast<const u32x4*>(pw + 256 * h);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) c.v[j][4 * h + e] = x[e];
+                    }
+                } else if constexpr (VW == 4) {
+                    const u32x4 x = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) c.v[j][e] = x[e];
+                } else {
+                    const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+                    c.v[j][0] = x.x;
+                    c.v[j][1] = x.y;
+                }
+            }
+        };
+
+        // This wave's blocks: round r's keys are shared out in turn.
+        constexpr int kStep = kRound / KB;   // blocks of a round
+        const int block_end = min(last * kStep, (q.length + KB - 1) / KB);
+        int block = first * kStep + wave;
+        Ids ids{0, 0};
+        Block c0, c1;
+        if (block < block_end) {
+            ids = lookup(block);
+            load(block, ids, c0);
+            ids = lookup(block + kWaves);
+        }
+
+        u32x4 qf[RT][KC];
+        int limit_key[RT];   // the last key that the row sees
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const int r = 16 * rt + lr, t = r / g;
+            const bool row_ok = t < q.todo;
+            limit_key[rt] = row_ok ? q.p0 + t : -1;
+            const T* qp = static_cast<const T*>(a.q) + static_cast<int64_t>(q.start + (row_ok ? t : 0)) * a.q_stride +
+                          (kh * g + r % g) * D;
+#pragma unroll
+            for (int s = 0; s < KC; ++s) {
+                qf[rt][s] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(qp) + 64 * s + 16 * lg);
+                if (!row_ok) qf[rt][s] = u32x4{0, 0, 0, 0};
+            }
+        }
+        f32x4 acc[RT][ND];
+        float m_run[RT];   // the score that weighs 1
+        float limit[RT];   // the score from which on it moves; -inf before the first key
+        float l_run[RT];   // sum of this lane's keys' weights
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+            for (int db = 0; db < ND; ++db) acc[rt][db] = f32x4{0.f, 0.f, 0.f, 0.f};
+            m_run[rt] = l_run[rt] = 0.0f;
+            limit[rt] = -INFINITY;
+        }
+
+        const auto compute = [&](auto masked_tag, int block, Block& c) {
+            constexpr bool kMasked = decltype(masked_tag)::value;
+            const int key0 = block * KB + KPL * lg;
+            f32x4 st[RT][NT];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int bt = 0; bt < NT; ++bt) st[rt][bt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < KC; ++s)
+#pragma unroll
+                for (int bt = 0; bt < NT; ++bt)
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) {
+                        if constexpr (kWide) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                st[rt][bt] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                    __uint_as_float(c.k[bt][s][e]), __uint_as_float(qf[rt][s][e]), st[rt][bt], 0, 0, 0);
+                        } else {
+                            st[rt][bt] = mfma16<T>(c.k[bt][s], qf[rt][s], st[rt][bt]);
+                        }
+                    }
+            bool odd = false;   // a value that is not finite, where not every row sees it
+            if (kMasked) {
+#pragma unroll
+                for (int j = 0; j < KPL; ++j)
+#pragma unroll
+                    for (int u = 0; u < VW; ++u) odd |= odd_element<T>(c.v[j][u]);
+                odd = __any(odd);
+            }
+            float mt[RT];
+            bool moves = false;
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                mt[rt] = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < KPL; ++j) {
+                    if (kMasked && !(c.there && key0 + j <= limit_key[rt])) st[rt][j / 4][j % 4] = -INFINITY;
+                    mt[rt] = fmaxf(mt[rt], st[rt][j / 4][j % 4]);
+                }
+                moves |= mt[rt] > limit[rt];
+            }
+            if (__any(moves)) {
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    const float most = max_groups(mt[rt]);
+                    if (most > -INFINITY) {
+                        const float m = limit[rt] == -INFINITY ? most : fmaxf(m_run[rt], most);
+                        const float fall = __builtin_amdgcn_exp2f((m_run[rt] - m) * a.c);
+                        if (limit[rt] > -INFINITY) {
+                            l_run[rt] *= fall;
+#pragma unroll
+                            for (int db = 0; db < ND; ++db) acc[rt][db] *= fall;
+                        }
+                        m_run[rt] = m;
+                        limit[rt] = m + kHeadroom / a.c;
+                    }
+                }
+            }
+            float p[RT][KPL];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                const float base = m_run[rt] * a.c;
+#pragma unroll
+                for (int j = 0; j < KPL; ++j) {
+                    p[rt][j] = __builtin_amdgcn_exp2f(fmaf(st[rt][j / 4][j % 4], a.c, -base));
+                    l_run[rt] += p[rt][j];
+                }
+            }
+            if (kMasked && odd) {
+                // Values that are not finite go to the rows that see them by
+                // hand, whatever their weight: 0 times them would not be 0.
+                for (int j = 0; j < KB; ++j) {
+                    const int key = block * KB + j;
+                    const int id = table[min(key >> a.shift, last_page)];
+                    if (id < 0 || id >= a.pages) continue;
+                    const T* vp = reinterpret_cast<const T*>(vbase + id * page_bytes + (key & in_page) * row_bytes);
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) {
+                        if (key > limit_key[rt]) continue;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+#pragma unroll
+                            for (int db = 0; db < ND; ++db) {
+                                const float x = widen(vp[kWide ? 64 * (db / 4) + 16 * lg + 4 * e + db % 4 : ND * (4 * lg + e) + db]);
+                                if (!(fabsf(x) < INFINITY)) acc[rt][db][e] += x;
+                            }
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < KPL; ++j)
+#pragma unroll
+                    for (int u = 0; u < VW; ++u) c.v[j][u] = finite_elements<T>(c.v[j][u]);
+            }
+            if constexpr (kWide) {
+#pragma unroll
+                for (int db = 0; db < ND; ++db)
+#pragma unroll
+                    for (int j = 0; j < KPL; ++j)
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt)
+                            acc[rt][db] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(c.v[j][db]), p[rt][j], acc[rt][db], 0, 0, 0);
+            } else {
+                u32x4 pf[RT];
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) pf[rt] = pack8<T>(p[rt]);
+#pragma unroll
+                for (int db = 0; db < ND; ++db) {
+                    u32x4 vf;
+#pragma unroll
+                    for (int jp = 0; jp < 4; ++jp)
+                        vf[jp] = __builtin_amdgcn_perm(c.v[2 * jp + 1][db / 2], c.v[2 * jp][db / 2],
+                                                       db % 2 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) acc[rt][db] = mfma16<T>(vf, pf[rt], acc[rt][db]);
+                }
+            }
+        };
+        const auto step = [&](Block& now, Block& next) {
+            if (block + kWaves < block_end) {
+                load(block + kWaves, ids, next);
+                ids = lookup(block + 2 * kWaves);
+            }
+            if ((block + 1) * KB <= whole && __all(now.there))
+                compute(std::false_type{}, block, now);
+            else
+                compute(std::true_type{}, block, now);
+            block += kWaves;
+        };
+        while (block < block_end) {
+            step(c0, c1);
+            if (block >= block_end) break;
+            step(c1, c0);
+        }
+
+        // Every wave's (reference, sum, output) to LDS; then thread (row, four
+        // dims) merges the four.
+        __syncthreads();   // (the last segment's merge has been read)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const float l = sum_groups(l_run[rt]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int u = 0; u < ND / 4; ++u) {
+                    const int dim = kWide ? 64 * u + 16 * lg + 4 * e : ND * (4 * lg + e) + 4 * u;
+                    const float y[4] = {acc[rt][4 * u][e], acc[rt][4 * u + 1][e], acc[rt][4 * u + 2][e], acc[rt][4 * u + 3][e]};
+                    store4(merge_o[wave] + (16 * rt + lr) * D + dim, y);
+                }
+            if (lg == 0) {
+                merge_m[wave][16 * rt + lr] = limit[rt] == -INFINITY ? -INFINITY : m_run[rt] * a.c;
+                merge_l[wave][16 * rt + lr] = l;
+            }
+        }
+        __syncthreads();
+        const auto part = [&](int s) {   // the first group's part is its second one
+            return (static_cast<int64_t>(first_group + s) * 2 + (s == 0)) * part_bytes(kRows, D);
+        };
+        const int mine = static_cast<int>(blockIdx.x) - first_group;
+        char* out_part = a.parts + (active > 1 ? part(mine) : 0);
+        const __amdgpu_buffer_rsrc_t prs = buffer_rsrc(out_part, part_bytes(kRows, D));
+        for (int item = threadIdx.x; item < kRows * D / 4; item += kThreads) {
+            const int row = item / (D / 4), d4 = item % (D / 4);
+            float m = merge_m[0][row];
+#pragma unroll
+            for (int k = 1; k < kWaves; ++k) m = fmaxf(m, merge_m[k][row]);
+            const float m_ref = m == -INFINITY ? 0.0f : m;
+            float l = 0.0f, y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < kWaves; ++k) {
+                const float f = __builtin_amdgcn_exp2f(merge_m[k][row] - m_ref);
+                l = fmaf(merge_l[k][row], f, l);
+                const float4 o = *reinterpret_cast<const float4*>(&merge_o[k][row * D + 4 * d4]);
+                y[0] = fmaf(o.x, f, y[0]);
+                y[1] = fmaf(o.y, f, y[1]);
+                y[2] = fmaf(o.z, f, y[2]);
+                y[3] = fmaf(o.w, f, y[3]);
+            }
+            if (active == 1) {
+                put<T>(a, q, kh, g, row, 4 * d4, y, l, D);
+                continue;
+            }
+            coherent_store16(prs, static_cast<uint32_t>(item) * 16,
+                             u32x4{__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3])});
+            if (d4 == 0) {
+                float* ml = reinterpret_cast<float*>(out_part) + kRows * D;
+                coherent_store(ml + row, m);
+                coherent_store(ml + kRows + row, l);
+            }
+        }
+        if (active > 1 && last_arrival(a.tickets + first_group * kTicketStride, active, &ticket)) {
+            static_assert(kMaxSplits * kRows <= kWaves * kRows * D, "factors fit");
+            join_parts<T, D, kRows>(a, q, kh, g, 0, active, part, merge_o[0], merge_m[0]);
+        }
+    }
+}
+
+// ---- Many rows: 32-wide tiles, 32 RT query rows a wave, KT keys at a time in
+// LDS for all four waves, the next tile's on their way in registers.  A[i][k] and
+// B[k][j] of a 32x32x16 product sit in lane i (j) + 32 (k / 8), element k % 8; of
+// a 32x32x2 fp32 product in lane i (j) + 32 k; D[i][j] in lane j + 32 (i / 4 %
+// 2), element i % 4 + 4 (i / 8).  A lane of half lh = lane / 32 holds the
+// scores of keys 8 a + 4 lh + b: as weights they are the second product's k
+// positions if V^T's operand has the same keys there, which two transposing LDS
+// reads of four keys give (16 bits), or plain reads (fp32).
+// LDS rows hold their 16-byte pieces exchanged by the row's number, so that
+// the rows that are read together lie in different banks.
+template <typename T, int D>
+struct Tile {
+    static constexpr int KT = sizeof(T) == 4 ? 32 : 64;         // keys
+    static constexpr int CH = D * sizeof(T) / 16;               // 16-byte pieces of a row
+    static constexpr int PER = KT * CH / kThreads;              // pieces of a thread
+    static constexpr int kBytes = KT * D * static_cast<int>(sizeof(T));
+    static __device__ __forceinline__ int swap(int row) { return CH == 8 ? row & 7 : 2 * (row & 7); }
+};
+
+template <typename T, int D, int RT, bool kPaged>
+__global__ __launch_bounds__(kThreads, 2) void attention_many_kernel(const Args a) {
+    constexpr bool kWide = sizeof(T) == 4;
+    using L = Tile<T, D>;
+    constexpr int KT = L::KT, CH = L::CH, PER = L::PER;
+    constexpr int NK = KT / 32;             // score tiles
+    constexpr int NQ = D * sizeof(T) / 32;  // 16-byte pieces of a query row that a lane holds
+    constexpr int ND = D / 32;              // dim tiles
+    constexpr int kRows = 32 * RT * kWaves;
+    constexpr int kRowBytes = D * sizeof(T);
+    __shared__ __align__(16) char lds[2][2][L::kBytes];   // [buffer][keys, values]
+    __shared__ unsigned ticket;
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lc = lane & 31, lh = lane >> 5;
+    const int g = a.heads / a.kv_heads;
+
+    // Workgroups go to the XCDs in turn: the tiles of a (KV head, share of the
+    // keys) stay on one where the count of those allows, the last tiles, which
+    // see the most keys, first.
+    int slot, share;
+    {
+        const int id = static_cast<int>(blockIdx.x), shares = a.kv_heads * a.splits;
+        if (shares % 8 == 0) {
+            const int j = id / 8;
+            slot = a.slots - 1 - j % a.slots;
+            share = j / a.slots * 8 + id % 8;
+        } else {
+            slot = a.slots - 1 - id / shares;
+            share = id % shares;
+        }
+    }
+    const int kh = share % a.kv_heads, split = share / a.kv_heads;
+
+    // Request b's tiles have the slots from row_start[b] G / kRows + b on (a
+    // slot more than it may need).
+    const auto first_slot = [&](int b) {
+        return static_cast<int>(static_cast<int64_t>(min(max(a.row_start[b], 0), a.rows)) * g / kRows) + b;
+    };
+    int b = 0;
+    for (int width = a.batch; width > 1;) {
+        // the last of 64 probes that starts at or before the slot
+        const int stride = (width + 63) / 64;
+        const int at = b + lane * stride;
+        const bool below = lane * stride < width && first_slot(at) <= slot;
+        const int n = max(__popcll(__ballot(below)), 1) - 1;
+        b += n * stride;
+        width = min(stride, width - n * stride);
+    }
+    b = __builtin_amdgcn_readfirstlane(b);
+    const Request q = request<kPaged>(a, b);
+    const int tile = slot - first_slot(b);
+    const int r0 = tile * kRows;
+    if (tile < 0 || r0 >= q.todo * g || q.todo * g <= a.few) return;
+    const int t_last = min((r0 + kRows - 1) / g, q.todo - 1);
+    const int seen = min(max(q.p0 + t_last + 1, 0), q.length);      // keys that some row sees
+    const int whole = min(max(q.p0 + r0 / g + 1, 0), q.length);     // that every row sees
+    const int tiles = (seen + KT - 1) / KT;
+    const int each = (tiles + a.splits - 1) / a.splits;
+    const int active = each > 0 ? (tiles + each - 1) / each : 1;
+    if (split >= active) return;
+    const int first = split * each, last = min(tiles, first + each);
+
+    // Where a thread's pieces of a tile lie.
+    const int64_t kv_row = static_cast<int64_t>(kh) << a.shift;
+    const int32_t* table = kPaged ? a.tables + static_cast<int64_t>(b) * a.max_pages : nullptr;
+    const int in_page = (1 << a.shift) - 1;
+    const int last_page = max(q.length - 1, 0) >> a.shift;
+    struct Ids {
+        int id[KT / 16];
+    };
+    const auto lookup = [&](int t) {
+        Ids i{};
+        if constexpr (kPaged) {
+#pragma unroll
+            for (int u = 0; u < KT / 16; ++u) i.id[u] = table[min((t * KT + 16 * u) >> a.shift, last_page)];
+        }
+        return i;
+    };
+    const auto there = [&](const Ids& i) {   // bit u: keys 16 u .. + 15 have a page
+        unsigned bits = (1u << (KT / 16)) - 1;
+        if constexpr (kPaged) {
+#pragma unroll
+            for (int u = 0; u < KT / 16; ++u)
+                if (i.id[u] < 0 || i.id[u] >= a.pages) bits &= ~(1u << u);
+        }
+        return bits;
+    };
+    u32x4 kreg[PER], vreg[PER];
+    const auto load = [&](int t, const Ids& ids) {
+#pragma unroll
+        for (int u = 0; u < PER; ++u) {
+            const int piece = u * kThreads + threadIdx.x;
+            const int row = piece / CH, c = (piece % CH) ^ L::swap(row);
+            if constexpr (kPaged) {
+                const int group = __builtin_amdgcn_readfirstlane(row / 16);
+                int id = ids.id[0];
+#pragma unroll
+                for (int w = 1; w < KT / 16; ++w)
+                    if (group == w) id = ids.id[w];
+                if (id < 0 || id >= a.pages) id = 0;
+                const int64_t at = (((static_cast<int64_t>(id) * a.kv_heads) << a.shift) + kv_row +
+                                    ((t * KT + 16 * group) & in_page)) * kRowBytes;
+                const int off = (row & 15) * kRowBytes + 16 * c;
+                kreg[u] = *reinterpret_cast<const u32x4*>(static_cast<const char*>(a.k) + at + off);
+                vreg[u] = *reinterpret_cast<const u32x4*>(static_cast<const char*>(a.v) + at + off);
+            } else {
+                const int64_t at = q.start + min(t * KT + row, q.length - 1);
+                kreg[u] = *reinterpret_cast<const u32x4*>(static_cast<const char*>(a.k) +
+                                                          (at * a.k_stride + kh * D) * static_cast<int>(sizeof(T)) + 16 * c);
+                vreg[u] = *reinterpret_cast<const u32x4*>(static_cast<const char*>(a.v) +
+                                                          (at * a.v_stride + kh * D) * static_cast<int>(sizeof(T)) + 16 * c);
+            }
+        }
+    };
+    // Puts the loaded tile into LDS and meets the other waves; true: it holds a
+    // value that is not finite (asked only of tiles that not every row sees whole).
+    const auto publish = [&](int buffer, bool ask) {
+        bool odd = false;
+#pragma unroll
+        for (int u = 0; u < PER; ++u) {
+            const int at = (u * kThreads + threadIdx.x) * 16;
+            *reinterpret_cast<u32x4*>(lds[buffer][0] + at) = kreg[u];
+            *reinterpret_cast<u32x4*>(lds[buffer][1] + at) = vreg[u];
+            if (ask) odd |= odd_vector<T>(vreg[u]);
+        }
+        if (ask) return __syncthreads_or(odd) != 0;
+        __syncthreads();
+        return false;
+    };
+
+    Ids ids = lookup(first);
+    if (first < last) load(first, ids);
+    unsigned pages_there = there(ids);
+
+    u32x4 qf[RT][NQ];
+    int limit_key[RT];
+    const int w0 = r0 + 32 * RT * wave;   // the wave's first row
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int r = w0 + 32 * rt + lc, t = r / g;
+        const bool row_ok = t < q.todo;
+        limit_key[rt] = row_ok ? q.p0 + t : -1;
+        const T* qp = static_cast<const T*>(a.q) + static_cast<int64_t>(q.start + (row_ok ? t : 0)) * a.q_stride +
+                      (kh * g + r % g) * D;
+#pragma unroll
+        for (int s = 0; s < NQ; ++s) {
+            qf[rt][s] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(qp) + 32 * s + 16 * lh);
+            if (!row_ok) qf[rt][s] = u32x4{0, 0, 0, 0};
+        }
+    }
+    // Keys below wave_whole are seen by every row of the wave, from wave_seen on by none.
+    const int wave_whole = w0 / g < q.todo ? min(max(q.p0 + w0 / g + 1, 0), q.length) : 0;
+    const int wave_seen = w0 / g < q.todo ? min(seen, max(q.p0 + min((w0 + 32 * RT - 1) / g, q.todo - 1) + 1, 0)) : 0;
+
+    f32x16 acc[RT][ND];
+    float m_run[RT], limit[RT], l_run[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+        for (int db = 0; db < ND; ++db)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[rt][db][e] = 0.0f;
+        m_run[rt] = l_run[rt] = 0.0f;
+        limit[rt] = -INFINITY;
+    }
+
+    const auto compute = [&](auto masked_tag, int t, int buffer, unsigned bits, bool odd) {
+        constexpr bool kMasked = decltype(masked_tag)::value;
+        const char* kt = lds[buffer][0];
+        const char* vt = lds[buffer][1];
+        f32x16 st[RT][NK];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int n = 0; n < NK; ++n)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) st[rt][n][e] = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NK; ++n)
+#pragma unroll
+            for (int s = 0; s < NQ; ++s) {
+                const int row = 32 * n + lc;
+                const u32x4 kf = *reinterpret_cast<const u32x4*>(kt + row * kRowBytes + 16 * ((2 * s + lh) ^ L::swap(row)));
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    if constexpr (kWide) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            st[rt][n] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kf[e]), __uint_as_float(qf[rt][s][e]),
+                                                                             st[rt][n], 0, 0, 0);
+                    } else {
+                        st[rt][n] = mfma32<T>(kf, qf[rt][s], st[rt][n]);
+                    }
+                }
+            }
+        float mt[RT];
+        bool moves = false;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            mt[rt] = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < NK; ++n)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int key = t * KT + 32 * n + 8 * (e / 4) + 4 * lh + e % 4;
+                    if (kMasked && !(key <= limit_key[rt] && (bits >> (2 * n + e / 8) & 1))) st[rt][n][e] = -INFINITY;
+                    mt[rt] = fmaxf(mt[rt], st[rt][n][e]);
+                }
+            moves |= mt[rt] > limit[rt];
+        }
+        if (__any(moves)) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                const float most = max_halves(mt[rt]);
+                if (most > -INFINITY) {
+                    const float m = limit[rt] == -INFINITY ? most : fmaxf(m_run[rt], most);
+                    const float fall = __builtin_amdgcn_exp2f((m_run[rt] - m) * a.c);
+                    if (limit[rt] > -INFINITY) {
+                        l_run[rt] *= fall;
+#pragma unroll
+                        for (int db = 0; db < ND; ++db)
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) acc[rt][db][e] *= fall;
+                    }
+                    m_run[rt] = m;
+                    limit[rt] = m + kHeadroom / a.c;
+                }
+            }
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const float base = m_run[rt] * a.c;
+#pragma unroll
+            for (int n = 0; n < NK; ++n)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float p = __builtin_amdgcn_exp2f(fmaf(st[rt][n][e], a.c, -base));
+                    st[rt][n][e] = p;
+                    l_run[rt] += p;
+                }
+        }
+        if (kMasked && odd) {
+            // Values that are not finite go to the rows that see them by hand,
+            // whatever their weight: 0 times them would not be 0.
+            for (int j = 0; j < KT; ++j) {
+                if (!(bits >> (j / 16) & 1)) continue;
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    if (t * KT + j > limit_key[rt]) continue;
+#pragma unroll
+                    for (int db = 0; db < ND; ++db)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const int at = (32 * db + 8 * (e / 4) + 4 * lh + e % 4) * static_cast<int>(sizeof(T));
+                            const float x = widen(*reinterpret_cast<const T*>(vt + j * kRowBytes +
+                                                                              16 * ((at / 16) ^ L::swap(j)) + at % 16));
+                            if (!(fabsf(x) < INFINITY)) acc[rt][db][e] += x;
+                        }
+                }
+            }
+        }
+        if constexpr (kWide) {
+#pragma unroll
+            for (int n = 0; n < NK; ++n)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+#pragma unroll
+                    for (int db = 0; db < ND; ++db) {
+                        const int row = 32 * n + 8 * (e / 4) + 4 * lh + e % 4;
+                        const int c = 8 * db + lc / 4;
+                        uint32_t x = *reinterpret_cast<const uint32_t*>(vt + row * kRowBytes + 16 * (c ^ L::swap(row)) + 4 * (lc & 3));
+                        if (kMasked && odd) x = finite_elements<T>(x);
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt)
+                            acc[rt][db] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(x), st[rt][n][e], acc[rt][db], 0, 0, 0);
+                    }
+        } else {
+            const int l16 = lane & 15;
+#pragma unroll
+            for (int n = 0; n < NK; ++n)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    u32x4 pf[RT];
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) {
+                        float p[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) p[e] = st[rt][n][8 * s + e];
+                        pf[rt] = pack8<T>(p);
+                    }
+#pragma unroll
+                    for (int db = 0; db < ND; ++db) {
+                        // lane 4 k + x of 16 reads dims 4 x .. + 3 of key k
+                        uint32_t x[4];
+#pragma unroll
+                        for (int w = 0; w < 2; ++w) {
+                            const int row = 32 * n + 16 * s + 8 * w + 4 * lh + l16 / 4;
+                            const int c = 4 * db + 2 * (lane >> 4 & 1) + (l16 % 4) / 2;
+                            const char* at = vt + row * kRowBytes + 16 * (c ^ L::swap(row)) + 8 * (l16 & 1);
+                            const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                (__attribute__((address_space(3))) s16x4*)(at));
+                            __builtin_memcpy(x + 2 * w, &y, 8);
+                        }
+                        u32x4 vf{x[0], x[1], x[2], x[3]};
+                        if (kMasked && odd) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) vf[e] = finite_elements<T>(vf[e]);
+                        }
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt) acc[rt][db] = mfma32<T>(vf, pf[rt], acc[rt][db]);
+                    }
+                }
+        }
+    };
+
+    const auto partly = [&](int t, unsigned bits) { return (t + 1) * KT > whole || bits != (1u << (KT / 16)) - 1; };
+    if (first < last) {
+        Ids next = lookup(first + 1);
+        bool odd = publish(first & 1, partly(first, pages_there));
+        for (int t = first; t < last; ++t) {
+            unsigned bits = pages_there;
+            if (t + 1 < last) {
+                pages_there = there(next);
+                load(t + 1, next);
+                next = lookup(t + 2);
+            }
+            if (t * KT < wave_seen) {
+                if ((t + 1) * KT <= wave_whole && bits == (1u << (KT / 16)) - 1)
+                    compute(std::false_type{}, t, t & 1, bits, false);
+                else
+                    compute(std::true_type{}, t, t & 1, bits, odd);
+            }
+            if (t + 1 < last) odd = publish((t + 1) & 1, partly(t + 1, pages_there));
+        }
+    }
+
+    const auto part = [&](int s) {
+        return ((static_cast<int64_t>(kh) * a.slots + slot) * a.splits + s) * part_bytes(kRows, D);
+    };
+    char* out_part = a.parts + (active > 1 ? part(split) : 0);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const float l = sum_halves(l_run[rt]);
+        const int row = 32 * (RT * wave + rt) + lc;
+#pragma unroll
+        for (int db = 0; db < ND; ++db)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int dim = 32 * db + 8 * u + 4 * lh;
+                const float y[4] = {acc[rt][db][4 * u], acc[rt][db][4 * u + 1], acc[rt][db][4 * u + 2], acc[rt][db][4 * u + 3]};
+                if (active == 1)
+                    put<T>(a, q, kh, g, r0 + row, dim, y, l, D);
+                else
+                    coherent_store16(buffer_rsrc(out_part, kRows * D * 4), (row * D + dim) * 4,
+                                     u32x4{__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3])});
+            }
+        if (active > 1 && lh == 0) {
+            float* ml = reinterpret_cast<float*>(out_part) + kRows * D;
+            coherent_store(ml + row, limit[rt] == -INFINITY ? -INFINITY : m_run[rt] * a.c);
+            coherent_store(ml + kRows + row, l);
+        }
+    }
+    if (active > 1) {
+        __syncthreads();   // (LDS is free)
+        if (last_arrival(a.tickets + (kh * a.slots + slot) * kTicketStride, active, &ticket)) {
+            float* f = reinterpret_cast<float*>(lds[0][0]);
+            static_assert((kManySplits + 1) * kRows * 4 <= static_cast<int>(sizeof lds), "factors fit");
+            join_parts<T, D, kRows>(a, q, kh, g, r0, active, part, f, f + kManySplits * kRows);
+        }
+    }
+}
+
+// ---- Host
+
+// Row tiles of a wave in attention_many_kernel.
+int many_tiles(int64_t d, bool wide) { return d == 64 && !wide ? 2 : 1; }
+
+struct Plan {
+    bool few, many;
+    int few_tiles;        // RT of attention_few_kernel
+    int few_rows;         // query rows up to which a request is its
+    int splits;
+    int64_t slots;
+    int64_t bytes;        // of the workspace: tickets, then parts; the kernels run one after the other
+};
+
+// bytes grows with rows and max_rows: a workspace serves smaller calls too.
+Plan plan(int64_t batch, int64_t rows, int64_t max_rows, int64_t heads, int64_t kv_heads, int64_t d,
+          int64_t max_tokens, bool wide, bool paged) {
+    Plan p{};
+    const int64_t g = heads / kv_heads;
+    const int64_t most = std::min(rows, max_rows > 0 ? max_rows : rows) * g;   // query rows of a request
+    p.few_tiles = most <= 16 ? 1 : 2;
+    p.few_rows = 16 * p.few_tiles;
+    // One request with more rows than that: all of it is the other kernel's.
+    p.few = paged && g <= p.few_rows && (batch > 1 || most <= p.few_rows);
+    if (!p.few) p.few_rows = 0;
+    p.many = most > p.few_rows;
+    if (p.few) p.bytes = kTicketBytes + 2 * kTargetGroups * part_bytes(16 * p.few_tiles, d);
+    if (p.many) {
+        const int64_t tile = 32 * many_tiles(d, wide) * kWaves;
+        p.slots = rows * g / tile + batch;
+        const int64_t units = p.slots * kv_heads;
+        const int64_t share = std::max<int64_t>(1, max_tokens / 256);   // 256 keys are worth a workgroup
+        p.splits = static_cast<int>(std::max<int64_t>(1, std::min({kTargetGroups / units, static_cast<int64_t>(kManySplits), share})));
+        if (share > 1) p.bytes = std::max(p.bytes, kTicketBytes + kTargetGroups * part_bytes(tile, d));
+    }
+    return p;
+}
+
+int check_call(const char* who, int64_t batch, int64_t rows, int64_t max_rows, int64_t heads, int64_t kv_heads,
+               int64_t d) {
+    const std::string w(who);
+    if (d != 64 && d != 128) return fail_inval(w + ": head_dim must be 64 or 128");
+    if (batch < 0 || batch > kMaxBatch || rows < 0 || rows > VM_HIP_PAGED_MAX_ROWS || max_rows < 0)
+        return fail_inval(w + ": batch or rows out of range");
+    if (kv_heads < 1 || kv_heads > 4096 || heads < 1 || heads > 65536 || heads % kv_heads)
+        return fail_inval(w + ": bad heads");
+    if (rows * heads >= (int64_t{1} << 30)) return fail_inval(w + ": too many rows for one call");
+    return 0;
+}
+
+int64_t workspace_bytes_of(int64_t batch, int64_t rows, int64_t max_rows, int64_t heads, int64_t kv_heads, int64_t d,
+                           int64_t max_tokens, bool paged) {
+    if (batch == 0 || rows == 0) return 0;
+    int64_t most = 0;
+    for (bool wide : {false, true})
+        most = std::max(most, plan(batch, rows, max_rows, heads, kv_heads, d, max_tokens, wide, paged).bytes);
+    return most;
+}
+
+template <typename T, int D>
+void launch_few(const Args& a, int tiles, hipStream_t s) {
+    const dim3 grid(kTargetGroups), block(kThreads);
+    if (tiles == 1)
+        hipLaunchKernelGGL((attention_few_kernel<T, D, 1>), grid, block, 0, s, a);
+    else
+        hipLaunchKernelGGL((attention_few_kernel<T, D, 2>), grid, block, 0, s, a);
+}
+
+template <typename T, int D, bool kPaged>
+void launch_many(const Args& a, int64_t grid, hipStream_t s) {
+    constexpr int RT = D == 64 && sizeof(T) == 2 ? 2 : 1;   // many_tiles()
+    hipLaunchKernelGGL((attention_many_kernel<T, D, RT, kPaged>), dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, s, a);
+}
+
+template <typename T, int D>
+void launch_type(const Args& a, const Plan& p, bool paged, hipStream_t s) {
+    if (p.few) launch_few<T, D>(a, p.few_tiles, s);
+    if (p.many) {
+        const int64_t grid = p.slots * a.kv_heads * p.splits;
+        if (paged)
+            launch_many<T, D, true>(a, grid, s);
+        else
+            launch_many<T, D, false>(a, grid, s);
+    }
+}
+
+int run(const char* who, Args a, const Plan& p, int dtype, int64_t d, bool paged, void* workspace, void* stream) {
+    a.few = p.few_rows;
+    a.splits = std::max(p.splits, 1);
+    a.slots = static_cast<int>(p.slots);
+    a.tickets = static_cast<unsigned*>(workspace);
+    a.parts = static_cast<char*>(workspace) + kTicketBytes;
+    auto s = static_cast<hipStream_t>(stream);
+    if (d == 64) {
+        if (dtype == VM_HIP_DTYPE_F32)
+            launch_type<float, 64>(a, p, paged, s);
+        else if (dtype == VM_HIP_DTYPE_F16)
+            launch_type<F16, 64>(a, p, paged, s);
+        else
+            launch_type<BF16, 64>(a, p, paged, s);
+    } else {
+        if (dtype == VM_HIP_DTYPE_F32)
+            launch_type<float, 128>(a, p, paged, s);
+        else if (dtype == VM_HIP_DTYPE_F16)
+            launch_type<F16, 128>(a, p, paged, s);
+        else
+            launch_type<BF16, 128>(a, p, paged, s);
+    }
+    return check_launch(who, s);
+}
+
+float scale_of(float scale, int64_t d) {
+    return (scale > 0.0f ? scale : 1.0f / std::sqrt(static_cast<float>(d))) * 1.44269504f;
+}
+
+bool off16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
+bool off4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) != 0; }
+
+}  // namespace
+}  // namespace vmhip
+
+using namespace vmhip;
+
+extern "C" {
+
+int64_t vm_hip_attention_packed_workspace_bytes(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads,
+                                                int64_t head_dim) {
+    clear_error();
+    VM_TRY(check_call("attention_packed", batch, rows, 0, heads, kv_heads, head_dim));
+    return workspace_bytes_of(batch, rows, 0, heads, kv_heads, head_dim, rows, false);
+}
+
+int vm_hip_attention_packed(const void* q, const void* k, const void* v, void* out, int dtype, int64_t q_stride,
+                            int64_t k_stride, int64_t v_stride, int64_t batch, int64_t rows, int64_t heads,
+                            int64_t kv_heads, int64_t head_dim, const int32_t* row_start, float scale, void* workspace,
+                            int64_t workspace_bytes, void* stream) {
+    clear_error();
+    if (dtype != VM_HIP_DTYPE_F32 && dtype != VM_HIP_DTYPE_F16 && dtype != VM_HIP_DTYPE_BF16)
+        return fail_inval("attention_packed: dtype must be F32, F16 or BF16");
+    VM_TRY(check_call("attention_packed", batch, rows, 0, heads, kv_heads, head_dim));
+    const int64_t unit = dtype == VM_HIP_DTYPE_F32 ? 4 : 8;   // elements of 16 bytes
+    for (int64_t s : {q_stride, k_stride, v_stride})
+        if (s % unit || s > (1 << 24)) return fail_inval("attention_packed: strides must be multiples of 16 bytes, at most 2^24 elements");
+    if (q_stride < heads * head_dim || k_stride < kv_heads * head_dim || v_stride < kv_heads * head_dim)
+        return fail_inval("attention_packed: strides must hold a row's heads");
+    if (!(scale < INFINITY)) return fail_inval("attention_packed: scale must be finite");
+    if (rows == 0 || batch == 0) return 0;
+    if (!q || !k || !v || !out || !row_start) return fail_inval("attention_packed: null pointer");
+    if (off16(q) || off16(k) || off16(v) || off16(out))
+        return fail_inval("attention_packed: q, k, v and out must be 16-byte aligned");
+    if (off4(row_start)) return fail_inval("attention_packed: row_start must be 4-byte aligned");
+    const int64_t need = vm_hip_attention_packed_workspace_bytes(batch, rows, heads, kv_heads, head_dim);
+    if (need > 0 && (!workspace || workspace_bytes < need || off16(workspace)))
+        return fail_inval("attention_packed: workspace smaller than vm_hip_attention_packed_workspace_bytes or unaligned");
+    const Plan p = plan(batch, rows, 0, heads, kv_heads, head_dim, rows, dtype == VM_HIP_DTYPE_F32, false);
+    if (p.slots * kv_heads * p.splits >= (1 << 24)) return fail_inval("attention_packed: too many rows for one call");
+    Args a{};
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.out = out;
+    a.row_start = row_start;
+    a.q_stride = q_stride;
+    a.k_stride = k_stride;
+    a.v_stride = v_stride;
+    a.batch = static_cast<int>(batch);
+    a.rows = a.max_rows = static_cast<int>(rows);
+    a.heads = static_cast<int>(heads);
+    a.kv_heads = static_cast<int>(kv_heads);
+    a.c = scale_of(scale, head_dim);
+    return run("attention_packed", a, p, dtype, head_dim, false, workspace, stream);
+}
+
+int64_t vm_hip_attention_paged_workspace_bytes(int64_t batch, int64_t rows, int64_t max_rows, int64_t heads,
+                                               int64_t kv_heads, int64_t head_dim, int64_t max_tokens) {
+    clear_error();
+    VM_TRY(check_call("attention_paged", batch, rows, max_rows, heads, kv_heads, head_dim));
+    if (max_tokens < 1 || max_tokens > (1 << 30)) return fail_inval("attention_paged: max_tokens out of range");
+    return workspace_bytes_of(batch, rows, max_rows, heads, kv_heads, head_dim, max_tokens, true);
+}
+
+int vm_hip_attention_paged(const vm_hip_kv_paged* cache, const int32_t* tables, int64_t max_pages, const void* q,
+                           void* out, int64_t batch, int64_t rows, int64_t max_rows, int64_t heads,
+                           const int32_t* row_start, const int32_t* lengths, float scale, void* workspace,
+                           int64_t workspace_bytes, void* stream) {
+    clear_error();
+    VM_TRY(check_kv_paged(cache, "attention_paged"));
+    const int64_t d = cache->head_dim, hk = cache->kv_heads;
+    VM_TRY(check_call("attention_paged", batch, rows, max_rows, heads, hk, d));
+    if (max_pages < 1 || max_pages > (1 << 30) / cache->page_size)
+        return fail_inval("attention_paged: max_pages * page_size must be at most 2^30");
+    if (batch * hk * ((max_pages * cache->page_size + kRound - 1) / kRound) >= (int64_t{1} << 31))
+        return fail_inval("attention_paged: batch * kv_heads * max_pages * page_size must be below 2^38");
+    if (!(scale < INFINITY)) return fail_inval("attention_paged: scale must be finite");
+    if (rows == 0 || batch == 0) return 0;
+    if (!tables || !q || !out || !row_start || !lengths) return fail_inval("attention_paged: null pointer");
+    if (off16(q) || off16(out)) return fail_inval("attention_paged: q and out must be 16-byte aligned");
+    if (off4(tables) || off4(row_start) || off4(lengths))
+        return fail_inval("attention_paged: tables, row_start and lengths must be 4-byte aligned");
+    const int64_t tokens = max_pages * cache->page_size;
+    const int64_t need = vm_hip_attention_paged_workspace_bytes(batch, rows, max_rows, heads, hk, d, tokens);
+    if (need > 0 && (!workspace || workspace_bytes < need || off16(workspace)))
+        return fail_inval("attention_paged: workspace smaller than vm_hip_attention_paged_workspace_bytes or unaligned");
+    const Plan p = plan(batch, rows, max_rows, heads, hk, d, tokens, cache->dtype == VM_HIP_DTYPE_F32, true);
+    if (p.many && p.slots * hk * p.splits >= (1 << 24)) return fail_inval("attention_paged: too many rows for one call");
+    Args a{};
+    a.q = q;
+    a.k = cache->k;
+    a.v = cache->v;
+    a.out = out;
+    a.row_start = row_start;
+    a.lengths = lengths;
+    a.tables = tables;
+    a.q_stride = heads * d;
+    a.max_pages = max_pages;
+    a.pages = cache->pages;
+    a.batch = static_cast<int>(batch);
+    a.rows = static_cast<int>(rows);
+    a.max_rows = static_cast<int>(max_rows > 0 ? std::min(max_rows, rows) : rows);
+    a.heads = static_cast<int>(heads);
+    a.kv_heads = static_cast<int>(hk);
+    a.shift = log2_of(cache->page_size);
+    a.c = scale_of(scale, d);
+    return run("attention_paged", a, p, cache->dtype, d, true, workspace, stream);
+}
+
+}  // extern "C"

@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, byref, c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p
+from ctypes import POINTER, byref, c_char_p, c_double, c_float, c_int, c_int64, c_size_t, c_void_p
 
 import numpy as np
 
@@ -21,6 +21,8 @@ QUANT_INT8 = 1
 QUANT_INT4 = 2
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 4, 5
 EINVAL, EUNSUPPORTED, EINJECTED, ENODEVICE = -1, -2, -3, -4
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BANDS, ROPE_RAMP = 0, 1, 2, 3   # vm_hip_rope_scaling.kind
+ROPE_HALVES, ROPE_PAIRS = 0, 1                               # vm_hip_rope.layout
 A_FP32, A_ROWS, A_PIECES = 0, 1, 2   # prefill GEMM activation layouts (vm_hip_qmm_a_layout)
 
 _lib: ctypes.CDLL | None = None
@@ -62,6 +64,37 @@ class LogitsRules(ctypes.Structure):
                 ("repetition", c_void_p), ("frequency", c_void_p), ("presence", c_void_p), ("bias_tokens", c_void_p),
                 ("bias_values", c_void_p), ("bias_lengths", c_void_p), ("bias_stride", c_int64), ("allowed", c_void_p),
                 ("drafted", c_void_p), ("tree", c_void_p)]
+
+
+class KvPaged(ctypes.Structure):
+    """vm_hip_kv_paged (include/vm_hip.h): device addresses and shape of a cache in pages."""
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("dtype", c_int), ("pages", c_int64), ("page_size", c_int64),
+                ("kv_heads", c_int64), ("head_dim", c_int64)]
+
+
+class PagePlan(ctypes.Structure):
+    """vm_hip_page_plan (include/vm_hip.h): sizes and device addresses of a step's plan."""
+    _fields_ = [("batch", c_int64), ("rows", c_int64), ("max_pages", c_int64), ("pages", c_int64),
+                ("page_size", c_int64), ("lengths", c_void_p), ("counts", c_void_p), ("free_pages", c_void_p),
+                ("free_count", c_void_p), ("tables", c_void_p), ("row_start", c_void_p), ("lengths_out", c_void_p),
+                ("free_count_out", c_void_p), ("positions", c_void_p), ("slots", c_void_p)]
+
+
+class RopeScaling(ctypes.Structure):
+    """vm_hip_rope_scaling (include/vm_hip.h)."""
+    _fields_ = [("kind", c_int), ("factor", c_double), ("low", c_double), ("high", c_double), ("original", c_double),
+                ("attention", c_double)]
+
+
+class Rope(ctypes.Structure):
+    """vm_hip_rope (include/vm_hip.h): device addresses of the tables, their size and the pairs' layout."""
+    _fields_ = [("cos_table", c_void_p), ("sin_table", c_void_p), ("rows", c_int64), ("dim", c_int64),
+                ("layout", c_int)]
+
+
+class QkNorm(ctypes.Structure):
+    """vm_hip_qk_norm (include/vm_hip.h)."""
+    _fields_ = [("q_weight", c_void_p), ("k_weight", c_void_p), ("eps", c_float)]
 
 
 def _declare(L: ctypes.CDLL) -> None:
@@ -159,6 +192,18 @@ def _declare(L: ctypes.CDLL) -> None:
         "vm_hip_a8_pack": ([p, c_int64, c_int64, p, p], c_int),
         "vm_hip_a8_stage": ([p, c_int, c_int64, c_int64, p, p], c_int),
         "vm_hip_qmm_a8": ([p, p, p, p, c_int, c_int64, c_int64, c_int64, p, c_int64, p], c_int),
+        "vm_hip_kv_paged_plan_workspace_bytes": ([c_int64] * 2, c_int64),
+        "vm_hip_kv_paged_plan": ([POINTER(PagePlan), p, c_int64, p], c_int),
+        "vm_hip_kv_paged_release": ([c_int64] * 4 + [p] * 6, c_int),
+        "vm_hip_rope_tables": ([p, p, c_int64, c_int64, c_int64, c_double, POINTER(RopeScaling), p], c_int),
+        "vm_hip_kv_paged_append": ([POINTER(KvPaged), p, c_int64, c_int64, POINTER(QkNorm), POINTER(Rope), p, p, p, p],
+                                   c_int),
+        "vm_hip_qk_norm_rope": ([p, c_int] + [c_int64] * 4 + [POINTER(QkNorm), POINTER(Rope), p, p, p, p], c_int),
+        "vm_hip_attention_packed_workspace_bytes": ([c_int64] * 5, c_int64),
+        "vm_hip_attention_packed": ([p] * 4 + [c_int] + [c_int64] * 8 + [p, c_float, p, c_int64, p], c_int),
+        "vm_hip_attention_paged_workspace_bytes": ([c_int64] * 7, c_int64),
+        "vm_hip_attention_paged": ([POINTER(KvPaged), p, c_int64, p, p] + [c_int64] * 4 + [p, p, c_float, p, c_int64, p],
+                                   c_int),
         "vm_hip_logits_rules_workspace_bytes": ([c_int64] * 3, c_int64),
         "vm_hip_logits_rules_apply": ([POINTER(LogitsRules), p, p, c_int, p, c_int64, c_int64, c_int64, p, p, c_int64, p],
                                       c_int),
@@ -198,7 +243,10 @@ def exported_symbols() -> list[str]:
             "vm_hip_kv_q8_append", "vm_hip_kv_q8_read", "vm_hip_kv_q8_keep", "vm_hip_attention_q8_workspace_bytes",
             "vm_hip_attention_q8", "vm_hip_a8_weights_bytes", "vm_hip_a8_stage_bytes", "vm_hip_qmm_a8_workspace_bytes",
             "vm_hip_a8_pack", "vm_hip_a8_stage", "vm_hip_qmm_a8", "vm_hip_logits_rules_workspace_bytes",
-            "vm_hip_logits_rules_apply"]
+            "vm_hip_logits_rules_apply", "vm_hip_kv_paged_plan_workspace_bytes", "vm_hip_kv_paged_plan",
+            "vm_hip_kv_paged_release", "vm_hip_rope_tables", "vm_hip_kv_paged_append", "vm_hip_qk_norm_rope",
+            "vm_hip_attention_packed_workspace_bytes", "vm_hip_attention_packed",
+            "vm_hip_attention_paged_workspace_bytes", "vm_hip_attention_paged"]
 
 
 def open_library() -> ctypes.CDLL:
@@ -464,6 +512,74 @@ def logits_rules(rules: LogitsRules, logits: int, out, dtype: int, tokens, seqs:
     """vm_hip_logits_rules_apply: penalties, biases and masks on logits, and the greedy token of each row."""
     check(open_library().vm_hip_logits_rules_apply(byref(rules), logits, out, dtype, tokens, seqs, rows, vocab, counts,
                                                    workspace, workspace_bytes, _h(stream)))
+
+
+# ---- A step over requests that share a pool of cache pages (raw device addresses) ----
+
+def kv_paged_plan_workspace_bytes(batch: int, rows: int) -> int:
+    return _size(open_library().vm_hip_kv_paged_plan_workspace_bytes(batch, rows))
+
+
+def kv_paged_plan(plan: PagePlan, workspace, workspace_bytes: int, stream=None) -> None:
+    """vm_hip_kv_paged_plan: block tables, row offsets, positions and slots of a step."""
+    check(open_library().vm_hip_kv_paged_plan(byref(plan), workspace, workspace_bytes, _h(stream)))
+
+
+def kv_paged_release(batch: int, max_pages: int, pages: int, page_size: int, finished, lengths, tables, free_pages,
+                     free_count, stream=None) -> None:
+    """vm_hip_kv_paged_release: the pages of finished requests back to the pool."""
+    check(open_library().vm_hip_kv_paged_release(batch, max_pages, pages, page_size, finished, lengths, tables,
+                                                 free_pages, free_count, _h(stream)))
+
+
+def rope_tables(cos, sin, first: int, rows: int, dim: int, theta: float, scaling: RopeScaling | None = None,
+                stream=None) -> None:
+    """vm_hip_rope_tables: cosines and sines of positions first .. first + rows - 1."""
+    check(open_library().vm_hip_rope_tables(cos, sin, first, rows, dim, theta, _ref(scaling), _h(stream)))
+
+
+def kv_paged_append(cache: KvPaged, qkv, rows: int, heads: int, norm: QkNorm | None, rope: Rope | None, positions,
+                    slots, q_out, stream=None) -> None:
+    """vm_hip_kv_paged_append: norm and rotate q and k, store k and v at their slots."""
+    check(open_library().vm_hip_kv_paged_append(byref(cache), qkv, rows, heads, _ref(norm), _ref(rope), positions,
+                                                slots, q_out, _h(stream)))
+
+
+def qk_norm_rope(qkv, dtype: int, rows: int, heads: int, kv_heads: int, head_dim: int, norm: QkNorm | None,
+                 rope: Rope | None, positions, q_out, k_out, stream=None) -> None:
+    """vm_hip_qk_norm_rope: norm and rotate q and k of packed rows."""
+    check(open_library().vm_hip_qk_norm_rope(qkv, dtype, rows, heads, kv_heads, head_dim, _ref(norm), _ref(rope),
+                                             positions, q_out, k_out, _h(stream)))
+
+
+def attention_packed_workspace_bytes(batch: int, rows: int, heads: int, kv_heads: int, head_dim: int) -> int:
+    return _size(open_library().vm_hip_attention_packed_workspace_bytes(batch, rows, heads, kv_heads, head_dim))
+
+
+def attention_packed(q, k, v, out, dtype: int, q_stride: int, k_stride: int, v_stride: int, batch: int, rows: int,
+                     heads: int, kv_heads: int, head_dim: int, row_start, scale: float, workspace,
+                     workspace_bytes: int, stream=None) -> None:
+    """vm_hip_attention_packed: causal attention of whole prompts, one behind the other."""
+    check(open_library().vm_hip_attention_packed(q, k, v, out, dtype, q_stride, k_stride, v_stride, batch, rows, heads,
+                                                 kv_heads, head_dim, row_start, scale, workspace, workspace_bytes,
+                                                 _h(stream)))
+
+
+def attention_paged_workspace_bytes(batch: int, rows: int, max_rows: int, heads: int, kv_heads: int, head_dim: int,
+                                    max_tokens: int) -> int:
+    return _size(open_library().vm_hip_attention_paged_workspace_bytes(batch, rows, max_rows, heads, kv_heads, head_dim,
+                                                                       max_tokens))
+
+
+def attention_paged(cache: KvPaged, tables, max_pages: int, q, out, batch: int, rows: int, max_rows: int, heads: int,
+                    row_start, lengths, scale: float, workspace, workspace_bytes: int, stream=None) -> None:
+    """vm_hip_attention_paged: decoded tokens and prompts' chunks over a cache in pages."""
+    check(open_library().vm_hip_attention_paged(byref(cache), tables, max_pages, q, out, batch, rows, max_rows, heads,
+                                                row_start, lengths, scale, workspace, workspace_bytes, _h(stream)))
+
+
+def _ref(struct):
+    return None if struct is None else byref(struct)
 
 
 def _size(n: int) -> int:
