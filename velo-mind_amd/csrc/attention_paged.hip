@@ -167,6 +167,17 @@ __device__ __forceinline__ u32x4 pack8(const float* p) {
     }
 }
 
+// Sixteen bytes a lane from memory to LDS, lane by lane behind `to` (uniform).
+// Written as statements of their own because the compiler would have every LDS
+// read wait for them, also reads of another buffer; wait_loads() waits.  (No
+// other instruction of these kernels uses m0.)
+__device__ __forceinline__ void lds_load16(const void* from, void* to) {
+    const uint32_t at = __builtin_amdgcn_readfirstlane(
+        static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)(to))));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(at), "v"(from) : "memory");
+}
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
+
 __device__ __forceinline__ void store4(float* p, const float* y) { *reinterpret_cast<float4*>(p) = make_float4(y[0], y[1], y[2], y[3]); }
 template <typename T>
 __device__ __forceinline__ void store4(T* p, const float* y) {
@@ -737,65 +748,78 @@ __global__ __launch_bounds__(kThreads, 2) void attention_many_kernel(const Args 
     const int32_t* table = kPaged ? a.tables + static_cast<int64_t>(b) * a.max_pages : nullptr;
     const int in_page = (1 << a.shift) - 1;
     const int last_page = max(q.length - 1, 0) >> a.shift;
-    struct Ids {
-        int id[KT / 16];
-    };
+    typedef int Ids __attribute__((ext_vector_type(KT / 16)));   // pages of a tile's keys, 16 each
     const auto lookup = [&](int t) {
         Ids i{};
         if constexpr (kPaged) {
 #pragma unroll
-            for (int u = 0; u < KT / 16; ++u) i.id[u] = table[min((t * KT + 16 * u) >> a.shift, last_page)];
+            for (int u = 0; u < KT / 16; ++u) i[u] = table[min((t * KT + 16 * u) >> a.shift, last_page)];
         }
         return i;
     };
-    const auto there = [&](const Ids& i) {   // bit u: keys 16 u .. + 15 have a page
+    const auto there = [&](Ids i) {   // bit u: keys 16 u .. + 15 have a page
         unsigned bits = (1u << (KT / 16)) - 1;
         if constexpr (kPaged) {
 #pragma unroll
             for (int u = 0; u < KT / 16; ++u)
-                if (i.id[u] < 0 || i.id[u] >= a.pages) bits &= ~(1u << u);
+                if (i[u] < 0 || i[u] >= a.pages) bits &= ~(1u << u);
         }
         return bits;
     };
-    u32x4 kreg[PER], vreg[PER];
-    const auto load = [&](int t, const Ids& ids) {
+    // A wave's piece u of a tile: 1 KB, 64 / CH rows, of one 16-key group.
+    constexpr int kWaveRows = 64 / CH;
+    static_assert(kWaves * kWaveRows <= 32, "a step's rows lie in two groups at most");
+    const int my_row = lane / CH;                                   // of the piece
+    // (a piece starts at a multiple of kWaveRows; rows are exchanged by row & 7)
+    const auto load = [&](int t, Ids ids) {
+        char* kl = lds[t & 1][0];
+        char* vl = lds[t & 1][1];
 #pragma unroll
         for (int u = 0; u < PER; ++u) {
-            const int piece = u * kThreads + threadIdx.x;
-            const int row = piece / CH, c = (piece % CH) ^ L::swap(row);
+            const int row0 = (u * kWaves + wave) * kWaveRows;       // uniform
+            const int row = row0 + my_row;
+            const int c = (lane % CH) ^ L::swap(row);
+            const char *kp, *vp;
             if constexpr (kPaged) {
-                const int group = __builtin_amdgcn_readfirstlane(row / 16);
-                int id = ids.id[0];
-#pragma unroll
-                for (int w = 1; w < KT / 16; ++w)
-                    if (group == w) id = ids.id[w];
+                const int group = row0 / 16;
+                constexpr int kStep = kWaves * kWaveRows;   // rows that the waves' pieces u have
+                int id = ids[u * kStep / 16];
+                if constexpr (kStep > 16) id = wave < kWaves / 2 ? id : ids[u * kStep / 16 + 1];
                 if (id < 0 || id >= a.pages) id = 0;
                 const int64_t at = (((static_cast<int64_t>(id) * a.kv_heads) << a.shift) + kv_row +
-                                    ((t * KT + 16 * group) & in_page)) * kRowBytes;
-                const int off = (row & 15) * kRowBytes + 16 * c;
-                kreg[u] = *reinterpret_cast<const u32x4*>(static_cast<const char*>(a.k) + at + off);
-                vreg[u] = *reinterpret_cast<const u32x4*>(static_cast<const char*>(a.v) + at + off);
+                                    ((t * KT + 16 * group) & in_page) + row0 % 16) * kRowBytes;
+                const int off = my_row * kRowBytes + 16 * c;
+                kp = static_cast<const char*>(a.k) + at + off;
+                vp = static_cast<const char*>(a.v) + at + off;
             } else {
                 const int64_t at = q.start + min(t * KT + row, q.length - 1);
-                kreg[u] = *reinterpret_cast<const u32x4*>(static_cast<const char*>(a.k) +
-                                                          (at * a.k_stride + kh * D) * static_cast<int>(sizeof(T)) + 16 * c);
-                vreg[u] = *reinterpret_cast<const u32x4*>(static_cast<const char*>(a.v) +
-                                                          (at * a.v_stride + kh * D) * static_cast<int>(sizeof(T)) + 16 * c);
+                kp = static_cast<const char*>(a.k) + (at * a.k_stride + kh * D) * static_cast<int>(sizeof(T)) + 16 * c;
+                vp = static_cast<const char*>(a.v) + (at * a.v_stride + kh * D) * static_cast<int>(sizeof(T)) + 16 * c;
             }
+            lds_load16(kp, kl + (u * kWaves + wave) * 1024);
+            lds_load16(vp, vl + (u * kWaves + wave) * 1024);
         }
     };
-    // Puts the loaded tile into LDS and meets the other waves; true: it holds a
-    // value that is not finite (asked only of tiles that not every row sees whole).
-    const auto publish = [&](int buffer, bool ask) {
-        bool odd = false;
+    // Waits for the wave's pieces of the tile and meets the other waves.  `ask`
+    // (tiles that not every row sees whole): values that are not finite are
+    // taken out; true: there were some.
+    const auto arrive = [&](int t, bool ask) {
+        wait_loads();
+        if (ask) {
+            bool odd = false;
 #pragma unroll
-        for (int u = 0; u < PER; ++u) {
-            const int at = (u * kThreads + threadIdx.x) * 16;
-            *reinterpret_cast<u32x4*>(lds[buffer][0] + at) = kreg[u];
-            *reinterpret_cast<u32x4*>(lds[buffer][1] + at) = vreg[u];
-            if (ask) odd |= odd_vector<T>(vreg[u]);
+            for (int u = 0; u < PER; ++u) {
+                u32x4* at = reinterpret_cast<u32x4*>(lds[t & 1][1] + (u * kWaves + wave) * 1024 + lane * 16);
+                u32x4 v = *at;
+                if (odd_vector<T>(v)) {
+                    odd = true;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = finite_elements<T>(v[e]);
+                    *at = v;
+                }
+            }
+            return __syncthreads_or(odd) != 0;
         }
-        if (ask) return __syncthreads_or(odd) != 0;
         __syncthreads();
         return false;
     };
@@ -836,10 +860,9 @@ __global__ __launch_bounds__(kThreads, 2) void attention_many_kernel(const Args 
         limit[rt] = -INFINITY;
     }
 
-    const auto compute = [&](auto masked_tag, int t, int buffer, unsigned bits, bool odd) {
-        constexpr bool kMasked = decltype(masked_tag)::value;
-        const char* kt = lds[buffer][0];
-        const char* vt = lds[buffer][1];
+    const auto compute = [&](int t, bool masked, unsigned bits) {
+        const char* kt = lds[t & 1][0];
+        const char* vt = lds[t & 1][1];
         f32x16 st[RT][NK];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
@@ -865,6 +888,17 @@ __global__ __launch_bounds__(kThreads, 2) void attention_many_kernel(const Args 
                     }
                 }
             }
+        if (masked) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int n = 0; n < NK; ++n)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int key = t * KT + 32 * n + 8 * (e / 4) + 4 * lh + e % 4;
+                        if (!(key <= limit_key[rt] && (bits >> (2 * n + e / 8) & 1))) st[rt][n][e] = -INFINITY;
+                    }
+        }
         float mt[RT];
         bool moves = false;
 #pragma unroll
@@ -873,11 +907,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_many_kernel(const Args 
 #pragma unroll
             for (int n = 0; n < NK; ++n)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int key = t * KT + 32 * n + 8 * (e / 4) + 4 * lh + e % 4;
-                    if (kMasked && !(key <= limit_key[rt] && (bits >> (2 * n + e / 8) & 1))) st[rt][n][e] = -INFINITY;
-                    mt[rt] = fmaxf(mt[rt], st[rt][n][e]);
-                }
+                for (int e = 0; e < 16; ++e) mt[rt] = fmaxf(mt[rt], st[rt][n][e]);
             moves |= mt[rt] > limit[rt];
         }
         if (__any(moves)) {
@@ -911,26 +941,6 @@ __global__ __launch_bounds__(kThreads, 2) void attention_many_kernel(const Args 
                     l_run[rt] += p;
                 }
         }
-        if (kMasked && odd) {
-            // Values that are not finite go to the rows that see them by hand,
-            // whatever their weight: 0 times them would not be 0.
-            for (int j = 0; j < KT; ++j) {
-                if (!(bits >> (j / 16) & 1)) continue;
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    if (t * KT + j > limit_key[rt]) continue;
-#pragma unroll
-                    for (int db = 0; db < ND; ++db)
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const int at = (32 * db + 8 * (e / 4) + 4 * lh + e % 4) * static_cast<int>(sizeof(T));
-                            const float x = widen(*reinterpret_cast<const T*>(vt + j * kRowBytes +
-                                                                              16 * ((at / 16) ^ L::swap(j)) + at % 16));
-                            if (!(fabsf(x) < INFINITY)) acc[rt][db][e] += x;
-                        }
-                }
-            }
-        }
         if constexpr (kWide) {
 #pragma unroll
             for (int n = 0; n < NK; ++n)
@@ -940,11 +950,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_many_kernel(const Args 
                     for (int db = 0; db < ND; ++db) {
                         const int row = 32 * n + 8 * (e / 4) + 4 * lh + e % 4;
                         const int c = 8 * db + lc / 4;
-                        uint32_t x = *reinterpret_cast<const uint32_t*>(vt + row * kRowBytes + 16 * (c ^ L::swap(row)) + 4 * (lc & 3));
-                        if (kMasked && odd) x = finite_elements<T>(x);
+                        const float x = *reinterpret_cast<const float*>(vt + row * kRowBytes + 16 * (c ^ L::swap(row)) + 4 * (lc & 3));
 #pragma unroll
                         for (int rt = 0; rt < RT; ++rt)
-                            acc[rt][db] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(x), st[rt][n][e], acc[rt][db], 0, 0, 0);
+                            acc[rt][db] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, st[rt][n][e], acc[rt][db], 0, 0, 0);
                     }
         } else {
             const int l16 = lane & 15;
@@ -973,36 +982,54 @@ __global__ __launch_bounds__(kThreads, 2) void attention_many_kernel(const Args 
                                 (__attribute__((address_space(3))) s16x4*)(at));
                             __builtin_memcpy(x + 2 * w, &y, 8);
                         }
-                        u32x4 vf{x[0], x[1], x[2], x[3]};
-                        if (kMasked && odd) {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) vf[e] = finite_elements<T>(vf[e]);
-                        }
+                        const u32x4 vf{x[0], x[1], x[2], x[3]};
 #pragma unroll
                         for (int rt = 0; rt < RT; ++rt) acc[rt][db] = mfma32<T>(vf, pf[rt], acc[rt][db]);
                     }
                 }
         }
     };
+    // The values of a tile that are not finite, to the rows that see them,
+    // whatever their weight: 0 times them would not be 0.
+    const auto add_odd = [&](int t, unsigned bits) {
+        for (int j = 0; j < KT; ++j) {
+            if (!(bits >> (j / 16) & 1)) continue;
+            const int key = min(t * KT + j, q.length - 1);
+            int64_t at;
+            if constexpr (kPaged)
+                at = ((((static_cast<int64_t>(table[key >> a.shift]) * a.kv_heads) << a.shift) + kv_row + (key & in_page)) * D);
+            else
+                at = static_cast<int64_t>(q.start + key) * a.v_stride + kh * D;
+            const T* vp = static_cast<const T*>(a.v) + at + 4 * lh;
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                if (t * KT + j > limit_key[rt]) continue;
+#pragma unroll
+                for (int db = 0; db < ND; ++db)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float x = widen(vp[32 * db + 8 * (e / 4) + e % 4]);
+                        if (!(fabsf(x) < INFINITY)) acc[rt][db][e] += x;
+                    }
+            }
+        }
+    };
 
-    const auto partly = [&](int t, unsigned bits) { return (t + 1) * KT > whole || bits != (1u << (KT / 16)) - 1; };
     if (first < last) {
         Ids next = lookup(first + 1);
-        bool odd = publish(first & 1, partly(first, pages_there));
         for (int t = first; t < last; ++t) {
-            unsigned bits = pages_there;
+            const unsigned bits = pages_there;
+            const bool all_there = bits == (1u << (KT / 16)) - 1;
+            const bool odd = arrive(t, (t + 1) * KT > whole || !all_there);
+            // (the other buffer's tile is behind all waves)
             if (t + 1 < last) {
                 pages_there = there(next);
                 load(t + 1, next);
                 next = lookup(t + 2);
             }
-            if (t * KT < wave_seen) {
-                if ((t + 1) * KT <= wave_whole && bits == (1u << (KT / 16)) - 1)
-                    compute(std::false_type{}, t, t & 1, bits, false);
-                else
-                    compute(std::true_type{}, t, t & 1, bits, odd);
-            }
-            if (t + 1 < last) odd = publish((t + 1) & 1, partly(t + 1, pages_there));
+            if (t * KT >= wave_seen) continue;
+            if (odd) add_odd(t, bits);
+            compute(t, (t + 1) * KT > wave_whole || !all_there, bits);
         }
     }
 
