@@ -45,7 +45,8 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kMaxBatch = VM_HIP_PAGED_MAX_BATCH;
 constexpr int kMaxSplits = 64;        // workgroups that share a request's keys: few rows,
-constexpr int kManySplits = 16;       // many rows
+constexpr int kManySplits = 28;       // many rows
+constexpr int kManyLeast = 512;       // keys that are worth a workgroup there
 constexpr int kTargetGroups = 512;    // workgroups that fill 256 compute units twice
 constexpr int kTicketStride = 16;     // a ticket has a 64-byte line of its own
 constexpr int64_t kTicketBytes = kTargetGroups * kTicketStride * 4;
@@ -68,10 +69,9 @@ struct Args {
     int64_t q_stride, k_stride, v_stride;   // elements
     int64_t max_pages, pages;
     int batch, rows, max_rows, heads, kv_heads, shift;
-    int few;      // query rows up to which a request is attention_few_kernel's
-    int splits;   // attention_many_kernel: workgroups that share a tile's keys
-    int slots;    // tiles that a KV head's requests may have
-    float c;      // scale / ln 2
+    int few;          // query rows up to which a request is attention_few_kernel's
+    int max_splits;   // attention_many_kernel: workgroups that may share a tile's keys
+    float c;   // scale / ln 2
 };
 
 // A request's rows and the tokens in front of them.
@@ -235,28 +235,92 @@ __device__ __forceinline__ void join_parts(const Args& a, const Request& q, int 
         if (s0 == 0) totals[row] = l;
     }
     __syncthreads();
-    for (int item = threadIdx.x; item < kRows * D / 4; item += kThreads) {
-        const int row = item / (D / 4), d4 = item % (D / 4);
-        float y[4] = {0.f, 0.f, 0.f, 0.f};
+    // Four items of a thread and eight parts at a time, 32 loads in flight.
+    constexpr int kItems = kRows * D / 4 / kThreads;
+    constexpr int kTake = kItems < 4 ? kItems : 4;
+    for (int i0 = 0; i0 < kItems; i0 += kTake) {
+        float y[kTake][4] = {};
         for (int s0 = 0; s0 < active; s0 += 8) {
-            u32x4 x[8];
-#pragma unroll
-            for (int u = 0; u < 8; ++u)
-                if (s0 + u < active)
-                    x[u] = coherent_load16(buffer_rsrc(a.parts + part(s0 + u), kRows * D * 4), item * 16);
+            u32x4 x[kTake][8];
 #pragma unroll
             for (int u = 0; u < 8; ++u)
                 if (s0 + u < active) {
-                    const float f = factors[(s0 + u) * kRows + row];
+                    const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(a.parts + part(s0 + u), kRows * D * 4);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) y[e] = fmaf(__uint_as_float(x[u][e]), f, y[e]);
+                    for (int i = 0; i < kTake; ++i) x[i][u] = coherent_load16(rs, ((i0 + i) * kThreads + threadIdx.x) * 16);
+                }
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (s0 + u < active) {
+#pragma unroll
+                    for (int i = 0; i < kTake; ++i) {
+                        const float f = factors[(s0 + u) * kRows + ((i0 + i) * kThreads + threadIdx.x) / (D / 4)];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) y[i][e] = fmaf(__uint_as_float(x[i][u][e]), f, y[i][e]);
+                    }
                 }
         }
-        put<T>(a, q, kh, g, r0 + row, 4 * d4, y, totals[row], D);
+#pragma unroll
+        for (int i = 0; i < kTake; ++i) {
+            const int item = (i0 + i) * kThreads + threadIdx.x, row = item / (D / 4);
+            put<T>(a, q, kh, g, r0 + row, 4 * (item % (D / 4)), y[i], totals[row], D);
+        }
     }
 }
 
 constexpr int64_t part_bytes(int64_t rows, int64_t d) { return rows * (d + 2) * 4; }
+
+// Running sums, up to and with each request, of what count(b) says of it, by
+// the whole workgroup; their total and, if asked, the largest count.
+struct Sums {
+    int upto[kMaxBatch];
+    int waves[kWaves], most[kWaves];
+};
+template <typename Count>
+__device__ __forceinline__ int sum_requests(int batch, Sums& s, Count count, int* largest) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int each = (batch + kThreads - 1) / kThreads, b0 = threadIdx.x * each;
+    int sum = 0, most = 0;
+    for (int b = b0; b < min(b0 + each, batch); ++b) {
+        const int w = count(b);
+        sum += w;
+        most = max(most, w);
+        s.upto[b] = sum;
+    }
+    int run = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_up(run, o, 64);
+        if (lane >= o) run += x;
+        if (largest) most = max(most, __shfl_xor(most, o, 64));
+    }
+    if (lane == 63) s.waves[wave] = run, s.most[wave] = most;
+    __syncthreads();
+    int before = run - sum, total = 0;
+    most = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        if (w < wave) before += s.waves[w];
+        total += s.waves[w];
+        most = max(most, s.most[w]);
+    }
+    if (largest) *largest = most;
+    for (int b = b0; b < min(b0 + each, batch); ++b) s.upto[b] += before;
+    __syncthreads();
+    return total;
+}
+// The first request whose running sum is above x.
+__device__ __forceinline__ int request_of(const Sums& s, int batch, int x) {
+    int lo = 0, hi = batch - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (s.upto[mid] > x)
+            hi = mid;
+        else
+            lo = mid + 1;
+    }
+    return __builtin_amdgcn_readfirstlane(lo);
+}
 
 // Clears the ticket and says whether this workgroup drew the last one.
 __device__ __forceinline__ bool last_arrival(unsigned* counter, int active, unsigned* drawn) {
@@ -291,8 +355,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_few_kernel(const Args a
     constexpr int kRows = 16 * RT;
     __shared__ __align__(16) float merge_o[kWaves][kRows * D];
     __shared__ float merge_m[kWaves][kRows], merge_l[kWaves][kRows];
-    __shared__ int work[kMaxBatch];              // rounds of the requests up to this one, of a KV head
-    __shared__ int waves_sum[kWaves], waves_max[kWaves];
+    __shared__ Sums sums;                        // rounds of a KV head
     __shared__ unsigned ticket;
 
     const int lane = threadIdx.x & 63;
@@ -304,37 +367,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_few_kernel(const Args a
     };
 
     // Rounds of all requests, summed up by every workgroup for itself.
-    int total, longest;
-    {
-        const int each = (a.batch + kThreads - 1) / kThreads, b0 = threadIdx.x * each;
-        int sum = 0, most = 0;
-        for (int b = b0; b < min(b0 + each, a.batch); ++b) {
-            const int w = rounds_of(request<true>(a, b));
-            sum += w;
-            most = max(most, w);
-            work[b] = sum;
-        }
-        int run = sum;
-#pragma unroll
-        for (int s = 1; s < 64; s <<= 1) {
-            const int o = __shfl_up(run, s, 64);
-            if (lane >= s) run += o;
-            most = max(most, __shfl_xor(most, s, 64));
-        }
-        if (lane == 63) waves_sum[wave] = run, waves_max[wave] = most;
-        __syncthreads();
-        int before = run - sum;
-        total = longest = 0;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            if (w < wave) before += waves_sum[w];
-            total += waves_sum[w];
-            longest = max(longest, waves_max[w]);
-        }
-        for (int b = b0; b < min(b0 + each, a.batch); ++b) work[b] += before;
-        __syncthreads();
-    }
-    total *= a.kv_heads;
+    int longest;
+    const int total = a.kv_heads * sum_requests(a.batch, sums, [&](int b) { return rounds_of(request<true>(a, b)); }, &longest);
     // Shares: even, worth a workgroup, and no more than kMaxSplits of a request's keys.
     const int per = max(max((total + kTargetGroups - 1) / kTargetGroups, kLeast),
                         (longest + kMaxSplits - 2) / (kMaxSplits - 1));
@@ -343,18 +377,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_few_kernel(const Args a
 
     while (pos < end) {
         // The request, KV head and rounds that this share goes on with.
-        int lo = 0, hi = a.batch - 1;            // the first request with more rounds than pos / kv_heads
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (work[mid] * a.kv_heads > pos)
-                hi = mid;
-            else
-                lo = mid + 1;
-        }
-        const int b = __builtin_amdgcn_readfirstlane(lo);
+        const int b = request_of(sums, a.batch, pos / a.kv_heads);
         const Request q = request<true>(a, b);
         const int rounds = rounds_of(q);
-        const int request_start = (work[b] - rounds) * a.kv_heads;
+        const int request_start = (sums.upto[b] - rounds) * a.kv_heads;
         const int kh = (pos - request_start) / rounds;
         const int unit_start = request_start + kh * rounds;
         const int first = pos - unit_start, last = min(rounds, end - unit_start);
@@ -371,68 +397,56 @@ __global__ __launch_bounds__(kThreads, 2) void attention_few_kernel(const Args a
         const int last_page = max(q.length - 1, 0) >> a.shift;
         const int whole = min(q.p0 + 1, q.length);   // keys that every row sees
 
-        struct Ids {
-            int k, v;
-        };
-        // (a block's keys have one page, or, of 16 tokens, two)
-        const auto lookup = [&](int block) {
-            Ids i;
-            i.k = table[min((block * KB + (kWide ? 0 : 8 * (lr / 4))) >> a.shift, last_page)];
-            i.v = table[min((block * KB + KPL * lg) >> a.shift, last_page)];
-            return i;
-        };
-        struct Block {
-            u32x4 k[NT][KC];
-            uint32_t v[KPL][VW];
-            bool there;   // the page of this lane's keys
-        };
-        const auto load = [&](int block, Ids ids, Block& c) {
-            const int k0 = block * KB;
-            const bool k_there = ids.k >= 0 && ids.k < a.pages;
-            c.there = ids.v >= 0 && ids.v < a.pages;
-            const char* kp = kbase + (k_there ? ids.k : 0) * page_bytes + 16 * lg;
-            const char* vp = vbase + (c.there ? ids.v : 0) * page_bytes + 4 * VW * lr;
-#pragma unroll
-            for (int bt = 0; bt < NT; ++bt) {
-                const int key = k0 + (kWide ? lr : 8 * (lr / 4) + 4 * bt + lr % 4);
-                const char* p = kp + (key & in_page) * row_bytes;
-#pragma unroll
-                for (int s = 0; s < KC; ++s) c.k[bt][s] = *reinterpret_cast<const u32x4*>(p + 64 * s);
-            }
-#pragma unroll
-            for (int j = 0; j < KPL; ++j) {
-                const char* p = vp + ((k0 + KPL * lg + j) & in_page) * row_bytes;
-                if constexpr (kWide) {
-                    // (rows of 64 dims apart: tile 4 h + u)
-                    const char* pw = vbase + (c.there ? ids.v : 0) * page_bytes + 16 * lr + ((k0 + KPL * lg + j) & in_page) * row_bytes;
-#pragma unroll
-                    for (int h = 0; h < D / 64; ++h) {
-                        const u32x4 x = *reinterpret_cast<const u32x4*>(pw + 256 * h);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) c.v[j][4 * h + e] = x[e];
-                    }
-                } else if constexpr (VW == 4) {
-                    const u32x4 x = *reinterpret_cast<const u32x4*>(p);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) c.v[j][e] = x[e];
-                } else {
-                    const u32x2 x = *reinterpret_cast<const u32x2*>(p);
-                    c.v[j][0] = x.x;
-                    c.v[j][1] = x.y;
-                }
-            }
-        };
-
         // This wave's blocks: round r's keys are shared out in turn.
         constexpr int kStep = kRound / KB;   // blocks of a round
         const int block_end = min(last * kStep, (q.length + KB - 1) / KB);
         int block = first * kStep + wave;
-        Ids ids{0, 0};
-        Block c0, c1;
+        // (a block's keys have one page, or, of 16 tokens, two)
+        const auto page_of = [&](int block, int octet) {
+            return table[min((min(block, block_end - 1) * KB + octet) >> a.shift, last_page)];
+        };
+        const int k_at = kWide ? 0 : 8 * (lr / 4), v_at = KPL * lg;   // this lane's keys of a block
+        const auto valid = [&](int id) { return id >= 0 && id < a.pages; };
+        // Loads go on past the last block with that block again: without a
+        // branch around them, waits need not be for all.
+        u32x4 kreg[NT][KC];
+        uint32_t vreg[KPL][VW];
+        const auto load_keys = [&](int block, int id) {
+            const int at = (min(block, block_end - 1) * KB + k_at) & in_page;
+            const char* p = kbase + (valid(id) ? id : 0) * page_bytes + (at + (kWide ? lr : lr % 4)) * row_bytes + 16 * lg;
+#pragma unroll
+            for (int bt = 0; bt < NT; ++bt)
+#pragma unroll
+                for (int s = 0; s < KC; ++s) kreg[bt][s] = *reinterpret_cast<const u32x4*>(p + 4 * bt * row_bytes + 64 * s);
+        };
+        const auto load_values = [&](int block, int id) {
+            const int at = (min(block, block_end - 1) * KB + v_at) & in_page;
+            const char* p = vbase + (valid(id) ? id : 0) * page_bytes + at * row_bytes + (kWide ? 16 : 4 * VW) * lr;
+#pragma unroll
+            for (int j = 0; j < KPL; ++j) {
+                if constexpr (VW == 2) {
+                    const u32x2 x = *reinterpret_cast<const u32x2*>(p + j * row_bytes);
+                    vreg[j][0] = x.x;
+                    vreg[j][1] = x.y;
+                } else {   // (fp32: rows of 64 dims apart, tiles 4 h + u)
+#pragma unroll
+                    for (int h = 0; h < VW / 4; ++h) {
+                        const u32x4 x = *reinterpret_cast<const u32x4*>(p + j * row_bytes + 256 * h);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) vreg[j][4 * h + e] = x[e];
+                    }
+                }
+            }
+        };
+
+        int id_k = 0, id_v = 0, next_k = 0, next_v = 0;
         if (block < block_end) {
-            ids = lookup(block);
-            load(block, ids, c0);
-            ids = lookup(block + kWaves);
+            id_k = page_of(block, k_at);
+            id_v = page_of(block, v_at);
+            next_k = page_of(block + kWaves, k_at);
+            next_v = page_of(block + kWaves, v_at);
+            load_keys(block, id_k);
+            load_values(block, id_v);
         }
 
         u32x4 qf[RT][KC];
@@ -462,9 +476,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_few_kernel(const Args a
             limit[rt] = -INFINITY;
         }
 
-        const auto compute = [&](auto masked_tag, int block, Block& c) {
-            constexpr bool kMasked = decltype(masked_tag)::value;
-            const int key0 = block * KB + KPL * lg;
+        for (; block < block_end; block += kWaves) {
+            const bool there = valid(id_v);
             f32x4 st[RT][NT];
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
@@ -480,18 +493,20 @@ __global__ __launch_bounds__(kThreads, 2) void attention_few_kernel(const Args a
 #pragma unroll
                             for (int e = 0; e < 4; ++e)
                                 st[rt][bt] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                                    __uint_as_float(c.k[bt][s][e]), __uint_as_float(qf[rt][s][e]), st[rt][bt], 0, 0, 0);
+                                    __uint_as_float(kreg[bt][s][e]), __uint_as_float(qf[rt][s][e]), st[rt][bt], 0, 0, 0);
                         } else {
-                            st[rt][bt] = mfma16<T>(c.k[bt][s], qf[rt][s], st[rt][bt]);
+                            st[rt][bt] = mfma16<T>(kreg[bt][s], qf[rt][s], st[rt][bt]);
                         }
                     }
-            bool odd = false;   // a value that is not finite, where not every row sees it
-            if (kMasked) {
+            load_keys(block + kWaves, next_k);
+            const bool masked = (block + 1) * KB > whole || !__all(there);
+            if (masked) {
+                const int key0 = block * KB + v_at;
 #pragma unroll
-                for (int j = 0; j < KPL; ++j)
+                for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-                    for (int u = 0; u < VW; ++u) odd |= odd_element<T>(c.v[j][u]);
-                odd = __any(odd);
+                    for (int j = 0; j < KPL; ++j)
+                        if (!(there && key0 + j <= limit_key[rt])) st[rt][j / 4][j % 4] = -INFINITY;
             }
             float mt[RT];
             bool moves = false;
@@ -499,10 +514,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_few_kernel(const Args a
             for (int rt = 0; rt < RT; ++rt) {
                 mt[rt] = -INFINITY;
 #pragma unroll
-                for (int j = 0; j < KPL; ++j) {
-                    if (kMasked && !(c.there && key0 + j <= limit_key[rt])) st[rt][j / 4][j % 4] = -INFINITY;
-                    mt[rt] = fmaxf(mt[rt], st[rt][j / 4][j % 4]);
-                }
+                for (int j = 0; j < KPL; ++j) mt[rt] = fmaxf(mt[rt], st[rt][j / 4][j % 4]);
                 moves |= mt[rt] > limit[rt];
             }
             if (__any(moves)) {
@@ -532,30 +544,38 @@ __global__ __launch_bounds__(kThreads, 2) void attention_few_kernel(const Args a
                     l_run[rt] += p[rt][j];
                 }
             }
-            if (kMasked && odd) {
-                // Values that are not finite go to the rows that see them by
-                // hand, whatever their weight: 0 times them would not be 0.
-                for (int j = 0; j < KB; ++j) {
-                    const int key = block * KB + j;
-                    const int id = table[min(key >> a.shift, last_page)];
-                    if (id < 0 || id >= a.pages) continue;
-                    const T* vp = reinterpret_cast<const T*>(vbase + id * page_bytes + (key & in_page) * row_bytes);
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) {
-                        if (key > limit_key[rt]) continue;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-#pragma unroll
-                            for (int db = 0; db < ND; ++db) {
-                                const float x = widen(vp[kWide ? 64 * (db / 4) + 16 * lg + 4 * e + db % 4 : ND * (4 * lg + e) + db]);
-                                if (!(fabsf(x) < INFINITY)) acc[rt][db][e] += x;
-                            }
-                    }
-                }
+            if (masked) {
+                // Values that are not finite, where not every row sees them: to
+                // the rows that do by hand, whatever their weight (0 times them
+                // would not be 0).
+                bool odd = false;
 #pragma unroll
                 for (int j = 0; j < KPL; ++j)
 #pragma unroll
-                    for (int u = 0; u < VW; ++u) c.v[j][u] = finite_elements<T>(c.v[j][u]);
+                    for (int u = 0; u < VW; ++u) {
+                        odd |= odd_element<T>(vreg[j][u]);
+                        vreg[j][u] = finite_elements<T>(vreg[j][u]);
+                    }
+                if (__any(odd)) {
+                    for (int j = 0; j < KB; ++j) {
+                        const int key = block * KB + j;
+                        const int id = table[min(key >> a.shift, last_page)];
+                        if (!valid(id)) continue;
+                        const T* vp = reinterpret_cast<const T*>(vbase + id * page_bytes + (key & in_page) * row_bytes);
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt) {
+                            if (key > limit_key[rt]) continue;
+                            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                                for (int db = 0; db < ND; ++db) {
+                                    const float x = widen(vp[kWide ? 64 * (db / 4) + 16 * lg + 4 * e + db % 4 : ND * (4 * lg + e) + db]);
+#pragma unroll
+                                    for (int w = 0; w < 4; ++w)
+                                        if (w == e && !(fabsf(x) < INFINITY)) acc[rt][db][w] += x;
+                                }
+                        }
+                    }
+                }
             }
             if constexpr (kWide) {
 #pragma unroll
@@ -564,7 +584,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_few_kernel(const Args a
                     for (int j = 0; j < KPL; ++j)
 #pragma unroll
                         for (int rt = 0; rt < RT; ++rt)
-                            acc[rt][db] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(c.v[j][db]), p[rt][j], acc[rt][db], 0, 0, 0);
+                            acc[rt][db] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vreg[j][db]), p[rt][j], acc[rt][db], 0, 0, 0);
             } else {
                 u32x4 pf[RT];
 #pragma unroll
@@ -574,28 +594,16 @@ __global__ __launch_bounds__(kThreads, 2) void attention_few_kernel(const Args a
                     u32x4 vf;
 #pragma unroll
                     for (int jp = 0; jp < 4; ++jp)
-                        vf[jp] = __builtin_amdgcn_perm(c.v[2 * jp + 1][db / 2], c.v[2 * jp][db / 2],
+                        vf[jp] = __builtin_amdgcn_perm(vreg[2 * jp + 1][db / 2], vreg[2 * jp][db / 2],
                                                        db % 2 ? 0x07060302u : 0x05040100u);
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt) acc[rt][db] = mfma16<T>(vf, pf[rt], acc[rt][db]);
                 }
             }
-        };
-        const auto step = [&](Block& now, Block& next) {
-            if (block + kWaves < block_end) {
-                load(block + kWaves, ids, next);
-                ids = lookup(block + 2 * kWaves);
-            }
-            if ((block + 1) * KB <= whole && __all(now.there))
-                compute(std::false_type{}, block, now);
-            else
-                compute(std::true_type{}, block, now);
-            block += kWaves;
-        };
-        while (block < block_end) {
-            step(c0, c1);
-            if (block >= block_end) break;
-            step(c1, c0);
+            load_values(block + kWaves, next_v);
+            id_v = next_v;
+            next_k = page_of(block + 2 * kWaves, k_at);
+            next_v = page_of(block + 2 * kWaves, v_at);
         }
 
         // Every wave's (reference, sum, output) to LDS; then thread (row, four
@@ -690,6 +698,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_many_kernel(const Args 
     constexpr int kRows = 32 * RT * kWaves;
     constexpr int kRowBytes = D * sizeof(T);
     __shared__ __align__(16) char lds[2][2][L::kBytes];   // [buffer][keys, values]
+    __shared__ Sums sums;                                 // tiles of a KV head
     __shared__ unsigned ticket;
 
     const int lane = threadIdx.x & 63;
@@ -697,49 +706,38 @@ __global__ __launch_bounds__(kThreads, 2) void attention_many_kernel(const Args 
     const int lc = lane & 31, lh = lane >> 5;
     const int g = a.heads / a.kv_heads;
 
+    // Tiles of all requests, and the workgroups that share a tile's keys.
+    const int tiles_all = sum_requests(a.batch, sums, [&](int b) {
+        const int r = request<kPaged>(a, b).todo * g;
+        return r > a.few ? (r + kRows - 1) / kRows : 0;
+    }, nullptr);
+    if (tiles_all == 0) return;
+    const int splits = max(min(kTargetGroups / (tiles_all * a.kv_heads), a.max_splits), 1);
+    const int shares = a.kv_heads * splits;
+    const int id = static_cast<int>(blockIdx.x);
+    if (id >= tiles_all * shares) return;
     // Workgroups go to the XCDs in turn: the tiles of a (KV head, share of the
     // keys) stay on one where the count of those allows, the last tiles, which
     // see the most keys, first.
     int slot, share;
-    {
-        const int id = static_cast<int>(blockIdx.x), shares = a.kv_heads * a.splits;
-        if (shares % 8 == 0) {
-            const int j = id / 8;
-            slot = a.slots - 1 - j % a.slots;
-            share = j / a.slots * 8 + id % 8;
-        } else {
-            slot = a.slots - 1 - id / shares;
-            share = id % shares;
-        }
+    if (shares % 8 == 0) {
+        const int j = id / 8;
+        slot = tiles_all - 1 - j % tiles_all;
+        share = j / tiles_all * 8 + id % 8;
+    } else {
+        slot = tiles_all - 1 - id / shares;
+        share = id % shares;
     }
     const int kh = share % a.kv_heads, split = share / a.kv_heads;
-
-    // Request b's tiles have the slots from row_start[b] G / kRows + b on (a
-    // slot more than it may need).
-    const auto first_slot = [&](int b) {
-        return static_cast<int>(static_cast<int64_t>(min(max(a.row_start[b], 0), a.rows)) * g / kRows) + b;
-    };
-    int b = 0;
-    for (int width = a.batch; width > 1;) {
-        // the last of 64 probes that starts at or before the slot
-        const int stride = (width + 63) / 64;
-        const int at = b + lane * stride;
-        const bool below = lane * stride < width && first_slot(at) <= slot;
-        const int n = max(__popcll(__ballot(below)), 1) - 1;
-        b += n * stride;
-        width = min(stride, width - n * stride);
-    }
-    b = __builtin_amdgcn_readfirstlane(b);
+    const int b = request_of(sums, a.batch, slot);
     const Request q = request<kPaged>(a, b);
-    const int tile = slot - first_slot(b);
-    const int r0 = tile * kRows;
-    if (tile < 0 || r0 >= q.todo * g || q.todo * g <= a.few) return;
+    const int r0 = (slot - (sums.upto[b] - (q.todo * g + kRows - 1) / kRows)) * kRows;
     const int t_last = min((r0 + kRows - 1) / g, q.todo - 1);
     const int seen = min(max(q.p0 + t_last + 1, 0), q.length);      // keys that some row sees
     const int whole = min(max(q.p0 + r0 / g + 1, 0), q.length);     // that every row sees
     const int tiles = (seen + KT - 1) / KT;
-    const int each = (tiles + a.splits - 1) / a.splits;
-    const int active = each > 0 ? (tiles + each - 1) / each : 1;
+    const int each = max((tiles + splits - 1) / splits, kManyLeast / KT);
+    const int active = max((tiles + each - 1) / each, 1);
     if (split >= active) return;
     const int first = split * each, last = min(tiles, first + each);
 
@@ -1034,7 +1032,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_many_kernel(const Args 
     }
 
     const auto part = [&](int s) {
-        return ((static_cast<int64_t>(kh) * a.slots + slot) * a.splits + s) * part_bytes(kRows, D);
+        return ((static_cast<int64_t>(kh) * tiles_all + slot) * splits + s) * part_bytes(kRows, D);
     };
     char* out_part = a.parts + (active > 1 ? part(split) : 0);
 #pragma unroll
@@ -1061,7 +1059,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_many_kernel(const Args 
     }
     if (active > 1) {
         __syncthreads();   // (LDS is free)
-        if (last_arrival(a.tickets + (kh * a.slots + slot) * kTicketStride, active, &ticket)) {
+        if (last_arrival(a.tickets + (kh * tiles_all + slot) * kTicketStride, active, &ticket)) {
             float* f = reinterpret_cast<float*>(lds[0][0]);
             static_assert((kManySplits + 1) * kRows * 4 <= static_cast<int>(sizeof lds), "factors fit");
             join_parts<T, D, kRows>(a, q, kh, g, r0, active, part, f, f + kManySplits * kRows);
@@ -1078,8 +1076,8 @@ struct Plan {
     bool few, many;
     int few_tiles;        // RT of attention_few_kernel
     int few_rows;         // query rows up to which a request is its
-    int splits;
-    int64_t slots;
+    int max_splits;
+    int64_t many_groups;
     int64_t bytes;        // of the workspace: tickets, then parts; the kernels run one after the other
 };
 
@@ -1098,11 +1096,10 @@ Plan plan(int64_t batch, int64_t rows, int64_t max_rows, int64_t heads, int64_t 
     if (p.few) p.bytes = kTicketBytes + 2 * kTargetGroups * part_bytes(16 * p.few_tiles, d);
     if (p.many) {
         const int64_t tile = 32 * many_tiles(d, wide) * kWaves;
-        p.slots = rows * g / tile + batch;
-        const int64_t units = p.slots * kv_heads;
-        const int64_t share = std::max<int64_t>(1, max_tokens / 256);   // 256 keys are worth a workgroup
-        p.splits = static_cast<int>(std::max<int64_t>(1, std::min({kTargetGroups / units, static_cast<int64_t>(kManySplits), share})));
-        if (share > 1) p.bytes = std::max(p.bytes, kTicketBytes + kTargetGroups * part_bytes(tile, d));
+        const int64_t units = (rows * g / tile + batch) * kv_heads;   // at most
+        p.max_splits = max_tokens > kManyLeast ? kManySplits : 1;
+        p.many_groups = p.max_splits > 1 ? std::max<int64_t>(units, kTargetGroups) : units;
+        if (p.max_splits > 1) p.bytes = std::max(p.bytes, kTicketBytes + kTargetGroups * part_bytes(tile, d));
     }
     return p;
 }
@@ -1147,18 +1144,16 @@ template <typename T, int D>
 void launch_type(const Args& a, const Plan& p, bool paged, hipStream_t s) {
     if (p.few) launch_few<T, D>(a, p.few_tiles, s);
     if (p.many) {
-        const int64_t grid = p.slots * a.kv_heads * p.splits;
         if (paged)
-            launch_many<T, D, true>(a, grid, s);
+            launch_many<T, D, true>(a, p.many_groups, s);
         else
-            launch_many<T, D, false>(a, grid, s);
+            launch_many<T, D, false>(a, p.many_groups, s);
     }
 }
 
 int run(const char* who, Args a, const Plan& p, int dtype, int64_t d, bool paged, void* workspace, void* stream) {
     a.few = p.few_rows;
-    a.splits = std::max(p.splits, 1);
-    a.slots = static_cast<int>(p.slots);
+    a.max_splits = p.max_splits;
     a.tickets = static_cast<unsigned*>(workspace);
     a.parts = static_cast<char*>(workspace) + kTicketBytes;
     auto s = static_cast<hipStream_t>(stream);
@@ -1224,7 +1219,7 @@ int vm_hip_attention_packed(const void* q, const void* k, const void* v, void* o
     if (need > 0 && (!workspace || workspace_bytes < need || off16(workspace)))
         return fail_inval("attention_packed: workspace smaller than vm_hip_attention_packed_workspace_bytes or unaligned");
     const Plan p = plan(batch, rows, 0, heads, kv_heads, head_dim, rows, dtype == VM_HIP_DTYPE_F32, false);
-    if (p.slots * kv_heads * p.splits >= (1 << 24)) return fail_inval("attention_packed: too many rows for one call");
+    if (p.many_groups >= (1 << 24)) return fail_inval("attention_packed: too many rows for one call");
     Args a{};
     a.q = q;
     a.k = k;
@@ -1273,7 +1268,7 @@ int vm_hip_attention_paged(const vm_hip_kv_paged* cache, const int32_t* tables, 
     if (need > 0 && (!workspace || workspace_bytes < need || off16(workspace)))
         return fail_inval("attention_paged: workspace smaller than vm_hip_attention_paged_workspace_bytes or unaligned");
     const Plan p = plan(batch, rows, max_rows, heads, hk, d, tokens, cache->dtype == VM_HIP_DTYPE_F32, true);
-    if (p.many && p.slots * hk * p.splits >= (1 << 24)) return fail_inval("attention_paged: too many rows for one call");
+    if (p.many_groups >= (1 << 24)) return fail_inval("attention_paged: too many rows for one call");
     Args a{};
     a.q = q;
     a.k = cache->k;
