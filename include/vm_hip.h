@@ -1046,7 +1046,7 @@ int vm_hip_qk_norm_rope(const void* qkv, int dtype, int64_t rows, int64_t heads,
 /* Causal attention of whole prompts that lie one behind the other: row i of
  * request b (rows row_start[b] + i) sees the request's rows 0 .. i.
  *   q, k, v  rows of dtype, q_stride, k_stride, v_stride elements apart (each a
- *            multiple of 16 bytes), query head h at h * head_dim of its row,
+ *            multiple of 16 bytes, at most 2^22), query head h at h * head_dim of its row,
  *            with KV head h / (heads / kv_heads); they may be parts of one
  *            projection's rows
  *   out      [rows, heads * head_dim] of dtype; all 16-byte aligned
@@ -1080,7 +1080,7 @@ int vm_hip_attention_packed(const void* q, const void* k, const void* v, void* o
  *        planned); a request's rows past it are left as they were.  0: not
  *        known.  Kernels and the workspace are chosen by it: 1 where all
  *        requests decode.
- * max_pages * page_size <= 2^30, and times batch * kv_heads below 2^38.
+ * max_pages * page_size <= 2^24, and times batch * kv_heads below 2^38.
  * row_start and lengths are held to [0, rows] and [0, max_pages * page_size];
  * tokens in table entries that are no page do not exist; a row that sees none
  * gets zeros.  Roundings, scores, infinities, scale and the workspace are those

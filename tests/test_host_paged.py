@@ -135,9 +135,9 @@ def test_attention_paged_arguments():
     _each_refused(H.attention_paged, ok,
                   [(i, None) for i in (1, 3, 4, 9, 10, 12)] + [(i, P + 8) for i in (3, 4, 12)]
                   + [(i, P + 2) for i in (1, 9, 10)]
-                  + [(2, 0), (2, (1 << 26) + 1), (5, -1), (5, 2049), (6, -1), (6, (1 << 24) + 1), (7, -1), (8, 3), (8, 0),
+                  + [(2, 0), (2, (1 << 20) + 1), (5, -1), (5, 2049), (6, -1), (6, (1 << 24) + 1), (7, -1), (8, 3), (8, 0),
                      (8, 1 << 20), (11, math.inf), (11, math.nan), (13, 0)])
-    _refused(H.attention_paged, _cache(kv_heads=4096), P, 1 << 26, P, P, 2048, 5, 3, 4096, P, P, 0.0, P, 1 << 40)
+    _refused(H.attention_paged, _cache(kv_heads=4096), P, 1 << 20, P, P, 2048, 5, 3, 4096, P, P, 0.0, P, 1 << 40)
     H.attention_paged(_cache(), None, 4, None, None, 0, 5, 3, 4, None, None, 0.0, None, 0)
     H.attention_paged(_cache(), None, 4, None, None, 2, 0, 3, 4, None, None, 0.0, None, 0)
 
@@ -153,6 +153,6 @@ def test_attention_workspaces():
             assert H.attention_packed_workspace_bytes(batch, 100, heads, hk, d) >= 0
     _refused(H.attention_paged_workspace_bytes, 1, 1, 1, 4, 3, 64, 16)
     _refused(H.attention_paged_workspace_bytes, 1, 1, 1, 4, 2, 64, 0)
-    _refused(H.attention_paged_workspace_bytes, 1, 1, 1, 4, 2, 64, (1 << 30) + 1)
+    _refused(H.attention_paged_workspace_bytes, 1, 1, 1, 4, 2, 64, (1 << 24) + 1)
     _refused(H.attention_packed_workspace_bytes, 1, 1, 4, 2, 32)
     assert H.attention_paged_workspace_bytes(0, 5, 1, 4, 2, 64, 16) == 0

@@ -46,7 +46,8 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kMaxBatch = VM_HIP_PAGED_MAX_BATCH;
 constexpr int kMaxSplits = 64;        // workgroups that share a request's keys: few rows,
 constexpr int kManySplits = 28;       // many rows
-constexpr int kManyLeast = 512;       // keys that are worth a workgroup there
+constexpr int kMaxShared = 1024;      // row tiles of a KV head that may share workgroups,
+constexpr int kShareUnits = 2048;     // and of all
 constexpr int kTargetGroups = 512;    // workgroups that fill 256 compute units twice
 constexpr int kTicketStride = 16;     // a ticket has a 64-byte line of its own
 constexpr int64_t kTicketBytes = kTargetGroups * kTicketStride * 4;
@@ -64,13 +65,13 @@ struct Args {
     const int32_t* row_start;
     const int32_t* lengths;   // with pages
     const int32_t* tables;
-    unsigned* tickets;
+    unsigned* tickets;   // kTargetGroups
     char* parts;
     int64_t q_stride, k_stride, v_stride;   // elements
-    int64_t max_pages, pages;
+    int max_pages, pages;
     int batch, rows, max_rows, heads, kv_heads, shift;
-    int few;          // query rows up to which a request is attention_few_kernel's
-    int max_splits;   // attention_many_kernel: workgroups that may share a tile's keys
+    int few;       // query rows up to which a request is of few rows
+    bool shared;   // whether a tile of many rows may have several workgroups
     float c;   // scale / ln 2
 };
 
@@ -86,14 +87,18 @@ __device__ __forceinline__ Request request(const Args& a, int b) {
     r.start = min(max(a.row_start[b], 0), a.rows);
     r.n = min(max(a.row_start[b + 1], r.start), a.rows) - r.start;
     if (kPaged) {
-        const int64_t most = a.max_pages << a.shift;
-        r.length = static_cast<int>(min(static_cast<int64_t>(max(a.lengths[b], 0)), most));
+        r.length = min(max(a.lengths[b], 0), a.max_pages << a.shift);
     } else {
         r.length = r.n;
     }
     r.p0 = r.length - r.n;
     r.todo = min(r.n, a.max_rows);
     return r;
+}
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ Request uniform(const Request& r) {
+    return {uniform(r.start), uniform(r.n), uniform(r.length), uniform(r.p0), uniform(r.todo)};
 }
 
 __device__ __forceinline__ float max_halves(float v) {
@@ -167,14 +172,17 @@ __device__ __forceinline__ u32x4 pack8(const float* p) {
     }
 }
 
-// Sixteen bytes a lane from memory to LDS, lane by lane behind `to` (uniform).
-// Written as statements of their own because the compiler would have every LDS
-// read wait for them, also reads of another buffer; wait_loads() waits.  (No
-// other instruction of these kernels uses m0.)
-__device__ __forceinline__ void lds_load16(const void* from, void* to) {
-    const uint32_t at = __builtin_amdgcn_readfirstlane(
-        static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)(to))));
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(at), "v"(from) : "memory");
+// Sixteen bytes a lane from memory (a uniform address and a lane's offset) to
+// LDS, lane by lane behind `to` (uniform).  Written as a statement of its own
+// because the compiler would have every LDS read wait for it, also reads of
+// another buffer; wait_loads() waits.  (No other instruction of these kernels
+// uses m0.)
+__device__ __forceinline__ void lds_load16(const char* from, uint32_t offset, char* to) {
+    const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)(to)));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(__builtin_amdgcn_readfirstlane(at)), "v"(offset), "s"(from)
+                 : "memory");
 }
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
 
@@ -198,20 +206,25 @@ __device__ __forceinline__ void put(const Args& a, const Request& q, int kh, int
     store4(static_cast<T*>(a.out) + (static_cast<int64_t>(q.start + t) * a.heads + kh * g + r % g) * d + dim, z);
 }
 
-// Parts of a tile's keys in the workspace, [rows][D] outputs, then references
-// (log2) and sums of the rows; the workgroup that draws the last ticket joins
-// them.  part(s): byte offset of workgroup s's; factors: LDS for kMaxSplits x
-// kRows floats, totals for kRows.
-template <typename T, int D, int kRows, typename Part>
+struct RowDim {
+    int row, dim;
+};
+
+// Parts of a tile's keys in the workspace: four outputs for each thread in turn
+// (place(i): the row and first dim of the i-th), then references (log2) and sums
+// of the rows; the workgroup that draws the last ticket joins them.  part(s):
+// byte offset of workgroup s's; factors: LDS for active x kRows floats, totals
+// for kRows.
+template <typename T, int D, int kRows, typename Part, typename Place>
 __device__ __forceinline__ void join_parts(const Args& a, const Request& q, int kh, int g, int r0, int active,
-                                           Part part, float* factors, float* totals) {
+                                           const char* parts, Part part, Place place, float* factors, float* totals) {
     for (int row = threadIdx.x / 16; row < kRows; row += kThreads / 16) {
         const int s0 = threadIdx.x % 16;
         float mv[kMaxSplits / 16], lv[kMaxSplits / 16], m = -INFINITY;
 #pragma unroll
         for (int u = 0; u < kMaxSplits / 16; ++u) {
             const int s = s0 + 16 * u;
-            const float* ml = reinterpret_cast<const float*>(a.parts + part(min(s, active - 1))) + kRows * D + row;
+            const float* ml = reinterpret_cast<const float*>(parts + part(min(s, active - 1))) + kRows * D + row;
             mv[u] = s < active ? coherent_load(ml) : -INFINITY;
             lv[u] = s < active ? coherent_load(ml + kRows) : 0.0f;
         }
@@ -235,9 +248,9 @@ __device__ __forceinline__ void join_parts(const Args& a, const Request& q, int 
         if (s0 == 0) totals[row] = l;
     }
     __syncthreads();
-    // Four items of a thread and eight parts at a time, 32 loads in flight.
+    // Two items of a thread and eight parts at a time, 16 loads in flight.
     constexpr int kItems = kRows * D / 4 / kThreads;
-    constexpr int kTake = kItems < 4 ? kItems : 4;
+    constexpr int kTake = kItems < 2 ? kItems : 2;
     for (int i0 = 0; i0 < kItems; i0 += kTake) {
         float y[kTake][4] = {};
         for (int s0 = 0; s0 < active; s0 += 8) {
@@ -245,7 +258,7 @@ __device__ __forceinline__ void join_parts(const Args& a, const Request& q, int 
 #pragma unroll
             for (int u = 0; u < 8; ++u)
                 if (s0 + u < active) {
-                    const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(a.parts + part(s0 + u), kRows * D * 4);
+                    const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(parts + part(s0 + u), kRows * D * 4);
 #pragma unroll
                     for (int i = 0; i < kTake; ++i) x[i][u] = coherent_load16(rs, ((i0 + i) * kThreads + threadIdx.x) * 16);
                 }
@@ -254,7 +267,7 @@ __device__ __forceinline__ void join_parts(const Args& a, const Request& q, int 
                 if (s0 + u < active) {
 #pragma unroll
                     for (int i = 0; i < kTake; ++i) {
-                        const float f = factors[(s0 + u) * kRows + ((i0 + i) * kThreads + threadIdx.x) / (D / 4)];
+                        const float f = factors[(s0 + u) * kRows + place(i0 + i).row];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) y[i][e] = fmaf(__uint_as_float(x[i][u][e]), f, y[i][e]);
                     }
@@ -262,65 +275,14 @@ __device__ __forceinline__ void join_parts(const Args& a, const Request& q, int 
         }
 #pragma unroll
         for (int i = 0; i < kTake; ++i) {
-            const int item = (i0 + i) * kThreads + threadIdx.x, row = item / (D / 4);
-            put<T>(a, q, kh, g, r0 + row, 4 * (item % (D / 4)), y[i], totals[row], D);
+            const RowDim at = place(i0 + i);
+            put<T>(a, q, kh, g, r0 + at.row, at.dim, y[i], totals[at.row], D);
         }
     }
 }
 
-constexpr int64_t part_bytes(int64_t rows, int64_t d) { return rows * (d + 2) * 4; }
 
-// Running sums, up to and with each request, of what count(b) says of it, by
-// the whole workgroup; their total and, if asked, the largest count.
-struct Sums {
-    int upto[kMaxBatch];
-    int waves[kWaves], most[kWaves];
-};
-template <typename Count>
-__device__ __forceinline__ int sum_requests(int batch, Sums& s, Count count, int* largest) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int each = (batch + kThreads - 1) / kThreads, b0 = threadIdx.x * each;
-    int sum = 0, most = 0;
-    for (int b = b0; b < min(b0 + each, batch); ++b) {
-        const int w = count(b);
-        sum += w;
-        most = max(most, w);
-        s.upto[b] = sum;
-    }
-    int run = sum;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int x = __shfl_up(run, o, 64);
-        if (lane >= o) run += x;
-        if (largest) most = max(most, __shfl_xor(most, o, 64));
-    }
-    if (lane == 63) s.waves[wave] = run, s.most[wave] = most;
-    __syncthreads();
-    int before = run - sum, total = 0;
-    most = 0;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-        if (w < wave) before += s.waves[w];
-        total += s.waves[w];
-        most = max(most, s.most[w]);
-    }
-    if (largest) *largest = most;
-    for (int b = b0; b < min(b0 + each, batch); ++b) s.upto[b] += before;
-    __syncthreads();
-    return total;
-}
-// The first request whose running sum is above x.
-__device__ __forceinline__ int request_of(const Sums& s, int batch, int x) {
-    int lo = 0, hi = batch - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (s.upto[mid] > x)
-            hi = mid;
-        else
-            lo = mid + 1;
-    }
-    return __builtin_amdgcn_readfirstlane(lo);
-}
+constexpr int64_t part_bytes(int64_t rows, int64_t d) { return rows * (d + 2) * 4; }
 
 // Clears the ticket and says whether this workgroup drew the last one.
 __device__ __forceinline__ bool last_arrival(unsigned* counter, int active, unsigned* drawn) {
@@ -333,6 +295,60 @@ __device__ __forceinline__ bool last_arrival(unsigned* counter, int active, unsi
     return true;
 }
 
+// Running sums, up to and with each of `count` things, of what size(i) says of
+// them, by the whole workgroup; their total and the largest size.
+template <int kMost>
+struct Sums {
+    int upto[kMost];
+    int waves[kWaves], most[kWaves];
+};
+template <int kMost, typename Size>
+__device__ __forceinline__ int sum_up(int count, Sums<kMost>& s, Size size, int* largest) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int each = (count + kThreads - 1) / kThreads, i0 = threadIdx.x * each;
+    int sum = 0, most = 0;
+    for (int i = i0; i < min(i0 + each, count); ++i) {
+        const int w = size(i);
+        sum += w;
+        most = max(most, w);
+        s.upto[i] = sum;
+    }
+    int run = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_up(run, o, 64);
+        if (lane >= o) run += x;
+        most = max(most, __shfl_xor(most, o, 64));
+    }
+    if (lane == 63) s.waves[wave] = run, s.most[wave] = most;
+    __syncthreads();
+    int before = run - sum, total = 0;
+    most = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        if (w < wave) before += s.waves[w];
+        total += s.waves[w];
+        most = max(most, s.most[w]);
+    }
+    *largest = most;
+    for (int i = i0; i < min(i0 + each, count); ++i) s.upto[i] += before;
+    __syncthreads();
+    return total;
+}
+// The first whose running sum is above x.
+template <int kMost>
+__device__ __forceinline__ int first_above(const Sums<kMost>& s, int count, int x) {
+    int lo = 0, hi = count - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (s.upto[mid] > x)
+            hi = mid;
+        else
+            lo = mid + 1;
+    }
+    return lo;
+}
+
 // ---- Few rows: 16-wide tiles.  A[i][k] and B[k][j] of a 16x16x32 product
 // sit in lane i (j) + 16 (k / 8), element k % 8; of a 16x16x4 fp32 product in lane
 // i (j) + 16 k; D[i][j] in lane j + 16 (i / 4), element i % 4.
@@ -343,8 +359,16 @@ __device__ __forceinline__ bool last_arrival(unsigned* counter, int active, unsi
 //   O^T  16 bits: row i of tile db is dim (D / 16) i + db: a lane reads D / 16
 //        adjacent elements of each of its eight keys and transposes them with
 //        byte permutes; fp32: tile 4 h + u has dim 64 h + 4 i + u: nothing moves
+template <int D, int RT>
+struct FewShared {
+    float merge_o[kWaves][16 * RT * D];
+    float merge_m[kWaves][16 * RT], merge_l[kWaves][16 * RT];
+    Sums<kMaxBatch> sums;   // rounds of a KV head
+    unsigned ticket;
+};
+
 template <typename T, int D, int RT>
-__global__ __launch_bounds__(kThreads, 2) void attention_few_kernel(const Args a) {
+__device__ __forceinline__ void few_rows(const Args& a, int id, FewShared<D, RT>& sh) {
     constexpr bool kWide = sizeof(T) == 4;
     constexpr int KB = kWide ? 16 : 32;          // keys of a block
     constexpr int KPL = KB / 4;                  // of a lane
@@ -353,11 +377,9 @@ __global__ __launch_bounds__(kThreads, 2) void attention_few_kernel(const Args a
     constexpr int ND = D / 16;                   // dim tiles
     constexpr int VW = ND * sizeof(T) / 4;       // dwords of a value's row that a lane reads
     constexpr int kRows = 16 * RT;
-    __shared__ __align__(16) float merge_o[kWaves][kRows * D];
-    __shared__ float merge_m[kWaves][kRows], merge_l[kWaves][kRows];
-    __shared__ Sums sums;                        // rounds of a KV head
-    __shared__ unsigned ticket;
-
+    auto& merge_o = sh.merge_o;
+    auto& merge_m = sh.merge_m;
+    auto& merge_l = sh.merge_l;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lr = lane & 15, lg = lane >> 4;
@@ -368,19 +390,19 @@ __global__ __launch_bounds__(kThreads, 2) void attention_few_kernel(const Args a
 
     // Rounds of all requests, summed up by every workgroup for itself.
     int longest;
-    const int total = a.kv_heads * sum_requests(a.batch, sums, [&](int b) { return rounds_of(request<true>(a, b)); }, &longest);
+    const int total = a.kv_heads * sum_up(a.batch, sh.sums, [&](int b) { return rounds_of(request<true>(a, b)); }, &longest);
     // Shares: even, worth a workgroup, and no more than kMaxSplits of a request's keys.
     const int per = max(max((total + kTargetGroups - 1) / kTargetGroups, kLeast),
                         (longest + kMaxSplits - 2) / (kMaxSplits - 1));
-    int pos = static_cast<int>(blockIdx.x) * per;
+    int pos = id * per;
     const int end = min(total, pos + per);
 
     while (pos < end) {
         // The request, KV head and rounds that this share goes on with.
-        const int b = request_of(sums, a.batch, pos / a.kv_heads);
-        const Request q = request<true>(a, b);
+        const int b = __builtin_amdgcn_readfirstlane(first_above(sh.sums, a.batch, pos / a.kv_heads));
+        const Request q = uniform(request<true>(a, b));
         const int rounds = rounds_of(q);
-        const int request_start = (sums.upto[b] - rounds) * a.kv_heads;
+        const int request_start = (sh.sums.upto[b] - rounds) * a.kv_heads;
         const int kh = (pos - request_start) / rounds;
         const int unit_start = request_start + kh * rounds;
         const int first = pos - unit_start, last = min(rounds, end - unit_start);
@@ -629,8 +651,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_few_kernel(const Args a
         const auto part = [&](int s) {   // the first group's part is its second one
             return (static_cast<int64_t>(first_group + s) * 2 + (s == 0)) * part_bytes(kRows, D);
         };
-        const int mine = static_cast<int>(blockIdx.x) - first_group;
-        char* out_part = a.parts + (active > 1 ? part(mine) : 0);
+        char* out_part = a.parts + (active > 1 ? part(id - first_group) : 0);
         const __amdgpu_buffer_rsrc_t prs = buffer_rsrc(out_part, part_bytes(kRows, D));
         for (int item = threadIdx.x; item < kRows * D / 4; item += kThreads) {
             const int row = item / (D / 4), d4 = item % (D / 4);
@@ -661,9 +682,13 @@ __global__ __launch_bounds__(kThreads, 2) void attention_few_kernel(const Args a
                 coherent_store(ml + kRows + row, l);
             }
         }
-        if (active > 1 && last_arrival(a.tickets + first_group * kTicketStride, active, &ticket)) {
+        if (active > 1 && last_arrival(a.tickets + first_group * kTicketStride, active, &sh.ticket)) {
             static_assert(kMaxSplits * kRows <= kWaves * kRows * D, "factors fit");
-            join_parts<T, D, kRows>(a, q, kh, g, 0, active, part, merge_o[0], merge_m[0]);
+            const auto place = [&](int i) {
+                const int item = i * kThreads + static_cast<int>(threadIdx.x);
+                return RowDim{item / (D / 4), 4 * (item % (D / 4))};
+            };
+            join_parts<T, D, kRows>(a, q, kh, g, 0, active, a.parts, part, place, merge_o[0], merge_m[0]);
         }
     }
 }
@@ -687,8 +712,16 @@ struct Tile {
     static __device__ __forceinline__ int swap(int row) { return CH == 8 ? row & 7 : 2 * (row & 7); }
 };
 
+template <typename T, int D>
+struct ManyShared {
+    char tile[2][2][Tile<T, D>::kBytes];   // [buffer][keys, values]
+    Sums<kMaxBatch> requests;              // tiles of a KV head
+    Sums<kMaxShared> tiles;                // rounds of a KV head
+    unsigned ticket;
+};
+
 template <typename T, int D, int RT, bool kPaged>
-__global__ __launch_bounds__(kThreads, 2) void attention_many_kernel(const Args a) {
+__device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D>& sh) {
     constexpr bool kWide = sizeof(T) == 4;
     using L = Tile<T, D>;
     constexpr int KT = L::KT, CH = L::CH, PER = L::PER;
@@ -697,105 +730,151 @@ __global__ __launch_bounds__(kThreads, 2) void attention_many_kernel(const Args 
     constexpr int ND = D / 32;              // dim tiles
     constexpr int kRows = 32 * RT * kWaves;
     constexpr int kRowBytes = D * sizeof(T);
-    __shared__ __align__(16) char lds[2][2][L::kBytes];   // [buffer][keys, values]
-    __shared__ Sums sums;                                 // tiles of a KV head
-    __shared__ unsigned ticket;
+    constexpr int kLeastTiles = kWide ? 2 : 4;   // key tiles that are worth a workgroup
+    constexpr int kStart = kWide ? 1 : 2;        // key tiles' time that a row tile takes beside its keys
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lc = lane & 31, lh = lane >> 5;
     const int g = a.heads / a.kv_heads;
-
-    // Tiles of all requests, and the workgroups that share a tile's keys.
-    const int tiles_all = sum_requests(a.batch, sums, [&](int b) {
-        const int r = request<kPaged>(a, b).todo * g;
+    const auto tiles_of = [&](const Request& q) {
+        const int r = q.todo * g;
         return r > a.few ? (r + kRows - 1) / kRows : 0;
-    }, nullptr);
+    };
+
+    int longest;
+    const int tiles_all = sum_up(a.batch, sh.requests, [&](int b) { return tiles_of(request<kPaged>(a, b)); }, &longest);
     if (tiles_all == 0) return;
-    const int splits = max(min(kTargetGroups / (tiles_all * a.kv_heads), a.max_splits), 1);
-    const int shares = a.kv_heads * splits;
-    const int id = static_cast<int>(blockIdx.x);
-    if (id >= tiles_all * shares) return;
-    // Workgroups go to the XCDs in turn: the tiles of a (KV head, share of the
-    // keys) stay on one where the count of those allows, the last tiles, which
-    // see the most keys, first.
-    int slot, share;
-    if (shares % 8 == 0) {
-        const int j = id / 8;
-        slot = tiles_all - 1 - j % tiles_all;
-        share = j / tiles_all * 8 + id % 8;
-    } else {
-        slot = tiles_all - 1 - id / shares;
-        share = id % shares;
+    // While there are few row tiles for the workgroups, their keys are dealt
+    // out evenly (as attention_few_kernel's are): a causal prompt's tiles are
+    // of all lengths, and the longest would be waited for.
+    bool shared = a.shared && tiles_all <= kMaxShared && tiles_all * a.kv_heads <= kShareUnits;
+    int of_head = 0;
+    if (shared) {
+        of_head = sum_up(tiles_all, sh.tiles, [&](int i) {
+            const int b = first_above(sh.requests, a.batch, i);
+            const Request q = request<kPaged>(a, b);
+            const int r0 = (i - (sh.requests.upto[b] - tiles_of(q))) * kRows;
+            const int seen = min(q.p0 + min((r0 + kRows - 1) / g, q.todo - 1) + 1, q.length);
+            return kStart + max((seen + KT - 1) / KT, 1);
+        }, &longest);
+        shared = longest > kStart + kLeastTiles;
     }
-    const int kh = share % a.kv_heads, split = share / a.kv_heads;
-    const int b = request_of(sums, a.batch, slot);
-    const Request q = request<kPaged>(a, b);
-    const int r0 = (slot - (sums.upto[b] - (q.todo * g + kRows - 1) / kRows)) * kRows;
+    int pos = id, end = id + 1, share = 1;   // of the units (KV head, row tile), or of their key tiles
+    if (shared) {
+        const int total = of_head * a.kv_heads;
+        share = max(max((total + kTargetGroups - 1) / kTargetGroups, kStart + kLeastTiles),
+                    (longest + kManySplits - 2) / (kManySplits - 1));
+        if (id >= kTargetGroups) return;
+        // neighbours, which read the same keys, on one XCD
+        id = id % 8 * (kTargetGroups / 8) + id / 8;
+        pos = id * share;
+        end = min(total, pos + share);
+    } else {
+        end = min(end, tiles_all * a.kv_heads);
+    }
+
+    while (pos < end) {
+    int kh, slot, first = 0, last = 0x7fffffff, active = 1, first_group = 0;
+    if (shared) {
+        kh = pos / of_head;
+        slot = first_above(sh.tiles, tiles_all, pos - kh * of_head);
+        const int before = slot ? sh.tiles.upto[slot - 1] : 0;
+        const int size = sh.tiles.upto[slot] - before, start = kh * of_head + before;
+        first = max(pos - start - kStart, 0);
+        last = min(end - start, size) - kStart;
+        first_group = (start + kStart) / share;
+        active = (start + size - 1) / share - first_group + 1;
+        pos = start + size;
+        if (last <= first) continue;
+    } else {
+        // Workgroups go to the XCDs in turn: a KV head's tiles stay on one where
+        // the count of those allows, the last tiles, which see the most keys, first.
+        if (a.kv_heads % 8 == 0) {
+            const int j = pos / 8;
+            slot = tiles_all - 1 - j % tiles_all;
+            kh = j / tiles_all * 8 + pos % 8;
+        } else {
+            slot = tiles_all - 1 - pos / a.kv_heads;
+            kh = pos % a.kv_heads;
+        }
+        pos = end;
+    }
+    kh = uniform(kh);
+    first = uniform(first);
+    last = uniform(last);
+    active = uniform(active);
+    first_group = uniform(first_group);
+    const int b = uniform(first_above(sh.requests, a.batch, slot));
+    const Request q = uniform(request<kPaged>(a, b));
+    const int r0 = uniform(slot - (sh.requests.upto[b] - tiles_of(q))) * kRows;
     const int t_last = min((r0 + kRows - 1) / g, q.todo - 1);
     const int seen = min(max(q.p0 + t_last + 1, 0), q.length);      // keys that some row sees
     const int whole = min(max(q.p0 + r0 / g + 1, 0), q.length);     // that every row sees
-    const int tiles = (seen + KT - 1) / KT;
-    const int each = max((tiles + splits - 1) / splits, kManyLeast / KT);
-    const int active = max((tiles + each - 1) / each, 1);
-    if (split >= active) return;
-    const int first = split * each, last = min(tiles, first + each);
+    last = min(last, (seen + KT - 1) / KT);
 
-    // Where a thread's pieces of a tile lie.
-    const int64_t kv_row = static_cast<int64_t>(kh) << a.shift;
-    const int32_t* table = kPaged ? a.tables + static_cast<int64_t>(b) * a.max_pages : nullptr;
+    // Where the tile's pieces lie: a wave's piece u is 1 KB, kWaveRows rows.
+    constexpr int kWaveRows = 64 / CH, kStep = kWaves * kWaveRows;   // rows of a piece, of the waves' pieces u
+    static_assert(kStep <= 32, "those rows lie in two 16-key groups at most");
+    const int my_row = wave * kWaveRows + lane / CH;
+    // (kStep is a multiple of 8, and rows are exchanged by row & 7)
+    const uint32_t my_piece = 16 * ((lane % CH) ^ L::swap(my_row));
     const int in_page = (1 << a.shift) - 1;
     const int last_page = max(q.length - 1, 0) >> a.shift;
-    typedef int Ids __attribute__((ext_vector_type(KT / 16)));   // pages of a tile's keys, 16 each
+    const int32_t* table = kPaged ? a.tables + static_cast<int64_t>(b) * a.max_pages : nullptr;
+    const uint32_t page_bytes = kPaged ? static_cast<uint32_t>(a.kv_heads << a.shift) * kRowBytes : 0;
+    const int k_row = kPaged ? kRowBytes : static_cast<int>(a.k_stride * sizeof(T));
+    const int v_row = kPaged ? kRowBytes : static_cast<int>(a.v_stride * sizeof(T));
+    const char* k_base = static_cast<const char*>(a.k) +
+                         (kPaged ? static_cast<int64_t>(kh << a.shift) * kRowBytes
+                                 : static_cast<int64_t>(q.start) * k_row + kh * kRowBytes);
+    const char* v_base = static_cast<const char*>(a.v) +
+                         (kPaged ? static_cast<int64_t>(kh << a.shift) * kRowBytes
+                                 : static_cast<int64_t>(q.start) * v_row + kh * kRowBytes);
+    // The pages of a tile's keys, one a lane for the 16 keys from 16 (lane % kGroups) on.
+    constexpr int kGroups = KT / 16;
+    constexpr unsigned kAll = (1u << kGroups) - 1;
     const auto lookup = [&](int t) {
-        Ids i{};
-        if constexpr (kPaged) {
-#pragma unroll
-            for (int u = 0; u < KT / 16; ++u) i[u] = table[min((t * KT + 16 * u) >> a.shift, last_page)];
-        }
-        return i;
+        if constexpr (kPaged)
+            return table[min((t * KT + 16 * (lane % kGroups)) >> a.shift, last_page)];
+        else
+            return 0;
     };
-    const auto there = [&](Ids i) {   // bit u: keys 16 u .. + 15 have a page
-        unsigned bits = (1u << (KT / 16)) - 1;
+    const auto valid = [&](int id) { return !kPaged || static_cast<unsigned>(id) < static_cast<unsigned>(a.pages); };
+    const uint32_t k_mine = (kPaged ? my_row % 16 : my_row) * k_row + my_piece;
+    const uint32_t v_mine = (kPaged ? my_row % 16 : my_row) * v_row + my_piece;
+    const auto load = [&](int t, int ids) {
+        char* kl = sh.tile[t & 1][0] + wave * 1024;
+        char* vl = sh.tile[t & 1][1] + wave * 1024;
         if constexpr (kPaged) {
+            const int pages = valid(ids) ? ids : 0;
 #pragma unroll
-            for (int u = 0; u < KT / 16; ++u)
-                if (i[u] < 0 || i[u] >= a.pages) bits &= ~(1u << u);
-        }
-        return bits;
-    };
-    // A wave's piece u of a tile: 1 KB, 64 / CH rows, of one 16-key group.
-    constexpr int kWaveRows = 64 / CH;
-    static_assert(kWaves * kWaveRows <= 32, "a step's rows lie in two groups at most");
-    const int my_row = lane / CH;                                   // of the piece
-    // (a piece starts at a multiple of kWaveRows; rows are exchanged by row & 7)
-    const auto load = [&](int t, Ids ids) {
-        char* kl = lds[t & 1][0];
-        char* vl = lds[t & 1][1];
-#pragma unroll
-        for (int u = 0; u < PER; ++u) {
-            const int row0 = (u * kWaves + wave) * kWaveRows;       // uniform
-            const int row = row0 + my_row;
-            const int c = (lane % CH) ^ L::swap(row);
-            const char *kp, *vp;
-            if constexpr (kPaged) {
-                const int group = row0 / 16;
-                constexpr int kStep = kWaves * kWaveRows;   // rows that the waves' pieces u have
-                int id = ids[u * kStep / 16];
-                if constexpr (kStep > 16) id = wave < kWaves / 2 ? id : ids[u * kStep / 16 + 1];
-                if (id < 0 || id >= a.pages) id = 0;
-                const int64_t at = (((static_cast<int64_t>(id) * a.kv_heads) << a.shift) + kv_row +
-                                    ((t * KT + 16 * group) & in_page) + row0 % 16) * kRowBytes;
-                const int off = my_row * kRowBytes + 16 * c;
-                kp = static_cast<const char*>(a.k) + at + off;
-                vp = static_cast<const char*>(a.v) + at + off;
-            } else {
-                const int64_t at = q.start + min(t * KT + row, q.length - 1);
-                kp = static_cast<const char*>(a.k) + (at * a.k_stride + kh * D) * static_cast<int>(sizeof(T)) + 16 * c;
-                vp = static_cast<const char*>(a.v) + (at * a.v_stride + kh * D) * static_cast<int>(sizeof(T)) + 16 * c;
+            for (int u = 0; u < PER; ++u) {
+                const int group = u * kStep / 16 + (kStep > 16 ? wave / (kWaves / 2) : 0);
+                const uint32_t id = __builtin_amdgcn_readlane(pages, group);
+                const uint32_t at = ((t * KT + 16 * group) & in_page) + (kStep < 16 ? u * kStep % 16 : 0);
+                const uint64_t offset = static_cast<uint64_t>(id) * page_bytes + at * kRowBytes;
+                lds_load16(k_base + offset, k_mine, kl + u * (kWaves * 1024));
+                lds_load16(v_base + offset, v_mine, vl + u * (kWaves * 1024));
             }
-            lds_load16(kp, kl + (u * kWaves + wave) * 1024);
-            lds_load16(vp, vl + (u * kWaves + wave) * 1024);
+        } else {
+            const char* kp = k_base + static_cast<int64_t>(t * KT) * k_row;
+            const char* vp = v_base + static_cast<int64_t>(t * KT) * v_row;
+            const int left = q.length - 1 - t * KT;   // the last row there is
+            if (left >= KT - 1) {
+#pragma unroll
+                for (int u = 0; u < PER; ++u) {
+                    lds_load16(kp + u * kStep * k_row, k_mine, kl + u * (kWaves * 1024));
+                    lds_load16(vp + u * kStep * v_row, v_mine, vl + u * (kWaves * 1024));
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < PER; ++u) {
+                    const int row = min(my_row + u * kStep, left);
+                    lds_load16(kp, row * k_row + my_piece, kl + u * (kWaves * 1024));
+                    lds_load16(vp, row * v_row + my_piece, vl + u * (kWaves * 1024));
+                }
+            }
         }
     };
     // Waits for the wave's pieces of the tile and meets the other waves.  `ask`
@@ -807,7 +886,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_many_kernel(const Args 
             bool odd = false;
 #pragma unroll
             for (int u = 0; u < PER; ++u) {
-                u32x4* at = reinterpret_cast<u32x4*>(lds[t & 1][1] + (u * kWaves + wave) * 1024 + lane * 16);
+                u32x4* at = reinterpret_cast<u32x4*>(sh.tile[t & 1][1] + (u * kWaves + wave) * 1024 + lane * 16);
                 u32x4 v = *at;
                 if (odd_vector<T>(v)) {
                     odd = true;
@@ -822,9 +901,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_many_kernel(const Args 
         return false;
     };
 
-    Ids ids = lookup(first);
+    int ids = lookup(first), next = lookup(first + 1);   // of the tile that is computed, and of the next one
     if (first < last) load(first, ids);
-    unsigned pages_there = there(ids);
 
     u32x4 qf[RT][NQ];
     int limit_key[RT];
@@ -859,8 +937,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_many_kernel(const Args 
     }
 
     const auto compute = [&](int t, bool masked, unsigned bits) {
-        const char* kt = lds[t & 1][0];
-        const char* vt = lds[t & 1][1];
+        const char* kt = sh.tile[t & 1][0];
+        const char* vt = sh.tile[t & 1][1];
         f32x16 st[RT][NK];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
@@ -993,12 +1071,12 @@ __global__ __launch_bounds__(kThreads, 2) void attention_many_kernel(const Args 
         for (int j = 0; j < KT; ++j) {
             if (!(bits >> (j / 16) & 1)) continue;
             const int key = min(t * KT + j, q.length - 1);
-            int64_t at;
+            const char* row = v_base;
             if constexpr (kPaged)
-                at = ((((static_cast<int64_t>(table[key >> a.shift]) * a.kv_heads) << a.shift) + kv_row + (key & in_page)) * D);
+                row += static_cast<uint64_t>(static_cast<uint32_t>(table[key >> a.shift])) * page_bytes + (key & in_page) * kRowBytes;
             else
-                at = static_cast<int64_t>(q.start + key) * a.v_stride + kh * D;
-            const T* vp = static_cast<const T*>(a.v) + at + 4 * lh;
+                row += static_cast<int64_t>(key) * v_row;
+            const T* vp = reinterpret_cast<const T*>(row) + 4 * lh;
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 if (t * KT + j > limit_key[rt]) continue;
@@ -1013,28 +1091,26 @@ __global__ __launch_bounds__(kThreads, 2) void attention_many_kernel(const Args 
         }
     };
 
-    if (first < last) {
-        Ids next = lookup(first + 1);
-        for (int t = first; t < last; ++t) {
-            const unsigned bits = pages_there;
-            const bool all_there = bits == (1u << (KT / 16)) - 1;
-            const bool odd = arrive(t, (t + 1) * KT > whole || !all_there);
-            // (the other buffer's tile is behind all waves)
-            if (t + 1 < last) {
-                pages_there = there(next);
-                load(t + 1, next);
-                next = lookup(t + 2);
-            }
-            if (t * KT >= wave_seen) continue;
-            if (odd) add_odd(t, bits);
-            compute(t, (t + 1) * KT > wave_whole || !all_there, bits);
-        }
+    for (int t = first; t < last; ++t) {
+        const unsigned bits = __ballot(valid(ids)) & kAll;   // keys 16 u .. + 15 have a page
+        const bool odd = arrive(t, (t + 1) * KT > whole || bits != kAll);
+        // (the other buffer's tile is behind all waves)
+        if (t + 1 < last) load(t + 1, next);
+        ids = next;
+        next = lookup(t + 2);
+        if (t * KT >= wave_seen) continue;
+        if (odd) add_odd(t, bits);
+        compute(t, (t + 1) * KT > wave_whole || bits != kAll, bits);
     }
 
-    const auto part = [&](int s) {
-        return ((static_cast<int64_t>(kh) * tiles_all + slot) * splits + s) * part_bytes(kRows, D);
+    const auto part = [&](int s) {   // the first group's part is its second one
+        return (static_cast<int64_t>(first_group + s) * 2 + (s == 0)) * part_bytes(kRows, D);
     };
-    char* out_part = a.parts + (active > 1 ? part(split) : 0);
+    const auto place = [&](int i) {   // i = 4 (ND rt + db) + u
+        return RowDim{32 * (RT * wave + i / (4 * ND)) + lc, 8 * (i % (4 * ND)) + 4 * lh};
+    };
+    char* out_part = a.parts + (active > 1 ? part(id - first_group) : 0);
+    const __amdgpu_buffer_rsrc_t prs = buffer_rsrc(out_part, part_bytes(kRows, D));
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         const float l = sum_halves(l_run[rt]);
@@ -1043,12 +1119,12 @@ __global__ __launch_bounds__(kThreads, 2) void attention_many_kernel(const Args 
         for (int db = 0; db < ND; ++db)
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const int dim = 32 * db + 8 * u + 4 * lh;
                 const float y[4] = {acc[rt][db][4 * u], acc[rt][db][4 * u + 1], acc[rt][db][4 * u + 2], acc[rt][db][4 * u + 3]};
+                const int i = 4 * (ND * rt + db) + u;
                 if (active == 1)
-                    put<T>(a, q, kh, g, r0 + row, dim, y, l, D);
+                    put<T>(a, q, kh, g, r0 + row, place(i).dim, y, l, D);
                 else
-                    coherent_store16(buffer_rsrc(out_part, kRows * D * 4), (row * D + dim) * 4,
+                    coherent_store16(prs, (i * kThreads + static_cast<int>(threadIdx.x)) * 16,
                                      u32x4{__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3])});
             }
         if (active > 1 && lh == 0) {
@@ -1057,31 +1133,39 @@ __global__ __launch_bounds__(kThreads, 2) void attention_many_kernel(const Args 
             coherent_store(ml + kRows + row, l);
         }
     }
-    if (active > 1) {
-        __syncthreads();   // (LDS is free)
-        if (last_arrival(a.tickets + (kh * tiles_all + slot) * kTicketStride, active, &ticket)) {
-            float* f = reinterpret_cast<float*>(lds[0][0]);
-            static_assert((kManySplits + 1) * kRows * 4 <= static_cast<int>(sizeof lds), "factors fit");
-            join_parts<T, D, kRows>(a, q, kh, g, r0, active, part, f, f + kManySplits * kRows);
-        }
+    __syncthreads();   // (LDS is free)
+    if (active > 1 && last_arrival(a.tickets + first_group * kTicketStride, active, &sh.ticket)) {
+        float* f = reinterpret_cast<float*>(sh.tile[0][0]);
+        static_assert((kManySplits + 1) * kRows * 4 <= static_cast<int>(sizeof sh.tile), "factors fit");
+        join_parts<T, D, kRows>(a, q, kh, g, r0, active, a.parts, part, place, f, f + kManySplits * kRows);
+        __syncthreads();
+    }
     }
 }
 
+template <typename T, int D, int RT>
+__global__ __launch_bounds__(kThreads, 2) void attention_few_kernel(const Args a) {
+    __shared__ __align__(16) FewShared<D, RT> sh;
+    few_rows<T, D, RT>(a, blockIdx.x, sh);
+}
+template <typename T, int D, int RT, bool kPaged>
+__global__ __launch_bounds__(kThreads, 2) void attention_many_kernel(const Args a) {
+    __shared__ __align__(16) ManyShared<T, D> sh;
+    many_rows<T, D, RT, kPaged>(a, blockIdx.x, sh);
+}
 // ---- Host
-
-// Row tiles of a wave in attention_many_kernel.
-int many_tiles(int64_t d, bool wide) { return d == 64 && !wide ? 2 : 1; }
 
 struct Plan {
     bool few, many;
     int few_tiles;        // RT of attention_few_kernel
     int few_rows;         // query rows up to which a request is its
-    int max_splits;
+    int many_tiles;       // RT of attention_many_kernel
+    bool shared;          // whether row tiles may have several workgroups
     int64_t many_groups;
-    int64_t bytes;        // of the workspace: tickets, then parts; the kernels run one after the other
+    int64_t bytes;        // of the parts; the kernels run one after the other
 };
 
-// bytes grows with rows and max_rows: a workspace serves smaller calls too.
+// The bytes grow with rows and max_rows: a workspace serves smaller calls too.
 Plan plan(int64_t batch, int64_t rows, int64_t max_rows, int64_t heads, int64_t kv_heads, int64_t d,
           int64_t max_tokens, bool wide, bool paged) {
     Plan p{};
@@ -1093,13 +1177,16 @@ Plan plan(int64_t batch, int64_t rows, int64_t max_rows, int64_t heads, int64_t 
     p.few = paged && g <= p.few_rows && (batch > 1 || most <= p.few_rows);
     if (!p.few) p.few_rows = 0;
     p.many = most > p.few_rows;
-    if (p.few) p.bytes = kTicketBytes + 2 * kTargetGroups * part_bytes(16 * p.few_tiles, d);
+    if (p.few) p.bytes = 2 * kTargetGroups * part_bytes(16 * p.few_tiles, d);
     if (p.many) {
-        const int64_t tile = 32 * many_tiles(d, wide) * kWaves;
+        // Two row tiles a wave read a key tile's operands once for both, where
+        // registers allow and enough tiles are left for the workgroups.
+        p.many_tiles = d == 64 && !wide && rows * g / 256 * kv_heads >= kTargetGroups ? 2 : 1;
+        const int64_t tile = 32 * p.many_tiles * kWaves;
         const int64_t units = (rows * g / tile + batch) * kv_heads;   // at most
-        p.max_splits = max_tokens > kManyLeast ? kManySplits : 1;
-        p.many_groups = p.max_splits > 1 ? std::max<int64_t>(units, kTargetGroups) : units;
-        if (p.max_splits > 1) p.bytes = std::max(p.bytes, kTicketBytes + kTargetGroups * part_bytes(tile, d));
+        p.shared = max_tokens > 64;
+        p.many_groups = p.shared ? std::max<int64_t>(units, kTargetGroups) : units;
+        if (p.shared) p.bytes = 2 * kTargetGroups * part_bytes(d == 64 ? 256 : 128, d);
     }
     return p;
 }
@@ -1119,58 +1206,50 @@ int check_call(const char* who, int64_t batch, int64_t rows, int64_t max_rows, i
 int64_t workspace_bytes_of(int64_t batch, int64_t rows, int64_t max_rows, int64_t heads, int64_t kv_heads, int64_t d,
                            int64_t max_tokens, bool paged) {
     if (batch == 0 || rows == 0) return 0;
-    int64_t most = 0;
-    for (bool wide : {false, true})
-        most = std::max(most, plan(batch, rows, max_rows, heads, kv_heads, d, max_tokens, wide, paged).bytes);
-    return most;
-}
-
-template <typename T, int D>
-void launch_few(const Args& a, int tiles, hipStream_t s) {
-    const dim3 grid(kTargetGroups), block(kThreads);
-    if (tiles == 1)
-        hipLaunchKernelGGL((attention_few_kernel<T, D, 1>), grid, block, 0, s, a);
-    else
-        hipLaunchKernelGGL((attention_few_kernel<T, D, 2>), grid, block, 0, s, a);
+    const Plan p = plan(batch, rows, max_rows, heads, kv_heads, d, max_tokens, false, paged);
+    return kTicketBytes + p.bytes;   // (the same for every type)
 }
 
 template <typename T, int D, bool kPaged>
-void launch_many(const Args& a, int64_t grid, hipStream_t s) {
-    constexpr int RT = D == 64 && sizeof(T) == 2 ? 2 : 1;   // many_tiles()
-    hipLaunchKernelGGL((attention_many_kernel<T, D, RT, kPaged>), dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, s, a);
-}
-
-template <typename T, int D>
-void launch_type(const Args& a, const Plan& p, bool paged, hipStream_t s) {
-    if (p.few) launch_few<T, D>(a, p.few_tiles, s);
-    if (p.many) {
-        if (paged)
-            launch_many<T, D, true>(a, p.many_groups, s);
-        else
-            launch_many<T, D, false>(a, p.many_groups, s);
+void launch_type(const Args& a, const Plan& p, hipStream_t s) {
+    const dim3 block(kThreads), few(kTargetGroups), many(static_cast<unsigned>(p.many_groups));
+    if constexpr (kPaged) {
+        if (p.few && p.few_tiles == 1)
+            hipLaunchKernelGGL((attention_few_kernel<T, D, 1>), few, block, 0, s, a);
+        else if (p.few)
+            hipLaunchKernelGGL((attention_few_kernel<T, D, 2>), few, block, 0, s, a);
     }
+    if (!p.many) return;
+    if constexpr (D == 64 && sizeof(T) == 2) {
+        if (p.many_tiles == 2) {
+            hipLaunchKernelGGL((attention_many_kernel<T, D, 2, kPaged>), many, block, 0, s, a);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((attention_many_kernel<T, D, 1, kPaged>), many, block, 0, s, a);
 }
 
-int run(const char* who, Args a, const Plan& p, int dtype, int64_t d, bool paged, void* workspace, void* stream) {
+template <bool kPaged>
+int run(const char* who, Args a, const Plan& p, int dtype, int64_t d, void* workspace, void* stream) {
     a.few = p.few_rows;
-    a.max_splits = p.max_splits;
+    a.shared = p.shared;
     a.tickets = static_cast<unsigned*>(workspace);
     a.parts = static_cast<char*>(workspace) + kTicketBytes;
     auto s = static_cast<hipStream_t>(stream);
     if (d == 64) {
         if (dtype == VM_HIP_DTYPE_F32)
-            launch_type<float, 64>(a, p, paged, s);
+            launch_type<float, 64, kPaged>(a, p, s);
         else if (dtype == VM_HIP_DTYPE_F16)
-            launch_type<F16, 64>(a, p, paged, s);
+            launch_type<F16, 64, kPaged>(a, p, s);
         else
-            launch_type<BF16, 64>(a, p, paged, s);
+            launch_type<BF16, 64, kPaged>(a, p, s);
     } else {
         if (dtype == VM_HIP_DTYPE_F32)
-            launch_type<float, 128>(a, p, paged, s);
+            launch_type<float, 128, kPaged>(a, p, s);
         else if (dtype == VM_HIP_DTYPE_F16)
-            launch_type<F16, 128>(a, p, paged, s);
+            launch_type<F16, 128, kPaged>(a, p, s);
         else
-            launch_type<BF16, 128>(a, p, paged, s);
+            launch_type<BF16, 128, kPaged>(a, p, s);
     }
     return check_launch(who, s);
 }
@@ -1206,7 +1285,8 @@ int vm_hip_attention_packed(const void* q, const void* k, const void* v, void* o
     VM_TRY(check_call("attention_packed", batch, rows, 0, heads, kv_heads, head_dim));
     const int64_t unit = dtype == VM_HIP_DTYPE_F32 ? 4 : 8;   // elements of 16 bytes
     for (int64_t s : {q_stride, k_stride, v_stride})
-        if (s % unit || s > (1 << 24)) return fail_inval("attention_packed: strides must be multiples of 16 bytes, at most 2^24 elements");
+        if (s % unit || s > (1 << 22))
+            return fail_inval("attention_packed: strides must be multiples of 16 bytes, at most 2^22 elements");
     if (q_stride < heads * head_dim || k_stride < kv_heads * head_dim || v_stride < kv_heads * head_dim)
         return fail_inval("attention_packed: strides must hold a row's heads");
     if (!(scale < INFINITY)) return fail_inval("attention_packed: scale must be finite");
@@ -1234,14 +1314,14 @@ int vm_hip_attention_packed(const void* q, const void* k, const void* v, void* o
     a.heads = static_cast<int>(heads);
     a.kv_heads = static_cast<int>(kv_heads);
     a.c = scale_of(scale, head_dim);
-    return run("attention_packed", a, p, dtype, head_dim, false, workspace, stream);
+    return run<false>("attention_packed", a, p, dtype, head_dim, workspace, stream);
 }
 
 int64_t vm_hip_attention_paged_workspace_bytes(int64_t batch, int64_t rows, int64_t max_rows, int64_t heads,
                                                int64_t kv_heads, int64_t head_dim, int64_t max_tokens) {
     clear_error();
     VM_TRY(check_call("attention_paged", batch, rows, max_rows, heads, kv_heads, head_dim));
-    if (max_tokens < 1 || max_tokens > (1 << 30)) return fail_inval("attention_paged: max_tokens out of range");
+    if (max_tokens < 1 || max_tokens > (1 << 24)) return fail_inval("attention_paged: max_tokens out of range");
     return workspace_bytes_of(batch, rows, max_rows, heads, kv_heads, head_dim, max_tokens, true);
 }
 
@@ -1253,8 +1333,8 @@ int vm_hip_attention_paged(const vm_hip_kv_paged* cache, const int32_t* tables, 
     VM_TRY(check_kv_paged(cache, "attention_paged"));
     const int64_t d = cache->head_dim, hk = cache->kv_heads;
     VM_TRY(check_call("attention_paged", batch, rows, max_rows, heads, hk, d));
-    if (max_pages < 1 || max_pages > (1 << 30) / cache->page_size)
-        return fail_inval("attention_paged: max_pages * page_size must be at most 2^30");
+    if (max_pages < 1 || max_pages > (1 << 24) / cache->page_size)
+        return fail_inval("attention_paged: max_pages * page_size must be at most 2^24");
     if (batch * hk * ((max_pages * cache->page_size + kRound - 1) / kRound) >= (int64_t{1} << 31))
         return fail_inval("attention_paged: batch * kv_heads * max_pages * page_size must be below 2^38");
     if (!(scale < INFINITY)) return fail_inval("attention_paged: scale must be finite");
@@ -1278,8 +1358,8 @@ int vm_hip_attention_paged(const vm_hip_kv_paged* cache, const int32_t* tables, 
     a.lengths = lengths;
     a.tables = tables;
     a.q_stride = heads * d;
-    a.max_pages = max_pages;
-    a.pages = cache->pages;
+    a.max_pages = static_cast<int>(max_pages);
+    a.pages = static_cast<int>(cache->pages);
     a.batch = static_cast<int>(batch);
     a.rows = static_cast<int>(rows);
     a.max_rows = static_cast<int>(max_rows > 0 ? std::min(max_rows, rows) : rows);
@@ -1287,7 +1367,7 @@ int vm_hip_attention_paged(const vm_hip_kv_paged* cache, const int32_t* tables, 
     a.kv_heads = static_cast<int>(hk);
     a.shift = log2_of(cache->page_size);
     a.c = scale_of(scale, d);
-    return run("attention_paged", a, p, cache->dtype, d, true, workspace, stream);
+    return run<true>("attention_paged", a, p, cache->dtype, d, workspace, stream);
 }
 
 }  // extern "C"
