@@ -709,7 +709,13 @@ struct Tile {
     static constexpr int CH = D * sizeof(T) / 16;               // 16-byte pieces of a row
     static constexpr int PER = KT * CH / kThreads;              // pieces of a thread
     static constexpr int kBytes = KT * D * static_cast<int>(sizeof(T));
-    static __device__ __forceinline__ int swap(int row) { return CH == 8 ? row & 7 : 2 * (row & 7); }
+    // Which piece of a row lies where: pieces are exchanged so that the 16 rows
+    // of keys, and the 4 (or, fp32, 2) rows of values, that are read at a time
+    // lie in different banks (64 of 4 bytes).
+    static __device__ __forceinline__ int swap_k(int row) { return CH == 8 ? row >> 1 & 7 : row & 15; }
+    static __device__ __forceinline__ int swap_v(int row) {
+        return sizeof(T) == 4 ? 8 * (row >> 2 & 1) : CH == 8 ? 4 * (row >> 1 & 1) : 4 * (row & 3);
+    }
 };
 
 template <typename T, int D>
@@ -817,8 +823,9 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
     constexpr int kWaveRows = 64 / CH, kStep = kWaves * kWaveRows;   // rows of a piece, of the waves' pieces u
     static_assert(kStep <= 32, "those rows lie in two 16-key groups at most");
     const int my_row = wave * kWaveRows + lane / CH;
-    // (kStep is a multiple of 8, and rows are exchanged by row & 7)
-    const uint32_t my_piece = 16 * ((lane % CH) ^ L::swap(my_row));
+    static_assert(kStep % 8 == 0, "pieces u and u + 2 of a lane are exchanged alike");
+    const auto k_piece = [&](int u) { return 16 * ((lane % CH) ^ L::swap_k(my_row + u % 2 * kStep)); };
+    const uint32_t v_piece = 16 * ((lane % CH) ^ L::swap_v(my_row));
     const int in_page = (1 << a.shift) - 1;
     const int last_page = max(q.length - 1, 0) >> a.shift;
     const int32_t* table = kPaged ? a.tables + static_cast<int64_t>(b) * a.max_pages : nullptr;
@@ -841,8 +848,9 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
             return 0;
     };
     const auto valid = [&](int id) { return !kPaged || static_cast<unsigned>(id) < static_cast<unsigned>(a.pages); };
-    const uint32_t k_mine = (kPaged ? my_row % 16 : my_row) * k_row + my_piece;
-    const uint32_t v_mine = (kPaged ? my_row % 16 : my_row) * v_row + my_piece;
+    const uint32_t k_mine[2] = {static_cast<uint32_t>((kPaged ? my_row % 16 : my_row) * k_row + k_piece(0)),
+                                static_cast<uint32_t>((kPaged ? my_row % 16 : my_row) * k_row + k_piece(1))};
+    const uint32_t v_mine = (kPaged ? my_row % 16 : my_row) * v_row + v_piece;
     const auto load = [&](int t, int ids) {
         char* kl = sh.tile[t & 1][0] + wave * 1024;
         char* vl = sh.tile[t & 1][1] + wave * 1024;
@@ -854,7 +862,7 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
                 const uint32_t id = __builtin_amdgcn_readlane(pages, group);
                 const uint32_t at = ((t * KT + 16 * group) & in_page) + (kStep < 16 ? u * kStep % 16 : 0);
                 const uint64_t offset = static_cast<uint64_t>(id) * page_bytes + at * kRowBytes;
-                lds_load16(k_base + offset, k_mine, kl + u * (kWaves * 1024));
+                lds_load16(k_base + offset, k_mine[u % 2], kl + u * (kWaves * 1024));
                 lds_load16(v_base + offset, v_mine, vl + u * (kWaves * 1024));
             }
         } else {
@@ -864,15 +872,15 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
             if (left >= KT - 1) {
 #pragma unroll
                 for (int u = 0; u < PER; ++u) {
-                    lds_load16(kp + u * kStep * k_row, k_mine, kl + u * (kWaves * 1024));
+                    lds_load16(kp + u * kStep * k_row, k_mine[u % 2], kl + u * (kWaves * 1024));
                     lds_load16(vp + u * kStep * v_row, v_mine, vl + u * (kWaves * 1024));
                 }
             } else {
 #pragma unroll
                 for (int u = 0; u < PER; ++u) {
                     const int row = min(my_row + u * kStep, left);
-                    lds_load16(kp, row * k_row + my_piece, kl + u * (kWaves * 1024));
-                    lds_load16(vp, row * v_row + my_piece, vl + u * (kWaves * 1024));
+                    lds_load16(kp, row * k_row + k_piece(u), kl + u * (kWaves * 1024));
+                    lds_load16(vp, row * v_row + v_piece, vl + u * (kWaves * 1024));
                 }
             }
         }
@@ -951,7 +959,7 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
 #pragma unroll
             for (int s = 0; s < NQ; ++s) {
                 const int row = 32 * n + lc;
-                const u32x4 kf = *reinterpret_cast<const u32x4*>(kt + row * kRowBytes + 16 * ((2 * s + lh) ^ L::swap(row)));
+                const u32x4 kf = *reinterpret_cast<const u32x4*>(kt + row * kRowBytes + 16 * ((2 * s + lh) ^ L::swap_k(row)));
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
                     if constexpr (kWide) {
@@ -1026,7 +1034,7 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
                     for (int db = 0; db < ND; ++db) {
                         const int row = 32 * n + 8 * (e / 4) + 4 * lh + e % 4;
                         const int c = 8 * db + lc / 4;
-                        const float x = *reinterpret_cast<const float*>(vt + row * kRowBytes + 16 * (c ^ L::swap(row)) + 4 * (lc & 3));
+                        const float x = *reinterpret_cast<const float*>(vt + row * kRowBytes + 16 * (c ^ L::swap_v(row)) + 4 * (lc & 3));
 #pragma unroll
                         for (int rt = 0; rt < RT; ++rt)
                             acc[rt][db] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, st[rt][n][e], acc[rt][db], 0, 0, 0);
@@ -1053,7 +1061,7 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
                         for (int w = 0; w < 2; ++w) {
                             const int row = 32 * n + 16 * s + 8 * w + 4 * lh + l16 / 4;
                             const int c = 4 * db + 2 * (lane >> 4 & 1) + (l16 % 4) / 2;
-                            const char* at = vt + row * kRowBytes + 16 * (c ^ L::swap(row)) + 8 * (l16 & 1);
+                            const char* at = vt + row * kRowBytes + 16 * (c ^ L::swap_v(row)) + 8 * (l16 & 1);
                             const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                 (__attribute__((address_space(3))) s16x4*)(at));
                             __builtin_memcpy(x + 2 * w, &y, 8);
