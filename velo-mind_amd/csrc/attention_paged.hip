@@ -72,6 +72,8 @@ struct Args {
     int batch, rows, max_rows, heads, kv_heads, shift;
     int few;       // query rows up to which a request is of few rows
     bool shared;   // whether a tile of many rows may have several workgroups
+    int group;     // query heads of a KV head
+    unsigned per_group;   // 2^32 / group, rounded up (group 1: not used)
     float c;   // scale / ln 2
 };
 
@@ -120,25 +122,25 @@ __device__ __forceinline__ float sum_groups(float v) {
     return swap_halves_add(v, v);
 }
 
-// Whether a dword holds an element that is not finite, and the dword without
-// those elements.
+// Elements that are not finite: bits that odd_bits() leaves in kOddMask (adding
+// one to an exponent of all ones carries into the sign's place), and a dword
+// without them.
 template <typename T>
-__device__ __forceinline__ bool odd_element(uint32_t bits) {
-    if constexpr (sizeof(T) == 4) return (bits & 0x7f800000u) == 0x7f800000u;
-    constexpr uint32_t e = std::is_same<T, F16>::value ? 0x7c00u : 0x7f80u;
-    return (bits & e) == e || (bits >> 16 & e) == e;
+constexpr uint32_t kExponent = sizeof(T) == 4 ? 0x7f800000u : std::is_same<T, F16>::value ? 0x7c007c00u : 0x7f807f80u;
+template <typename T>
+constexpr uint32_t kOddMask = sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
+template <typename T>
+__device__ __forceinline__ uint32_t odd_bits(uint32_t bits) {
+    constexpr uint32_t kStep = kExponent<T> & ~(kExponent<T> << 1);   // the exponents' lowest bits
+    return (bits & kExponent<T>) + kStep;
 }
 template <typename T>
 __device__ __forceinline__ uint32_t finite_elements(uint32_t bits) {
-    if constexpr (sizeof(T) == 4) return odd_element<T>(bits) ? 0u : bits;
-    constexpr uint32_t e = std::is_same<T, F16>::value ? 0x7c00u : 0x7f80u;
-    if ((bits & e) == e) bits &= 0xffff0000u;
-    if ((bits >> 16 & e) == e) bits &= 0x0000ffffu;
+    const uint32_t odd = odd_bits<T>(bits) & kOddMask<T>;
+    if constexpr (sizeof(T) == 4) return odd ? 0u : bits;
+    if (odd & 0x8000u) bits &= 0xffff0000u;
+    if (odd & 0x80000000u) bits &= 0x0000ffffu;
     return bits;
-}
-template <typename T>
-__device__ __forceinline__ bool odd_vector(u32x4 v) {
-    return odd_element<T>(v.x) || odd_element<T>(v.y) || odd_element<T>(v.z) || odd_element<T>(v.w);
 }
 
 template <typename T>
@@ -184,26 +186,41 @@ __device__ __forceinline__ void lds_load16(const char* from, uint32_t offset, ch
                  : "s"(__builtin_amdgcn_readfirstlane(at)), "v"(offset), "s"(from)
                  : "memory");
 }
+// The compiler moves vector and scalar arithmetic across this, nothing else.
+__device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0x406); }
+
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
 
 __device__ __forceinline__ void store4(float* p, const float* y) { *reinterpret_cast<float4*>(p) = make_float4(y[0], y[1], y[2], y[3]); }
-template <typename T>
-__device__ __forceinline__ void store4(T* p, const float* y) {
-    uint16_t h[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) h[e] = narrow<T>(y[e]).bits;
-    *reinterpret_cast<u32x2*>(p) = u32x2{h[0] | static_cast<uint32_t>(h[1]) << 16, h[2] | static_cast<uint32_t>(h[3]) << 16};
+__device__ __forceinline__ void store4(F16* p, const float* y) {
+    typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+    const half4 h{static_cast<_Float16>(y[0]), static_cast<_Float16>(y[1]), static_cast<_Float16>(y[2]), static_cast<_Float16>(y[3])};
+    *reinterpret_cast<half4*>(p) = h;
+}
+__device__ __forceinline__ void store4(BF16* p, const float* y) {
+    typedef __bf16 bf4 __attribute__((ext_vector_type(4)));
+    const bf4 h{static_cast<__bf16>(y[0]), static_cast<__bf16>(y[1]), static_cast<__bf16>(y[2]), static_cast<__bf16>(y[3])};
+    *reinterpret_cast<bf4*>(p) = h;
+}
+
+// A query row's token and head of the group: rows are counted from the first
+// of token t0, and are few (less than the group's size and 256).
+struct Row {
+    int t, head;
+};
+__device__ __forceinline__ Row row_of(const Args& a, int t0, int r) {
+    // r / group as the upper half of r times 2^32 / group, rounded up
+    const int t = static_cast<int>(__umulhi(static_cast<unsigned>(r), a.per_group)) + (a.group == 1 ? r : 0);
+    return {t0 + t, r - t * a.group};
 }
 
 // One row's four dims: outputs over the sum of weights; a row that saw nothing: zeros.
 template <typename T>
-__device__ __forceinline__ void put(const Args& a, const Request& q, int kh, int g, int r, int dim, const float* y,
-                                    float l, int d) {
-    const int t = r / g;
-    if (t >= q.todo) return;
+__device__ __forceinline__ void put(const Args& a, const Request& q, int kh, Row r, int dim, const float* y, float l, int d) {
+    if (r.t >= q.todo) return;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const float z[4] = {y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv};
-    store4(static_cast<T*>(a.out) + (static_cast<int64_t>(q.start + t) * a.heads + kh * g + r % g) * d + dim, z);
+    store4(static_cast<T*>(a.out) + (static_cast<int64_t>(q.start + r.t) * a.heads + kh * a.group + r.head) * d + dim, z);
 }
 
 struct RowDim {
@@ -216,7 +233,7 @@ struct RowDim {
 // byte offset of workgroup s's; factors: LDS for active x kRows floats, totals
 // for kRows.
 template <typename T, int D, int kRows, typename Part, typename Place>
-__device__ __forceinline__ void join_parts(const Args& a, const Request& q, int kh, int g, int r0, int active,
+__device__ __forceinline__ void join_parts(const Args& a, const Request& q, int kh, int t0, int r0, int active,
                                            const char* parts, Part part, Place place, float* factors, float* totals) {
     for (int row = threadIdx.x / 16; row < kRows; row += kThreads / 16) {
         const int s0 = threadIdx.x % 16;
@@ -276,7 +293,7 @@ __device__ __forceinline__ void join_parts(const Args& a, const Request& q, int 
 #pragma unroll
         for (int i = 0; i < kTake; ++i) {
             const RowDim at = place(i0 + i);
-            put<T>(a, q, kh, g, r0 + at.row, at.dim, y[i], totals[at.row], D);
+            put<T>(a, q, kh, row_of(a, t0, r0 + at.row), at.dim, y[i], totals[at.row], D);
         }
     }
 }
@@ -305,6 +322,10 @@ struct Sums {
 template <int kMost, typename Size>
 __device__ __forceinline__ int sum_up(int count, Sums<kMost>& s, Size size, int* largest) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (count == 1) {   // (every thread writes the same)
+        s.upto[0] = *largest = size(0);
+        return *largest;
+    }
     const int each = (count + kThreads - 1) / kThreads, i0 = threadIdx.x * each;
     int sum = 0, most = 0;
     for (int i = i0; i < min(i0 + each, count); ++i) {
@@ -383,7 +404,7 @@ __device__ __forceinline__ void few_rows(const Args& a, int id, FewShared<D, RT>
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lr = lane & 15, lg = lane >> 4;
-    const int g = a.heads / a.kv_heads;
+    const int g = a.group;
     const auto rounds_of = [&](const Request& q) {
         return q.todo > 0 && q.todo * g <= a.few ? max((q.length + kRound - 1) / kRound, 1) : 0;
     };
@@ -475,11 +496,11 @@ __device__ __forceinline__ void few_rows(const Args& a, int id, FewShared<D, RT>
         int limit_key[RT];   // the last key that the row sees
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            const int r = 16 * rt + lr, t = r / g;
-            const bool row_ok = t < q.todo;
-            limit_key[rt] = row_ok ? q.p0 + t : -1;
-            const T* qp = static_cast<const T*>(a.q) + static_cast<int64_t>(q.start + (row_ok ? t : 0)) * a.q_stride +
-                          (kh * g + r % g) * D;
+            const Row r = row_of(a, 0, 16 * rt + lr);
+            const bool row_ok = r.t < q.todo;
+            limit_key[rt] = row_ok ? q.p0 + r.t : -1;
+            const T* qp = static_cast<const T*>(a.q) + static_cast<int64_t>(q.start + (row_ok ? r.t : 0)) * a.q_stride +
+                          (kh * g + r.head) * D;
 #pragma unroll
             for (int s = 0; s < KC; ++s) {
                 qf[rt][s] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(qp) + 64 * s + 16 * lg);
@@ -570,15 +591,16 @@ __device__ __forceinline__ void few_rows(const Args& a, int id, FewShared<D, RT>
                 // Values that are not finite, where not every row sees them: to
                 // the rows that do by hand, whatever their weight (0 times them
                 // would not be 0).
-                bool odd = false;
+                uint32_t odd = 0;
 #pragma unroll
                 for (int j = 0; j < KPL; ++j)
 #pragma unroll
-                    for (int u = 0; u < VW; ++u) {
-                        odd |= odd_element<T>(vreg[j][u]);
-                        vreg[j][u] = finite_elements<T>(vreg[j][u]);
-                    }
-                if (__any(odd)) {
+                    for (int u = 0; u < VW; ++u) odd |= odd_bits<T>(vreg[j][u]);
+                if (__any((odd & kOddMask<T>) != 0)) {
+#pragma unroll
+                    for (int j = 0; j < KPL; ++j)
+#pragma unroll
+                        for (int u = 0; u < VW; ++u) vreg[j][u] = finite_elements<T>(vreg[j][u]);
                     for (int j = 0; j < KB; ++j) {
                         const int key = block * KB + j;
                         const int id = table[min(key >> a.shift, last_page)];
@@ -671,7 +693,7 @@ __device__ __forceinline__ void few_rows(const Args& a, int id, FewShared<D, RT>
                 y[3] = fmaf(o.w, f, y[3]);
             }
             if (active == 1) {
-                put<T>(a, q, kh, g, row, 4 * d4, y, l, D);
+                put<T>(a, q, kh, row_of(a, 0, row), 4 * d4, y, l, D);
                 continue;
             }
             coherent_store16(prs, static_cast<uint32_t>(item) * 16,
@@ -688,7 +710,7 @@ __device__ __forceinline__ void few_rows(const Args& a, int id, FewShared<D, RT>
                 const int item = i * kThreads + static_cast<int>(threadIdx.x);
                 return RowDim{item / (D / 4), 4 * (item % (D / 4))};
             };
-            join_parts<T, D, kRows>(a, q, kh, g, 0, active, a.parts, part, place, merge_o[0], merge_m[0]);
+            join_parts<T, D, kRows>(a, q, kh, 0, 0, active, a.parts, part, place, merge_o[0], merge_m[0]);
         }
     }
 }
@@ -737,12 +759,14 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
     constexpr int kRows = 32 * RT * kWaves;
     constexpr int kRowBytes = D * sizeof(T);
     constexpr int kLeastTiles = kWide ? 2 : 4;   // key tiles that are worth a workgroup
+    constexpr int kAhead = 4;                    // LDS operands in front of their products
+    constexpr int kJoin = kWide ? 3 : 16;        // key tiles' time that parts take
     constexpr int kStart = kWide ? 1 : 2;        // key tiles' time that a row tile takes beside its keys
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lc = lane & 31, lh = lane >> 5;
-    const int g = a.heads / a.kv_heads;
+    const int g = a.group;
     const auto tiles_of = [&](const Request& q) {
         const int r = q.todo * g;
         return r > a.few ? (r + kRows - 1) / kRows : 0;
@@ -751,10 +775,14 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
     int longest;
     const int tiles_all = sum_up(a.batch, sh.requests, [&](int b) { return tiles_of(request<kPaged>(a, b)); }, &longest);
     if (tiles_all == 0) return;
-    // While there are few row tiles for the workgroups, their keys are dealt
-    // out evenly (as attention_few_kernel's are): a causal prompt's tiles are
-    // of all lengths, and the longest would be waited for.
-    bool shared = a.shared && tiles_all <= kMaxShared && tiles_all * a.kv_heads <= kShareUnits;
+    // A row tile's keys go to one workgroup, or all tiles' keys are dealt out
+    // evenly (as attention_few_kernel's are): where the longest tile (of a causal
+    // prompt: twice the mean) would be waited for longer than the parts take to
+    // store and join (25 us for 512 workgroups' 16-bit tiles, about kJoin key
+    // tiles' time).  32 heads of 64 on 4, f16, 3000 rows: 55 us against 79 dealt
+    // out; 500 rows behind 30000: 340 against 700.
+    const int units = tiles_all * a.kv_heads;
+    bool shared = a.shared && tiles_all <= kMaxShared && units <= kShareUnits;
     int of_head = 0;
     if (shared) {
         of_head = sum_up(tiles_all, sh.tiles, [&](int i) {
@@ -764,7 +792,10 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
             const int seen = min(q.p0 + min((r0 + kRows - 1) / g, q.todo - 1) + 1, q.length);
             return kStart + max((seen + KT - 1) / KT, 1);
         }, &longest);
-        shared = longest > kStart + kLeastTiles;
+        const int each = of_head * a.kv_heads / kTargetGroups;
+        // the last workgroups to start: none, or, of tiles of equal length, whole ones
+        const int alone = units <= kTargetGroups ? longest : each + max(2 * (of_head / tiles_all) - longest, 0);
+        shared = longest > kStart + kLeastTiles && alone > max(each, kStart + kLeastTiles) + kJoin;
     }
     int pos = id, end = id + 1, share = 1;   // of the units (KV head, row tile), or of their key tiles
     if (shared) {
@@ -814,9 +845,10 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
     const int b = uniform(first_above(sh.requests, a.batch, slot));
     const Request q = uniform(request<kPaged>(a, b));
     const int r0 = uniform(slot - (sh.requests.upto[b] - tiles_of(q))) * kRows;
-    const int t_last = min((r0 + kRows - 1) / g, q.todo - 1);
+    const int t0 = r0 / g, rem0 = r0 - t0 * g;   // its token, and the rows of that in front
+    const int t_last = min(uniform(row_of(a, t0, rem0 + kRows - 1).t), q.todo - 1);
     const int seen = min(max(q.p0 + t_last + 1, 0), q.length);      // keys that some row sees
-    const int whole = min(max(q.p0 + r0 / g + 1, 0), q.length);     // that every row sees
+    const int whole = min(max(q.p0 + t0 + 1, 0), q.length);         // that every row sees
     last = min(last, (seen + KT - 1) / KT);
 
     // Where the tile's pieces lie: a wave's piece u is 1 KB, kWaveRows rows.
@@ -891,19 +923,17 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
     const auto arrive = [&](int t, bool ask) {
         wait_loads();
         if (ask) {
-            bool odd = false;
+            uint32_t odd = 0;
 #pragma unroll
             for (int u = 0; u < PER; ++u) {
                 u32x4* at = reinterpret_cast<u32x4*>(sh.tile[t & 1][1] + (u * kWaves + wave) * 1024 + lane * 16);
-                u32x4 v = *at;
-                if (odd_vector<T>(v)) {
-                    odd = true;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = finite_elements<T>(v[e]);
-                    *at = v;
-                }
+                const u32x4 v = *at;
+                const uint32_t bits = (odd_bits<T>(v.x) | odd_bits<T>(v.y) | odd_bits<T>(v.z) | odd_bits<T>(v.w)) & kOddMask<T>;
+                if (bits)
+                    *at = u32x4{finite_elements<T>(v.x), finite_elements<T>(v.y), finite_elements<T>(v.z), finite_elements<T>(v.w)};
+                odd |= bits;
             }
-            return __syncthreads_or(odd) != 0;
+            return __syncthreads_or(odd != 0) != 0;
         }
         __syncthreads();
         return false;
@@ -914,14 +944,13 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
 
     u32x4 qf[RT][NQ];
     int limit_key[RT];
-    const int w0 = r0 + 32 * RT * wave;   // the wave's first row
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const int r = w0 + 32 * rt + lc, t = r / g;
-        const bool row_ok = t < q.todo;
-        limit_key[rt] = row_ok ? q.p0 + t : -1;
-        const T* qp = static_cast<const T*>(a.q) + static_cast<int64_t>(q.start + (row_ok ? t : 0)) * a.q_stride +
-                      (kh * g + r % g) * D;
+        const Row r = row_of(a, t0, rem0 + 32 * (RT * wave + rt) + lc);
+        const bool row_ok = r.t < q.todo;
+        limit_key[rt] = row_ok ? q.p0 + r.t : -1;
+        const T* qp = static_cast<const T*>(a.q) + static_cast<int64_t>(q.start + (row_ok ? r.t : 0)) * a.q_stride +
+                      (kh * g + r.head) * D;
 #pragma unroll
         for (int s = 0; s < NQ; ++s) {
             qf[rt][s] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(qp) + 32 * s + 16 * lh);
@@ -929,8 +958,9 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
         }
     }
     // Keys below wave_whole are seen by every row of the wave, from wave_seen on by none.
-    const int wave_whole = w0 / g < q.todo ? min(max(q.p0 + w0 / g + 1, 0), q.length) : 0;
-    const int wave_seen = w0 / g < q.todo ? min(seen, max(q.p0 + min((w0 + 32 * RT - 1) / g, q.todo - 1) + 1, 0)) : 0;
+    const int w0 = uniform(row_of(a, t0, rem0 + 32 * RT * wave).t), w1 = uniform(row_of(a, t0, rem0 + 32 * RT * (wave + 1) - 1).t);
+    const int wave_whole = w0 < q.todo ? min(max(q.p0 + w0 + 1, 0), q.length) : 0;
+    const int wave_seen = w0 < q.todo ? min(seen, max(q.p0 + min(w1, q.todo - 1) + 1, 0)) : 0;
 
     f32x16 acc[RT][ND];
     float m_run[RT], limit[RT], l_run[RT];
@@ -954,24 +984,32 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
             for (int n = 0; n < NK; ++n)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) st[rt][n][e] = 0.0f;
+        // LDS reads run kAhead operands in front of their products: left to
+        // itself, the compiler waits for each before the next.
+        const auto key_piece = [&](int i) {   // of score tile i / NQ, 16-byte piece i % NQ
+            const int row = 32 * (i / NQ) + lc;
+            return *reinterpret_cast<const u32x4*>(kt + row * kRowBytes + 16 * ((2 * (i % NQ) + lh) ^ L::swap_k(row)));
+        };
+        u32x4 kf[kAhead];
 #pragma unroll
-        for (int n = 0; n < NK; ++n)
+        for (int i = 0; i < kAhead; ++i) kf[i] = key_piece(i);
+        keep_order();
 #pragma unroll
-            for (int s = 0; s < NQ; ++s) {
-                const int row = 32 * n + lc;
-                const u32x4 kf = *reinterpret_cast<const u32x4*>(kt + row * kRowBytes + 16 * ((2 * s + lh) ^ L::swap_k(row)));
+        for (int i = 0; i < NK * NQ; ++i) {
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    if constexpr (kWide) {
+            for (int rt = 0; rt < RT; ++rt) {
+                if constexpr (kWide) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            st[rt][n] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kf[e]), __uint_as_float(qf[rt][s][e]),
-                                                                             st[rt][n], 0, 0, 0);
-                    } else {
-                        st[rt][n] = mfma32<T>(kf, qf[rt][s], st[rt][n]);
-                    }
+                    for (int e = 0; e < 4; ++e)
+                        st[rt][i / NQ] = __builtin_amdgcn_mfma_f32_32x32x2f32(
+                            __uint_as_float(kf[i % kAhead][e]), __uint_as_float(qf[rt][i % NQ][e]), st[rt][i / NQ], 0, 0, 0);
+                } else {
+                    st[rt][i / NQ] = mfma32<T>(kf[i % kAhead], qf[rt][i % NQ], st[rt][i / NQ]);
                 }
             }
+            if (i + kAhead < NK * NQ) kf[i % kAhead] = key_piece(i + kAhead);
+            keep_order();
+        }
         if (masked) {
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
@@ -1041,36 +1079,40 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
                     }
         } else {
             const int l16 = lane & 15;
+            const auto value_piece = [&](int i) {   // of 16 keys i / ND, dim tile i % ND
+                u32x4 x;
 #pragma unroll
-            for (int n = 0; n < NK; ++n)
+                for (int w = 0; w < 2; ++w) {
+                    // lane 4 k + x of 16 reads dims 4 x .. + 3 of key k
+                    const int row = 16 * (i / ND) + 8 * w + 4 * lh + l16 / 4;
+                    const int c = 4 * (i % ND) + 2 * (lane >> 4 & 1) + (l16 % 4) / 2;
+                    const char* at = vt + row * kRowBytes + 16 * (c ^ L::swap_v(row)) + 8 * (l16 & 1);
+                    const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                                  (__attribute__((address_space(3))) s16x4*)(at)));
+                    x[2 * w] = y.x;
+                    x[2 * w + 1] = y.y;
+                }
+                return x;
+            };
+            u32x4 vf[kAhead], pf[RT];
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    u32x4 pf[RT];
+            for (int i = 0; i < kAhead; ++i) vf[i] = value_piece(i);
+            keep_order();
 #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) {
+            for (int i = 0; i < 2 * NK * ND; ++i) {
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    if (i % ND == 0) {
                         float p[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) p[e] = st[rt][n][8 * s + e];
+                        for (int e = 0; e < 8; ++e) p[e] = st[rt][i / ND / 2][i / ND % 2 * 8 + e];
                         pf[rt] = pack8<T>(p);
                     }
-#pragma unroll
-                    for (int db = 0; db < ND; ++db) {
-                        // lane 4 k + x of 16 reads dims 4 x .. + 3 of key k
-                        uint32_t x[4];
-#pragma unroll
-                        for (int w = 0; w < 2; ++w) {
-                            const int row = 32 * n + 16 * s + 8 * w + 4 * lh + l16 / 4;
-                            const int c = 4 * db + 2 * (lane >> 4 & 1) + (l16 % 4) / 2;
-                            const char* at = vt + row * kRowBytes + 16 * (c ^ L::swap_v(row)) + 8 * (l16 & 1);
-                            const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                (__attribute__((address_space(3))) s16x4*)(at));
-                            __builtin_memcpy(x + 2 * w, &y, 8);
-                        }
-                        const u32x4 vf{x[0], x[1], x[2], x[3]};
-#pragma unroll
-                        for (int rt = 0; rt < RT; ++rt) acc[rt][db] = mfma32<T>(vf, pf[rt], acc[rt][db]);
-                    }
+                    acc[rt][i % ND] = mfma32<T>(vf[i % kAhead], pf[rt], acc[rt][i % ND]);
                 }
+                if (i + kAhead < 2 * NK * ND) vf[i % kAhead] = value_piece(i + kAhead);
+                keep_order();
+            }
         }
     };
     // The values of a tile that are not finite, to the rows that see them,
@@ -1130,7 +1172,7 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
                 const float y[4] = {acc[rt][db][4 * u], acc[rt][db][4 * u + 1], acc[rt][db][4 * u + 2], acc[rt][db][4 * u + 3]};
                 const int i = 4 * (ND * rt + db) + u;
                 if (active == 1)
-                    put<T>(a, q, kh, g, r0 + row, place(i).dim, y, l, D);
+                    put<T>(a, q, kh, row_of(a, t0, rem0 + row), place(i).dim, y, l, D);
                 else
                     coherent_store16(prs, (i * kThreads + static_cast<int>(threadIdx.x)) * 16,
                                      u32x4{__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3])});
@@ -1145,7 +1187,7 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
     if (active > 1 && last_arrival(a.tickets + first_group * kTicketStride, active, &sh.ticket)) {
         float* f = reinterpret_cast<float*>(sh.tile[0][0]);
         static_assert((kManySplits + 1) * kRows * 4 <= static_cast<int>(sizeof sh.tile), "factors fit");
-        join_parts<T, D, kRows>(a, q, kh, g, r0, active, a.parts, part, place, f, f + kManySplits * kRows);
+        join_parts<T, D, kRows>(a, q, kh, t0, rem0, active, a.parts, part, place, f, f + kManySplits * kRows);
         __syncthreads();
     }
     }
@@ -1205,7 +1247,7 @@ int check_call(const char* who, int64_t batch, int64_t rows, int64_t max_rows, i
     if (d != 64 && d != 128) return fail_inval(w + ": head_dim must be 64 or 128");
     if (batch < 0 || batch > kMaxBatch || rows < 0 || rows > VM_HIP_PAGED_MAX_ROWS || max_rows < 0)
         return fail_inval(w + ": batch or rows out of range");
-    if (kv_heads < 1 || kv_heads > 4096 || heads < 1 || heads > 65536 || heads % kv_heads)
+    if (kv_heads < 1 || kv_heads > 4096 || heads < 1 || heads > 65536 || heads % kv_heads || heads / kv_heads > 4096)
         return fail_inval(w + ": bad heads");
     if (rows * heads >= (int64_t{1} << 30)) return fail_inval(w + ": too many rows for one call");
     return 0;
@@ -1240,6 +1282,8 @@ void launch_type(const Args& a, const Plan& p, hipStream_t s) {
 template <bool kPaged>
 int run(const char* who, Args a, const Plan& p, int dtype, int64_t d, void* workspace, void* stream) {
     a.few = p.few_rows;
+    a.group = a.heads / a.kv_heads;
+    a.per_group = static_cast<unsigned>(((uint64_t{1} << 32) + a.group - 1) / a.group);
     a.shared = p.shared;
     a.tickets = static_cast<unsigned*>(workspace);
     a.parts = static_cast<char*>(workspace) + kTicketBytes;
