@@ -52,7 +52,6 @@ constexpr int kTargetGroups = 512;    // workgroups that fill 256 compute units 
 constexpr int kTicketStride = 16;     // a ticket has a 64-byte line of its own
 constexpr int64_t kTicketBytes = kTargetGroups * kTicketStride * 4;
 constexpr int kRound = 128;           // keys that the waves of attention_few_kernel take at once
-constexpr int kLeast = 2;             // rounds that are worth a workgroup
 // A weight may exceed 1 by this much (log2) before its row's reference moves:
 // references then move in the first blocks and rarely later.
 constexpr float kHeadroom = 7.0f;
@@ -235,6 +234,21 @@ struct RowDim {
 template <typename T, int D, int kRows, typename Part, typename Place>
 __device__ __forceinline__ void join_parts(const Args& a, const Request& q, int kh, int t0, int r0, int active,
                                            const char* parts, Part part, Place place, float* factors, float* totals) {
+    // Two items of a thread and eight parts at a time, 16 loads in flight; the
+    // first are requested before the factors' inputs.
+    constexpr int kItems = kRows * D / 4 / kThreads;
+    constexpr int kTake = kItems < 2 ? kItems : 2;
+    u32x4 x[kTake][8];
+    const auto request_parts = [&](int i0, int s0) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            if (s0 + u >= active) break;
+            const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(parts + part(s0 + u), kRows * D * 4);
+#pragma unroll
+            for (int i = 0; i < kTake; ++i) x[i][u] = coherent_load16(rs, ((i0 + i) * kThreads + threadIdx.x) * 16);
+        }
+    };
+    request_parts(0, 0);
     for (int row = threadIdx.x / 16; row < kRows; row += kThreads / 16) {
         const int s0 = threadIdx.x % 16;
         float mv[kMaxSplits / 16], lv[kMaxSplits / 16], m = -INFINITY;
@@ -265,30 +279,20 @@ __device__ __forceinline__ void join_parts(const Args& a, const Request& q, int 
         if (s0 == 0) totals[row] = l;
     }
     __syncthreads();
-    // Two items of a thread and eight parts at a time, 16 loads in flight.
-    constexpr int kItems = kRows * D / 4 / kThreads;
-    constexpr int kTake = kItems < 2 ? kItems : 2;
     for (int i0 = 0; i0 < kItems; i0 += kTake) {
         float y[kTake][4] = {};
         for (int s0 = 0; s0 < active; s0 += 8) {
-            u32x4 x[kTake][8];
+            if (i0 + s0 > 0) request_parts(i0, s0);
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
-                if (s0 + u < active) {
-                    const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(parts + part(s0 + u), kRows * D * 4);
+            for (int u = 0; u < 8; ++u) {
+                if (s0 + u >= active) break;
 #pragma unroll
-                    for (int i = 0; i < kTake; ++i) x[i][u] = coherent_load16(rs, ((i0 + i) * kThreads + threadIdx.x) * 16);
+                for (int i = 0; i < kTake; ++i) {
+                    const float f = factors[(s0 + u) * kRows + place(i0 + i).row];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[i][e] = fmaf(__uint_as_float(x[i][u][e]), f, y[i][e]);
                 }
-#pragma unroll
-            for (int u = 0; u < 8; ++u)
-                if (s0 + u < active) {
-#pragma unroll
-                    for (int i = 0; i < kTake; ++i) {
-                        const float f = factors[(s0 + u) * kRows + place(i0 + i).row];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) y[i][e] = fmaf(__uint_as_float(x[i][u][e]), f, y[i][e]);
-                    }
-                }
+            }
         }
 #pragma unroll
         for (int i = 0; i < kTake; ++i) {
@@ -297,7 +301,6 @@ __device__ __forceinline__ void join_parts(const Args& a, const Request& q, int 
         }
     }
 }
-
 
 constexpr int64_t part_bytes(int64_t rows, int64_t d) { return rows * (d + 2) * 4; }
 
@@ -412,8 +415,10 @@ __device__ __forceinline__ void few_rows(const Args& a, int id, FewShared<D, RT>
     // Rounds of all requests, summed up by every workgroup for itself.
     int longest;
     const int total = a.kv_heads * sum_up(a.batch, sh.sums, [&](int b) { return rounds_of(request<true>(a, b)); }, &longest);
-    // Shares: even, worth a workgroup, and no more than kMaxSplits of a request's keys.
-    const int per = max(max((total + kTargetGroups - 1) / kTargetGroups, kLeast),
+    // Shares: even, worth a workgroup (64 KB of keys and values or so; one fp32
+    // token over 2000: 9.0 us with one round, 9.9 with two; one of 64 heads of 128
+    // over 8000, bf16: 23 and 17, with four 18.7), and no more than kMaxSplits of a request's keys.
+    const int per = max(max((total + kTargetGroups - 1) / kTargetGroups, kWide ? 1 : 2),
                         (longest + kMaxSplits - 2) / (kMaxSplits - 1));
     int pos = id * per;
     const int end = min(total, pos + per);
