@@ -497,8 +497,14 @@ __device__ __forceinline__ void few_rows(const Args& a, int id, FewShared<D, RT>
             load_values(block, id_v);
         }
 
-        u32x4 qf[RT][KC];
+        // Queries: in registers, or, where these do not do, in LDS (where the
+        // outputs are merged later).
+        constexpr bool kQueriesInLds = RT == 2 && D == 128;
+        u32x4 qf[kQueriesInLds ? 1 : RT][kQueriesInLds ? 1 : KC];
+        u32x4* q_lds = reinterpret_cast<u32x4*>(merge_o[0]) + lane;
+        static_assert(RT * KC * 1024 <= static_cast<int>(sizeof merge_o), "queries fit");
         int limit_key[RT];   // the last key that the row sees
+        if (kQueriesInLds) __syncthreads();   // (the last segment's merge has been read)
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             const Row r = row_of(a, 0, 16 * rt + lr);
@@ -508,10 +514,22 @@ __device__ __forceinline__ void few_rows(const Args& a, int id, FewShared<D, RT>
                           (kh * g + r.head) * D;
 #pragma unroll
             for (int s = 0; s < KC; ++s) {
-                qf[rt][s] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(qp) + 64 * s + 16 * lg);
-                if (!row_ok) qf[rt][s] = u32x4{0, 0, 0, 0};
+                if (kQueriesInLds && s % kWaves != wave) continue;
+                u32x4 x = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(qp) + 64 * s + 16 * lg);
+                if (!row_ok) x = u32x4{0, 0, 0, 0};
+                if constexpr (kQueriesInLds)
+                    q_lds[(rt * KC + s) * 64] = x;
+                else
+                    qf[rt][s] = x;
             }
         }
+        if (kQueriesInLds) __syncthreads();
+        const auto query = [&](int rt, int s) {
+            if constexpr (kQueriesInLds)
+                return q_lds[(rt * KC + s) * 64];
+            else
+                return qf[rt][s];
+        };
         f32x4 acc[RT][ND];
         float m_run[RT];   // the score that weighs 1
         float limit[RT];   // the score from which on it moves; -inf before the first key
@@ -525,6 +543,7 @@ __device__ __forceinline__ void few_rows(const Args& a, int id, FewShared<D, RT>
         }
 
         for (; block < block_end; block += kWaves) {
+            if (kQueriesInLds) asm volatile("" : : : "memory");   // (read again: not kept in registers)
             const bool there = valid(id_v);
             f32x4 st[RT][NT];
 #pragma unroll
@@ -534,18 +553,20 @@ __device__ __forceinline__ void few_rows(const Args& a, int id, FewShared<D, RT>
 #pragma unroll
             for (int s = 0; s < KC; ++s)
 #pragma unroll
-                for (int bt = 0; bt < NT; ++bt)
+                for (int rt = 0; rt < RT; ++rt) {
+                    const u32x4 x = query(rt, s);
 #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) {
+                    for (int bt = 0; bt < NT; ++bt) {
                         if constexpr (kWide) {
 #pragma unroll
                             for (int e = 0; e < 4; ++e)
-                                st[rt][bt] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                                    __uint_as_float(kreg[bt][s][e]), __uint_as_float(qf[rt][s][e]), st[rt][bt], 0, 0, 0);
+                                st[rt][bt] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kreg[bt][s][e]), __uint_as_float(x[e]),
+                                                                                  st[rt][bt], 0, 0, 0);
                         } else {
-                            st[rt][bt] = mfma16<T>(kreg[bt][s], qf[rt][s], st[rt][bt]);
+                            st[rt][bt] = mfma16<T>(kreg[bt][s], x, st[rt][bt]);
                         }
                     }
+                }
             load_keys(block + kWaves, next_k);
             const bool masked = (block + 1) * KB > whole || !__all(there);
             if (masked) {
@@ -1226,13 +1247,14 @@ Plan plan(int64_t batch, int64_t rows, int64_t max_rows, int64_t heads, int64_t 
     Plan p{};
     const int64_t g = heads / kv_heads;
     const int64_t most = std::min(rows, max_rows > 0 ? max_rows : rows) * g;   // query rows of a request
-    p.few_tiles = most <= 16 ? 1 : 2;
+    // (requests between 17 and 32 rows are the other kernel's where that runs anyway)
+    p.few_tiles = most <= 16 || (most > 32 && g <= 16) ? 1 : 2;
     p.few_rows = 16 * p.few_tiles;
     // One request with more rows than that: all of it is the other kernel's.
     p.few = paged && g <= p.few_rows && (batch > 1 || most <= p.few_rows);
     if (!p.few) p.few_rows = 0;
     p.many = most > p.few_rows;
-    if (p.few) p.bytes = 2 * kTargetGroups * part_bytes(16 * p.few_tiles, d);
+    if (p.few) p.bytes = 2 * kTargetGroups * part_bytes(32, d);
     if (p.many) {
         // Two row tiles a wave read a key tile's operands once for both, where
         // registers allow and enough tiles are left for the workgroups.
