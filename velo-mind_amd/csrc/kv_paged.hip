@@ -87,24 +87,24 @@ __device__ __forceinline__ int last_at_most(const int* start, int n, int x) {
 
 // ---- The plan.  Every workgroup sums all requests up for itself (E
 // consecutive ones a thread; 2048 requests are 16 KB, read from L2) and then
-// places kPlanRows rows: a search in LDS, one page id, two stores.  One launch
+// places a row a thread: a search in LDS, one page id, two stores.  One launch
 // and no second pass, because a page that is handed out starts with a row of
 // this step: the row at its first position writes the table's entry.  The
-// pool's count and the lengths may be updated in place: the workgroup that
+// pool's count and the lengths may be updated in place: then the workgroup that
 // draws the last ticket, when all have read them, writes both.  Bound by the
-// launch and three round trips (requests, page ids, stores).
-constexpr int kPlanRows = 4 * kT;
-
+// launch and three round trips (requests, page ids, stores): 32 rows of 32
+// requests 3.8 us, 128000 of 256 6.7 (four rows a thread: 9.3).
 struct PlanArgs {
     vm_hip_page_plan p;
     int shift;          // log2 of the page size
-    unsigned* ticket;   // with more than one workgroup
+    unsigned* ticket;   // with more than one workgroup and results in place
 };
 
 template <int E>
 __global__ __launch_bounds__(kT) void kv_paged_plan_kernel(const PlanArgs a) {
     __shared__ int row_start[kMaxBatch + 1];   // rows in front of a request's
     __shared__ int page_start[kMaxBatch];      // pages handed out in front of a request's
+    __shared__ int lengths[kMaxBatch];
     __shared__ int waves[kT / 64];
     __shared__ int handed_out;
     __shared__ unsigned drawn;
@@ -161,7 +161,7 @@ __global__ __launch_bounds__(kT) void kv_paged_plan_kernel(const PlanArgs a) {
     run = sum_before(mine, 0x3fffffff, waves, &total);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        if (b0 + e < batch) row_start[b0 + e] = run;
+        if (b0 + e < batch) row_start[b0 + e] = run, lengths[b0 + e] = length[e];
         run += count[e];
     }
     if (threadIdx.x == 0) row_start[batch] = total, handed_out = 0;
@@ -169,38 +169,25 @@ __global__ __launch_bounds__(kT) void kv_paged_plan_kernel(const PlanArgs a) {
     if (taken > 0) atomicMax(&handed_out, taken);
     __syncthreads();
 
-    const int r0 = static_cast<int>(blockIdx.x) * kPlanRows + threadIdx.x;
-    int position[4], slot[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-        const int r = r0 + u * kT;
-        position[u] = slot[u] = -1;
-        if (r >= total) continue;
+    const int r = static_cast<int>(blockIdx.x) * kT + threadIdx.x;
+    if (r < total) {
         const int b = last_at_most(row_start, batch, r);
-        const int n = p.lengths[b];
-        position[u] = n + r - row_start[b];
-        const int held = (n + page - 1) >> a.shift, at = position[u] >> a.shift;
+        const int n = lengths[b];
+        const int position = n + r - row_start[b];
+        const int held = (n + page - 1) >> a.shift, at = position >> a.shift;
         int32_t* entry = p.tables + static_cast<int64_t>(b) * p.max_pages + at;
-        int id;
-        if (at < held) {
-            id = *entry;
-        } else {
-            id = p.free_pages[free_pages - 1 - (page_start[b] + at - held)];
-            if ((position[u] & (page - 1)) == 0) *entry = id;
-        }
-        if (id >= 0 && id < p.pages) slot[u] = (id << a.shift) + (position[u] & (page - 1));
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-        const int r = r0 + u * kT;
-        if (r < rows) {
-            p.positions[r] = position[u];
-            p.slots[r] = slot[u];
-        }
+        const int id = at < held ? *entry : p.free_pages[free_pages - 1 - (page_start[b] + at - held)];
+        if (at >= held && (position & (page - 1)) == 0) *entry = id;
+        p.positions[r] = position;
+        p.slots[r] = id >= 0 && id < p.pages ? (id << a.shift) + (position & (page - 1)) : -1;
+    } else if (r < rows) {
+        p.positions[r] = p.slots[r] = -1;
     }
     if (blockIdx.x == 0)
         for (int b = threadIdx.x; b <= batch; b += kT) p.row_start[b] = row_start[b];
-    if (gridDim.x > 1) {
+    if (!a.ticket) {
+        if (blockIdx.x != 0) return;
+    } else if (gridDim.x > 1) {
         __syncthreads();   // this workgroup has read the lengths and the count
         if (threadIdx.x == 0) drawn = ticket_take(a.ticket, gridDim.x);
         __syncthreads();
@@ -260,12 +247,14 @@ __global__ __launch_bounds__(kT) void kv_paged_release_kernel(int batch, int64_t
 
 // ---- Tables of the rotation.  Angles of far positions need 64 bits (131071
 // radians leave 2^-7 of a turn in fp32): the first of a thread's R rows takes
-// a sine and cosine in fp64, the others turn it on by the frequency's own,
-// four products a row (each adds 2^-52 or so).  Pairs are adjacent lanes.
+// a sine and cosine in fp64, of its part of a turn, the others turn it on by the
+// frequency's own, four products a row (each adds 2^-52 or so).  Pairs are
+// adjacent lanes.  Bound by the stores (131072 rows of 64 pairs: 12.2 us, 5.5
+// TB/s); small tables by the launch and one sine (2000 of 32: 4.5).
 constexpr int kMaxPairs = 64;
 
 struct RopeArgs {
-    double f[kMaxPairs], c[kMaxPairs], s[kMaxPairs];   // radians a position, and their cosines and sines
+    double turns[kMaxPairs], c[kMaxPairs], s[kMaxPairs];   // of a position: turns, cosine and sine
     double factor;
     float* cos_t;
     float* sin_t;
@@ -280,7 +269,8 @@ __global__ __launch_bounds__(kT) void rope_tables_kernel(const RopeArgs a) {
     const int i = static_cast<int>(u % a.pairs);
     if (r0 >= a.rows) return;
     double s, c;
-    sincos(static_cast<double>(a.first + r0) * a.f[i], &s, &c);
+    const double t = static_cast<double>(a.first + r0) * a.turns[i];
+    sincospi(2.0 * (t - rint(t)), &s, &c);
     c *= a.factor;
     s *= a.factor;
     const double tc = a.c[i], ts = a.s[i];
@@ -300,8 +290,10 @@ __global__ __launch_bounds__(kT) void rope_tables_kernel(const RopeArgs a) {
 // steps away, pairs of the interleaved layout are a lane's own, and those of
 // halves are exchanged through LDS (any even number of rotated elements does).
 // A group takes the heads h0, h0 + step, ... of its token, with the table's
-// row and the norms' weights in registers.  Bound: one read of qkv, one write
-// of q, keys and values.
+// row and the norms' weights in registers and the next head's row on its way.
+// Bound: one read of qkv, one write of q, keys and values (4000 rows of 80 heads
+// of 128, bf16, normed, half of each rotated in pairs: 28 us, 5.8 TB/s, part of it
+// from the caches that hold what was written last; one row of 40 heads of 64: 3.7).
 template <typename T, int N>
 struct alignas(sizeof(T) * N >= 16 ? 16 : sizeof(T) * N) Vec {
     T e[N];
@@ -372,8 +364,11 @@ __global__ __launch_bounds__(kT) void kv_paged_append_kernel(const AppendArgs a)
         }
     }
     const T* src = static_cast<const T*>(a.qkv) + token * width * D + i * N;
-    for (int h = static_cast<int>(u % a.step); h < all; h += a.step) {
-        Vec<T, N> x = *reinterpret_cast<const Vec<T, N>*>(src + static_cast<int64_t>(h) * D);
+    const int h0 = static_cast<int>(u % a.step);
+    Vec<T, N> next = *reinterpret_cast<const Vec<T, N>*>(src + static_cast<int64_t>(h0) * D);
+    for (int h = h0; h < all; h += a.step) {
+        Vec<T, N> x = next;
+        next = *reinterpret_cast<const Vec<T, N>*>(src + static_cast<int64_t>(min(h + a.step, all - 1)) * D);
         T* dst;
         if (h < a.heads) {
             dst = static_cast<T*>(a.q_out) + (token * a.heads + h) * D;
@@ -474,9 +469,10 @@ int append(const char* who, AppendArgs a, int dtype, int64_t heads, int64_t kv_h
     a.heads = static_cast<int>(heads);
     a.kv_heads = static_cast<int>(kv_heads);
     // Groups of a token: one a head while they do not fill the GPU, so that no
-    // head waits for another.
+    // head waits for another (65536 of them instead of 16384: 2000 fp32 rows of 40
+    // heads of 64 11.8 us, 8.4).
     const int all = a.heads + 2 * a.kv_heads;
-    a.step = static_cast<int>(std::min<int64_t>(all, std::max<int64_t>(1, 65536 / a.rows)));
+    a.step = static_cast<int>(std::min<int64_t>(all, std::max<int64_t>(1, 16384 / a.rows)));
     auto s = static_cast<hipStream_t>(stream);
     if (head_dim == 64) {
         if (dtype == VM_HIP_DTYPE_F32)
@@ -528,8 +524,9 @@ int vm_hip_kv_paged_plan(const vm_hip_page_plan* plan, void* workspace, int64_t 
         return fail_inval("kv_paged_plan: null or unaligned pointer");
     if (!workspace || workspace_bytes < need || off16(workspace))
         return fail_inval("kv_paged_plan: workspace smaller than vm_hip_kv_paged_plan_workspace_bytes or unaligned");
-    PlanArgs a{p, log2_of(p.page_size), static_cast<unsigned*>(workspace)};
-    const dim3 grid(static_cast<unsigned>(std::max<int64_t>(1, (p.rows + kPlanRows - 1) / kPlanRows))), block(kT);
+    const bool in_place = p.lengths_out == p.lengths || p.free_count_out == p.free_count;
+    PlanArgs a{p, log2_of(p.page_size), in_place ? static_cast<unsigned*>(workspace) : nullptr};
+    const dim3 grid(static_cast<unsigned>(std::max<int64_t>(1, (p.rows + kT - 1) / kT))), block(kT);
     auto s = static_cast<hipStream_t>(stream);
     if (p.batch <= kT)
         hipLaunchKernelGGL(kv_paged_plan_kernel<1>, grid, block, 0, s, a);
@@ -611,7 +608,7 @@ int vm_hip_rope_tables(float* cos_table, float* sin_table, int64_t first, int64_
             const double r = std::min(1.0, std::max(0.0, (i - low) / std::max(high - low, 0.001)));
             f = f / scaling->factor * r + f * (1.0 - r);
         }
-        a.f[i] = f;
+        a.turns[i] = f / two_pi;
         a.c[i] = std::cos(f);
         a.s[i] = std::sin(f);
     }
