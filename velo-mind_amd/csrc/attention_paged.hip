@@ -786,7 +786,7 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
     constexpr int kRowBytes = D * sizeof(T);
     constexpr int kLeastTiles = kWide ? 2 : 4;   // key tiles that are worth a workgroup
     constexpr int kAhead = 4;                    // LDS operands in front of their products
-    constexpr int kJoin = kWide ? 3 : 16;        // key tiles' time that parts take
+    constexpr int kJoin = kWide ? 3 : D == 64 ? 28 : 16;      // key tiles' time that parts take
     constexpr int kStart = kWide ? 1 : 2;        // key tiles' time that a row tile takes beside its keys
 
     const int lane = threadIdx.x & 63;
@@ -851,15 +851,19 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
         pos = start + size;
         if (last <= first) continue;
     } else {
-        // Workgroups go to the XCDs in turn: a KV head's tiles stay on one where
-        // the count of those allows, the last tiles, which see the most keys, first.
+        // Workgroups go to the XCDs in turn, eight at a time: a KV head's tiles
+        // stay on one where the count of those allows, the last tiles, which see
+        // the most keys, first.  Of the 512 that start at once a compute unit has
+        // the n-th and the 256 + n-th: the second half goes backwards.
+        int at = pos / 8;
+        const int half = kTargetGroups / 16, both = min(kTargetGroups, tiles_all * a.kv_heads) / 8;
+        if (at >= half && at < both) at = half + both - 1 - at;
         if (a.kv_heads % 8 == 0) {
-            const int j = pos / 8;
-            slot = tiles_all - 1 - j % tiles_all;
-            kh = j / tiles_all * 8 + pos % 8;
+            slot = tiles_all - 1 - at % tiles_all;
+            kh = at / tiles_all * 8 + pos % 8;
         } else {
-            slot = tiles_all - 1 - pos / a.kv_heads;
-            kh = pos % a.kv_heads;
+            slot = tiles_all - 1 - (8 * at + pos % 8) / a.kv_heads;
+            kh = (8 * at + pos % 8) % a.kv_heads;
         }
         pos = end;
     }
