@@ -459,6 +459,35 @@ def test_packed_later_rows_count_for_nothing(hip, dtype, d, odd):
         assert not np.isfinite(got[t:n]).any()
 
 
+@pytest.mark.parametrize("dtype,heads,hk,d,n", [(4, 64, 8, 64, [2300, 77]), (5, 64, 8, 64, [2100]), (5, 64, 8, 128, [900, 700]),
+                                                (4, 48, 16, 64, [1400]), (0, 40, 5, 64, [1300, 1]), (0, 16, 16, 128, [700]),
+                                                (4, 32, 32, 128, [1000, 600])], ids=str)
+def test_packed_large(hip, dtype, heads, hk, d, n):
+    """More row tiles than workgroups run at once, and both tile sizes, by some of the heads."""
+    c = Packed(hip, dtype, n, heads, hk, d, 30).upload()
+    c.call()
+    got, x = c.result(), held(c.qkv, dtype)
+    g = heads // hk
+    for a, b in zip(c.start[:-1], c.start[1:]):
+        for h in (0, hk // 2, hk - 1):
+            u = [h * g, h * g + g - 1]
+            want, tol = reference(x[a:b, u], x[a:b, [heads + h]], x[a:b, [heads + hk + h]], 0, d ** -0.5, dtype)
+            close(got[a:b, u], want, tol)
+    first = got
+    c.call()
+    assert np.array_equal(first, c.result())
+
+
+@pytest.mark.parametrize("dtype", [0, 5], ids=["f32", "bf16"])
+def test_chunks_large(hip, dtype):
+    """Chunks whose keys several workgroups share, and chunks that have one each."""
+    for n, lengths, heads, hk, d in [([600, 90, 300], [2600, 4000, 300], 16, 4, 64), ([300] * 5, [500] * 5, 32, 8, 128)]:
+        c = Paged(hip, dtype, n, lengths, heads, hk, d, 32, 31).upload()
+        for _ in range(2):
+            c.call()
+        c.check()
+
+
 @TYPES
 def test_packed_many_requests(hip, dtype):
     r = np.random.default_rng(23)

@@ -149,8 +149,12 @@ def test_attention_workspaces():
         for batch in (1, 2, 7, 64, 2048):
             sizes = [H.attention_paged_workspace_bytes(batch, r, m, heads, hk, d, 4096)
                      for r, m in [(1, 1), (batch, 1), (batch + 1, 2), (batch + 99, 100), (batch + 5000, 0)]]
-            assert all(s >= 0 and s % 4 == 0 for s in sizes)
-            assert H.attention_packed_workspace_bytes(batch, 100, heads, hk, d) >= 0
+            assert sizes == sorted(sizes) and sizes[0] >= 0 and not any(s % 16 for s in sizes)
+            for tokens in (16, 64, 100, 128, 129, 300):
+                few, many = (H.attention_paged_workspace_bytes(batch, r, 0, heads, hk, d, tokens) for r in (1, 5000))
+                assert 0 <= few <= many
+            sizes = [H.attention_packed_workspace_bytes(batch, rows, heads, hk, d) for rows in (1, 60, 128, 129, 5000)]
+            assert sizes == sorted(sizes)
     _refused(H.attention_paged_workspace_bytes, 1, 1, 1, 4, 3, 64, 16)
     _refused(H.attention_paged_workspace_bytes, 1, 1, 1, 4, 2, 64, 0)
     _refused(H.attention_paged_workspace_bytes, 1, 1, 1, 4, 2, 64, (1 << 24) + 1)

@@ -742,15 +742,23 @@ __device__ __forceinline__ void few_rows(const Args& a, int id, FewShared<D, RT>
 }
 
 // ---- Many rows: 32-wide tiles, 32 RT query rows a wave, KT keys at a time in
-// LDS for all four waves, the next tile's on their way in registers.  A[i][k] and
-// B[k][j] of a 32x32x16 product sit in lane i (j) + 32 (k / 8), element k % 8; of
+// LDS for all four waves, the next tile's on their way into a second buffer.
+// A[i][k] and B[k][j] of a 32x32x16 product sit in lane i (j) + 32 (k / 8), element k % 8; of
 // a 32x32x2 fp32 product in lane i (j) + 32 k; D[i][j] in lane j + 32 (i / 4 %
 // 2), element i % 4 + 4 (i / 8).  A lane of half lh = lane / 32 holds the
 // scores of keys 8 a + 4 lh + b: as weights they are the second product's k
 // positions if V^T's operand has the same keys there, which two transposing LDS
 // reads of four keys give (16 bits), or plain reads (fp32).
-// LDS rows hold their 16-byte pieces exchanged by the row's number, so that
-// the rows that are read together lie in different banks.
+//
+// MI355X, passes back to back: 3 prompts of 12000 tokens, 64 heads of 128 on 8,
+// bf16: 963 us, 948 TFLOP/s (a large product: 1150); one of 6500, 64 heads of 64
+// on 8, f16: 380 us, 910 TFLOP/s; 500 tokens behind 30000, 32 heads of 128 on 8,
+// f16: 292 us, 850 TFLOP/s; one fp32 prompt of 2000, 64 heads of 128: 536 us, 122
+// TFLOP/s (153).  The matrix cores are busy 40 % of the cycles: what is left is
+// softmax between the products of two waves a SIMD (without the loads 496 us
+// where it takes 640, without barriers too 472, without exponentials 436).  Eight
+// waves and 128 keys a tile: 743 us for 625; a tile's scores beside the weights
+// of the one before: registers spill, 1310.
 template <typename T, int D>
 struct Tile {
     static constexpr int KT = sizeof(T) == 4 ? 32 : 64;         // keys
@@ -786,7 +794,7 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
     constexpr int kRowBytes = D * sizeof(T);
     constexpr int kLeastTiles = kWide ? 2 : 4;   // key tiles that are worth a workgroup
     constexpr int kAhead = 4;                    // LDS operands in front of their products
-    constexpr int kJoin = kWide ? 3 : D == 64 ? 28 : 16;      // key tiles' time that parts take
+    constexpr int kJoin = kWide ? 3 : D == 64 ? 28 : 16;   // key tiles' time that parts take
     constexpr int kStart = kWide ? 1 : 2;        // key tiles' time that a row tile takes beside its keys
 
     const int lane = threadIdx.x & 63;
@@ -838,388 +846,389 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
     }
 
     while (pos < end) {
-    int kh, slot, first = 0, last = 0x7fffffff, active = 1, first_group = 0;
-    if (shared) {
-        kh = pos / of_head;
-        slot = first_above(sh.tiles, tiles_all, pos - kh * of_head);
-        const int before = slot ? sh.tiles.upto[slot - 1] : 0;
-        const int size = sh.tiles.upto[slot] - before, start = kh * of_head + before;
-        first = max(pos - start - kStart, 0);
-        last = min(end - start, size) - kStart;
-        first_group = (start + kStart) / share;
-        active = (start + size - 1) / share - first_group + 1;
-        pos = start + size;
-        if (last <= first) continue;
-    } else {
-        // Workgroups go to the XCDs in turn, eight at a time: a KV head's tiles
-        // stay on one where the count of those allows, the last tiles, which see
-        // the most keys, first.  Of the 512 that start at once a compute unit has
-        // the n-th and the 256 + n-th: the second half goes backwards.
-        int at = pos / 8;
-        const int half = kTargetGroups / 16, both = min(kTargetGroups, tiles_all * a.kv_heads) / 8;
-        if (at >= half && at < both) at = half + both - 1 - at;
-        if (a.kv_heads % 8 == 0) {
-            slot = tiles_all - 1 - at % tiles_all;
-            kh = at / tiles_all * 8 + pos % 8;
+        int kh, slot, first = 0, last = 0x7fffffff, active = 1, first_group = 0;
+        if (shared) {
+            kh = pos / of_head;
+            slot = first_above(sh.tiles, tiles_all, pos - kh * of_head);
+            const int before = slot ? sh.tiles.upto[slot - 1] : 0;
+            const int size = sh.tiles.upto[slot] - before, start = kh * of_head + before;
+            first = max(pos - start - kStart, 0);
+            last = min(end - start, size) - kStart;
+            first_group = (start + kStart) / share;
+            active = (start + size - 1) / share - first_group + 1;
+            pos = start + size;
+            if (last <= first) continue;
         } else {
-            slot = tiles_all - 1 - (8 * at + pos % 8) / a.kv_heads;
-            kh = (8 * at + pos % 8) % a.kv_heads;
-        }
-        pos = end;
-    }
-    kh = uniform(kh);
-    first = uniform(first);
-    last = uniform(last);
-    active = uniform(active);
-    first_group = uniform(first_group);
-    const int b = uniform(first_above(sh.requests, a.batch, slot));
-    const Request q = uniform(request<kPaged>(a, b));
-    const int r0 = uniform(slot - (sh.requests.upto[b] - tiles_of(q))) * kRows;
-    const int t0 = r0 / g, rem0 = r0 - t0 * g;   // its token, and the rows of that in front
-    const int t_last = min(uniform(row_of(a, t0, rem0 + kRows - 1).t), q.todo - 1);
-    const int seen = min(max(q.p0 + t_last + 1, 0), q.length);      // keys that some row sees
-    const int whole = min(max(q.p0 + t0 + 1, 0), q.length);         // that every row sees
-    last = min(last, (seen + KT - 1) / KT);
-
-    // Where the tile's pieces lie: a wave's piece u is 1 KB, kWaveRows rows.
-    constexpr int kWaveRows = 64 / CH, kStep = kWaves * kWaveRows;   // rows of a piece, of the waves' pieces u
-    static_assert(kStep <= 32, "those rows lie in two 16-key groups at most");
-    const int my_row = wave * kWaveRows + lane / CH;
-    static_assert(kStep % 8 == 0, "pieces u and u + 2 of a lane are exchanged alike");
-    const auto k_piece = [&](int u) { return 16 * ((lane % CH) ^ L::swap_k(my_row + u % 2 * kStep)); };
-    const uint32_t v_piece = 16 * ((lane % CH) ^ L::swap_v(my_row));
-    const int in_page = (1 << a.shift) - 1;
-    const int last_page = max(q.length - 1, 0) >> a.shift;
-    const int32_t* table = kPaged ? a.tables + static_cast<int64_t>(b) * a.max_pages : nullptr;
-    const uint32_t page_bytes = kPaged ? static_cast<uint32_t>(a.kv_heads << a.shift) * kRowBytes : 0;
-    const int k_row = kPaged ? kRowBytes : static_cast<int>(a.k_stride * sizeof(T));
-    const int v_row = kPaged ? kRowBytes : static_cast<int>(a.v_stride * sizeof(T));
-    const char* k_base = static_cast<const char*>(a.k) +
-                         (kPaged ? static_cast<int64_t>(kh << a.shift) * kRowBytes
-                                 : static_cast<int64_t>(q.start) * k_row + kh * kRowBytes);
-    const char* v_base = static_cast<const char*>(a.v) +
-                         (kPaged ? static_cast<int64_t>(kh << a.shift) * kRowBytes
-                                 : static_cast<int64_t>(q.start) * v_row + kh * kRowBytes);
-    // The pages of a tile's keys, one a lane for the 16 keys from 16 (lane % kGroups) on.
-    constexpr int kGroups = KT / 16;
-    constexpr unsigned kAll = (1u << kGroups) - 1;
-    const auto lookup = [&](int t) {
-        if constexpr (kPaged)
-            return table[min((t * KT + 16 * (lane % kGroups)) >> a.shift, last_page)];
-        else
-            return 0;
-    };
-    const auto valid = [&](int id) { return !kPaged || static_cast<unsigned>(id) < static_cast<unsigned>(a.pages); };
-    const uint32_t k_mine[2] = {static_cast<uint32_t>((kPaged ? my_row % 16 : my_row) * k_row + k_piece(0)),
-                                static_cast<uint32_t>((kPaged ? my_row % 16 : my_row) * k_row + k_piece(1))};
-    const uint32_t v_mine = (kPaged ? my_row % 16 : my_row) * v_row + v_piece;
-    const auto load = [&](int t, int ids) {
-        char* kl = sh.tile[t & 1][0] + wave * 1024;
-        char* vl = sh.tile[t & 1][1] + wave * 1024;
-        if constexpr (kPaged) {
-            const int pages = valid(ids) ? ids : 0;
-#pragma unroll
-            for (int u = 0; u < PER; ++u) {
-                const int group = u * kStep / 16 + (kStep > 16 ? wave / (kWaves / 2) : 0);
-                const uint32_t id = __builtin_amdgcn_readlane(pages, group);
-                const uint32_t at = ((t * KT + 16 * group) & in_page) + (kStep < 16 ? u * kStep % 16 : 0);
-                const uint64_t offset = static_cast<uint64_t>(id) * page_bytes + at * kRowBytes;
-                lds_load16(k_base + offset, k_mine[u % 2], kl + u * (kWaves * 1024));
-                lds_load16(v_base + offset, v_mine, vl + u * (kWaves * 1024));
+            // Workgroups go to the XCDs in turn, eight at a time: a KV head's tiles
+            // stay on one where the count of those allows, the last tiles, which see
+            // the most keys, first.  Of the 512 that start at once a compute unit has
+            // the n-th and the 256 + n-th: the second half goes backwards.
+            int at = pos / 8;
+            const int half = kTargetGroups / 16, both = min(kTargetGroups, tiles_all * a.kv_heads) / 8;
+            if (at >= half && at < both) at = half + both - 1 - at;
+            if (a.kv_heads % 8 == 0) {
+                slot = tiles_all - 1 - at % tiles_all;
+                kh = at / tiles_all * 8 + pos % 8;
+            } else {
+                slot = tiles_all - 1 - (8 * at + pos % 8) / a.kv_heads;
+                kh = (8 * at + pos % 8) % a.kv_heads;
             }
-        } else {
-            const char* kp = k_base + static_cast<int64_t>(t * KT) * k_row;
-            const char* vp = v_base + static_cast<int64_t>(t * KT) * v_row;
-            const int left = q.length - 1 - t * KT;   // the last row there is
-            if (left >= KT - 1) {
+            pos = end;
+        }
+        kh = uniform(kh);
+        first = uniform(first);
+        last = uniform(last);
+        active = uniform(active);
+        first_group = uniform(first_group);
+        const int b = uniform(first_above(sh.requests, a.batch, slot));
+        const Request q = uniform(request<kPaged>(a, b));
+        const int r0 = uniform(slot - (sh.requests.upto[b] - tiles_of(q))) * kRows;
+        if (r0 < 0 || r0 >= q.todo * g) continue;   // (row_start that does not rise)
+        const int t0 = r0 / g, rem0 = r0 - t0 * g;   // its token, and the rows of that in front
+        const int t_last = min(uniform(row_of(a, t0, rem0 + kRows - 1).t), q.todo - 1);
+        const int seen = min(max(q.p0 + t_last + 1, 0), q.length);      // keys that some row sees
+        const int whole = min(max(q.p0 + t0 + 1, 0), q.length);         // that every row sees
+        last = min(last, (seen + KT - 1) / KT);
+
+        // Where the tile's pieces lie: a wave's piece u is 1 KB, kWaveRows rows.
+        constexpr int kWaveRows = 64 / CH, kStep = kWaves * kWaveRows;   // rows of a piece, of the waves' pieces u
+        static_assert(kStep <= 32, "those rows lie in two 16-key groups at most");
+        const int my_row = wave * kWaveRows + lane / CH;
+        static_assert(kStep % 8 == 0, "pieces u and u + 2 of a lane are exchanged alike");
+        const auto k_piece = [&](int u) { return 16 * ((lane % CH) ^ L::swap_k(my_row + u % 2 * kStep)); };
+        const uint32_t v_piece = 16 * ((lane % CH) ^ L::swap_v(my_row));
+        const int in_page = (1 << a.shift) - 1;
+        const int last_page = max(q.length - 1, 0) >> a.shift;
+        const int32_t* table = kPaged ? a.tables + static_cast<int64_t>(b) * a.max_pages : nullptr;
+        const uint32_t page_bytes = kPaged ? static_cast<uint32_t>(a.kv_heads << a.shift) * kRowBytes : 0;
+        const int k_row = kPaged ? kRowBytes : static_cast<int>(a.k_stride * sizeof(T));
+        const int v_row = kPaged ? kRowBytes : static_cast<int>(a.v_stride * sizeof(T));
+        const char* k_base = static_cast<const char*>(a.k) +
+                             (kPaged ? static_cast<int64_t>(kh << a.shift) * kRowBytes
+                                     : static_cast<int64_t>(q.start) * k_row + kh * kRowBytes);
+        const char* v_base = static_cast<const char*>(a.v) +
+                             (kPaged ? static_cast<int64_t>(kh << a.shift) * kRowBytes
+                                     : static_cast<int64_t>(q.start) * v_row + kh * kRowBytes);
+        // The pages of a tile's keys, one a lane for the 16 keys from 16 (lane % kGroups) on.
+        constexpr int kGroups = KT / 16;
+        constexpr unsigned kAll = (1u << kGroups) - 1;
+        const auto lookup = [&](int t) {
+            if constexpr (kPaged)
+                return table[min((t * KT + 16 * (lane % kGroups)) >> a.shift, last_page)];
+            else
+                return 0;
+        };
+        const auto valid = [&](int id) { return !kPaged || static_cast<unsigned>(id) < static_cast<unsigned>(a.pages); };
+        const uint32_t k_mine[2] = {static_cast<uint32_t>((kPaged ? my_row % 16 : my_row) * k_row + k_piece(0)),
+                                    static_cast<uint32_t>((kPaged ? my_row % 16 : my_row) * k_row + k_piece(1))};
+        const uint32_t v_mine = (kPaged ? my_row % 16 : my_row) * v_row + v_piece;
+        const auto load = [&](int t, int ids) {
+            char* kl = sh.tile[t & 1][0] + wave * 1024;
+            char* vl = sh.tile[t & 1][1] + wave * 1024;
+            if constexpr (kPaged) {
+                const int pages = valid(ids) ? ids : 0;
 #pragma unroll
                 for (int u = 0; u < PER; ++u) {
-                    lds_load16(kp + u * kStep * k_row, k_mine[u % 2], kl + u * (kWaves * 1024));
-                    lds_load16(vp + u * kStep * v_row, v_mine, vl + u * (kWaves * 1024));
+                    const int group = u * kStep / 16 + (kStep > 16 ? wave / (kWaves / 2) : 0);
+                    const uint32_t id = __builtin_amdgcn_readlane(pages, group);
+                    const uint32_t at = ((t * KT + 16 * group) & in_page) + (kStep < 16 ? u * kStep % 16 : 0);
+                    const uint64_t offset = static_cast<uint64_t>(id) * page_bytes + at * kRowBytes;
+                    lds_load16(k_base + offset, k_mine[u % 2], kl + u * (kWaves * 1024));
+                    lds_load16(v_base + offset, v_mine, vl + u * (kWaves * 1024));
                 }
             } else {
+                const char* kp = k_base + static_cast<int64_t>(t * KT) * k_row;
+                const char* vp = v_base + static_cast<int64_t>(t * KT) * v_row;
+                const int left = q.length - 1 - t * KT;   // the last row there is
+                if (left >= KT - 1) {
+#pragma unroll
+                    for (int u = 0; u < PER; ++u) {
+                        lds_load16(kp + u * kStep * k_row, k_mine[u % 2], kl + u * (kWaves * 1024));
+                        lds_load16(vp + u * kStep * v_row, v_mine, vl + u * (kWaves * 1024));
+                    }
+                } else {
+#pragma unroll
+                    for (int u = 0; u < PER; ++u) {
+                        const int row = min(my_row + u * kStep, left);
+                        lds_load16(kp, row * k_row + k_piece(u), kl + u * (kWaves * 1024));
+                        lds_load16(vp, row * v_row + v_piece, vl + u * (kWaves * 1024));
+                    }
+                }
+            }
+        };
+        // Waits for the wave's pieces of the tile and meets the other waves.  `ask`
+        // (tiles that not every row sees whole): values that are not finite are
+        // taken out; true: there were some.
+        const auto arrive = [&](int t, bool ask) {
+            wait_loads();
+            if (ask) {
+                uint32_t odd = 0;
 #pragma unroll
                 for (int u = 0; u < PER; ++u) {
-                    const int row = min(my_row + u * kStep, left);
-                    lds_load16(kp, row * k_row + k_piece(u), kl + u * (kWaves * 1024));
-                    lds_load16(vp, row * v_row + v_piece, vl + u * (kWaves * 1024));
+                    u32x4* at = reinterpret_cast<u32x4*>(sh.tile[t & 1][1] + (u * kWaves + wave) * 1024 + lane * 16);
+                    const u32x4 v = *at;
+                    const uint32_t bits = (odd_bits<T>(v.x) | odd_bits<T>(v.y) | odd_bits<T>(v.z) | odd_bits<T>(v.w)) & kOddMask<T>;
+                    if (bits)
+                        *at = u32x4{finite_elements<T>(v.x), finite_elements<T>(v.y), finite_elements<T>(v.z), finite_elements<T>(v.w)};
+                    odd |= bits;
                 }
+                return __syncthreads_or(odd != 0) != 0;
             }
-        }
-    };
-    // Waits for the wave's pieces of the tile and meets the other waves.  `ask`
-    // (tiles that not every row sees whole): values that are not finite are
-    // taken out; true: there were some.
-    const auto arrive = [&](int t, bool ask) {
-        wait_loads();
-        if (ask) {
-            uint32_t odd = 0;
-#pragma unroll
-            for (int u = 0; u < PER; ++u) {
-                u32x4* at = reinterpret_cast<u32x4*>(sh.tile[t & 1][1] + (u * kWaves + wave) * 1024 + lane * 16);
-                const u32x4 v = *at;
-                const uint32_t bits = (odd_bits<T>(v.x) | odd_bits<T>(v.y) | odd_bits<T>(v.z) | odd_bits<T>(v.w)) & kOddMask<T>;
-                if (bits)
-                    *at = u32x4{finite_elements<T>(v.x), finite_elements<T>(v.y), finite_elements<T>(v.z), finite_elements<T>(v.w)};
-                odd |= bits;
-            }
-            return __syncthreads_or(odd != 0) != 0;
-        }
-        __syncthreads();
-        return false;
-    };
-
-    int ids = lookup(first), next = lookup(first + 1);   // of the tile that is computed, and of the next one
-    if (first < last) load(first, ids);
-
-    u32x4 qf[RT][NQ];
-    int limit_key[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const Row r = row_of(a, t0, rem0 + 32 * (RT * wave + rt) + lc);
-        const bool row_ok = r.t < q.todo;
-        limit_key[rt] = row_ok ? q.p0 + r.t : -1;
-        const T* qp = static_cast<const T*>(a.q) + static_cast<int64_t>(q.start + (row_ok ? r.t : 0)) * a.q_stride +
-                      (kh * g + r.head) * D;
-#pragma unroll
-        for (int s = 0; s < NQ; ++s) {
-            qf[rt][s] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(qp) + 32 * s + 16 * lh);
-            if (!row_ok) qf[rt][s] = u32x4{0, 0, 0, 0};
-        }
-    }
-    // Keys below wave_whole are seen by every row of the wave, from wave_seen on by none.
-    const int w0 = uniform(row_of(a, t0, rem0 + 32 * RT * wave).t), w1 = uniform(row_of(a, t0, rem0 + 32 * RT * (wave + 1) - 1).t);
-    const int wave_whole = w0 < q.todo ? min(max(q.p0 + w0 + 1, 0), q.length) : 0;
-    const int wave_seen = w0 < q.todo ? min(seen, max(q.p0 + min(w1, q.todo - 1) + 1, 0)) : 0;
-
-    f32x16 acc[RT][ND];
-    float m_run[RT], limit[RT], l_run[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-#pragma unroll
-        for (int db = 0; db < ND; ++db)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[rt][db][e] = 0.0f;
-        m_run[rt] = l_run[rt] = 0.0f;
-        limit[rt] = -INFINITY;
-    }
-
-    const auto compute = [&](int t, bool masked, unsigned bits) {
-        const char* kt = sh.tile[t & 1][0];
-        const char* vt = sh.tile[t & 1][1];
-        f32x16 st[RT][NK];
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int n = 0; n < NK; ++n)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) st[rt][n][e] = 0.0f;
-        // LDS reads run kAhead operands in front of their products: left to
-        // itself, the compiler waits for each before the next.
-        const auto key_piece = [&](int i) {   // of score tile i / NQ, 16-byte piece i % NQ
-            const int row = 32 * (i / NQ) + lc;
-            return *reinterpret_cast<const u32x4*>(kt + row * kRowBytes + 16 * ((2 * (i % NQ) + lh) ^ L::swap_k(row)));
+            __syncthreads();
+            return false;
         };
-        u32x4 kf[kAhead];
+
+        int ids = lookup(first), next = lookup(first + 1);   // of the tile that is computed, and of the next one
+        if (first < last) load(first, ids);
+
+        u32x4 qf[RT][NQ];
+        int limit_key[RT];
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) kf[i] = key_piece(i);
-        keep_order();
+        for (int rt = 0; rt < RT; ++rt) {
+            const Row r = row_of(a, t0, rem0 + 32 * (RT * wave + rt) + lc);
+            const bool row_ok = r.t < q.todo;
+            limit_key[rt] = row_ok ? q.p0 + r.t : -1;
+            const T* qp = static_cast<const T*>(a.q) + static_cast<int64_t>(q.start + (row_ok ? r.t : 0)) * a.q_stride +
+                          (kh * g + r.head) * D;
 #pragma unroll
-        for (int i = 0; i < NK * NQ; ++i) {
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                if constexpr (kWide) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        st[rt][i / NQ] = __builtin_amdgcn_mfma_f32_32x32x2f32(
-                            __uint_as_float(kf[i % kAhead][e]), __uint_as_float(qf[rt][i % NQ][e]), st[rt][i / NQ], 0, 0, 0);
-                } else {
-                    st[rt][i / NQ] = mfma32<T>(kf[i % kAhead], qf[rt][i % NQ], st[rt][i / NQ]);
-                }
+            for (int s = 0; s < NQ; ++s) {
+                qf[rt][s] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(qp) + 32 * s + 16 * lh);
+                if (!row_ok) qf[rt][s] = u32x4{0, 0, 0, 0};
             }
-            if (i + kAhead < NK * NQ) kf[i % kAhead] = key_piece(i + kAhead);
-            keep_order();
         }
-        if (masked) {
+        // Keys below wave_whole are seen by every row of the wave, from wave_seen on by none.
+        const int w0 = uniform(row_of(a, t0, rem0 + 32 * RT * wave).t), w1 = uniform(row_of(a, t0, rem0 + 32 * RT * (wave + 1) - 1).t);
+        const int wave_whole = w0 < q.todo ? min(max(q.p0 + w0 + 1, 0), q.length) : 0;
+        const int wave_seen = w0 < q.todo ? min(seen, max(q.p0 + min(w1, q.todo - 1) + 1, 0)) : 0;
+
+        f32x16 acc[RT][ND];
+        float m_run[RT], limit[RT], l_run[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+            for (int db = 0; db < ND; ++db)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[rt][db][e] = 0.0f;
+            m_run[rt] = l_run[rt] = 0.0f;
+            limit[rt] = -INFINITY;
+        }
+
+        const auto compute = [&](int t, bool masked, unsigned bits) {
+            const char* kt = sh.tile[t & 1][0];
+            const char* vt = sh.tile[t & 1][1];
+            f32x16 st[RT][NK];
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
                 for (int n = 0; n < NK; ++n)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int key = t * KT + 32 * n + 8 * (e / 4) + 4 * lh + e % 4;
-                        if (!(key <= limit_key[rt] && (bits >> (2 * n + e / 8) & 1))) st[rt][n][e] = -INFINITY;
-                    }
-        }
-        float mt[RT];
-        bool moves = false;
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            mt[rt] = -INFINITY;
-#pragma unroll
-            for (int n = 0; n < NK; ++n)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) mt[rt] = fmaxf(mt[rt], st[rt][n][e]);
-            moves |= mt[rt] > limit[rt];
-        }
-        if (__any(moves)) {
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                const float most = max_halves(mt[rt]);
-                if (most > -INFINITY) {
-                    const float m = limit[rt] == -INFINITY ? most : fmaxf(m_run[rt], most);
-                    const float fall = __builtin_amdgcn_exp2f((m_run[rt] - m) * a.c);
-                    if (limit[rt] > -INFINITY) {
-                        l_run[rt] *= fall;
-#pragma unroll
-                        for (int db = 0; db < ND; ++db)
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) acc[rt][db][e] *= fall;
-                    }
-                    m_run[rt] = m;
-                    limit[rt] = m + kHeadroom / a.c;
-                }
-            }
-        }
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            const float base = m_run[rt] * a.c;
-#pragma unroll
-            for (int n = 0; n < NK; ++n)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const float p = __builtin_amdgcn_exp2f(fmaf(st[rt][n][e], a.c, -base));
-                    st[rt][n][e] = p;
-                    l_run[rt] += p;
-                }
-        }
-        if constexpr (kWide) {
-#pragma unroll
-            for (int n = 0; n < NK; ++n)
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-#pragma unroll
-                    for (int db = 0; db < ND; ++db) {
-                        const int row = 32 * n + 8 * (e / 4) + 4 * lh + e % 4;
-                        const int c = 8 * db + lc / 4;
-                        const float x = *reinterpret_cast<const float*>(vt + row * kRowBytes + 16 * (c ^ L::swap_v(row)) + 4 * (lc & 3));
-#pragma unroll
-                        for (int rt = 0; rt < RT; ++rt)
-                            acc[rt][db] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, st[rt][n][e], acc[rt][db], 0, 0, 0);
-                    }
-        } else {
-            const int l16 = lane & 15;
-            const auto value_piece = [&](int i) {   // of 16 keys i / ND, dim tile i % ND
-                u32x4 x;
-#pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    // lane 4 k + x of 16 reads dims 4 x .. + 3 of key k
-                    const int row = 16 * (i / ND) + 8 * w + 4 * lh + l16 / 4;
-                    const int c = 4 * (i % ND) + 2 * (lane >> 4 & 1) + (l16 % 4) / 2;
-                    const char* at = vt + row * kRowBytes + 16 * (c ^ L::swap_v(row)) + 8 * (l16 & 1);
-                    const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                                                  (__attribute__((address_space(3))) s16x4*)(at)));
-                    x[2 * w] = y.x;
-                    x[2 * w + 1] = y.y;
-                }
-                return x;
+                    for (int e = 0; e < 16; ++e) st[rt][n][e] = 0.0f;
+            // LDS reads run kAhead operands in front of their products: left to
+            // itself, the compiler waits for each before the next.
+            const auto key_piece = [&](int i) {   // of score tile i / NQ, 16-byte piece i % NQ
+                const int row = 32 * (i / NQ) + lc;
+                return *reinterpret_cast<const u32x4*>(kt + row * kRowBytes + 16 * ((2 * (i % NQ) + lh) ^ L::swap_k(row)));
             };
-            u32x4 vf[kAhead], pf[RT];
+            u32x4 kf[kAhead];
 #pragma unroll
-            for (int i = 0; i < kAhead; ++i) vf[i] = value_piece(i);
+            for (int i = 0; i < kAhead; ++i) kf[i] = key_piece(i);
             keep_order();
 #pragma unroll
-            for (int i = 0; i < 2 * NK * ND; ++i) {
+            for (int i = 0; i < NK * NQ; ++i) {
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
-                    if (i % ND == 0) {
-                        float p[8];
+                    if constexpr (kWide) {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) p[e] = st[rt][i / ND / 2][i / ND % 2 * 8 + e];
-                        pf[rt] = pack8<T>(p);
+                        for (int e = 0; e < 4; ++e)
+                            st[rt][i / NQ] = __builtin_amdgcn_mfma_f32_32x32x2f32(
+                                __uint_as_float(kf[i % kAhead][e]), __uint_as_float(qf[rt][i % NQ][e]), st[rt][i / NQ], 0, 0, 0);
+                    } else {
+                        st[rt][i / NQ] = mfma32<T>(kf[i % kAhead], qf[rt][i % NQ], st[rt][i / NQ]);
                     }
-                    acc[rt][i % ND] = mfma32<T>(vf[i % kAhead], pf[rt], acc[rt][i % ND]);
                 }
-                if (i + kAhead < 2 * NK * ND) vf[i % kAhead] = value_piece(i + kAhead);
+                if (i + kAhead < NK * NQ) kf[i % kAhead] = key_piece(i + kAhead);
                 keep_order();
             }
-        }
-    };
-    // The values of a tile that are not finite, to the rows that see them,
-    // whatever their weight: 0 times them would not be 0.
-    const auto add_odd = [&](int t, unsigned bits) {
-        for (int j = 0; j < KT; ++j) {
-            if (!(bits >> (j / 16) & 1)) continue;
-            const int key = min(t * KT + j, q.length - 1);
-            const char* row = v_base;
-            if constexpr (kPaged)
-                row += static_cast<uint64_t>(static_cast<uint32_t>(table[key >> a.shift])) * page_bytes + (key & in_page) * kRowBytes;
-            else
-                row += static_cast<int64_t>(key) * v_row;
-            const T* vp = reinterpret_cast<const T*>(row) + 4 * lh;
+            if (masked) {
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                    for (int n = 0; n < NK; ++n)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const int key = t * KT + 32 * n + 8 * (e / 4) + 4 * lh + e % 4;
+                            if (!(key <= limit_key[rt] && (bits >> (2 * n + e / 8) & 1))) st[rt][n][e] = -INFINITY;
+                        }
+            }
+            float mt[RT];
+            bool moves = false;
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                if (t * KT + j > limit_key[rt]) continue;
+                mt[rt] = -INFINITY;
 #pragma unroll
-                for (int db = 0; db < ND; ++db)
+                for (int n = 0; n < NK; ++n)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) mt[rt] = fmaxf(mt[rt], st[rt][n][e]);
+                moves |= mt[rt] > limit[rt];
+            }
+            if (__any(moves)) {
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    const float most = max_halves(mt[rt]);
+                    if (most > -INFINITY) {
+                        const float m = limit[rt] == -INFINITY ? most : fmaxf(m_run[rt], most);
+                        const float fall = __builtin_amdgcn_exp2f((m_run[rt] - m) * a.c);
+                        if (limit[rt] > -INFINITY) {
+                            l_run[rt] *= fall;
+#pragma unroll
+                            for (int db = 0; db < ND; ++db)
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) acc[rt][db][e] *= fall;
+                        }
+                        m_run[rt] = m;
+                        limit[rt] = m + kHeadroom / a.c;
+                    }
+                }
+            }
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                const float base = m_run[rt] * a.c;
+#pragma unroll
+                for (int n = 0; n < NK; ++n)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        const float x = widen(vp[32 * db + 8 * (e / 4) + e % 4]);
-                        if (!(fabsf(x) < INFINITY)) acc[rt][db][e] += x;
+                        const float p = __builtin_amdgcn_exp2f(fmaf(st[rt][n][e], a.c, -base));
+                        st[rt][n][e] = p;
+                        l_run[rt] += p;
                     }
             }
-        }
-    };
-
-    for (int t = first; t < last; ++t) {
-        const unsigned bits = __ballot(valid(ids)) & kAll;   // keys 16 u .. + 15 have a page
-        const bool odd = arrive(t, (t + 1) * KT > whole || bits != kAll);
-        // (the other buffer's tile is behind all waves)
-        if (t + 1 < last) load(t + 1, next);
-        ids = next;
-        next = lookup(t + 2);
-        if (t * KT >= wave_seen) continue;
-        if (odd) add_odd(t, bits);
-        compute(t, (t + 1) * KT > wave_whole || bits != kAll, bits);
-    }
-
-    const auto part = [&](int s) {   // the first group's part is its second one
-        return (static_cast<int64_t>(first_group + s) * 2 + (s == 0)) * part_bytes(kRows, D);
-    };
-    const auto place = [&](int i) {   // i = 4 (ND rt + db) + u
-        return RowDim{32 * (RT * wave + i / (4 * ND)) + lc, 8 * (i % (4 * ND)) + 4 * lh};
-    };
-    char* out_part = a.parts + (active > 1 ? part(id - first_group) : 0);
-    const __amdgpu_buffer_rsrc_t prs = buffer_rsrc(out_part, part_bytes(kRows, D));
+            if constexpr (kWide) {
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const float l = sum_halves(l_run[rt]);
-        const int row = 32 * (RT * wave + rt) + lc;
+                for (int n = 0; n < NK; ++n)
 #pragma unroll
-        for (int db = 0; db < ND; ++db)
+                    for (int e = 0; e < 16; ++e)
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const float y[4] = {acc[rt][db][4 * u], acc[rt][db][4 * u + 1], acc[rt][db][4 * u + 2], acc[rt][db][4 * u + 3]};
-                const int i = 4 * (ND * rt + db) + u;
-                if (active == 1)
-                    put<T>(a, q, kh, row_of(a, t0, rem0 + row), place(i).dim, y, l, D);
-                else
-                    coherent_store16(prs, (i * kThreads + static_cast<int>(threadIdx.x)) * 16,
-                                     u32x4{__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3])});
+                        for (int db = 0; db < ND; ++db) {
+                            const int row = 32 * n + 8 * (e / 4) + 4 * lh + e % 4;
+                            const int c = 8 * db + lc / 4;
+                            const float x = *reinterpret_cast<const float*>(vt + row * kRowBytes + 16 * (c ^ L::swap_v(row)) + 4 * (lc & 3));
+#pragma unroll
+                            for (int rt = 0; rt < RT; ++rt)
+                                acc[rt][db] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, st[rt][n][e], acc[rt][db], 0, 0, 0);
+                        }
+            } else {
+                const int l16 = lane & 15;
+                const auto value_piece = [&](int i) {   // of 16 keys i / ND, dim tile i % ND
+                    u32x4 x;
+#pragma unroll
+                    for (int w = 0; w < 2; ++w) {
+                        // lane 4 k + x of 16 reads dims 4 x .. + 3 of key k
+                        const int row = 16 * (i / ND) + 8 * w + 4 * lh + l16 / 4;
+                        const int c = 4 * (i % ND) + 2 * (lane >> 4 & 1) + (l16 % 4) / 2;
+                        const char* at = vt + row * kRowBytes + 16 * (c ^ L::swap_v(row)) + 8 * (l16 & 1);
+                        const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                                      (__attribute__((address_space(3))) s16x4*)(at)));
+                        x[2 * w] = y.x;
+                        x[2 * w + 1] = y.y;
+                    }
+                    return x;
+                };
+                u32x4 vf[kAhead], pf[RT];
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) vf[i] = value_piece(i);
+                keep_order();
+#pragma unroll
+                for (int i = 0; i < 2 * NK * ND; ++i) {
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) {
+                        if (i % ND == 0) {
+                            float p[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) p[e] = st[rt][i / ND / 2][i / ND % 2 * 8 + e];
+                            pf[rt] = pack8<T>(p);
+                        }
+                        acc[rt][i % ND] = mfma32<T>(vf[i % kAhead], pf[rt], acc[rt][i % ND]);
+                    }
+                    if (i + kAhead < 2 * NK * ND) vf[i % kAhead] = value_piece(i + kAhead);
+                    keep_order();
+                }
             }
-        if (active > 1 && lh == 0) {
-            float* ml = reinterpret_cast<float*>(out_part) + kRows * D;
-            coherent_store(ml + row, limit[rt] == -INFINITY ? -INFINITY : m_run[rt] * a.c);
-            coherent_store(ml + kRows + row, l);
+        };
+        // The values of a tile that are not finite, to the rows that see them,
+        // whatever their weight: 0 times them would not be 0.
+        const auto add_odd = [&](int t, unsigned bits) {
+            for (int j = 0; j < KT; ++j) {
+                if (!(bits >> (j / 16) & 1)) continue;
+                const int key = min(t * KT + j, q.length - 1);
+                const char* row = v_base;
+                if constexpr (kPaged)
+                    row += static_cast<uint64_t>(static_cast<uint32_t>(table[key >> a.shift])) * page_bytes + (key & in_page) * kRowBytes;
+                else
+                    row += static_cast<int64_t>(key) * v_row;
+                const T* vp = reinterpret_cast<const T*>(row) + 4 * lh;
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    if (t * KT + j > limit_key[rt]) continue;
+#pragma unroll
+                    for (int db = 0; db < ND; ++db)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const float x = widen(vp[32 * db + 8 * (e / 4) + e % 4]);
+                            if (!(fabsf(x) < INFINITY)) acc[rt][db][e] += x;
+                        }
+                }
+            }
+        };
+
+        for (int t = first; t < last; ++t) {
+            const unsigned bits = __ballot(valid(ids)) & kAll;   // keys 16 u .. + 15 have a page
+            const bool odd = arrive(t, (t + 1) * KT > whole || bits != kAll);
+            // (the other buffer's tile is behind all waves)
+            if (t + 1 < last) load(t + 1, next);
+            ids = next;
+            next = lookup(t + 2);
+            if (t * KT >= wave_seen) continue;
+            if (odd) add_odd(t, bits);
+            compute(t, (t + 1) * KT > wave_whole || bits != kAll, bits);
         }
-    }
-    __syncthreads();   // (LDS is free)
-    if (active > 1 && last_arrival(a.tickets + first_group * kTicketStride, active, &sh.ticket)) {
-        float* f = reinterpret_cast<float*>(sh.tile[0][0]);
-        static_assert((kManySplits + 1) * kRows * 4 <= static_cast<int>(sizeof sh.tile), "factors fit");
-        join_parts<T, D, kRows>(a, q, kh, t0, rem0, active, a.parts, part, place, f, f + kManySplits * kRows);
-        __syncthreads();
-    }
+
+        const auto part = [&](int s) {   // the first group's part is its second one
+            return (static_cast<int64_t>(first_group + s) * 2 + (s == 0)) * part_bytes(kRows, D);
+        };
+        const auto place = [&](int i) {   // i = 4 (ND rt + db) + u
+            return RowDim{32 * (RT * wave + i / (4 * ND)) + lc, 8 * (i % (4 * ND)) + 4 * lh};
+        };
+        char* out_part = a.parts + (active > 1 ? part(id - first_group) : 0);
+        const __amdgpu_buffer_rsrc_t prs = buffer_rsrc(out_part, part_bytes(kRows, D));
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const float l = sum_halves(l_run[rt]);
+            const int row = 32 * (RT * wave + rt) + lc;
+#pragma unroll
+            for (int db = 0; db < ND; ++db)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const float y[4] = {acc[rt][db][4 * u], acc[rt][db][4 * u + 1], acc[rt][db][4 * u + 2], acc[rt][db][4 * u + 3]};
+                    const int i = 4 * (ND * rt + db) + u;
+                    if (active == 1)
+                        put<T>(a, q, kh, row_of(a, t0, rem0 + row), place(i).dim, y, l, D);
+                    else
+                        coherent_store16(prs, (i * kThreads + static_cast<int>(threadIdx.x)) * 16,
+                                         u32x4{__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3])});
+                }
+            if (active > 1 && lh == 0) {
+                float* ml = reinterpret_cast<float*>(out_part) + kRows * D;
+                coherent_store(ml + row, limit[rt] == -INFINITY ? -INFINITY : m_run[rt] * a.c);
+                coherent_store(ml + kRows + row, l);
+            }
+        }
+        __syncthreads();   // (LDS is free)
+        if (active > 1 && last_arrival(a.tickets + first_group * kTicketStride, active, &sh.ticket)) {
+            float* f = reinterpret_cast<float*>(sh.tile[0][0]);
+            static_assert((kManySplits + 1) * kRows * 4 <= static_cast<int>(sizeof sh.tile), "factors fit");
+            join_parts<T, D, kRows>(a, q, kh, t0, rem0, active, a.parts, part, place, f, f + kManySplits * kRows);
+            __syncthreads();
+        }
     }
 }
 
@@ -1233,6 +1242,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_many_kernel(const Args 
     __shared__ __align__(16) ManyShared<T, D> sh;
     many_rows<T, D, RT, kPaged>(a, blockIdx.x, sh);
 }
+
 // ---- Host
 
 struct Plan {
@@ -1240,7 +1250,7 @@ struct Plan {
     int few_tiles;        // RT of attention_few_kernel
     int few_rows;         // query rows up to which a request is its
     int many_tiles;       // RT of attention_many_kernel
-    bool shared;          // whether row tiles may have several workgroups
+    bool shared;          // whether a request's keys may go to several workgroups
     int64_t many_groups;
     int64_t bytes;        // of the parts; the kernels run one after the other
 };
@@ -1258,14 +1268,16 @@ Plan plan(int64_t batch, int64_t rows, int64_t max_rows, int64_t heads, int64_t 
     p.few = paged && g <= p.few_rows && (batch > 1 || most <= p.few_rows);
     if (!p.few) p.few_rows = 0;
     p.many = most > p.few_rows;
-    if (p.few) p.bytes = 2 * kTargetGroups * part_bytes(32, d);
+    p.shared = max_tokens > kRound;
+    if (p.few && p.shared) p.bytes = 2 * kTargetGroups * part_bytes(32, d);
     if (p.many) {
         // Two row tiles a wave read a key tile's operands once for both, where
-        // registers allow and enough tiles are left for the workgroups.
-        p.many_tiles = d == 64 && !wide && rows * g / 256 * kv_heads >= kTargetGroups ? 2 : 1;
+        // registers allow, enough tiles are left for the workgroups and the tile's
+        // tokens are few (f16, 64 heads of 64 on 8, 6500 rows: 380 us against 414; 32
+        // on 4, 3000 rows: 75 against 55; 32 on 32, 6000 rows: 227 against 195).
+        p.many_tiles = d == 64 && !wide && g >= 4 && rows * g / 256 * kv_heads >= kTargetGroups ? 2 : 1;
         const int64_t tile = 32 * p.many_tiles * kWaves;
         const int64_t units = (rows * g / tile + batch) * kv_heads;   // at most
-        p.shared = max_tokens > 64;
         p.many_groups = p.shared ? std::max<int64_t>(units, kTargetGroups) : units;
         if (p.shared) p.bytes = 2 * kTargetGroups * part_bytes(d == 64 ? 256 : 128, d);
     }
