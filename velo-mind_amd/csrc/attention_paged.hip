@@ -794,7 +794,7 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
     constexpr int kRowBytes = D * sizeof(T);
     constexpr int kLeastTiles = kWide ? 2 : 4;   // key tiles that are worth a workgroup
     constexpr int kAhead = 4;                    // LDS operands in front of their products
-    constexpr int kJoin = kWide ? 3 : D == 64 ? 28 : 16;   // key tiles' time that parts take
+    constexpr int kJoin = kWide ? 6 : D == 64 ? 28 : 16;   // key tiles' time that parts take
     constexpr int kStart = kWide ? 1 : 2;        // key tiles' time that a row tile takes beside its keys
 
     const int lane = threadIdx.x & 63;
@@ -810,11 +810,13 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
     const int tiles_all = sum_up(a.batch, sh.requests, [&](int b) { return tiles_of(request<kPaged>(a, b)); }, &longest);
     if (tiles_all == 0) return;
     // A row tile's keys go to one workgroup, or all tiles' keys are dealt out
-    // evenly (as attention_few_kernel's are): where the longest tile (of a causal
-    // prompt: twice the mean) would be waited for longer than the parts take to
-    // store and join (25 us for 512 workgroups' 16-bit tiles, about kJoin key
-    // tiles' time).  32 heads of 64 on 4, f16, 3000 rows: 55 us against 79 dealt
-    // out; 500 rows behind 30000: 340 against 700.
+    // evenly (as attention_few_kernel's are), where the first would take longer
+    // than dealing out and the storing and joining of the parts (kJoin; 512
+    // workgroups' 16-bit parts take 25 us).  Times in key tiles of a compute unit:
+    // up to 256 tiles have one each, up to 512 share one by twos (below), more
+    // follow as others end (of tiles of equal length the last alone).  32 heads of 64
+    // on 4, f16, 3000 rows: 55 us against 79 dealt out; 40 rows of 64 heads of 128 on
+    // 8 behind 2000: 57 against 40, behind 1000: 36.5 against 39.5.
     const int units = tiles_all * a.kv_heads;
     bool shared = a.shared && tiles_all <= kMaxShared && units <= kShareUnits;
     int of_head = 0;
@@ -827,9 +829,10 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
             return kStart + max((seen + KT - 1) / KT, 1);
         }, &longest);
         const int each = of_head * a.kv_heads / kTargetGroups;
-        // the last workgroups to start: none, or, of tiles of equal length, whole ones
-        const int alone = units <= kTargetGroups ? longest : each + max(2 * (of_head / tiles_all) - longest, 0);
-        shared = longest > kStart + kLeastTiles && alone > max(each, kStart + kLeastTiles) + kJoin;
+        const int alone = units <= kTargetGroups / 2 ? longest
+                          : units <= kTargetGroups   ? max(longest, 2 * each)
+                                                     : 2 * each + max(2 * (of_head / tiles_all) - longest, 0);
+        shared = longest > kStart + kLeastTiles && alone > 2 * max(each, kStart + kLeastTiles) + kJoin;
     }
     int pos = id, end = id + 1, share = 1;   // of the units (KV head, row tile), or of their key tiles
     if (shared) {
@@ -844,6 +847,39 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
     } else {
         end = min(end, tiles_all * a.kv_heads);
     }
+
+    // The tile with `rank` tiles in front of it that see more keys (of up to 64
+    // requests, one a lane): tile t of a request sees about as many as tile t +
+    // p0 group / kRows of a request without tokens in front.
+    const auto by_length = [&](int rank) {
+        const bool real = lane < a.batch;
+        const Request q = request<kPaged>(a, real ? lane : 0);
+        const int mine = real ? tiles_of(q) : 0;
+        const int ahead = static_cast<int>(static_cast<int64_t>(max(q.p0, 0)) * g / kRows);
+        const int before = sh.requests.upto[real ? lane : 0] - mine;
+        const auto from = [&](int level) {   // tiles of all requests from this level on
+            int n = min(max(mine + ahead - level, 0), mine);
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) n += __shfl_xor(n, o, 64);
+            return uniform(n);
+        };
+        int lo = 0, hi = mine + ahead;       // from(lo) > rank >= from(hi)
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) hi = max(hi, __shfl_xor(hi, o, 64));
+        hi = uniform(hi);
+        while (hi - lo > 1) {
+            const int mid = lo + (hi - lo) / 2;
+            if (from(mid) > rank)
+                lo = mid;
+            else
+                hi = mid;
+        }
+        // the n-th of the requests that have a tile of this level
+        uint64_t has = __ballot(lo >= ahead && lo < ahead + mine);
+        for (int n = rank - from(lo + 1); n > 0; --n) has &= has - 1;
+        const int b = has ? __builtin_ctzll(has) : 0;
+        return __builtin_amdgcn_readlane(before + lo - ahead, b);
+    };
 
     while (pos < end) {
         int kh, slot, first = 0, last = 0x7fffffff, active = 1, first_group = 0;
@@ -860,19 +896,25 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
             if (last <= first) continue;
         } else {
             // Workgroups go to the XCDs in turn, eight at a time: a KV head's tiles
-            // stay on one where the count of those allows, the last tiles, which see
-            // the most keys, first.  Of the 512 that start at once a compute unit has
-            // the n-th and the 256 + n-th: the second half goes backwards.
+            // stay on one where the count of those allows, those that see the most
+            // keys first.  Of the 512 that start at once a compute unit has the n-th
+            // and the 256 + n-th: the second half goes backwards.
             int at = pos / 8;
             const int half = kTargetGroups / 16, both = min(kTargetGroups, tiles_all * a.kv_heads) / 8;
             if (at >= half && at < both) at = half + both - 1 - at;
             if (a.kv_heads % 8 == 0) {
-                slot = tiles_all - 1 - at % tiles_all;
+                slot = at % tiles_all;
                 kh = at / tiles_all * 8 + pos % 8;
             } else {
-                slot = tiles_all - 1 - (8 * at + pos % 8) / a.kv_heads;
+                slot = (8 * at + pos % 8) / a.kv_heads;
                 kh = (8 * at + pos % 8) % a.kv_heads;
             }
+            // Of several requests, by length where that balances compute units (4 of
+            // 4000 rows in all, 32 heads of 128 on 8, bf16: 64.6 us against 69.7);
+            // of more tiles, a request's together for the caches' sake (3 of 12000
+            // rows: 964 against 992).
+            const bool sorted = a.batch > 1 && a.batch <= 64 && units > kTargetGroups / 2 && units <= 2 * kTargetGroups;
+            slot = sorted ? by_length(uniform(slot)) : tiles_all - 1 - slot;
             pos = end;
         }
         kh = uniform(kh);
@@ -1103,19 +1145,25 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
                     }
             }
             if constexpr (kWide) {
+                const auto value = [&](int i) {   // of score element i / ND, dim tile i % ND
+                    const int e = i / ND;
+                    const int row = 8 * (e / 4) + 4 * lh + e % 4;
+                    const int c = 8 * (i % ND) + lc / 4;
+                    return *reinterpret_cast<const float*>(vt + row * kRowBytes + 16 * (c ^ L::swap_v(row)) + 4 * (lc & 3));
+                };
+                float x[2 * kAhead];
 #pragma unroll
-                for (int n = 0; n < NK; ++n)
+                for (int i = 0; i < 2 * kAhead; ++i) x[i] = value(i);
+                keep_order();
 #pragma unroll
-                    for (int e = 0; e < 16; ++e)
+                for (int i = 0; i < 16 * NK * ND; ++i) {
 #pragma unroll
-                        for (int db = 0; db < ND; ++db) {
-                            const int row = 32 * n + 8 * (e / 4) + 4 * lh + e % 4;
-                            const int c = 8 * db + lc / 4;
-                            const float x = *reinterpret_cast<const float*>(vt + row * kRowBytes + 16 * (c ^ L::swap_v(row)) + 4 * (lc & 3));
-#pragma unroll
-                            for (int rt = 0; rt < RT; ++rt)
-                                acc[rt][db] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, st[rt][n][e], acc[rt][db], 0, 0, 0);
-                        }
+                    for (int rt = 0; rt < RT; ++rt)
+                        acc[rt][i % ND] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[i % (2 * kAhead)], st[rt][i / ND / 16][i / ND % 16],
+                                                                               acc[rt][i % ND], 0, 0, 0);
+                    if (i + 2 * kAhead < 16 * NK * ND) x[i % (2 * kAhead)] = value(i + 2 * kAhead);
+                    if (i % 2) keep_order();
+                }
             } else {
                 const int l16 = lane & 15;
                 const auto value_piece = [&](int i) {   // of 16 keys i / ND, dim tile i % ND
