@@ -917,7 +917,8 @@ int vm_hip_logits_rules_apply(const vm_hip_logits_rules* rules, const void* logi
  * so that a captured step replays with others; indices that point outside
  * (a page id, a slot, a position) are never followed: their rows and keys
  * count as not there.  At most VM_HIP_PAGED_MAX_BATCH requests and
- * VM_HIP_PAGED_MAX_ROWS rows a call. */
+ * VM_HIP_PAGED_MAX_ROWS rows a call.  kv_heads is at most 4096, heads a multiple
+ * of it, at most 65536. */
 #define VM_HIP_PAGED_MAX_BATCH 2048
 #define VM_HIP_PAGED_MAX_ROWS  (1 << 24)
 
@@ -979,7 +980,8 @@ int vm_hip_kv_paged_release(int64_t batch, int64_t max_pages, int64_t pages, int
  * Tables of the cosines and sines of positions first .. first + rows - 1 for
  * `dim` rotated elements (even, 2 to 128): cos_table, sin_table [rows, dim / 2]
  * fp32, entry i of position p = cos(p f_i) and sin(p f_i), times the attention
- * factor, computed in fp64 (off by at most half a step of fp32 and 2^-40).
+ * factor, computed in fp64 (off by at most half a step of fp32, 2^-40, and what
+ * 64 bits leave of the angle, 2^-50 of it).
  * f_i = theta^(-2 i / dim), theta > 1, scaled for contexts longer than the
  * trained one (`original` positions):
  *   PLAIN   not (scaling may be NULL)
@@ -1031,8 +1033,8 @@ typedef struct vm_hip_qk_norm {
  * (rope, or NULL) at positions[row], in fp32, rounded once; queries go to
  * q_out [rows, heads * head_dim], keys and values to the cache's slots[row].
  * A row with a negative position or a slot outside the cache is padding: nothing
- * of it is written.  Slots that are given twice get one of the rows.  q_out must
- * not overlap qkv; both are 16-byte aligned. */
+ * of it is written.  A slot that is given twice gets parts of either row.  q_out
+ * must not overlap qkv; both are 16-byte aligned. */
 int vm_hip_kv_paged_append(const vm_hip_kv_paged* cache, const void* qkv, int64_t rows, int64_t heads,
                            const vm_hip_qk_norm* norm, const vm_hip_rope* rope, const int32_t* positions,
                            const int32_t* slots, void* q_out, void* stream);
@@ -1059,10 +1061,14 @@ int vm_hip_qk_norm_rope(const void* qkv, int dtype, int64_t rows, int64_t heads,
  * row does not see takes no part in it, whatever it holds; a value that is not
  * finite makes the element not finite in every row that sees it.
  *
- * workspace: vm_hip_attention_packed_workspace_bytes bytes (0 is possible: then
- * it may be NULL), 16-byte aligned and zeroed before its first use; every call
- * leaves it ready for the next one of any shape it is large enough for.  Calls
- * that share a workspace must not overlap. */
+ * Limits: heads / kv_heads <= 4096, rows * heads < 2^30, and at most 2^24 tiles of
+ * 128 query rows; a call past them is refused.  out overlaps no input.
+ *
+ * workspace: vm_hip_attention_packed_workspace_bytes bytes (0 without rows,
+ * else 32 KiB and, past 128 rows, up to 66 MiB, however many the rows are), 16-byte
+ * aligned and zeroed before its first use; every call leaves it ready for the
+ * next one of any shape it is large enough for.  Calls that share a workspace
+ * must not overlap. */
 int64_t vm_hip_attention_packed_workspace_bytes(int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads,
                                                 int64_t head_dim);
 int vm_hip_attention_packed(const void* q, const void* k, const void* v, void* out, int dtype, int64_t q_stride,
@@ -1083,8 +1089,8 @@ int vm_hip_attention_packed(const void* q, const void* k, const void* v, void* o
  * max_pages * page_size <= 2^24, and times batch * kv_heads below 2^38.
  * row_start and lengths are held to [0, rows] and [0, max_pages * page_size];
  * tokens in table entries that are no page do not exist; a row that sees none
- * gets zeros.  Roundings, scores, infinities, scale and the workspace are those
- * of vm_hip_attention_packed; the workspace is that of the largest rows and
+ * gets zeros.  Roundings, scores, infinities, scale, limits and the workspace are
+ * those of vm_hip_attention_packed; the workspace is that of the largest rows and
  * max_rows it is used with. */
 int64_t vm_hip_attention_paged_workspace_bytes(int64_t batch, int64_t rows, int64_t max_rows, int64_t heads,
                                                int64_t kv_heads, int64_t head_dim, int64_t max_tokens);

@@ -383,6 +383,15 @@ __device__ __forceinline__ int first_above(const Sums<kMost>& s, int count, int 
 //   O^T  16 bits: row i of tile db is dim (D / 16) i + db: a lane reads D / 16
 //        adjacent elements of each of its eight keys and transposes them with
 //        byte permutes; fp32: tile 4 h + u has dim 64 h + 4 i + u: nothing moves
+// K and V are read once and only used by one wave, so they skip LDS; a block's
+// loads are requested a block ahead.
+//
+// MI355X, passes back to back: one token each of 32 requests over 1 to 8000
+// tokens, 64 heads of 128 on 8, bf16: 151 us, 5.2 TB/s of K and V (a copy: 5.35),
+// bound by HBM; 16 requests of 4 tokens over 6000: 67.6 us (of 2: 57); one request
+// over 100000: 89 us, 4.6 TB/s, over 8000: 17 us.  One fp32 token of 32 heads of 64
+// on 4 over 2000: 9.2 us: the launch and a chain of trips (lengths, table, keys,
+// ticket, parts) of about a microsecond each.
 template <int D, int RT>
 struct FewShared {
     float merge_o[kWaves][16 * RT * D];
@@ -421,7 +430,7 @@ __device__ __forceinline__ void few_rows(const Args& a, int id, FewShared<D, RT>
     const int per = max(max((total + kTargetGroups - 1) / kTargetGroups, kWide ? 1 : 2),
                         (longest + kMaxSplits - 2) / (kMaxSplits - 1));
     int pos = id * per;
-    const int end = min(total, pos + per);
+    const int end = total - pos > per ? pos + per : total;   // (pos + per may pass 31 bits)
 
     while (pos < end) {
         // The request, KV head and rounds that this share goes on with.
@@ -750,7 +759,7 @@ __device__ __forceinline__ void few_rows(const Args& a, int id, FewShared<D, RT>
 // positions if V^T's operand has the same keys there, which two transposing LDS
 // reads of four keys give (16 bits), or plain reads (fp32).
 //
-// MI355X, passes back to back: 3 prompts of 12000 tokens, 64 heads of 128 on 8,
+// MI355X, passes back to back: 3 prompts, 12000 tokens in all, 64 heads of 128 on 8,
 // bf16: 963 us, 948 TFLOP/s (a large product: 1150); one of 6500, 64 heads of 64
 // on 8, f16: 380 us, 910 TFLOP/s; 500 tokens behind 30000, 32 heads of 128 on 8,
 // f16: 292 us, 850 TFLOP/s; one fp32 prompt of 2000, 64 heads of 128: 536 us, 122
@@ -912,7 +921,7 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
             // Of several requests, by length where that balances compute units (4 of
             // 4000 rows in all, 32 heads of 128 on 8, bf16: 64.6 us against 69.7);
             // of more tiles, a request's together for the caches' sake (3 of 12000
-            // rows: 964 against 992).
+            // in all: 964 against 992).
             const bool sorted = a.batch > 1 && a.batch <= 64 && units > kTargetGroups / 2 && units <= 2 * kTargetGroups;
             slot = sorted ? by_length(uniform(slot)) : tiles_all - 1 - slot;
             pos = end;
