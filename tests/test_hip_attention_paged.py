@@ -209,6 +209,22 @@ def test_long_contexts(hip, dtype, heads, hk, d, n, length):
 
 
 @TYPES
+@pytest.mark.parametrize("heads,hk,d", [(32, 8, 128), (32, 8, 64), (40, 5, 64)], ids=str)
+@pytest.mark.parametrize("known", [True, False], ids=["most rows known", "unknown"])
+@pytest.mark.parametrize("n,lengths", [([60, 1, 1, 3], [2060, 1500, 300, 40]), ([1, 10, 1], [1900, 1510, 1]),
+                                       ([1, 1, 33, 20], [700, 2600, 633, 2500])], ids=str)
+def test_chunks_beside_decoded_tokens(hip, dtype, heads, hk, d, known, n, lengths):
+    """Row tiles of which some waves have no rows, alone and joined from two to
+    many workgroups' parts."""
+    c = Paged(hip, dtype, n, lengths, heads, hk, d, 16, 31, max_rows=None if known else 0, pad=2).upload()
+    c.call()
+    c.check()
+    first = c.result()
+    c.call()
+    assert np.array_equal(first, c.result())
+
+
+@TYPES
 def test_one_workspace_for_many_shapes(hip, dtype):
     shapes = [([1] * 40, [700 + 13 * i for i in range(40)]), ([200, 1], [3000, 5000]), ([1], [9000]),
               ([3, 3, 3], [2000, 2500, 100]), ([90], [4000]), ([1, 2], [6000, 10])]

@@ -13,7 +13,7 @@
 // are the weights that the second product wants from it.
 //
 // Two kernels.  attention_few_kernel takes requests of at most 16 RT query
-// rows (decoded tokens): K and V straight from memory to operand registers, a
+// rows (decoded tokens, where plan() does not leave them to the other): K and V straight from memory to operand registers, a
 // wave its own blocks of keys, and the keys of all requests dealt out evenly
 // over the workgroups.  attention_many_kernel takes the others: 32 RT rows a
 // wave, key tiles in LDS for all four waves.  16-bit rows use the 16-bit matrix
@@ -229,27 +229,30 @@ struct RowDim {
 // Parts of a tile's keys in the workspace: four outputs for each thread in turn
 // (place(i): the row and first dim of the i-th), then references (log2) and sums
 // of the rows; the workgroup that draws the last ticket joins them.  part(s):
-// byte offset of workgroup s's; factors: LDS for active x kRows floats, totals
-// for kRows.
-template <typename T, int D, int kRows, typename Part, typename Place>
-__device__ __forceinline__ void join_parts(const Args& a, const Request& q, int kh, int t0, int r0, int active,
-                                           const char* parts, Part part, Place place, float* factors, float* totals) {
-    // Two items of a thread and eight parts at a time, 16 loads in flight; the
-    // first are requested before the factors' inputs.
+// byte offset of workgroup s's; rows: how many the parts hold, mine: whether
+// this wave's threads have any; factors: LDS for active x kRows floats, totals for
+// kRows.
+// kParts parts at a time and as many of a thread's items as make 16 loads in
+// flight; the first are requested before the factors' inputs.
+template <typename T, int D, int kRows, int kParts, typename Part, typename Place>
+__device__ __forceinline__ void join_by(const Args& a, const Request& q, int kh, int t0, int r0, int active, int rows,
+                                        bool mine, const char* parts, Part part, Place place, float* factors,
+                                        float* totals) {
     constexpr int kItems = kRows * D / 4 / kThreads;
-    constexpr int kTake = kItems < 2 ? kItems : 2;
-    u32x4 x[kTake][8];
+    constexpr int kTake = kItems < 16 / kParts ? kItems : 16 / kParts;
+    static_assert(kItems % kTake == 0, "items are taken evenly");
+    u32x4 x[kTake][kParts];
     const auto request_parts = [&](int i0, int s0) {
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
+        for (int u = 0; u < kParts; ++u) {
             if (s0 + u >= active) break;
             const __amdgpu_buffer_rsrc_t rs = buffer_rsrc(parts + part(s0 + u), kRows * D * 4);
 #pragma unroll
             for (int i = 0; i < kTake; ++i) x[i][u] = coherent_load16(rs, ((i0 + i) * kThreads + threadIdx.x) * 16);
         }
     };
-    request_parts(0, 0);
-    for (int row = threadIdx.x / 16; row < kRows; row += kThreads / 16) {
+    if (mine) request_parts(0, 0);
+    for (int row = threadIdx.x / 16; row < rows; row += kThreads / 16) {
         const int s0 = threadIdx.x % 16;
         float mv[kMaxSplits / 16], lv[kMaxSplits / 16], m = -INFINITY;
 #pragma unroll
@@ -279,12 +282,13 @@ __device__ __forceinline__ void join_parts(const Args& a, const Request& q, int 
         if (s0 == 0) totals[row] = l;
     }
     __syncthreads();
+    if (!mine) return;
     for (int i0 = 0; i0 < kItems; i0 += kTake) {
         float y[kTake][4] = {};
-        for (int s0 = 0; s0 < active; s0 += 8) {
+        for (int s0 = 0; s0 < active; s0 += kParts) {
             if (i0 + s0 > 0) request_parts(i0, s0);
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
+            for (int u = 0; u < kParts; ++u) {
                 if (s0 + u >= active) break;
 #pragma unroll
                 for (int i = 0; i < kTake; ++i) {
@@ -300,6 +304,15 @@ __device__ __forceinline__ void join_parts(const Args& a, const Request& q, int 
             put<T>(a, q, kh, row_of(a, t0, r0 + at.row), at.dim, y[i], totals[at.row], D);
         }
     }
+}
+template <typename T, int D, int kRows, typename Part, typename Place>
+__device__ __forceinline__ void join_parts(const Args& a, const Request& q, int kh, int t0, int r0, int active, int rows,
+                                           bool mine, const char* parts, Part part, Place place, float* factors,
+                                           float* totals) {
+    if (active <= 4 && kRows * D / 4 / kThreads > 8)
+        join_by<T, D, kRows, 4>(a, q, kh, t0, r0, active, rows, mine, parts, part, place, factors, totals);
+    else
+        join_by<T, D, kRows, 8>(a, q, kh, t0, r0, active, rows, mine, parts, part, place, factors, totals);
 }
 
 constexpr int64_t part_bytes(int64_t rows, int64_t d) { return rows * (d + 2) * 4; }
@@ -745,7 +758,7 @@ __device__ __forceinline__ void few_rows(const Args& a, int id, FewShared<D, RT>
                 const int item = i * kThreads + static_cast<int>(threadIdx.x);
                 return RowDim{item / (D / 4), 4 * (item % (D / 4))};
             };
-            join_parts<T, D, kRows>(a, q, kh, 0, 0, active, a.parts, part, place, merge_o[0], merge_m[0]);
+            join_parts<T, D, kRows>(a, q, kh, 0, 0, active, kRows, true, a.parts, part, place, merge_o[0], merge_m[0]);
         }
     }
 }
@@ -762,12 +775,14 @@ __device__ __forceinline__ void few_rows(const Args& a, int id, FewShared<D, RT>
 // MI355X, passes back to back: 3 prompts, 12000 tokens in all, 64 heads of 128 on 8,
 // bf16: 963 us, 948 TFLOP/s (a large product: 1150); one of 6500, 64 heads of 64
 // on 8, f16: 380 us, 910 TFLOP/s; 500 tokens behind 30000, 32 heads of 128 on 8,
-// f16: 292 us, 850 TFLOP/s; one fp32 prompt of 2000, 64 heads of 128: 536 us, 122
-// TFLOP/s (153).  The matrix cores are busy 40 % of the cycles: what is left is
-// softmax between the products of two waves a SIMD (without the loads 496 us
-// where it takes 640, without barriers too 472, without exponentials 436).  Eight
-// waves and 128 keys a tile: 743 us for 625; a tile's scores beside the weights
-// of the one before: registers spill, 1310.
+// f16: 292 us, 850 TFLOP/s, with 7 tokens of other requests over 22000 beside them
+// 411 to 430; one fp32 prompt of 2000, 64 heads of 128: 536 us, 122 TFLOP/s (153).
+// The matrix cores are busy 40 % of the cycles: what is left is softmax between
+// the products of two waves a SIMD (without the loads 496 us where it takes 640,
+// without barriers too 472, without exponentials 436).  Eight waves and 128 keys a
+// tile: 743 us for 625; a tile's scores beside the weights of the one before:
+// registers spill, 1310.  A single tile alone on its compute unit waits for its
+// keys: about 1.4 us for 64 of 128 dims, twice what its products take.
 template <typename T, int D>
 struct Tile {
     static constexpr int KT = sizeof(T) == 4 ? 32 : 64;         // keys
@@ -803,7 +818,8 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
     constexpr int kRowBytes = D * sizeof(T);
     constexpr int kLeastTiles = kWide ? 2 : 4;   // key tiles that are worth a workgroup
     constexpr int kAhead = 4;                    // LDS operands in front of their products
-    constexpr int kJoin = kWide ? 6 : D == 64 ? 28 : 16;   // key tiles' time that parts take
+    constexpr int kJoin = kWide ? 6 : D == 64 ? 28 : 16;   // key tiles' time that all workgroups' parts take,
+    constexpr int kJoinFew = kWide ? 6 : D == 64 ? 16 : 10;   // and those of fewer
     constexpr int kStart = kWide ? 1 : 2;        // key tiles' time that a row tile takes beside its keys
 
     const int lane = threadIdx.x & 63;
@@ -814,14 +830,17 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
         const int r = q.todo * g;
         return r > a.few ? (r + kRows - 1) / kRows : 0;
     };
+    constexpr int kLeast = kStart + kLeastTiles;
 
     int longest;
     const int tiles_all = sum_up(a.batch, sh.requests, [&](int b) { return tiles_of(request<kPaged>(a, b)); }, &longest);
     if (tiles_all == 0) return;
     // A row tile's keys go to one workgroup, or all tiles' keys are dealt out
     // evenly (as attention_few_kernel's are), where the first would take longer
-    // than dealing out and the storing and joining of the parts (kJoin; 512
-    // workgroups' 16-bit parts take 25 us).  Times in key tiles of a compute unit:
+    // than dealing out and the storing and joining of the parts (512 workgroups'
+    // 16-bit parts take 25 us: kJoin; less where the shares are the least that is
+    // worth a workgroup and fewer take part: kJoinFew, 100 rows beside 7 tokens over
+    // 2000, 32 heads of 64 on 8: 27.6 us, one workgroup a tile 38.9).  Times in key tiles of a compute unit:
     // up to 256 tiles have one each, up to 512 share one by twos (below), more
     // follow as others end (of tiles of equal length the last alone).  32 heads of 64
     // on 4, f16, 3000 rows: 55 us against 79 dealt out; 40 rows of 64 heads of 128 on
@@ -841,13 +860,12 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
         const int alone = units <= kTargetGroups / 2 ? longest
                           : units <= kTargetGroups   ? max(longest, 2 * each)
                                                      : 2 * each + max(2 * (of_head / tiles_all) - longest, 0);
-        shared = longest > kStart + kLeastTiles && alone > 2 * max(each, kStart + kLeastTiles) + kJoin;
+        shared = longest > kLeast && alone > 2 * max(each, kLeast) + (each >= kLeast ? kJoin : kJoinFew);
     }
     int pos = id, end = id + 1, share = 1;   // of the units (KV head, row tile), or of their key tiles
     if (shared) {
         const int total = of_head * a.kv_heads;
-        share = max(max((total + kTargetGroups - 1) / kTargetGroups, kStart + kLeastTiles),
-                    (longest + kManySplits - 2) / (kManySplits - 1));
+        share = max(max((total + kTargetGroups - 1) / kTargetGroups, kLeast), (longest + kManySplits - 2) / (kManySplits - 1));
         if (id >= kTargetGroups) return;
         // neighbours, which read the same keys, on one XCD
         id = id % 8 * (kTargetGroups / 8) + id / 8;
@@ -940,6 +958,8 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
         const int seen = min(max(q.p0 + t_last + 1, 0), q.length);      // keys that some row sees
         const int whole = min(max(q.p0 + t0 + 1, 0), q.length);         // that every row sees
         last = min(last, (seen + KT - 1) / KT);
+        const int rows = min(q.todo * g - r0, kRows);
+        const bool has_rows = 32 * RT * wave < rows;   // this wave
 
         // Where the tile's pieces lie: a wave's piece u is 1 KB, kWaveRows rows.
         constexpr int kWaveRows = 64 / CH, kStep = kWaves * kWaveRows;   // rows of a piece, of the waves' pieces u
@@ -1259,6 +1279,7 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
         const __amdgpu_buffer_rsrc_t prs = buffer_rsrc(out_part, part_bytes(kRows, D));
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
+            if (!has_rows) break;
             const float l = sum_halves(l_run[rt]);
             const int row = 32 * (RT * wave + rt) + lc;
 #pragma unroll
@@ -1283,7 +1304,7 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
         if (active > 1 && last_arrival(a.tickets + first_group * kTicketStride, active, &sh.ticket)) {
             float* f = reinterpret_cast<float*>(sh.tile[0][0]);
             static_assert((kManySplits + 1) * kRows * 4 <= static_cast<int>(sizeof sh.tile), "factors fit");
-            join_parts<T, D, kRows>(a, q, kh, t0, rem0, active, a.parts, part, place, f, f + kManySplits * kRows);
+            join_parts<T, D, kRows>(a, q, kh, t0, rem0, active, rows, has_rows, a.parts, part, place, f, f + kManySplits * kRows);
             __syncthreads();
         }
     }
@@ -1321,8 +1342,15 @@ Plan plan(int64_t batch, int64_t rows, int64_t max_rows, int64_t heads, int64_t 
     // (requests between 17 and 32 rows are the other kernel's where that runs anyway)
     p.few_tiles = most <= 16 || (most > 32 && g <= 16) ? 1 : 2;
     p.few_rows = 16 * p.few_tiles;
-    // One request with more rows than that: all of it is the other kernel's.
-    p.few = paged && g <= p.few_rows && (batch > 1 || most <= p.few_rows);
+    // Where some request is known to have more rows than that, 16-bit calls are the
+    // other kernel's altogether: tokens then run beside the chunk instead of before
+    // it (16 bits, 32 heads of 128 on 8: a chunk of 500 behind 30000 beside 7 tokens
+    // 430 us against 456, of 11 behind 769 beside 4 27.6 against 41.4).  fp32 tokens
+    // would take the matrix cores from it (100 rows beside 31 tokens over 2000, 32
+    // heads of 64 on 4: 91 us against 71).  Rows not known: most calls hold tokens
+    // alone, which are this kernel's (32 over 8000, 64 heads of 128 on 8: 151 us
+    // against 157, one over 2000, 32 of 64: 7.6 against 34.5).
+    p.few = paged && g <= p.few_rows && (most <= p.few_rows || (batch > 1 && (wide || max_rows == 0)));
     if (!p.few) p.few_rows = 0;
     p.many = most > p.few_rows;
     p.shared = max_tokens > kRound;
