@@ -1056,8 +1056,9 @@ int vm_hip_qk_norm_rope(const void* qkv, int dtype, int64_t rows, int64_t heads,
  * rising order.  scale <= 0 means 1/sqrt(head_dim).
  *
  * Products, maxima, sums and the output are fp32 (with 16-bit rows, each weight
- * is rounded to 16 bits for its product with the value; fp32 rows are
- * multiplied in fp32).  Scores below 2^100 in magnitude.  A key or value that a
+ * is rounded to the rows' type for its product with the value, half a step of it,
+ * and with F16 at most 2^-33 of the row's largest weight where that is more; fp32
+ * rows are multiplied in fp32).  Scores below 2^100 in magnitude.  A key or value that a
  * row does not see takes no part in it, whatever it holds; a value that is not
  * finite makes the element not finite in every row that sees it.
  *

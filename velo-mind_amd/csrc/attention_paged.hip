@@ -17,8 +17,8 @@
 // wave its own blocks of keys, and the keys of all requests dealt out evenly
 // over the workgroups.  attention_many_kernel takes the others: 32 RT rows a
 // wave, key tiles in LDS for all four waves.  16-bit rows use the 16-bit matrix
-// instructions (weights rounded to 16 bits: half a step of the result's type
-// for each), fp32 rows the fp32 ones.
+// instructions (weights rounded to 16 bits: half a step of the rows' type for
+// each, F16 as kLift says), fp32 rows the fp32 ones.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -55,6 +55,15 @@ constexpr int kRound = 128;           // keys that the waves of attention_few_ke
 // A weight may exceed 1 by this much (log2) before its row's reference moves:
 // references then move in the first blocks and rarely later.
 constexpr float kHeadroom = 7.0f;
+// What a row's reference weighs (log2).  F16 weights below 2^-14 have an error of
+// up to 2^-25 instead of half a step, below 2^-25 they are lost, and the sum of
+// weights, in fp32, keeps them: behind a key that weighs 1, 100000 others of e^-17
+// would count for half as much again.  The type goes to 65504, so its references
+// weigh 2^8, weights with the headroom 2^15: errors are half a step down to 2^-22 of
+// the reference and 2^-33 of it below.  All weights of a row are larger by the
+// same, which its sum takes out again.
+template <typename T>
+constexpr float kLift = std::is_same<T, F16>::value ? 8.0f : 0.0f;
 
 struct Args {
     const void* q;
@@ -628,7 +637,7 @@ __device__ __forceinline__ void few_rows(const Args& a, int id, FewShared<D, RT>
             float p[RT][KPL];
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                const float base = m_run[rt] * a.c;
+                const float base = m_run[rt] * a.c - kLift<T>;
 #pragma unroll
                 for (int j = 0; j < KPL; ++j) {
                     p[rt][j] = __builtin_amdgcn_exp2f(fmaf(st[rt][j / 4][j % 4], a.c, -base));
@@ -713,7 +722,7 @@ __device__ __forceinline__ void few_rows(const Args& a, int id, FewShared<D, RT>
                     store4(merge_o[wave] + (16 * rt + lr) * D + dim, y);
                 }
             if (lg == 0) {
-                merge_m[wave][16 * rt + lr] = limit[rt] == -INFINITY ? -INFINITY : m_run[rt] * a.c;
+                merge_m[wave][16 * rt + lr] = limit[rt] == -INFINITY ? -INFINITY : m_run[rt] * a.c - kLift<T>;
                 merge_l[wave][16 * rt + lr] = l;
             }
         }
@@ -1163,7 +1172,7 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
             }
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                const float base = m_run[rt] * a.c;
+                const float base = m_run[rt] * a.c - kLift<T>;
 #pragma unroll
                 for (int n = 0; n < NK; ++n)
 #pragma unroll
@@ -1296,7 +1305,7 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
                 }
             if (active > 1 && lh == 0) {
                 float* ml = reinterpret_cast<float*>(out_part) + kRows * D;
-                coherent_store(ml + row, limit[rt] == -INFINITY ? -INFINITY : m_run[rt] * a.c);
+                coherent_store(ml + row, limit[rt] == -INFINITY ? -INFINITY : m_run[rt] * a.c - kLift<T>);
                 coherent_store(ml + kRows + row, l);
             }
         }
