@@ -89,13 +89,22 @@ struct Args {
 struct Request {
     int start, n, length, p0;   // first row, rows, tokens, tokens in front of the first row (negative: rows without)
     int todo;                   // rows that are computed
+    bool falls;                 // the next offset is below this request's
 };
 
+// `falls`: some offset is below an earlier one, and the largest up to b counts
+// (every row is one request's).  Offsets of a plan rise, and only the others pay
+// for the walk.
 template <bool kPaged>
-__device__ __forceinline__ Request request(const Args& a, int b) {
+__device__ __forceinline__ Request request(const Args& a, int b, bool falls) {
     Request r;
-    r.start = min(max(a.row_start[b], 0), a.rows);
-    r.n = min(max(a.row_start[b + 1], r.start), a.rows) - r.start;
+    int from = a.row_start[b];
+    const int to = a.row_start[b + 1];
+    r.falls = to < from;
+    if (__builtin_expect(falls, false))
+        for (int i = 0; i < b; ++i) from = max(from, a.row_start[i]);
+    r.start = min(max(from, 0), a.rows);
+    r.n = min(max(to, r.start), a.rows) - r.start;
     if (kPaged) {
         r.length = min(max(a.lengths[b], 0), a.max_pages << a.shift);
     } else {
@@ -108,7 +117,7 @@ __device__ __forceinline__ Request request(const Args& a, int b) {
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ Request uniform(const Request& r) {
-    return {uniform(r.start), uniform(r.n), uniform(r.length), uniform(r.p0), uniform(r.todo)};
+    return {uniform(r.start), uniform(r.n), uniform(r.length), uniform(r.p0), uniform(r.todo), r.falls};
 }
 
 __device__ __forceinline__ float max_halves(float v) {
@@ -338,7 +347,9 @@ __device__ __forceinline__ bool last_arrival(unsigned* counter, int active, unsi
 }
 
 // Running sums, up to and with each of `count` things, of what size(i) says of
-// them, by the whole workgroup; their total and the largest size.
+// them, by the whole workgroup; their total and the largest size.  Some size
+// negative: the largest is kNoSums, and the sums are not valid.
+constexpr int kNoSums = 0x7fffffff;
 template <int kMost>
 struct Sums {
     int upto[kMost];
@@ -356,7 +367,7 @@ __device__ __forceinline__ int sum_up(int count, Sums<kMost>& s, Size size, int*
     for (int i = i0; i < min(i0 + each, count); ++i) {
         const int w = size(i);
         sum += w;
-        most = max(most, w);
+        most = w < 0 ? kNoSums : max(most, w);
         s.upto[i] = sum;
     }
     int run = sum;
@@ -380,6 +391,17 @@ __device__ __forceinline__ int sum_up(int count, Sums<kMost>& s, Size size, int*
     for (int i = i0; i < min(i0 + each, count); ++i) s.upto[i] += before;
     __syncthreads();
     return total;
+}
+// The sums of size(request) over all requests; whether offsets fall.
+template <bool kPaged, typename Size>
+__device__ __forceinline__ int sum_up_requests(const Args& a, Sums<kMaxBatch>& s, Size size, int* largest, bool* falls) {
+    const int total = sum_up(a.batch, s, [&](int b) {
+        const Request q = request<kPaged>(a, b, false);
+        return a.batch > 1 && q.falls ? -1 : size(q);   // (one request's rows are nobody else's)
+    }, largest);
+    *falls = uniform(*largest) == kNoSums;
+    if (__builtin_expect(!*falls, true)) return total;
+    return sum_up(a.batch, s, [&](int b) { return size(request<kPaged>(a, b, true)); }, largest);
 }
 // The first whose running sum is above x.
 template <int kMost>
@@ -445,7 +467,8 @@ __device__ __forceinline__ void few_rows(const Args& a, int id, FewShared<D, RT>
 
     // Rounds of all requests, summed up by every workgroup for itself.
     int longest;
-    const int total = a.kv_heads * sum_up(a.batch, sh.sums, [&](int b) { return rounds_of(request<true>(a, b)); }, &longest);
+    bool falls;
+    const int total = a.kv_heads * sum_up_requests<true>(a, sh.sums, rounds_of, &longest, &falls);
     // Shares: even, worth a workgroup (64 KB of keys and values or so; one fp32
     // token over 2000: 9.0 us with one round, 9.9 with two; one of 64 heads of 128
     // over 8000, bf16: 23 and 17, with four 18.7), and no more than kMaxSplits of a request's keys.
@@ -457,7 +480,7 @@ __device__ __forceinline__ void few_rows(const Args& a, int id, FewShared<D, RT>
     while (pos < end) {
         // The request, KV head and rounds that this share goes on with.
         const int b = __builtin_amdgcn_readfirstlane(first_above(sh.sums, a.batch, pos / a.kv_heads));
-        const Request q = uniform(request<true>(a, b));
+        const Request q = uniform(request<true>(a, b, falls));
         const int rounds = rounds_of(q);
         const int request_start = (sh.sums.upto[b] - rounds) * a.kv_heads;
         const int kh = (pos - request_start) / rounds;
@@ -842,7 +865,8 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
     constexpr int kLeast = kStart + kLeastTiles;
 
     int longest;
-    const int tiles_all = sum_up(a.batch, sh.requests, [&](int b) { return tiles_of(request<kPaged>(a, b)); }, &longest);
+    bool falls;
+    const int tiles_all = sum_up_requests<kPaged>(a, sh.requests, tiles_of, &longest, &falls);
     if (tiles_all == 0) return;
     // A row tile's keys go to one workgroup, or all tiles' keys are dealt out
     // evenly (as attention_few_kernel's are), where the first would take longer
@@ -860,7 +884,7 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
     if (shared) {
         of_head = sum_up(tiles_all, sh.tiles, [&](int i) {
             const int b = first_above(sh.requests, a.batch, i);
-            const Request q = request<kPaged>(a, b);
+            const Request q = request<kPaged>(a, b, falls);
             const int r0 = (i - (sh.requests.upto[b] - tiles_of(q))) * kRows;
             const int seen = min(q.p0 + min((r0 + kRows - 1) / g, q.todo - 1) + 1, q.length);
             return kStart + max((seen + KT - 1) / KT, 1);
@@ -889,7 +913,7 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
     // p0 group / kRows of a request without tokens in front.
     const auto by_length = [&](int rank) {
         const bool real = lane < a.batch;
-        const Request q = request<kPaged>(a, real ? lane : 0);
+        const Request q = request<kPaged>(a, real ? lane : 0, falls);
         const int mine = real ? tiles_of(q) : 0;
         const int ahead = static_cast<int>(static_cast<int64_t>(max(q.p0, 0)) * g / kRows);
         const int before = sh.requests.upto[real ? lane : 0] - mine;
@@ -959,9 +983,8 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
         active = uniform(active);
         first_group = uniform(first_group);
         const int b = uniform(first_above(sh.requests, a.batch, slot));
-        const Request q = uniform(request<kPaged>(a, b));
+        const Request q = uniform(request<kPaged>(a, b, falls));
         const int r0 = uniform(slot - (sh.requests.upto[b] - tiles_of(q))) * kRows;
-        if (r0 < 0 || r0 >= q.todo * g) continue;   // (row_start that does not rise)
         const int t0 = r0 / g, rem0 = r0 - t0 * g;   // its token, and the rows of that in front
         const int t_last = min(uniform(row_of(a, t0, rem0 + kRows - 1).t), q.todo - 1);
         const int seen = min(max(q.p0 + t_last + 1, 0), q.length);      // keys that some row sees
