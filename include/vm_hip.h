@@ -972,7 +972,8 @@ int vm_hip_kv_paged_plan(const vm_hip_page_plan* plan, void* workspace, int64_t 
 
 /* The pages of every request with finished[b] != 0 (int32 [batch]) go back to
  * the end of free_pages, in order of requests and tokens; their tables' entries
- * become -1, their lengths 0, and *free_count grows (never past `pages`). */
+ * become -1, their lengths 0, and *free_count grows (never past `pages`: the
+ * pages behind are dropped).  Entries that are no page are not given back. */
 int vm_hip_kv_paged_release(int64_t batch, int64_t max_pages, int64_t pages, int64_t page_size, const int32_t* finished,
                             int32_t* lengths, int32_t* tables, int32_t* free_pages, int32_t* free_count, void* stream);
 

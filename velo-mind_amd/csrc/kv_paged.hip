@@ -45,23 +45,25 @@ bool off16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; 
 bool off4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) != 0; }
 bool known_dtype(int d) { return d == VM_HIP_DTYPE_F32 || d == VM_HIP_DTYPE_F16 || d == VM_HIP_DTYPE_BF16; }
 
-// Sums of non-negative numbers that stop at `cap` (< 2^30): the order of the
-// additions does not matter, and nothing leaves 32 bits.
-__device__ __forceinline__ int add_capped(int a, int b, int cap) { return min(a + b, cap); }
+// Sums of non-negative numbers that stop at `cap` (half of what N holds at most):
+// the order of the additions does not matter, and nothing leaves N.
+template <typename N>
+__device__ __forceinline__ N add_capped(N a, N b, N cap) { return min(a + b, cap); }
 
 // The capped sum of the values of the threads in front of this one, and of all.
-__device__ __forceinline__ int sum_before(int v, int cap, int* waves, int* all) {
+template <typename N>
+__device__ __forceinline__ N sum_before(N v, N cap, N* waves, N* all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) {
-        const int o = __shfl_up(v, s, 64);
+        const N o = __shfl_up(v, s, 64);
         if (lane >= s) v = add_capped(v, o, cap);
     }
     __syncthreads();   // (the sums of an earlier call have been read)
     if (lane == 63) waves[wave] = v;
     __syncthreads();
-    const int left = __shfl_up(v, 1, 64);
-    int before = lane ? left : 0, total = 0;
+    const N left = __shfl_up(v, 1, 64);
+    N before = lane ? left : 0, total = 0;
 #pragma unroll
     for (int w = 0; w < kT / 64; ++w) {
         if (w < wave) before = add_capped(before, waves[w], cap);
@@ -73,7 +75,8 @@ __device__ __forceinline__ int sum_before(int v, int cap, int* waves, int* all) 
 
 // The last index of start[0 .. n - 1] (non-decreasing, start[0] <= x) whose
 // value is at most x.
-__device__ __forceinline__ int last_at_most(const int* start, int n, int x) {
+template <typename N>
+__device__ __forceinline__ int last_at_most(const N* start, int n, N x) {
     int lo = 0, hi = n;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -202,47 +205,72 @@ __global__ __launch_bounds__(kT) void kv_paged_plan_kernel(const PlanArgs a) {
     if (threadIdx.x == 0) *p.free_count_out = free_pages - handed_out;
 }
 
-// ---- Pages given back: one workgroup, E requests a thread summed up, then a
-// page a thread and step.  A launch and three round trips.
+// ---- Pages given back: one workgroup, E requests a thread summed up, then kRun
+// adjacent entries a thread and step.  Entries that are no page are cleared but not
+// given back (a plan would hand them out), so a step counts the others before it
+// stores them; a pool that is full takes no more.  Sums are 64 bits: requests whose
+// lengths are not valid hold whole tables.  A launch and four round trips for up to
+// 2048 pages (5 of 256 requests, 2500 pages: 3.3 us), three more for each further
+// 2048 (all 128000 pages of those: 213 us).
 template <int E>
 __global__ __launch_bounds__(kT) void kv_paged_release_kernel(int batch, int64_t max_pages, int64_t pages, int shift,
                                                               const int32_t* __restrict__ finished, int32_t* lengths,
                                                               int32_t* tables, int32_t* free_pages,
                                                               int32_t* free_count) {
-    __shared__ int start[kMaxBatch + 1];
-    __shared__ int waves[kT / 64];
-    const int left = min(max(*free_count, 0), static_cast<int>(pages));
-    const int room = static_cast<int>(pages) - left;   // a pool that is full takes no more
+    constexpr int kRun = 8;
+    __shared__ int64_t start[kMaxBatch + 1];   // entries in front of a request's
+    __shared__ int64_t waves[kT / 64];
+    __shared__ int valid_waves[kT / 64];
+    int64_t left = min(max(*free_count, 0), static_cast<int>(pages));
     const int b0 = threadIdx.x * E;
-    int n[E], sum = 0;
+    int64_t n[E], sum = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         n[e] = 0;
         if (b0 + e < batch && finished[b0 + e]) {
             const int64_t held = (static_cast<int64_t>(max(lengths[b0 + e], 0)) + (1 << shift) - 1) >> shift;
-            n[e] = static_cast<int>(min(held, max_pages));
+            n[e] = min(held, max_pages);
             lengths[b0 + e] = 0;
         }
-        n[e] = min(n[e], room + 1);
-        sum = add_capped(sum, n[e], room + 1);
+        sum += n[e];
     }
-    int all;
-    int at = sum_before(sum, room + 1, waves, &all);
+    int64_t all;
+    int64_t at = sum_before<int64_t>(sum, INT64_MAX / 2, waves, &all);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         if (b0 + e < batch) start[b0 + e] = at;
-        at = add_capped(at, n[e], room + 1);
+        at += n[e];
     }
     if (threadIdx.x == 0) start[batch] = all;
     __syncthreads();
-    const int total = min(all, room);
-    for (int i = threadIdx.x; i < total; i += kT) {
-        const int b = last_at_most(start, batch, i);
-        int32_t* entry = tables + static_cast<int64_t>(b) * max_pages + (i - start[b]);
-        free_pages[left + i] = *entry;
-        *entry = -1;
+    for (int64_t i0 = 0; i0 < all; i0 += kT * kRun) {
+        const int64_t i = i0 + threadIdx.x * kRun;
+        int id[kRun], valid = 0;
+        int32_t* entry[kRun];
+        int b = i < all ? last_at_most(start, batch, i) : 0;
+#pragma unroll
+        for (int u = 0; u < kRun; ++u) {
+            id[u] = -1;
+            if (i + u >= all) continue;
+            while (start[b + 1] <= i + u) ++b;   // (start[batch] is above)
+            entry[u] = tables + b * max_pages + (i + u - start[b]);
+            id[u] = *entry[u];
+        }
+#pragma unroll
+        for (int u = 0; u < kRun; ++u) valid += id[u] >= 0 && id[u] < pages;
+        int given;
+        int64_t to = left + sum_before<int>(valid, kT * kRun, valid_waves, &given);
+#pragma unroll
+        for (int u = 0; u < kRun; ++u) {
+            if (i + u >= all) continue;
+            *entry[u] = -1;
+            if (id[u] < 0 || id[u] >= pages) continue;
+            if (to < pages) free_pages[to] = id[u];
+            ++to;
+        }
+        left = min(left + given, pages);
     }
-    if (threadIdx.x == 0) *free_count = left + total;
+    if (threadIdx.x == 0) *free_count = static_cast<int>(left);
 }
 
 // ---- Tables of the rotation.  Angles of far positions need 64 bits (131071
