@@ -1088,7 +1088,8 @@ int vm_hip_attention_packed(const void* q, const void* k, const void* v, void* o
  *        planned); a request's rows past it are left as they were.  0: not
  *        known.  Kernels and the workspace are chosen by it: 1 where all
  *        requests decode.
- * max_pages * page_size <= 2^24, and times batch * kv_heads below 2^38.
+ * max_pages * page_size <= 2^24, and, as a multiple of 128, times batch * kv_heads at
+ * most 2^38 - 2^16.
  * row_start and lengths are held to [0, rows] and [0, max_pages * page_size];
  * tokens in table entries that are no page do not exist; a row that sees none
  * gets zeros.  Roundings, scores, infinities, scale, limits and the workspace are

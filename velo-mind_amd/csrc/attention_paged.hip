@@ -1547,8 +1547,9 @@ int vm_hip_attention_paged(const vm_hip_kv_paged* cache, const int32_t* tables, 
     VM_TRY(check_call("attention_paged", batch, rows, max_rows, heads, hk, d));
     if (max_pages < 1 || max_pages > (1 << 24) / cache->page_size)
         return fail_inval("attention_paged: max_pages * page_size must be at most 2^24");
-    if (batch * hk * ((max_pages * cache->page_size + kRound - 1) / kRound) >= (int64_t{1} << 31))
-        return fail_inval("attention_paged: batch * kv_heads * max_pages * page_size must be below 2^38");
+    // (attention_few_kernel rounds the requests' rounds up to workgroups in 32 bits)
+    if (batch * hk * ((max_pages * cache->page_size + kRound - 1) / kRound) > 0x7fffffff - (kTargetGroups - 1))
+        return fail_inval("attention_paged: batch * kv_heads * max_pages * page_size must be at most 2^38 - 2^16");
     if (!(scale < INFINITY)) return fail_inval("attention_paged: scale must be finite");
     if (rows == 0 || batch == 0) return 0;
     if (!tables || !q || !out || !row_start || !lengths) return fail_inval("attention_paged: null pointer");
