@@ -1054,7 +1054,8 @@ int vm_hip_qk_norm_rope(const void* qkv, int dtype, int64_t rows, int64_t heads,
  *            projection's rows
  *   out      [rows, heads * head_dim] of dtype; all 16-byte aligned
  * row_start (int32 [batch + 1] in device memory) is held to [0, rows] and to
- * rising order: an offset below an earlier one counts as the largest before it.  scale <= 0 means 1/sqrt(head_dim).
+ * rising order: an offset below an earlier one counts as the largest before it.
+ * scale <= 0 means 1/sqrt(head_dim); it is finite, also divided by ln 2.
  *
  * Products, maxima, sums and the output are fp32 (with 16-bit rows, each weight
  * is rounded to the rows' type for its product with the value, half a step of it,

@@ -33,3 +33,17 @@ def test_the_most_keys_that_are_taken():
     assert 512 * 2049 * 2047 == 2 ** 31 - 512
     assert "workspace" in _paged(512, 2049, 2047)
     assert "2^38" in _paged(512, 2049, 2048)
+
+
+@pytest.mark.parametrize("scale", [3.4e38, 2.4e38], ids=str)
+def test_scales_that_overflow_with_the_factor_of_exp2(scale):
+    assert "scale" in _paged(1, 2, 4, scale=scale)
+    assert "scale" in _message(H.attention_packed, P, P, P, P, H.DTYPE_F16, 512, 512, 512, 2, 10, 4, 2, 64, P, scale,
+                               None, 0)
+
+
+@pytest.mark.parametrize("scale", [2.3e38, 1e-38, 0.0, -1.0, float("-inf")], ids=str)
+def test_scales_that_are_taken(scale):
+    assert "workspace" in _paged(1, 2, 4, scale=scale)
+    assert "workspace" in _message(H.attention_packed, P, P, P, P, H.DTYPE_F16, 512, 512, 512, 2, 10, 4, 2, 64, P,
+                                   scale, None, 0)

@@ -1470,6 +1470,13 @@ float scale_of(float scale, int64_t d) {
     return (scale > 0.0f ? scale : 1.0f / std::sqrt(static_cast<float>(d))) * 1.44269504f;
 }
 
+// The factor that the kernels multiply scores by (scale / ln 2) has to be finite as well.
+int check_scale(const char* who, float scale, int64_t d) {
+    if (!(scale < INFINITY) || !(scale_of(scale, d) < INFINITY))
+        return fail_inval(std::string(who) + ": scale must be finite, also divided by ln 2");
+    return 0;
+}
+
 bool off16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
 bool off4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) != 0; }
 
@@ -1501,7 +1508,7 @@ int vm_hip_attention_packed(const void* q, const void* k, const void* v, void* o
             return fail_inval("attention_packed: strides must be multiples of 16 bytes, at most 2^22 elements");
     if (q_stride < heads * head_dim || k_stride < kv_heads * head_dim || v_stride < kv_heads * head_dim)
         return fail_inval("attention_packed: strides must hold a row's heads");
-    if (!(scale < INFINITY)) return fail_inval("attention_packed: scale must be finite");
+    VM_TRY(check_scale("attention_packed", scale, head_dim));
     if (rows == 0 || batch == 0) return 0;
     if (!q || !k || !v || !out || !row_start) return fail_inval("attention_packed: null pointer");
     if (off16(q) || off16(k) || off16(v) || off16(out))
@@ -1550,7 +1557,7 @@ int vm_hip_attention_paged(const vm_hip_kv_paged* cache, const int32_t* tables, 
     // (attention_few_kernel rounds the requests' rounds up to workgroups in 32 bits)
     if (batch * hk * ((max_pages * cache->page_size + kRound - 1) / kRound) > 0x7fffffff - (kTargetGroups - 1))
         return fail_inval("attention_paged: batch * kv_heads * max_pages * page_size must be at most 2^38 - 2^16");
-    if (!(scale < INFINITY)) return fail_inval("attention_paged: scale must be finite");
+    VM_TRY(check_scale("attention_paged", scale, d));
     if (rows == 0 || batch == 0) return 0;
     if (!tables || !q || !out || !row_start || !lengths) return fail_inval("attention_paged: null pointer");
     if (off16(q) || off16(out)) return fail_inval("attention_paged: q and out must be 16-byte aligned");
