@@ -1060,9 +1060,10 @@ int vm_hip_qk_norm_rope(const void* qkv, int dtype, int64_t rows, int64_t heads,
  * Products, maxima, sums and the output are fp32 (with 16-bit rows, each weight
  * is rounded to the rows' type for its product with the value, half a step of it,
  * and with F16 at most 2^-33 of the row's largest weight where that is more; fp32
- * rows are multiplied in fp32).  Scores below 2^100 in magnitude.  A key or value that a
- * row does not see takes no part in it, whatever it holds; a value that is not
- * finite makes the element not finite in every row that sees it.
+ * rows are multiplied in fp32).  Scores are below 2^100, finite values below 2^96 in
+ * magnitude.  A key or value that a row does not see takes no part in it, whatever
+ * it holds; a value that is not finite makes the element not finite in every row
+ * that sees it.
  *
  * Limits: heads / kv_heads <= 4096, rows * heads < 2^30, and at most 2^24 tiles of
  * 128 query rows; a call past them is refused.  out overlaps no input.

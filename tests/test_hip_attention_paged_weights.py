@@ -76,3 +76,39 @@ def test_many_small_weights_in_a_prompt(hip, dtype, d):
         scores[0] = low
         want, tol = small(values[first:i + 1], scores, dtype)
         close(got[i], np.broadcast_to(want, (heads, d)), np.broadcast_to(tol, (heads, d)))
+
+
+# A reference near 2^k has a step of 2^(k - 23): what its rounding adds to every exponent
+# (0.43 steps with queries of 167, -0.22 with 131) passes what F16 holds from 2^28 on,
+# and fp32 from 2^32.
+@TYPES
+@pytest.mark.parametrize("n,length,heads,hk,d", [(1, 700, 4, 4, 64), (3, 300, 16, 2, 128), (1, 9000, 8, 1, 64),
+                                                 (40, 2000, 16, 2, 128), (150, 150, 8, 2, 64), (40, 6000, 8, 8, 64)],
+                         ids=str)
+@pytest.mark.parametrize("power", [14, 17, 22, 28, 30, 34, 60, 99])
+@pytest.mark.parametrize("query", [167.0, 131.0])
+@pytest.mark.parametrize("sign", [1, -1], ids=["positive", "negative"])
+def test_large_scores(hip, dtype, n, length, heads, hk, d, power, query, sign):
+    """Scores of about 2^power, and half or twice that: some keys weigh 1, all others
+    nothing, and the outputs are means of the values of the first."""
+    c = Paged(hip, dtype, [n], [length], heads, hk, d, 16, 45)
+    c.scale = float(np.float32(2.0) ** (power - 14) * np.float32(1.1))
+    c.q[:] = c.k[:] = 0
+    c.q[:, :, 1] = query
+    t = np.arange(length)
+    large = np.random.default_rng(46).random(length) < 0.4
+    large[0] = True
+    key = np.where(large, 93.0, 46.5) if sign > 0 else np.where(large, -46.5, -93.0)
+    c.k[c.tables[0, t // 16], :, t % 16, 1] = key[:, None]
+    c.upload().call()
+    got = c.result()
+    _, values, _ = c.keys(0)
+    for i in {0, n // 2, n - 1}:
+        seen = np.flatnonzero(large[:length - n + i + 1])
+        for h in range(heads):
+            v = values[seen][:, h // (heads // hk)]
+            mean = v.mean(0)
+            # weights are alike, but not 1: at 2^14 167 adds 0.43 2^-9 to their exponents, so that
+            # 16 bits round each (1.0006, half a step of the rows' type, WEIGHT), their sum not
+            tol = np.abs(v).mean(0) * (len(seen) * 2.0 ** -23 + 2.0 ** -22 + WEIGHT[dtype]) + np.abs(mean) * STEP[dtype]
+            close(got[i, h], mean, tol + (2.0 ** -25 if dtype == 4 else 0))

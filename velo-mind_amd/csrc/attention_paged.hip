@@ -55,6 +55,13 @@ constexpr int kRound = 128;           // keys that the waves of attention_few_ke
 // A weight may exceed 1 by this much (log2) before its row's reference moves:
 // references then move in the first blocks and rarely later.
 constexpr float kHeadroom = 7.0f;
+// An exponent is one multiply-add, score times scale less the reference, whose
+// rounding (2^-24 of the reference) all weights share.  Where a reference is 2^16
+// or more, and it comes near a factor, the wave's scores lose theirs before they are
+// scaled: such rows have the lowest limit, so that every block goes where references
+// move.
+constexpr float kFar = 65536.0f;
+constexpr float kAlways = -3.402823466e38f;
 // What a row's reference weighs (log2).  F16 weights below 2^-14 have an error of
 // up to 2^-25 instead of half a step, below 2^-25 they are lost, and the sum of
 // weights, in fp32, keeps them: behind a key that weighs 1, 100000 others of e^-17
@@ -137,6 +144,22 @@ __device__ __forceinline__ float max_groups(float v) {
 __device__ __forceinline__ float sum_groups(float v) {
     v = swap_rows_add(v, v);
     return swap_halves_add(v, v);
+}
+
+// The rows' references, scaled; true: some row of the wave has a far one, and they
+// are to be taken from the scores.
+template <int RT>
+__device__ __forceinline__ bool references(const float (&m)[RT], float c, float (&ref)[RT]) {
+    bool far = false;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        ref[rt] = m[rt] * c;
+        far |= !(fabsf(ref[rt]) < kFar);
+    }
+    if (__builtin_expect(__any(far) == 0, true)) return false;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) ref[rt] = 0.0f;
+    return true;
 }
 
 // Elements that are not finite: bits that odd_bits() leaves in kOddMask (adding
@@ -586,7 +609,7 @@ __device__ __forceinline__ void few_rows(const Args& a, int id, FewShared<D, RT>
         };
         f32x4 acc[RT][ND];
         float m_run[RT];   // the score that weighs 1
-        float limit[RT];   // the score from which on it moves; -inf before the first key
+        float limit[RT];   // the score from which on it moves; -inf before the first key, or kAlways
         float l_run[RT];   // sum of this lane's keys' weights
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
@@ -640,6 +663,9 @@ __device__ __forceinline__ void few_rows(const Args& a, int id, FewShared<D, RT>
                 for (int j = 0; j < KPL; ++j) mt[rt] = fmaxf(mt[rt], st[rt][j / 4][j % 4]);
                 moves |= mt[rt] > limit[rt];
             }
+            float ref[RT];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) ref[rt] = m_run[rt] * a.c;
             if (__any(moves)) {
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
@@ -653,14 +679,20 @@ __device__ __forceinline__ void few_rows(const Args& a, int id, FewShared<D, RT>
                             for (int db = 0; db < ND; ++db) acc[rt][db] *= fall;
                         }
                         m_run[rt] = m;
-                        limit[rt] = m + kHeadroom / a.c;
+                        limit[rt] = fabsf(m * a.c) < kFar ? m + kHeadroom / a.c : kAlways;
                     }
+                }
+                if (references(m_run, a.c, ref)) {
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                        for (int bt = 0; bt < NT; ++bt) st[rt][bt] -= m_run[rt];
                 }
             }
             float p[RT][KPL];
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                const float base = m_run[rt] * a.c - kLift<T>;
+                const float base = ref[rt] - kLift<T>;
 #pragma unroll
                 for (int j = 0; j < KPL; ++j) {
                     p[rt][j] = __builtin_amdgcn_exp2f(fmaf(st[rt][j / 4][j % 4], a.c, -base));
@@ -1174,6 +1206,9 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
                     for (int e = 0; e < 16; ++e) mt[rt] = fmaxf(mt[rt], st[rt][n][e]);
                 moves |= mt[rt] > limit[rt];
             }
+            float ref[RT];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) ref[rt] = m_run[rt] * a.c;
             if (__any(moves)) {
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
@@ -1189,13 +1224,19 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
                                 for (int e = 0; e < 16; ++e) acc[rt][db][e] *= fall;
                         }
                         m_run[rt] = m;
-                        limit[rt] = m + kHeadroom / a.c;
+                        limit[rt] = fabsf(m * a.c) < kFar ? m + kHeadroom / a.c : kAlways;
                     }
+                }
+                if (references(m_run, a.c, ref)) {
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                        for (int n = 0; n < NK; ++n) st[rt][n] -= m_run[rt];
                 }
             }
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                const float base = m_run[rt] * a.c - kLift<T>;
+                const float base = ref[rt] - kLift<T>;
 #pragma unroll
                 for (int n = 0; n < NK; ++n)
 #pragma unroll
