@@ -28,6 +28,7 @@
 
 #include "kv_paged.h"
 #include "kv_q8.h"
+#include "lds_load.h"
 #include "vm_device.h"
 #include "vm_internal.h"
 
@@ -214,22 +215,8 @@ __device__ __forceinline__ u32x4 pack8(const float* p) {
     }
 }
 
-// Sixteen bytes a lane from memory (a uniform address and a lane's offset) to
-// LDS, lane by lane behind `to` (uniform).  Written as a statement of its own
-// because the compiler would have every LDS read wait for it, also reads of
-// another buffer; wait_loads() waits.  (No other instruction of these kernels
-// uses m0.)
-__device__ __forceinline__ void lds_load16(const char* from, uint32_t offset, char* to) {
-    const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)(to)));
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                 :
-                 : "s"(__builtin_amdgcn_readfirstlane(at)), "v"(offset), "s"(from)
-                 : "memory");
-}
 // The compiler moves vector and scalar arithmetic across this, nothing else.
 __device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0x406); }
-
-__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
 
 __device__ __forceinline__ void store4(float* p, const float* y) { *reinterpret_cast<float4*>(p) = make_float4(y[0], y[1], y[2], y[3]); }
 __device__ __forceinline__ void store4(F16* p, const float* y) {
