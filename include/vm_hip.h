@@ -973,7 +973,8 @@ int vm_hip_kv_paged_plan(const vm_hip_page_plan* plan, void* workspace, int64_t 
 /* The pages of every request with finished[b] != 0 (int32 [batch]) go back to
  * the end of free_pages, in order of requests and tokens; their tables' entries
  * become -1, their lengths 0, and *free_count grows (never past `pages`: the
- * pages behind are dropped).  Entries that are no page are not given back. */
+ * pages behind are dropped).  Entries that are no page are not given back; a page
+ * that two of the requests hold is given back twice. */
 int vm_hip_kv_paged_release(int64_t batch, int64_t max_pages, int64_t pages, int64_t page_size, const int32_t* finished,
                             int32_t* lengths, int32_t* tables, int32_t* free_pages, int32_t* free_count, void* stream);
 
@@ -1022,7 +1023,9 @@ typedef struct vm_hip_rope {
 } vm_hip_rope;
 
 /* The norm of a head row in front of the rotation: x / sqrt(mean(x^2) + eps) *
- * weight, with weights [head_dim] for query and for key heads. */
+ * weight, with weights [head_dim] for query and for key heads.  Squares are summed
+ * in fp32: elements are below 2^60 in magnitude, and without an eps a row's largest
+ * is above 2^-60. */
 typedef struct vm_hip_qk_norm {
     const float* q_weight;
     const float* k_weight;
@@ -1034,8 +1037,8 @@ typedef struct vm_hip_qk_norm {
  * (rope, or NULL) at positions[row], in fp32, rounded once; queries go to
  * q_out [rows, heads * head_dim], keys and values to the cache's slots[row].
  * A row with a negative position or a slot outside the cache is padding: nothing
- * of it is written.  A slot that is given twice gets parts of either row.  q_out
- * must not overlap qkv; both are 16-byte aligned. */
+ * of it is written.  A slot that is given twice gets parts of either row.  The
+ * outputs overlap neither qkv nor each other; qkv and q_out are 16-byte aligned. */
 int vm_hip_kv_paged_append(const vm_hip_kv_paged* cache, const void* qkv, int64_t rows, int64_t heads,
                            const vm_hip_qk_norm* norm, const vm_hip_rope* rope, const int32_t* positions,
                            const int32_t* slots, void* q_out, void* stream);
