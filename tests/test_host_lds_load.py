@@ -68,8 +68,9 @@ def test_the_address_is_there(listing):
 
 def test_a_wait_state_between_m0_and_the_load(listing):
     at = next(i for i, line in enumerate(listing) if line.startswith("global_load_lds_dwordx4"))
-    assert re.match(r"s_(mov|nop)", listing[at - 1]) and not re.match(r"s_\w+ m0,", listing[at - 1])
-    assert any(re.match(r"s_\w+ m0,", line) for line in listing[at - 3:at - 1])
+    wrote = max(i for i in range(at) if re.match(r"s_\w+ m0,", listing[i]))
+    assert wrote < at - 1
+    assert not any(line.startswith("global_load_lds") for line in listing[wrote:at]), "m0 is an earlier load's"
 
 
 def test_m0_is_written_again_behind_the_load(listing):
