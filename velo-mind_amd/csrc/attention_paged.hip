@@ -364,6 +364,7 @@ template <int kMost>
 struct Sums {
     int upto[kMost];
     int waves[kWaves], most[kWaves];
+    int falls;   // of requests: whether offsets do (here because scalar registers are short)
 };
 template <int kMost, typename Size>
 __device__ __forceinline__ int sum_up(int count, Sums<kMost>& s, Size size, int* largest) {
@@ -402,15 +403,16 @@ __device__ __forceinline__ int sum_up(int count, Sums<kMost>& s, Size size, int*
     __syncthreads();
     return total;
 }
-// The sums of size(request) over all requests; whether offsets fall.
+// The sums of size(request) over all requests, and whether offsets fall.
 template <bool kPaged, typename Size>
-__device__ __forceinline__ int sum_up_requests(const Args& a, Sums<kMaxBatch>& s, Size size, int* largest, bool* falls) {
+__device__ __forceinline__ int sum_up_requests(const Args& a, Sums<kMaxBatch>& s, Size size, int* largest) {
     const int total = sum_up(a.batch, s, [&](int b) {
         const Request q = request<kPaged>(a, b, false);
         return a.batch > 1 && q.falls ? -1 : size(q);   // (one request's rows are nobody else's)
     }, largest);
-    *falls = uniform(*largest) == kNoSums;
-    if (__builtin_expect(!*falls, true)) return total;
+    const bool falls = uniform(*largest) == kNoSums;
+    s.falls = falls;   // (every thread writes the same)
+    if (__builtin_expect(!falls, true)) return total;
     return sum_up(a.batch, s, [&](int b) { return size(request<kPaged>(a, b, true)); }, largest);
 }
 // The first whose running sum is above x.
@@ -477,8 +479,7 @@ __device__ __forceinline__ void few_rows(const Args& a, int id, FewShared<D, RT>
 
     // Rounds of all requests, summed up by every workgroup for itself.
     int longest;
-    bool falls;
-    const int total = a.kv_heads * sum_up_requests<true>(a, sh.sums, rounds_of, &longest, &falls);
+    const int total = a.kv_heads * sum_up_requests<true>(a, sh.sums, rounds_of, &longest);
     // Shares: even, worth a workgroup (64 KB of keys and values or so; one fp32
     // token over 2000: 9.0 us with one round, 9.9 with two; one of 64 heads of 128
     // over 8000, bf16: 23 and 17, with four 18.7), and no more than kMaxSplits of a request's keys.
@@ -490,7 +491,7 @@ __device__ __forceinline__ void few_rows(const Args& a, int id, FewShared<D, RT>
     while (pos < end) {
         // The request, KV head and rounds that this share goes on with.
         const int b = __builtin_amdgcn_readfirstlane(first_above(sh.sums, a.batch, pos / a.kv_heads));
-        const Request q = uniform(request<true>(a, b, falls));
+        const Request q = uniform(request<true>(a, b, sh.sums.falls));
         const int rounds = rounds_of(q);
         const int request_start = (sh.sums.upto[b] - rounds) * a.kv_heads;
         const int kh = (pos - request_start) / rounds;
@@ -884,8 +885,7 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
     constexpr int kLeast = kStart + kLeastTiles;
 
     int longest;
-    bool falls;
-    const int tiles_all = sum_up_requests<kPaged>(a, sh.requests, tiles_of, &longest, &falls);
+    const int tiles_all = sum_up_requests<kPaged>(a, sh.requests, tiles_of, &longest);
     if (tiles_all == 0) return;
     // A row tile's keys go to one workgroup, or all tiles' keys are dealt out
     // evenly (as attention_few_kernel's are), where the first would take longer
@@ -903,7 +903,7 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
     if (shared) {
         of_head = sum_up(tiles_all, sh.tiles, [&](int i) {
             const int b = first_above(sh.requests, a.batch, i);
-            const Request q = request<kPaged>(a, b, falls);
+            const Request q = request<kPaged>(a, b, sh.requests.falls);
             const int r0 = (i - (sh.requests.upto[b] - tiles_of(q))) * kRows;
             const int seen = min(q.p0 + min((r0 + kRows - 1) / g, q.todo - 1) + 1, q.length);
             return kStart + max((seen + KT - 1) / KT, 1);
@@ -932,7 +932,7 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
     // p0 group / kRows of a request without tokens in front.
     const auto by_length = [&](int rank) {
         const bool real = lane < a.batch;
-        const Request q = request<kPaged>(a, real ? lane : 0, falls);
+        const Request q = request<kPaged>(a, real ? lane : 0, sh.requests.falls);
         const int mine = real ? tiles_of(q) : 0;
         const int ahead = static_cast<int>(static_cast<int64_t>(max(q.p0, 0)) * g / kRows);
         const int before = sh.requests.upto[real ? lane : 0] - mine;
@@ -1002,7 +1002,7 @@ __device__ __forceinline__ void many_rows(const Args& a, int id, ManyShared<T, D
         active = uniform(active);
         first_group = uniform(first_group);
         const int b = uniform(first_above(sh.requests, a.batch, slot));
-        const Request q = uniform(request<kPaged>(a, b, falls));
+        const Request q = uniform(request<kPaged>(a, b, sh.requests.falls));
         const int r0 = uniform(slot - (sh.requests.upto[b] - tiles_of(q))) * kRows;
         const int t0 = r0 / g, rem0 = r0 - t0 * g;   // its token, and the rows of that in front
         const int t_last = min(uniform(row_of(a, t0, rem0 + kRows - 1).t), q.todo - 1);
