@@ -444,9 +444,9 @@ __device__ __forceinline__ int first_above(const Sums<kMost>& s, int count, int 
 //
 // MI355X, passes back to back: one token each of 32 requests over 1 to 8000
 // tokens, 64 heads of 128 on 8, bf16: 151 us, 5.2 TB/s of K and V (a copy: 5.35),
-// bound by HBM; 16 requests of 4 tokens over 6000: 67.6 us (of 2: 57); one request
+// bound by HBM; 16 requests of 4 tokens over 6000: 69 us (of 2: 57); one request
 // over 100000: 89 us, 4.6 TB/s, over 8000: 17 us.  One fp32 token of 32 heads of 64
-// on 4 over 2000: 9.2 us: the launch and a chain of trips (lengths, table, keys,
+// on 4 over 2000: 9.3 us: the launch and a chain of trips (lengths, table, keys,
 // ticket, parts) of about a microsecond each.
 template <int D, int RT>
 struct FewShared {
@@ -827,8 +827,8 @@ __device__ __forceinline__ void few_rows(const Args& a, int id, FewShared<D, RT>
 // MI355X, passes back to back: 3 prompts, 12000 tokens in all, 64 heads of 128 on 8,
 // bf16: 963 us, 948 TFLOP/s (a large product: 1150); one of 6500, 64 heads of 64
 // on 8, f16: 380 us, 910 TFLOP/s; 500 tokens behind 30000, 32 heads of 128 on 8,
-// f16: 292 us, 850 TFLOP/s, with 7 tokens of other requests over 22000 beside them
-// 411 to 430; one fp32 prompt of 2000, 64 heads of 128: 536 us, 122 TFLOP/s (153).
+// f16: 297 us, 835 TFLOP/s, with 7 tokens of other requests over 22000 beside them
+// 415 to 430; one fp32 prompt of 2000, 64 heads of 128: 536 us, 122 TFLOP/s (153).
 // The matrix cores are busy 40 % of the cycles: what is left is softmax between
 // the products of two waves a SIMD (without the loads 496 us where it takes 640,
 // without barriers too 472, without exponentials 436).  Eight waves and 128 keys a
